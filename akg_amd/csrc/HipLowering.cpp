@@ -20,6 +20,8 @@ const char *kernelFamilyName(KernelFamily f) {
     case KernelFamily::Indexed: return "indexed";
     case KernelFamily::SegmentSum: return "segment_sum";
     case KernelFamily::GemmRows: return "gemm_rows";
+    case KernelFamily::Rotary: return "rotary";
+    case KernelFamily::Attention: return "attention";
     case KernelFamily::Staged: return "staged";
   }
   return "?";
@@ -604,6 +606,9 @@ LoweredKernel lowerToHip(const OpGraph &described, const LoweringOptions &option
   bool hasMatMul = false;
   for (const OpNode &op : graph.ops) {
     if (op.kind == OpKind::MatMul) hasMatMul = true;
+  }
+  for (const OpNode &op : graph.ops) {
+    if (isLayerKind(op.kind)) return lowerLayerToHip(graph, options);
   }
   for (const OpNode &op : graph.ops) {
     if (op.kind == OpKind::SegmentSum) return lowerSegmentSumToHip(graph, options);

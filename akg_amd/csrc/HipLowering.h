@@ -31,7 +31,7 @@ class LoweringError : public std::runtime_error {
   explicit LoweringError(const std::string &msg) : std::runtime_error(msg) {}
 };
 
-enum class KernelFamily { Elementwise, RowReduce, GemmEpilogue, StreamReduce, Indexed, SegmentSum, Staged, ColumnReduce, GemmRows, PlaneReduce };
+enum class KernelFamily { Elementwise, RowReduce, GemmEpilogue, StreamReduce, Indexed, SegmentSum, Staged, ColumnReduce, GemmRows, PlaneReduce, Rotary, Attention };
 const char *kernelFamilyName(KernelFamily f);
 
 // Tuning knobs; 0 means "let the heuristic decide". They can be set through the environment
@@ -115,6 +115,8 @@ LoweredKernel lowerPlaneToHip(const OpGraph &graph, const LoweringOptions &optio
 LoweredKernel lowerTileToHip(const OpGraph &graph, const LoweringOptions &options);      // elementwise, row_reduce
 LoweredKernel lowerIndexedToHip(const OpGraph &graph, const LoweringOptions &options);
 LoweredKernel lowerSegmentSumToHip(const OpGraph &graph, const LoweringOptions &options);
+// One operator of an attention layer (HipLoweringAttention.cpp).
+LoweredKernel lowerLayerToHip(const OpGraph &graph, const LoweringOptions &options);
 // True when the graph contains a data-movement op (Transpose, Tile, Slice, StridedSlice, Pad, Concat).
 bool wantsIndexedKernel(const OpGraph &graph);
 // True when the reductions of `graph` belong to the streaming family: some reduced axis is not the innermost one

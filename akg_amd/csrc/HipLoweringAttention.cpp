@@ -1,0 +1,375 @@
+/**
+ * The operators of an attention layer (RotaryEmbedding, Attention, AttentionGrad, CacheAttention): descriptions of one op
+ * become an instance of the hand-written kernels in kernels/akg_rotary.hpp, akg_attention.hpp and akg_cache_attention.hpp.
+ * Types, channels, heads, layout and which operands there are go into the source; batch, sequence lengths and the number
+ * of blocks are kernel arguments (LoweredKernel::scalarArgs), so calls that differ there share a code object.
+ */
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <sstream>
+
+#include "HipLowering.h"
+
+namespace akg {
+namespace {
+
+using lowering::dtypeTag;
+
+int64_t ceilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+class LayerEmitter {
+ public:
+  LayerEmitter(const OpGraph &g, const LoweringOptions &options) : g_(g), op_(g.ops[0]), l_(op_.layer), cus_(options.computeUnits) {}
+
+  LoweredKernel run() {
+    for (size_t i = 0; i < g_.outputs.size(); ++i) {
+      for (size_t j = i + 1; j < g_.outputs.size(); ++j) {
+        if (g_.outputs[i] == g_.outputs[j]) throw LoweringError("op " + op_.name + ": a result is listed twice among the outputs");
+      }
+    }
+    k_.kernelName = g_.name + "_kernel";
+    switch (op_.kind) {
+      case OpKind::RotaryEmbedding: rotary(); break;
+      case OpKind::Attention: attention(); break;
+      case OpKind::AttentionGrad: attentionGrad(); break;
+      default: cacheAttention(); break;
+    }
+    for (const KernelPhase &p : k_.earlierPhases) checkGrid(p.grid[0]);
+    k_.shapeArgs = lowering::buildShapeArgs(g_);
+    if (k_.algorithmicBytes == 0) k_.algorithmicBytes = lowering::countAlgorithmicBytes(g_);
+    return k_;
+  }
+
+ private:
+  const OpGraph &g_;
+  const OpNode &op_;
+  const LayerAttributes &l_;
+  const int cus_;
+  LoweredKernel k_;
+
+  const TensorValue &in(size_t i) const { return g_.tensor(op_.inputs[i]); }
+  std::string inName(size_t i) const { return "in" + std::to_string(in(i).inputIndex); }
+  // Argument of result j, or a null pointer where the description does not return it.
+  std::string outName(size_t j) const {
+    if (j >= op_.outputs.size()) return "nullptr";
+    const int index = g_.tensor(op_.outputs[j]).outputIndex;
+    return index < 0 ? "nullptr" : "out" + std::to_string(index);
+  }
+  bool wanted(size_t j) const { return outName(j) != "nullptr"; }
+
+  static unsigned checkGrid(int64_t n) {
+    if (n <= 0 || n >= (1LL << 31)) throw LoweringError("more workgroups than a launch holds");
+    return static_cast<unsigned>(n);
+  }
+  static std::string number(double v) {
+    char buf[40];
+    std::snprintf(buf, sizeof(buf), "%af", static_cast<double>(static_cast<float>(v)));
+    return buf;
+  }
+  static const char *flag(bool b) { return b ? "true" : "false"; }
+
+  std::string signature(const std::vector<std::string> &scalars, bool workspace) const {
+    std::ostringstream o;
+    bool first = true;
+    auto sep = [&]() -> std::ostringstream & {
+      if (!first) o << ", ";
+      first = false;
+      return o;
+    };
+    for (size_t i = 0; i < g_.inputs.size(); ++i) sep() << "const " << dtypeTag(g_.tensor(g_.inputs[i]).dtype) << "::storage *in" << i;
+    for (size_t i = 0; i < g_.outputs.size(); ++i) sep() << dtypeTag(g_.tensor(g_.outputs[i]).dtype) << "::storage *out" << i;
+    for (const std::string &s : scalars) sep() << "long " << s;
+    if (workspace) sep() << "float *akg_ws";
+    return o.str();
+  }
+  std::string head(const char *header) const {
+    return "// Generated by the akg HIP lowering for gfx950. Op description: " + g_.name + "\n// family: attention, op: " + op_.name +
+           "\n#include \"akg_rt.hpp\"\n" + header + "\n";
+  }
+  static std::string kernel(const std::string &name, int threads, const std::string &args, const std::string &body) {
+    return "extern \"C\" __global__ __launch_bounds__(" + std::to_string(threads) + ") void " + name + "(" + args + ") {\n" + body + "}\n\n";
+  }
+  const char *trait() const { return in(0).dtype == DType::BF16 ? "akg::attn::BF16" : "akg::attn::F16"; }
+
+  // ---- RotaryEmbedding ------------------------------------------------------------------------------------------------
+  // Turns per position of every pair, as fractions of 2^64.
+  std::vector<uint64_t> rates() const {
+    std::vector<uint64_t> out;
+    const long double twoPi = 6.283185307179586476925286766559005768L;
+    for (int64_t i = 0; i < l_.rotaryDims / 2; ++i) {
+      long double w = std::pow(static_cast<long double>(l_.base), -2.0L * static_cast<long double>(i) / static_cast<long double>(l_.rotaryDims));
+      if (l_.scaling == LayerAttributes::Scaling::Linear) {
+        w /= static_cast<long double>(l_.factor);
+      } else if (l_.scaling == LayerAttributes::Scaling::Wavelength) {
+        // turns over the original length: at least `high`: as they are; at most `low`: divided; between: both, linearly
+        const long double turns = static_cast<long double>(l_.originalLength) * w / twoPi;
+        long double share = (turns - static_cast<long double>(l_.low)) / static_cast<long double>(l_.high - l_.low);
+        share = std::min(1.0L, std::max(0.0L, share));
+        w = (1.0L - share) * w / static_cast<long double>(l_.factor) + share * w;
+      }
+      out.push_back(static_cast<uint64_t>(std::floor(w / twoPi * 18446744073709551616.0L + 0.5L)));   // (w <= 1: below 2^62)
+    }
+    return out;
+  }
+
+  void rotary() {
+    const size_t tensors = op_.inputs.size() - 1;
+    const TensorValue &x = in(0), &positions = in(tensors);
+    const size_t seqDim = l_.headsFirst ? 2 : 1, headDim = l_.headsFirst ? 1 : 2;
+    const int64_t batch = x.shape[0], seq = x.shape[seqDim], dim = x.shape[3], r = l_.rotaryDims;
+    if (batch * seq >= (1LL << 31)) throw LoweringError("op " + op_.name + ": more than 2^31 tokens");
+    // pairs of a thread: as many as make 16-byte accesses, fewer where the pairs or the copied channels do not divide
+    int64_t pairs = x.dtype == DType::F32 ? 4 : 8;
+    while (pairs > 1 && ((r / 2) % pairs != 0 || (dim - r) % (2 * pairs) != 0)) pairs /= 2;
+    const int64_t chunks = r / 2 / pairs + ceilDiv(dim - r, 2 * pairs);
+    std::vector<int64_t> heads;
+    int64_t all = 0;
+    for (size_t t = 0; t < tensors; ++t) {
+      heads.push_back(in(t).shape[headDim]);
+      all += heads.back();
+    }
+    // heads of a thread: the angles are computed once for them, as long as that leaves enough threads
+    int64_t each = 8;
+    while (each > 1 && batch * seq * chunks * ceilDiv(all, each) < static_cast<int64_t>(cus_) * 512) each /= 2;
+    std::vector<int64_t> groups;
+    int64_t allGroups = 0;
+    for (int64_t h : heads) {
+      groups.push_back(wanted(groups.size()) ? ceilDiv(h, each) : 0);
+      allGroups += groups.back();
+    }
+    const std::vector<uint64_t> rate = rates();
+    std::ostringstream o;
+    o << head("#include \"akg_rotary.hpp\"\n");
+    o << "__device__ const akg::u64 akg_rates[" << rate.size() << "] = {";
+    for (size_t i = 0; i < rate.size(); ++i) o << (i ? ", " : "") << rate[i] << "ull";
+    o << "};\n\n";
+    std::ostringstream b;
+    const bool perBatch = positions.shape.size() == 2 && positions.shape[0] == batch;
+    b << "  constexpr int P = " << pairs << ", CHUNKS = " << chunks << ", GROUPS = " << allGroups << ";\n"
+      << "  const long at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;\n"
+      << "  const long token = at / (CHUNKS * GROUPS);\n  if (token >= akg_batch * akg_seq) return;\n"
+      << "  const int rest = static_cast<int>(at % (CHUNKS * GROUPS)), chunk = rest % CHUNKS, group = rest / CHUNKS;\n"
+      << "  const long b = token / akg_seq, s = token % akg_seq;\n"
+      << "  const akg::u64 position = static_cast<akg::u64>(static_cast<long long>(" << inName(tensors) << "[" << (perBatch ? "token" : "s") << "]));\n"
+      << "  float sine[P], cosine[P];\n#pragma unroll\n  for (int e = 0; e < P; ++e) {\n"
+      << "    const int pair = P * chunk + e;\n"
+      << "    akg::rotary::sine_cosine(position * akg_rates[pair < " << r / 2 << " ? pair : 0], sine[e], cosine[e]);\n"
+      << "    sine[e] *= " << number(l_.inverse ? -l_.magnitude : l_.magnitude) << ";\n    cosine[e] *= " << number(l_.magnitude) << ";\n  }\n";
+    int64_t before = 0;
+    for (size_t t = 0; t < tensors; ++t) {
+      if (groups[t] == 0) continue;
+      b << "  " << (before ? "else " : "") << "if (group < " << before + groups[t] << ") akg::rotary::turn<" << dtypeTag(x.dtype) << ", " << dim << ", " << r
+        << ", " << heads[t] << ", P, " << each << ", " << flag(l_.headsFirst) << ", " << flag(l_.interleaved) << ">(" << inName(t) << ", " << outName(t)
+        << ", b, s, akg_seq, (group - " << before << ") * " << each << ", chunk, sine, cosine);\n";
+      before += groups[t];
+    }
+    o << kernel(k_.kernelName, 256, signature({"akg_batch", "akg_seq"}, false), b.str());
+    k_.source = o.str();
+    k_.family = KernelFamily::Rotary;
+    k_.scalarArgs = {batch, seq};
+    k_.grid[0] = checkGrid(ceilDiv(batch * seq * chunks * allGroups, 256));
+    k_.block[0] = 256;
+    k_.scheduleNote = "pairs per thread " + std::to_string(pairs) + ", heads per thread " + std::to_string(each);
+  }
+
+  // ---- Attention and its gradient -------------------------------------------------------------------------------------
+  struct Sizes {
+    int64_t batch, sq, sk, heads, kvHeads, dk, dv, group, rows, keyHeads;
+  };
+  Sizes sizes(const TensorValue &q, const TensorValue &k, const TensorValue &v) const {
+    const size_t seqDim = l_.headsFirst ? 2 : 1, headDim = l_.headsFirst ? 1 : 2;
+    Sizes s;
+    s.batch = q.shape[0];
+    s.sq = q.shape[seqDim];
+    s.sk = k.shape[seqDim];
+    s.heads = q.shape[headDim];
+    s.kvHeads = k.shape[headDim];
+    s.dk = q.shape[3];
+    s.dv = v.shape[3];
+    s.group = s.heads / s.kvHeads;
+    s.rows = s.sq * s.group;
+    s.keyHeads = s.batch * s.kvHeads;
+    if (s.dk % 8 != 0 || s.dv % 8 != 0 || s.dk > 256 || s.dv > 256) {
+      throw LoweringError("op " + op_.name + ": the channels of a head must be a multiple of 8 up to 256");
+    }
+    // row numbers and key numbers are 32-bit values, and so are byte offsets between the heads that share a tile of rows
+    if (s.rows >= (1LL << 31) - 512 || s.sk >= (1LL << 31) - 512) throw LoweringError("op " + op_.name + ": more than 2^31 rows");
+    const int64_t widest = 2 * std::max(s.dk, s.dv);
+    if ((l_.headsFirst ? s.group * s.sq * widest : 64 * s.heads * widest) >= (1LL << 31) - 65536 || 64 * s.kvHeads * widest >= (1LL << 31) - 65536) {
+      throw LoweringError("op " + op_.name + ": the rows of a tile lie more than 2 GiB apart");
+    }
+    return s;
+  }
+  std::string config(const Sizes &s, size_t maskAt) const {
+    std::ostringstream o;
+    int kind = 0;
+    bool mb = false, mh = false, mq = false;
+    if (l_.hasMask) {
+      const TensorValue &m = in(maskAt);
+      kind = m.dtype == DType::Bool ? 1 : m.dtype == DType::F16 ? 2 : m.dtype == DType::BF16 ? 3 : 4;
+      mb = m.shape[0] > 1;
+      mh = m.shape[1] > 1;
+      mq = m.shape[2] > 1;
+    }
+    o << "typedef akg::attn::Config<" << trait() << ", " << s.dk << ", " << s.dv << ", " << s.kvHeads << ", " << s.group << ", " << flag(l_.headsFirst) << ", "
+      << flag(l_.causal) << ", " << kind << ", " << flag(mb) << ", " << flag(mh) << ", " << flag(mq) << "> akg_C;\n\n";
+    return o.str();
+  }
+  // Mask and lengths as arguments of the kernels' functions.
+  std::string optionals(size_t at) const {
+    std::string s;
+    s += l_.hasMask ? inName(at++) : "nullptr";
+    s += ", " + (l_.hasQueryLengths ? inName(at++) : std::string("nullptr"));
+    s += ", " + (l_.hasKeyLengths ? inName(at++) : std::string("nullptr"));
+    return s;
+  }
+  // Pairs of query and key that see each other where every sequence has its full length.
+  static int64_t pairs(const Sizes &s, bool causal) {
+    if (!causal) return s.sq * s.sk;
+    const int64_t first = s.sk - s.sq + 1, low = std::max<int64_t>(0, 1 - first), n = std::max<int64_t>(0, s.sq - low);
+    return n * (first + low) + n * (n - 1) / 2;
+  }
+  // Wavefronts of a workgroup that gives 32 rows to each: as many as keep every CU busy (a tile is fetched once for all of them).
+  int waves(const Sizes &s, int most) const {
+    int w = most;
+    while (w > 1 && (s.rows <= 32 * (w / 2) || s.keyHeads * ceilDiv(s.rows, 32 * w) < cus_)) w /= 2;
+    return w;
+  }
+
+  void attention() {
+    const Sizes s = sizes(in(0), in(1), in(2));
+    const int nw = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8);
+    const int64_t groups = s.keyHeads * ceilDiv(s.rows, 32 * nw);
+    // few rows and a long axis of keys: several workgroups share it, at least four tiles of 64 each
+    int64_t splits = 1;
+    if (groups < cus_) splits = std::max<int64_t>(1, std::min<int64_t>({ceilDiv(2 * cus_, groups), s.sk / 256, 64}));
+    std::ostringstream o;
+    o << head("#include \"akg_attention.hpp\"\n") << config(s, 3);
+    const std::string args = signature({"akg_batch", "akg_sq", "akg_sk", "akg_splits"}, splits > 1);
+    const std::string extents = "akg::attn::Extents{akg_batch, akg_sq, akg_sk}";
+    const std::string outs = outName(0) + ", " + outName(1);
+    auto call = [&](bool split) {
+      return "  akg::attn::forward<akg_C, " + std::to_string(nw) + ", " + flag(split) + ">(" + inName(0) + ", " + inName(1) + ", " + inName(2) + ", " +
+             optionals(3) + ", " + outs + ", " + (split ? "akg_ws" : "nullptr") + ", " + extents + ", " + number(l_.scale) + ", static_cast<int>(akg_splits));\n";
+    };
+    if (!wanted(0)) throw LoweringError("op " + op_.name + ": its first result must be an output");
+    if (splits > 1) {
+      KernelPhase ranges;
+      ranges.kernelName = g_.name + "_ranges";
+      ranges.grid[0] = checkGrid(groups * splits);
+      ranges.block[0] = static_cast<unsigned>(64 * nw);
+      k_.earlierPhases.push_back(ranges);
+      o << kernel(ranges.kernelName, 64 * nw, args, call(true));
+      o << kernel(k_.kernelName, 256, args, "  akg::attn::join<akg_C>(akg_ws, " + outs + ", " + extents + ", static_cast<int>(akg_splits));\n");
+      k_.grid[0] = checkGrid(ceilDiv(s.keyHeads * s.rows * (s.dv / 4), 256));
+      k_.block[0] = 256;
+      k_.workspaceBytes = static_cast<uint64_t>(splits * s.keyHeads * s.rows * (ceilDiv(s.dv, 32) * 32 + 2) * 4);
+    } else {
+      o << kernel(k_.kernelName, 64 * nw, args, call(false));
+      k_.grid[0] = checkGrid(groups);
+      k_.block[0] = static_cast<unsigned>(64 * nw);
+    }
+    k_.source = o.str();
+    k_.family = KernelFamily::Attention;
+    k_.scalarArgs = {s.batch, s.sq, s.sk, splits};
+    k_.algorithmicOps = static_cast<uint64_t>(2 * (s.dk + s.dv) * s.batch * s.heads * pairs(s, l_.causal));
+    k_.scheduleNote = "32 rows per wavefront, wavefronts " + std::to_string(nw) + ", key ranges " + std::to_string(splits);
+  }
+
+  void attentionGrad() {
+    const Sizes s = sizes(in(1), in(2), in(3));
+    const int nwq = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8), nwk = 4;
+    const int64_t tilesQ = ceilDiv(s.rows, 32 * nwq);
+    std::ostringstream o;
+    o << head("#include \"akg_attention.hpp\"\n") << config(s, 6);
+    const std::string args = signature({"akg_batch", "akg_sq", "akg_sk"}, true);
+    const std::string extents = "akg::attn::Extents{akg_batch, akg_sq, akg_sk}";
+    std::ostringstream queries, keys;
+    queries << "  akg::attn::backward_queries<akg_C, " << nwq << ">(" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << inName(3) << ", "
+            << inName(4) << ", " << inName(5) << ", " << optionals(6) << ", " << outName(0) << ", akg_ws, " << extents << ", " << number(l_.scale) << ");\n";
+    keys << "  akg::attn::backward_keys<akg_C, " << nwk << ", " << nwq << ">(" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << inName(3)
+         << ", " << inName(5) << ", " << optionals(6) << ", " << outName(1) << ", " << outName(2) << ", akg_ws, " << extents << ", " << number(l_.scale) << ");\n";
+    KernelPhase first;
+    first.kernelName = g_.name + "_queries";
+    first.grid[0] = checkGrid(s.keyHeads * tilesQ);
+    first.block[0] = static_cast<unsigned>(64 * nwq);
+    k_.earlierPhases.push_back(first);
+    o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(k_.kernelName, 64 * nwk, args, keys.str());
+    k_.grid[0] = checkGrid(s.keyHeads * ceilDiv(s.sk, 32 * nwk));
+    k_.block[0] = static_cast<unsigned>(64 * nwk);
+    // per row delta (and, for an added mask, two parts of its log-sum), per workgroup of the first kernel the largest |dout|
+    const bool added = l_.hasMask && in(6).dtype != DType::Bool;
+    k_.workspaceBytes = static_cast<uint64_t>(4 * s.keyHeads * ((added ? 3 : 1) * s.rows + tilesQ));
+    k_.source = o.str();
+    k_.family = KernelFamily::Attention;
+    k_.scalarArgs = {s.batch, s.sq, s.sk};
+    k_.algorithmicOps = static_cast<uint64_t>((6 * s.dk + 4 * s.dv) * s.batch * s.heads * pairs(s, l_.causal));
+    k_.scheduleNote = "32 rows per wavefront, wavefronts " + std::to_string(nwq) + " (dq), " + std::to_string(nwk) + " (dk, dv)";
+  }
+
+  // ---- CacheAttention -------------------------------------------------------------------------------------------------
+  void cacheAttention() {
+    const TensorValue &q = in(0), &cache = in(1), &table = in(5);
+    const int64_t batch = q.shape[0], sq = q.shape[1], heads = q.shape[2], dim = q.shape[3];
+    const int64_t blocks = cache.shape[0], kvHeads = cache.shape[1], page = cache.shape[2], perSequence = table.shape[1];
+    const int64_t group = heads / kvHeads, rows = sq * group;
+    if (dim % 16 != 0 || dim > 256) throw LoweringError("op " + op_.name + ": the channels of a head must be a multiple of 16 up to 256");
+    if (page % 16 != 0) throw LoweringError("op " + op_.name + ": the tokens of a block must be a multiple of 16");
+    if (rows >= (1LL << 30) || perSequence * page >= (1LL << 30)) throw LoweringError("op " + op_.name + ": more than 2^30 tokens or rows");
+    const int64_t units = ceilDiv(dim, 64);
+    const int64_t rt = std::min<int64_t>(ceilDiv(rows, 16), std::max<int64_t>(1, std::min<int64_t>(4, 8 / units)));
+    const int64_t groups = batch * kvHeads * ceilDiv(rows, 16 * rt);
+    // workgroups that share a sequence: four to a CU, at least one step of 32 tokens for each of their four wavefronts
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({ceilDiv(4 * cus_, groups), ceilDiv(perSequence * page, 128), 64}));
+    std::ostringstream o;
+    o << head("#include \"akg_attention.hpp\"\n#include \"akg_cache_attention.hpp\"\n")
+      << "typedef akg::attn::Config<" << trait() << ", " << dim << ", " << dim << ", " << kvHeads << ", " << group
+      << ", false, true, 0, false, false, false> akg_C;\n\n";
+    const std::string args = signature({"akg_batch", "akg_sq", "akg_blocks", "akg_per_sequence", "akg_splits"}, splits > 1);
+    auto call = [&](bool split) {
+      std::ostringstream c;
+      c << "  akg::attn::over_cache<akg_C, " << page << ", " << rt << ", " << flag(split) << ">(";
+      for (size_t i = 0; i < 7; ++i) c << inName(i) << ", ";
+      c << outName(0) << ", " << (split ? "akg_ws" : "nullptr") << ", akg::attn::CacheExtents{akg_batch, akg_sq, akg_blocks, akg_per_sequence}, "
+        << number(l_.scale) << ", static_cast<int>(akg_splits));\n";
+      return c.str();
+    };
+    if (splits > 1) {
+      KernelPhase ranges;
+      ranges.kernelName = g_.name + "_ranges";
+      ranges.grid[0] = checkGrid(groups * splits);
+      ranges.block[0] = 256;
+      k_.earlierPhases.push_back(ranges);
+      o << kernel(ranges.kernelName, 256, args, call(true))
+        << kernel(k_.kernelName, 256, args, "  akg::attn::join<akg_C>(akg_ws, " + outName(0) +
+                  ", nullptr, akg::attn::Extents{akg_batch, akg_sq, 0}, static_cast<int>(akg_splits));\n");
+      k_.grid[0] = checkGrid(ceilDiv(batch * kvHeads * rows * (dim / 4), 256));
+      k_.workspaceBytes = static_cast<uint64_t>(splits * batch * kvHeads * rows * (ceilDiv(dim, 32) * 32 + 2) * 4);
+    } else {
+      o << kernel(k_.kernelName, 256, args, call(false));
+      k_.grid[0] = checkGrid(groups);
+    }
+    k_.block[0] = 256;
+    k_.source = o.str();
+    k_.family = KernelFamily::Attention;
+    k_.scalarArgs = {batch, sq, blocks, perSequence, splits};
+    // (of the pool, at most the blocks that the table names)
+    const uint64_t live = static_cast<uint64_t>(std::min(blocks, batch * perSequence));
+    k_.algorithmicBytes = 2 * live * static_cast<uint64_t>(kvHeads) * static_cast<uint64_t>(page * dim + 4) + 4 * static_cast<uint64_t>(table.numel() + batch) +
+                          2 * 2 * static_cast<uint64_t>(q.numel());
+    k_.algorithmicOps = static_cast<uint64_t>(4 * dim * batch * heads * sq * perSequence * page);
+    k_.scheduleNote = "row tiles " + std::to_string(rt) + ", workgroups per sequence and key head " + std::to_string(splits);
+  }
+};
+
+}  // namespace
+
+LoweredKernel lowerLayerToHip(const OpGraph &graph, const LoweringOptions &options) {
+  // (operands that other ops compute lie in memory first: the description is cut there)
+  if (graph.ops.size() != 1) throw LoweringError("op " + graph.ops[0].name + ": operators of an attention layer are kernels of their own");
+  LayerEmitter emitter(graph, options);
+  return emitter.run();
+}
+
+}  // namespace akg

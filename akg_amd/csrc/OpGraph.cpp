@@ -1,6 +1,7 @@
 #include "OpGraph.h"
 
 #include <algorithm>
+#include <cmath>
 #include <sstream>
 
 #include "Json.h"
@@ -99,6 +100,11 @@ const OpTableEntry kOpTable[] = {
   {"MatMul", OpKind::MatMul},
   {"BatchMatMul", OpKind::MatMul},
   {"Cast", OpKind::Cast},
+  // not in the reference's table: the operators of an attention layer
+  {"RotaryEmbedding", OpKind::RotaryEmbedding},
+  {"Attention", OpKind::Attention},
+  {"AttentionGrad", OpKind::AttentionGrad},
+  {"CacheAttention", OpKind::CacheAttention},
 };
 
 OpKind lookupOpKind(const std::string &name) {
@@ -334,6 +340,7 @@ class GraphBuilder {
           least = most = 2;
         }
         if (node.kind == OpKind::Concat || node.kind == OpKind::AddN) most = static_cast<size_t>(-1);
+        if (isLayerKind(node.kind)) least = most = layerOperands(&node, attrs);
         if (node.inputs.size() < least || node.inputs.size() > most) {
           throw TranslateError("op " + node.name + ": " + std::to_string(node.inputs.size()) + " operands where " +
                                (most == least ? std::to_string(least) : "at least " + std::to_string(least)) + " are read");
@@ -409,6 +416,7 @@ class GraphBuilder {
         }
       }
       (void)fakeOutput;
+      std::vector<TensorValue> layerResults;   // types and shapes of every result (operators of an attention layer)
       std::vector<int64_t> inferred;  // result shape derived from the operands (empty: take the declared one)
       if (node.name == "Split") {
         // handled below, once the result tensors exist
@@ -416,6 +424,8 @@ class GraphBuilder {
           node.kind == OpKind::StridedSlice || node.kind == OpKind::Pad || node.kind == OpKind::Concat ||
           node.kind == OpKind::Gather) {
         inferred = parseDataMovement(&node, attrs, inputDesc, readShape(outputDesc[0]));
+      } else if (isLayerKind(node.kind)) {
+        layerResults = layerResultTensors(node, outputDesc.size());
       } else if (binding_ != nullptr) {
         inferred = inferResultShape(node, attrs, inputDesc, readShape(outputDesc[0]));
       }
@@ -430,6 +440,14 @@ class GraphBuilder {
         for (int64_t e : shape) dynamic = dynamic || e < 0;
         if (dynamic && binding_ != nullptr && j == 0 && !inferred.empty()) shape = inferred;
         if (node.kind == OpKind::Assign) shape = graph_.tensor(node.inputs[0]).shape;  // (:359-364, :398-404)
+        if (!layerResults.empty()) {
+          const TensorValue &r = layerResults[j];
+          bool same = shape.size() == r.shape.size();
+          for (size_t x = 0; same && x < shape.size(); ++x) same = shape[x] == r.shape[x] || (shape[x] < 0 && binding_ != nullptr);
+          if (!same) throw TranslateError("op " + node.name + ": the declared shape of result " + tensorName + " does not follow from the operands");
+          if (dtype != r.dtype) throw TranslateError("op " + node.name + ": result " + tensorName + " must be " + dtypeName(r.dtype));
+          shape = r.shape;
+        }
         int id = addTensor(tensorName, dtype, shape);
         graph_.tensors[static_cast<size_t>(id)].producer = opIndex;
         node.outputs.push_back(id);
@@ -570,6 +588,170 @@ class GraphBuilder {
       if (out.size() < declared.size()) out.insert(out.begin(), declared.size() - out.size(), 1);
     }
     return out;
+  }
+
+  // ---- operators of an attention layer ------------------------------------------------------------------------------
+  static double numberAttr(const json::Value &attrs, const char *name, double otherwise) {
+    const json::Value *a = findAttr(attrs, name);
+    if (a == nullptr) return otherwise;
+    if (!a->isNumber()) throw TranslateError(std::string("attribute ") + name + " must be a number");
+    return a->asDouble();
+  }
+  static bool boolAttr(const json::Value &attrs, const char *name) {
+    const json::Value *a = findAttr(attrs, name);
+    if (a == nullptr) return false;
+    if (!a->isBool()) throw TranslateError(std::string("attribute ") + name + " must be a bool");
+    return a->asBool();
+  }
+  static std::string textAttr(const json::Value &attrs, const char *name, const char *otherwise) {
+    const json::Value *a = findAttr(attrs, name);
+    if (a == nullptr) return otherwise;
+    if (!a->isString()) throw TranslateError(std::string("attribute ") + name + " must be a str");
+    return a->asString();
+  }
+
+  // Reads the attributes; returns how many operands they ask for.
+  size_t layerOperands(OpNode *node, const json::Value &attrs) {
+    LayerAttributes &l = node->layer;
+    const std::string at = "op " + node->name + ": ";
+    const std::string layout = textAttr(attrs, "layout", "BSND");
+    if (layout != "BSND" && layout != "BNSD") throw TranslateError(at + "layout must be BSND or BNSD");
+    l.headsFirst = layout == "BNSD";
+    if (node->kind == OpKind::RotaryEmbedding) {
+      l.base = numberAttr(attrs, "base", 10000.0);
+      l.magnitude = numberAttr(attrs, "magnitude", 1.0);
+      l.rotaryDims = static_cast<int64_t>(numberAttr(attrs, "rotary_dims", 0.0));
+      l.interleaved = boolAttr(attrs, "interleaved");
+      l.inverse = boolAttr(attrs, "inverse");
+      const std::string scaling = textAttr(attrs, "scaling", "none");
+      l.factor = numberAttr(attrs, "factor", 1.0);
+      l.low = numberAttr(attrs, "low", 1.0);
+      l.high = numberAttr(attrs, "high", 4.0);
+      l.originalLength = numberAttr(attrs, "original_length", 0.0);
+      if (scaling == "linear") {
+        l.scaling = LayerAttributes::Scaling::Linear;
+      } else if (scaling == "wavelength") {
+        l.scaling = LayerAttributes::Scaling::Wavelength;
+        if (!(l.originalLength > 0.0) || !(l.low > 0.0) || !(l.high > l.low)) {
+          throw TranslateError(at + "scaling by wavelength needs original_length > 0 and 0 < low < high");
+        }
+      } else if (scaling != "none") {
+        throw TranslateError(at + "scaling must be none, linear or wavelength");
+      }
+      if (!(l.base > 1.0) || !(l.factor >= 1.0)) throw TranslateError(at + "base must be above 1 and factor at least 1");
+      if (node->inputs.size() != 2 && node->inputs.size() != 3) throw TranslateError(at + "takes one or two tensors and their positions");
+      return node->inputs.size();
+    }
+    l.scale = numberAttr(attrs, "scale", 0.0);
+    if (findAttr(attrs, "scale") != nullptr && !(l.scale > 0.0)) throw TranslateError(at + "scale must be above 0");
+    if (node->kind == OpKind::CacheAttention) {
+      if (l.headsFirst) throw TranslateError(at + "layout must be BSND");
+      return 7;
+    }
+    l.causal = boolAttr(attrs, "causal");
+    l.hasMask = boolAttr(attrs, "has_mask");
+    l.hasQueryLengths = boolAttr(attrs, "has_query_lengths");
+    l.hasKeyLengths = boolAttr(attrs, "has_key_lengths");
+    return (node->kind == OpKind::Attention ? 3u : 6u) + (l.hasMask ? 1 : 0) + (l.hasQueryLengths ? 1 : 0) + (l.hasKeyLengths ? 1 : 0);
+  }
+
+  // Checks the operands; returns type and shape of every result.
+  std::vector<TensorValue> layerResultTensors(OpNode &node, size_t results) {
+    LayerAttributes &l = node.layer;
+    const std::string at = "op " + node.name + ": ";
+    auto operand = [&](size_t i) -> const TensorValue & { return graph_.tensor(node.inputs[i]); };
+    auto need = [&](bool ok, const std::string &what) {
+      if (!ok) throw TranslateError(at + what);
+    };
+    auto like = [](const TensorValue &t) {
+      TensorValue r;
+      r.dtype = t.dtype;
+      r.shape = t.shape;
+      return r;
+    };
+    for (int id : node.inputs) need(!graph_.tensor(id).isConst, "operands must be tensors, not constants");
+    const TensorValue &x = operand(0);
+    need(x.shape.size() == 4, "tensors of heads must have four dimensions");
+    need(x.dtype == DType::F16 || x.dtype == DType::BF16 || (x.dtype == DType::F32 && node.kind == OpKind::RotaryEmbedding),
+         node.kind == OpKind::RotaryEmbedding ? "tensors must be float16, bfloat16 or float32" : "tensors must be float16 or bfloat16");
+    const size_t seqDim = l.headsFirst ? 2 : 1, headDim = l.headsFirst ? 1 : 2;
+    const int64_t batch = x.shape[0], seq = x.shape[seqDim], heads = x.shape[headDim], dim = x.shape[3];
+    if (node.kind == OpKind::RotaryEmbedding) {
+      if (l.rotaryDims == 0) l.rotaryDims = dim;
+      need(l.rotaryDims > 0 && l.rotaryDims <= dim && l.rotaryDims % 2 == 0, "rotary_dims must be even and at most the channels of a head");
+      const size_t tensors = node.inputs.size() - 1;
+      need(results == tensors, "one result for every tensor turned");
+      std::vector<TensorValue> out;
+      for (size_t i = 0; i < tensors; ++i) {
+        const TensorValue &t = operand(i);
+        need(t.dtype == x.dtype && t.shape.size() == 4 && t.shape[0] == batch && t.shape[seqDim] == seq && t.shape[3] == dim,
+             "the two tensors may differ in their number of heads only");
+        out.push_back(like(t));
+      }
+      const TensorValue &p = operand(tensors);
+      need(p.dtype == DType::I32 || p.dtype == DType::I64, "positions must be int32 or int64");
+      need((p.shape.size() == 1 && p.shape[0] == seq) || (p.shape.size() == 2 && (p.shape[0] == batch || p.shape[0] == 1) && p.shape[1] == seq),
+           "positions must be [sequence] or [batch, sequence]");
+      return out;
+    }
+    auto lengths = [&](size_t i, const char *what) {
+      need(operand(i).dtype == DType::I32 && operand(i).shape.size() == 1 && operand(i).shape[0] == batch,
+           std::string(what) + " must be int32 [batch]");
+    };
+    if (node.kind == OpKind::CacheAttention) {
+      const TensorValue &kc = operand(1), &vc = operand(2), &ks = operand(3), &vs = operand(4), &table = operand(5);
+      need(kc.dtype == DType::I8 && vc.dtype == DType::I8 && kc.shape.size() == 4 && kc.shape == vc.shape,
+           "the caches must be int8 [blocks, key heads, tokens of a block, channels], both alike");
+      need(kc.shape[3] == dim, "queries and cache differ in the channels of a head");
+      need(heads % kc.shape[1] == 0, "the heads must be a multiple of the key heads");
+      const std::vector<int64_t> scales{kc.shape[0], kc.shape[1]};
+      need(ks.dtype == DType::F32 && vs.dtype == DType::F32 && ks.shape == scales && vs.shape == scales, "the scales must be float32 [blocks, key heads]");
+      need(table.dtype == DType::I32 && table.shape.size() == 2 && table.shape[0] == batch, "the block table must be int32 [batch, blocks of a sequence]");
+      lengths(6, "lengths");
+      need(results == 1, "has one result");
+      if (l.scale == 0.0) l.scale = 1.0 / std::sqrt(static_cast<double>(dim));
+      return {like(x)};
+    }
+    // Attention: q, k, v ...; AttentionGrad: dout, q, k, v, out, lse ...
+    const bool grad = node.kind == OpKind::AttentionGrad;
+    const TensorValue &q = operand(grad ? 1 : 0), &k = operand(grad ? 2 : 1), &v = operand(grad ? 3 : 2);
+    need(q.shape.size() == 4 && k.shape.size() == 4 && v.shape.size() == 4, "tensors of heads must have four dimensions");
+    need(q.dtype == x.dtype && k.dtype == x.dtype && v.dtype == x.dtype, "queries, keys and values must have one type");
+    need(q.shape[0] == batch && q.shape[seqDim] == seq && q.shape[headDim] == heads, "the gradient must have the shape of the result");
+    need(k.shape[0] == batch && v.shape[0] == batch, "queries, keys and values differ in their batch");
+    need(k.shape[seqDim] == v.shape[seqDim] && k.shape[headDim] == v.shape[headDim], "keys and values differ in length or heads");
+    need(k.shape[3] == q.shape[3], "queries and keys differ in the channels of a head");
+    need(heads % k.shape[headDim] == 0, "the heads must be a multiple of the key heads");
+    const int64_t keys = k.shape[seqDim];
+    if (l.scale == 0.0) l.scale = 1.0 / std::sqrt(static_cast<double>(q.shape[3]));
+    TensorValue out = like(q);
+    out.shape[3] = v.shape[3];
+    TensorValue lse;
+    lse.dtype = DType::F32;
+    lse.shape = {batch, heads, seq};
+    size_t next = 3;
+    if (grad) {
+      need(x.shape == out.shape && operand(4).shape == out.shape && operand(4).dtype == x.dtype, "result and its gradient must be [.., channels of the values]");
+      need(operand(5).dtype == DType::F32 && operand(5).shape == lse.shape, "lse must be float32 [batch, heads, sequence]");
+      next = 6;
+    }
+    if (l.hasMask) {
+      const TensorValue &m = operand(next++);
+      need(m.dtype == DType::Bool || m.dtype == DType::F16 || m.dtype == DType::BF16 || m.dtype == DType::F32, "the mask must be bool, float16, bfloat16 or float32");
+      const int64_t whole[3] = {batch, heads, seq};
+      bool fits = m.shape.size() == 4 && m.shape[3] == keys;
+      for (size_t d = 0; fits && d < 3; ++d) fits = m.shape[d] == whole[d] || m.shape[d] == 1;
+      need(fits, "the mask must be [batch or 1, heads or 1, queries or 1, keys]");
+    }
+    if (l.hasQueryLengths) lengths(next++, "query lengths");
+    if (l.hasKeyLengths) lengths(next++, "key lengths");
+    if (grad) {
+      need(results == 3, "has three results: the gradients of queries, keys and values");
+      return {like(q), like(k), like(v)};
+    }
+    need(results == 1 || results == 2, "has one or two results: the values' means and the log of the sums");
+    if (results == 1) return {out};
+    return {out, lse};
   }
 
   std::vector<int64_t> parseDataMovement(OpNode *node, const json::Value &attrs, const json::Value &inputDesc,
@@ -784,6 +966,9 @@ OperatorTemplate templateOfOp(const OpGraph &g, const OpNode &op) {
     case OpKind::ReduceAny:
       return OperatorTemplate::Reduction;
     case OpKind::MatMul:
+    case OpKind::Attention:
+    case OpKind::AttentionGrad:
+    case OpKind::CacheAttention:
       return OperatorTemplate::Matmul;
     case OpKind::Reshape:
       return OperatorTemplate::Reshape;
@@ -798,6 +983,7 @@ OperatorTemplate templateOfOp(const OpGraph &g, const OpNode &op) {
     case OpKind::Concat:
     case OpKind::Gather:
     case OpKind::SegmentSum:
+    case OpKind::RotaryEmbedding:
       return OperatorTemplate::Default;  // not classified by getOperatorTemplate (OperatorIdentify.cpp:51-75)
     case OpKind::Unknown:
     case OpKind::Unsupported:
@@ -932,11 +1118,19 @@ const char *opKindName(OpKind k) {
     case OpKind::SegmentSum: return "unsorted_segment_sum";
     case OpKind::MatMul: return "matmul";
     case OpKind::AddN: return "addn";
+    case OpKind::RotaryEmbedding: return "rotary_embedding";
+    case OpKind::Attention: return "attention";
+    case OpKind::AttentionGrad: return "attention_grad";
+    case OpKind::CacheAttention: return "cache_attention";
     case OpKind::Assign: return "inplace_assign";
     case OpKind::Unsupported: return "unsupported";
     case OpKind::Unknown: return "unknown";
   }
   return "?";
+}
+
+bool isLayerKind(OpKind k) {
+  return k == OpKind::RotaryEmbedding || k == OpKind::Attention || k == OpKind::AttentionGrad || k == OpKind::CacheAttention;
 }
 
 const char *operatorTemplateName(OperatorTemplate t) {
@@ -1224,6 +1418,18 @@ std::string printOpGraph(const OpGraph &g) {
       os << ", value = " << op.padValue << "}";
     } else if (op.kind == OpKind::Concat || op.kind == OpKind::Gather) {
       os << " {axis = " << op.concatAxis << "}";
+    }
+    if (isLayerKind(op.kind)) {
+      const LayerAttributes &l = op.layer;
+      os << " {layout = \"" << (l.headsFirst ? "BNSD" : "BSND") << "\"";
+      if (op.kind == OpKind::RotaryEmbedding) {
+        static const char *const kScaling[] = {"none", "linear", "wavelength"};
+        os << ", base = " << l.base << ", rotary_dims = " << l.rotaryDims << ", interleaved = " << (l.interleaved ? "true" : "false")
+           << ", inverse = " << (l.inverse ? "true" : "false") << ", scaling = \"" << kScaling[static_cast<int>(l.scaling)] << "\"";
+      } else {
+        os << ", scale = " << l.scale << ", causal = " << (l.causal ? "true" : "false");
+      }
+      os << "}";
     }
     if (op.kind == OpKind::Unknown) os << " {ori_op = \"" << op.name << "\"}";
     os << " : " << typeStr(g.tensor(op.outputs[0])) << "\n";

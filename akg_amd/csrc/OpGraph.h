@@ -55,6 +55,8 @@ enum class OpKind {
   Iota,
   // contraction
   MatMul,
+  // the operators of an attention layer, each a kernel of its own (LayerAttributes)
+  RotaryEmbedding, Attention, AttentionGrad, CacheAttention,
   // n-ary
   AddN,
   // Assign / InplaceAssign: the result is the second operand; as a side effect it is also written over the first
@@ -67,6 +69,8 @@ enum class OpKind {
 };
 
 const char *opKindName(OpKind k);
+// RotaryEmbedding, Attention, AttentionGrad, CacheAttention.
+bool isLayerKind(OpKind k);
 
 // OperatorTemplate lattice of akg-mlir/include/akg/Utils/AnalysisCommon.hpp:127; the fusion class of a kernel
 // is the maximum over its ops (akg-mlir/lib/Transforms/OperatorIdentify.cpp:51-93).
@@ -89,7 +93,24 @@ struct TensorValue {
   int64_t numel() const;
 };
 
+// Attributes of RotaryEmbedding, Attention, AttentionGrad and CacheAttention.
+struct LayerAttributes {
+  bool headsFirst = false;        // "layout": "BSND" (default) or "BNSD"
+  // Attention and its gradient: optional operands behind the fixed ones, in this order
+  bool hasMask = false, hasQueryLengths = false, hasKeyLengths = false;
+  bool causal = false;
+  double scale = 0.0;             // of the scores; the translator puts 1 / sqrt(channels) where none is given
+  // RotaryEmbedding
+  double base = 10000.0, magnitude = 1.0;
+  int64_t rotaryDims = 0;         // leading channels of a head that are turned
+  bool interleaved = false;       // pairs of adjacent channels (else channel i and i + rotaryDims / 2)
+  bool inverse = false;           // turned back: the gradient
+  enum class Scaling { None, Linear, Wavelength } scaling = Scaling::None;
+  double factor = 1.0, low = 1.0, high = 4.0, originalLength = 0.0;
+};
+
 struct OpNode {
+  LayerAttributes layer;
   std::string name;           // JSON op name, e.g. "RealDiv"
   OpKind kind = OpKind::Unknown;
   std::vector<int> inputs;    // tensor ids

@@ -117,7 +117,7 @@ bool planStages(const std::string &jsonText, const OpGraph &g, bool reductionsTo
       *why = "op " + op.name + " is not cut into stages";
       return false;
     }
-    if (op.outputs.size() != 1) {
+    if (op.outputs.size() != 1 && !isLayerKind(op.kind)) {
       *why = "op " + op.name + " has several results";
       return false;
     }
@@ -156,12 +156,15 @@ bool planStages(const std::string &jsonText, const OpGraph &g, bool reductionsTo
       }
     }
     for (const OpNode &op : g.ops) {
+      if (isLayerKind(op.kind)) {   // (a kernel of its own, with all its results)
+        for (int out : op.outputs) cutResult[static_cast<size_t>(out)] = true;
+      }
       const int out = op.outputs[0];
       if (isViewOp(op.kind) || (reductionsToo && lowering::isReduceKind(op.kind)) ||
           (op.kind == OpKind::MatMul && feedsReduction[static_cast<size_t>(out)]) || op.kind == OpKind::SegmentSum) {
         cutResult[static_cast<size_t>(out)] = true;
       }
-      if (op.kind == OpKind::MatMul || op.kind == OpKind::SegmentSum) {   // (their kernels read operands from memory)
+      if (op.kind == OpKind::MatMul || op.kind == OpKind::SegmentSum || isLayerKind(op.kind)) {   // (their kernels read operands from memory)
         for (int in : op.inputs) {
           if (g.tensor(in).producer >= 0) cutResult[static_cast<size_t>(in)] = true;
         }
@@ -319,6 +322,14 @@ bool planStages(const std::string &jsonText, const OpGraph &g, bool reductionsTo
     for (const OpNode &op : g.ops) {
       const bool isReduce = lowering::isReduceKind(op.kind);
       if (!cutResult[static_cast<size_t>(op.outputs[0])]) continue;
+      if (isLayerKind(op.kind)) {
+        for (int result : op.outputs) {
+          if (needed[static_cast<size_t>(result)] && level[static_cast<size_t>(result)] == s + 1) {
+            reduceGroups["op" + std::to_string(op.outputs[0])].push_back(result);
+          }
+        }
+        continue;
+      }
       const int out = op.outputs[0];
       if (!needed[static_cast<size_t>(out)] || level[static_cast<size_t>(out)] != s + 1) continue;
       std::ostringstream key;

@@ -1,0 +1,882 @@
+/**
+ * Attention for gfx950 that keeps no probabilities: the forward pass with the running maximum and sum of a softmax, and
+ * the backward pass, which recomputes the probabilities from the log of that sum.
+ *
+ *   s = scale q k^T (+ mask), lse = log sum_j exp s, out = exp(s - lse) v
+ *   delta = rowsum(dout out), p = exp(s - lse), ds = p (dout v^T - delta)
+ *   dv = p^T dout, dq = scale ds k, dk = scale ds^T q
+ *
+ * Every product runs on v_mfma_f32_32x32x16 with float32 accumulators. A wavefront owns 32 rows (queries, or keys in the
+ * kernel of dk and dv) as the COLUMNS of its MFMA results: lane n and n + 32 hold row n, so that the maximum, the sum and
+ * the rescaling of a row are values of one lane pair, and the probabilities that one MFMA leaves in a lane are already the
+ * operand of the next one. A lane holds of every 16 contracted positions those 4 h .. 4 h + 3 and 8 + 4 h .. 8 + 4 h + 3
+ * (h = lane / 32); the order of contracted positions does not matter as long as both operands have the same, and the
+ * transposing LDS reads fetch four adjacent positions each, so nothing is exchanged between lanes.
+ *
+ * The other side's tiles lie in LDS as they lie in memory (rows of channels). They are read two ways: along the row
+ * (16 bytes of a row per lane) and transposed (ds_read_b64_tr_b16: four rows of 16 columns per sixteen lanes). Rows are an
+ * odd multiple of 64 bytes apart, so four neighbouring rows of 64 bytes cover the 256 bytes of the banks (transposed
+ * reads), and the 16-byte chunks inside 64 bytes are permuted by (row / 4) % 4, so the sixteen rows that a 128-bit read
+ * serves at a time (the lane quads 0, 3, 5, 6 of a half wavefront, then 1, 2, 4, 7) fall into different bank groups.
+ *
+ * Heads that share keys are rows of one problem: row r of a key head is query r / G of head r % G, so the tiles of keys
+ * and values are fetched once for the group, and the gradients of keys and values are sums without atomics.
+ */
+#pragma once
+
+namespace akg {
+namespace attn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef u32 u32x4 __attribute__((ext_vector_type(4)));
+typedef u32 u32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+struct BF16 {
+  typedef bf16 dtype;
+  static constexpr bool kNarrowRange = false;
+  typedef __bf16 frag __attribute__((ext_vector_type(8)));
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  static AKG_DEV f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(frag, a), __builtin_bit_cast(frag, b), c, 0, 0, 0);
+  }
+  static AKG_DEV u32 pack(float lo, float hi) {
+    const pair p = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
+    return __builtin_bit_cast(u32, p);
+  }
+  static AKG_DEV float low(u32 w) { return __builtin_bit_cast(float, w << 16); }
+  static AKG_DEV float high(u32 w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+};
+struct F16 {
+  typedef f16 dtype;
+  static constexpr bool kNarrowRange = true;
+  typedef _Float16 frag __attribute__((ext_vector_type(8)));
+  typedef _Float16 pair __attribute__((ext_vector_type(2)));
+  static AKG_DEV f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(frag, a), __builtin_bit_cast(frag, b), c, 0, 0, 0);
+  }
+  static AKG_DEV u32 pack(float lo, float hi) {
+    const pair p = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
+    return __builtin_bit_cast(u32, p);
+  }
+  static AKG_DEV float low(u32 w) { return static_cast<float>(__builtin_bit_cast(pair, w)[0]); }
+  static AKG_DEV float high(u32 w) { return static_cast<float>(__builtin_bit_cast(pair, w)[1]); }
+};
+
+constexpr float kLog2e = 0x1.715476p+0f, kLn2 = 0x1.62e430p-1f;
+constexpr int kRows = 32;      // rows of a wavefront
+constexpr int kTile = 64;      // keys of a tile (forward, dq)
+constexpr int kTileRows = 32;  // queries of a tile (dk, dv)
+
+constexpr int padded(int d) { return (d + 31) / 32 * 32; }
+constexpr int pitch(int d) { return padded(d) / 32 % 2 == 1 ? padded(d) * 2 : padded(d) * 2 + 64; }
+
+AKG_DEV float neg_inf() { return -__builtin_inff(); }
+// The two halves of a row's lane pair (n and n + 32) joined.
+AKG_DEV float max_halves(float v) {
+  const u32 w = __builtin_bit_cast(u32, v);
+  const auto s = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __builtin_fmaxf(__builtin_bit_cast(float, static_cast<u32>(s[0])), __builtin_bit_cast(float, static_cast<u32>(s[1])));
+}
+AKG_DEV float add_halves(float v) {
+  const u32 w = __builtin_bit_cast(u32, v);
+  const auto s = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return __builtin_bit_cast(float, static_cast<u32>(s[0])) + __builtin_bit_cast(float, static_cast<u32>(s[1]));
+}
+
+// ---- what the emitted kernel states about its description -------------------------------------------------------------
+// Extents that are kernel arguments, and what follows from them.
+struct Extents {
+  long batch, sq, sk;
+};
+
+// MASK: 0 none, 1 bool (true: the pair counts), 2 float16, 3 bfloat16, 4 float32 (added to the scaled score).
+template <typename T_, int DK_, int DV_, int HKV_, int G_, bool HEADS_FIRST_, bool CAUSAL_, int MASK_, bool MASK_B_, bool MASK_H_, bool MASK_Q_>
+struct Config {
+  typedef T_ T;
+  static constexpr int DK = DK_, DV = DV_, HKV = HKV_, G = G_, H = HKV_ * G_, MASK = MASK_;
+  static constexpr bool HEADS_FIRST = HEADS_FIRST_, CAUSAL = CAUSAL_;
+  // which leading dimensions of the mask are the scores' (the others have extent 1)
+  static constexpr bool MASK_B = MASK_B_, MASK_H = MASK_H_, MASK_Q = MASK_Q_;
+  // Scores are exponents of 2 (scale log2 e in one factor), unless a mask is added: its lowest values times log2 e would
+  // leave float32, so sums of score and mask, and their maxima, are kept as they are and differences are multiplied.
+  static constexpr bool ADDED = MASK_ >= 2;
+};
+
+// Where the rows of one key head lie, in bytes: row r = query r / G of head r % G.
+template <typename C, int D>
+struct RowsOf {
+  const char *base;     // of (batch, first head of the group)
+  long stepI, stepG;    // from query to query, from head to head
+  AKG_DEV RowsOf(const void *p, long b, long hkv, const Extents &e) {
+    if (C::HEADS_FIRST) {
+      stepI = 2L * D;
+      stepG = 2L * D * e.sq;
+      base = static_cast<const char *>(p) + (b * C::H + hkv * C::G) * stepG;
+    } else {
+      stepI = 2L * D * C::H;
+      stepG = 2L * D;
+      base = static_cast<const char *>(p) + (b * e.sq) * stepI + hkv * C::G * stepG;
+    }
+  }
+  AKG_DEV long offset(long r) const { return r / C::G * stepI + r % C::G * stepG; }
+};
+template <typename C, int D>
+struct KeysOf {
+  const char *base;
+  long step;
+  AKG_DEV KeysOf(const void *p, long b, long hkv, const Extents &e) {
+    step = C::HEADS_FIRST ? 2L * D : 2L * D * C::HKV;
+    base = static_cast<const char *>(p) + (C::HEADS_FIRST ? (b * C::HKV + hkv) * e.sk * step : b * e.sk * step + hkv * 2L * D);
+  }
+};
+
+// How many keys query i sees, given the lengths of its sequence (none behind the queries' length).
+template <typename C>
+AKG_DEV int keys_seen(long i, int ql, int kl) {
+  if (i >= ql) return 0;
+  if (!C::CAUSAL) return kl;
+  const int n = static_cast<int>(i) + kl - ql + 1;
+  return n < 0 ? 0 : (n < kl ? n : kl);
+}
+
+template <typename C>
+AKG_DEV int clamped_length(const int *lengths, long b, long most) {
+  if (lengths == nullptr) return static_cast<int>(most);
+  const long n = lengths[b];
+  return static_cast<int>(n < 0 ? 0 : (n < most ? n : most));
+}
+
+// ---- tiles in LDS -----------------------------------------------------------------------------------------------------
+// A tile of ROWS rows of D 16-bit channels on its way from memory to LDS through the registers of THREADS threads.
+template <int ROWS, int D, int THREADS>
+struct TileLoad {
+  static constexpr int kPerRow = D / 8;
+  static constexpr int kChunks = ROWS * kPerRow;
+  static constexpr int kEach = (kChunks + THREADS - 1) / THREADS;
+  static constexpr bool kWhole = kChunks % THREADS == 0;
+  u32x4 held[kEach];
+  // `offset(row)`: byte offset of the row from the descriptor's base, or kBeyondEveryBuffer (reads zeros).
+  template <typename F>
+  AKG_DEV void load(Buffer buf, int tid, F offset) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int c = tid + i * THREADS;
+      const u32 off = offset(c / kPerRow) + static_cast<u32>(c % kPerRow) * 16u;
+      held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, (kWhole || c < kChunks) ? off : kBeyondEveryBuffer, 0, 0));
+    }
+  }
+  AKG_DEV void store(u8 *tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int c = tid + i * THREADS;
+      const int row = c / kPerRow, chunk = c % kPerRow;
+      if (kWhole || c < kChunks) *reinterpret_cast<u32x4 *>(tile + row * pitch(D) + ((chunk ^ ((row >> 2) & 3)) << 4)) = held[i];
+    }
+  }
+};
+
+// 16 bytes of row `row0 + lane % 32`: channels 16 c + 8 (lane / 32) ... + 7, the operand of 16 contracted channels.
+template <int D>
+AKG_DEV u32x4 read_row(const u8 *tile, int row0, int c, int lane) {
+  const int row = row0 + (lane & 31);
+  const int chunk = 2 * c + (lane >> 5);
+  return *reinterpret_cast<const u32x4 *>(tile + row * pitch(D) + ((chunk ^ ((row >> 2) & 3)) << 4));
+}
+// Column 32 dt + lane % 32 of the rows row0 + 4 h .. 4 h + 3 and row0 + 8 + 4 h .. (h = lane / 32; row0 a multiple of 16).
+template <int D>
+AKG_DEV u32x4 read_transposed(const u8 *tile, int row0, int dt, int lane) {
+  const int i = lane & 15;
+  const int row = row0 + 4 * (lane >> 5) + (i >> 2);
+  const int chunk = 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+  const u8 *p0 = tile + row * pitch(D) + ((chunk ^ ((row >> 2) & 3)) << 4) + (i & 1) * 8;
+  const u8 *p1 = tile + (row + 8) * pitch(D) + ((chunk ^ (((row + 8) >> 2) & 3)) << 4) + (i & 1) * 8;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p0));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p1));
+  const u32x2 l = __builtin_bit_cast(u32x2, lo), u = __builtin_bit_cast(u32x2, hi);
+  return u32x4{l[0], l[1], u[0], u[1]};
+}
+
+// The channels behind D of a tile's rows (D to the next multiple of 32) hold zeros: written once, never again.
+template <int ROWS, int D, int THREADS>
+AKG_DEV void clear_padding(u8 *tile, int tid) {
+  if constexpr (D % 32 != 0) {
+    constexpr int kPad = (padded(D) - D) / 8;
+    for (int c = tid; c < ROWS * kPad; c += THREADS) {
+      const int row = c / kPad, chunk = D / 8 + c % kPad;
+      *reinterpret_cast<u32x4 *>(tile + row * pitch(D) + ((chunk ^ ((row >> 2) & 3)) << 4)) = u32x4{0, 0, 0, 0};
+    }
+  }
+}
+
+// The operand of a wavefront's own 32 rows, straight from memory (channels behind D: zeros).
+template <int D>
+AKG_DEV void load_own(const char *row, bool ok, int lane, u32x4 (&own)[(D + 15) / 16]) {
+#pragma unroll
+  for (int c = 0; c < (D + 15) / 16; ++c) {
+    const int at = 16 * c + 8 * (lane >> 5);
+    own[c] = (ok && (D % 16 == 0 || at < D)) ? *reinterpret_cast<const u32x4 *>(row + 2 * at) : u32x4{0, 0, 0, 0};
+  }
+}
+
+AKG_DEV u32 records(long bytes) { return static_cast<u32>(bytes < 0 ? 0 : (bytes < 0x7fffffffL ? bytes : 0x7fffffffL)); }
+
+// ---- masks ------------------------------------------------------------------------------------------------------------
+template <typename C>
+AKG_DEV long mask_row(long b, long h, long i, const Extents &e) {
+  long r = 0;
+  if (C::MASK_B) r = b;
+  if (C::MASK_H) r = r * C::H + h;
+  if (C::MASK_Q) r = r * e.sq + i;
+  return r * e.sk;
+}
+// The score with the mask at element `at` applied; `factor`: scale log2 e, or the scale where the mask is added.
+template <typename C>
+AKG_DEV float with_mask(float s, float factor, const void *mask, long at) {
+  if constexpr (C::MASK == 1) return static_cast<const u8 *>(mask)[at] ? s * factor : neg_inf();
+  if constexpr (C::MASK == 2) return __builtin_fmaf(s, factor, f16::load(static_cast<const f16::storage *>(mask)[at]));
+  if constexpr (C::MASK == 3) return __builtin_fmaf(s, factor, bf16::load(static_cast<const bf16::storage *>(mask)[at]));
+  if constexpr (C::MASK == 4) return __builtin_fmaf(s, factor, static_cast<const float *>(mask)[at]);
+  return s * factor;
+}
+// 2^x or e^x of a difference of scores, and a row's log of the sum from its maximum and its sum.
+template <typename C>
+AKG_DEV float power(float x) {
+  return __builtin_amdgcn_exp2f(C::ADDED ? x * kLog2e : x);
+}
+template <typename C>
+AKG_DEV float log_sum(float top, float sum) {
+  const float l = __builtin_amdgcn_logf(sum);
+  return sum == 0.0f ? neg_inf() : C::ADDED ? __builtin_fmaf(l, kLn2, top) : (top + l) * kLn2;
+}
+
+// ---- workgroup -> (key head, tile) ------------------------------------------------------------------------------------
+// Workgroups go round robin to the 8 XCDs. With a multiple of 8 key heads (over the batch) a head stays on one XCD, whose
+// L2 then holds its keys and values once; else heads follow one another. Tiles in the given order, heads inside.
+AKG_DEV void head_and_tile(long id, long heads, long &head, long &tile) {
+  if (heads % 8 == 0) {
+    const long each = heads / 8, y = id / 8;
+    head = id % 8 + 8 * (y % each);
+    tile = y / each;
+  } else {
+    head = id % heads;
+    tile = id / heads;
+  }
+}
+
+// ---- forward ----------------------------------------------------------------------------------------------------------
+// SPLIT: the workgroup takes one of `splits` ranges of the keys and leaves accumulators, maximum and sum in `ws`.
+template <typename C, int NW, bool SPLIT>
+AKG_DEV void forward(const void *q, const void *k, const void *v, const void *mask, const int *qlens, const int *klens,
+                     void *out, float *lse, float *ws, Extents e, float scale, int splits) {
+  typedef typename C::T T;
+  constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, TV = padded(DV) / 32, kThreads = 64 * NW;
+  __shared__ __attribute__((aligned(16))) u8 lds[2][kTile * (pitch(DK) + pitch(DV))];
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const long rows = e.sq * C::G, tiles = (rows + kRows * NW - 1) / (kRows * NW), heads = e.batch * C::HKV;
+  long id = blockIdx.x;
+  const int split = SPLIT ? static_cast<int>(id % splits) : 0;
+  if (SPLIT) id /= splits;
+  long head, tile;
+  head_and_tile(id, heads, head, tile);
+  tile = tiles - 1 - tile;   // the rows that see most keys first
+  const long b = head / C::HKV, hkv = head % C::HKV;
+  const int ql = clamped_length<C>(qlens, b, e.sq), kl = clamped_length<C>(klens, b, e.sk);
+
+  const long row0 = tile * (kRows * NW), row = row0 + wave * kRows + (lane & 31);
+  const long i = row / C::G, g = row % C::G;
+  const bool exists = row < rows;
+  const int seen = exists ? keys_seen<C>(i, ql, kl) : 0;
+  // keys of the workgroup: those of its last row that has any
+  long last = (row0 + kRows * NW < rows ? row0 + kRows * NW : rows) - 1;
+  long lastI = last / C::G;
+  if (lastI >= ql) lastI = ql - 1;
+  const int most = row0 / C::G < ql ? keys_seen<C>(lastI, ql, kl) : 0;
+  int first = 0, end = most;
+  if (SPLIT) {
+    const int all = (most + kTile - 1) / kTile, each = (all + splits - 1) / splits;
+    first = split * each * kTile < most ? split * each * kTile : most;
+    end = first + each * kTile < most ? first + each * kTile : most;
+  }
+
+  const RowsOf<C, DK> qrows(q, b, hkv, e);
+  u32x4 own[CK];
+  load_own<DK>(qrows.base + qrows.offset(exists ? row : 0), seen > 0, lane, own);
+  const float c = C::ADDED ? scale : scale * kLog2e;
+
+  f32x16 acc[TV];
+#pragma unroll
+  for (int d = 0; d < TV; ++d) acc[d] = {};
+  float top = neg_inf(), sum = 0.0f;   // the row's maximum; the sum over this lane's keys
+
+  const KeysOf<C, DK> keys(k, b, hkv, e);
+  const KeysOf<C, DV> values(v, b, hkv, e);
+  TileLoad<kTile, DK, kThreads> kload;
+  TileLoad<kTile, DV, kThreads> vload;
+  auto fetch = [&](int k0) {
+    const Buffer kb = make_buffer(keys.base + k0 * keys.step, records((kl - k0 - 1) * keys.step + 2 * DK));
+    const Buffer vb = make_buffer(values.base + k0 * values.step, records((kl - k0 - 1) * values.step + 2 * DV));
+    // (rows behind the keys' length lie behind the descriptor and read zeros)
+    kload.load(kb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(keys.step)); });
+    vload.load(vb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(values.step)); });
+  };
+  auto put = [&](int buf) {
+    kload.store(lds[buf], tid);
+    vload.store(lds[buf] + kTile * pitch(DK), tid);
+  };
+#pragma unroll
+  for (int buf = 0; buf < 2; ++buf) {
+    clear_padding<kTile, DK, kThreads>(lds[buf], tid);
+    clear_padding<kTile, DV, kThreads>(lds[buf] + kTile * pitch(DK), tid);
+  }
+  if (first < end) {
+    fetch(first);
+    put(0);
+  }
+  __syncthreads();
+
+  const long maskAt = C::MASK != 0 ? mask_row<C>(b, hkv * C::G + g, exists ? i : 0, e) : 0;
+  int buf = 0;
+  for (int k0 = first; k0 < end; k0 += kTile, buf ^= 1) {
+    const bool more = k0 + kTile < end;
+    if (more) fetch(k0 + kTile);
+    const u8 *kt = lds[buf], *vt = lds[buf] + kTile * pitch(DK);
+    if (__any(k0 < seen)) {   // (wavefronts whose rows see nothing of the tile only help to fetch the next one)
+      f32x16 s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s[t] = {};
+#pragma unroll
+        for (int x = 0; x < CK; ++x) s[t] = T::mma(read_row<DK>(kt, 32 * t, x, lane), own[x], s[t]);
+      }
+      const bool ragged = __any(k0 + kTile > seen);
+      if (C::MASK != 0 || ragged) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = k0 + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
+            if (C::MASK != 0) {
+              s[t][r] = j < seen ? with_mask<C>(s[t][r], c, mask, maskAt + j) : neg_inf();
+            } else {
+              s[t][r] = j < seen ? s[t][r] : neg_inf();
+            }
+          }
+        }
+      }
+      float m = top;
+      {
+        float peak = s[0][0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) peak = __builtin_fmaxf(peak, s[t][r]);
+        }
+        if (C::MASK == 0) peak *= c;
+        m = __builtin_fmaxf(m, max_halves(peak));
+      }
+      const float base = m == neg_inf() ? 0.0f : m;
+      const float shrink = power<C>(top - base);
+      top = m;
+      sum *= shrink;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[t][r] = power<C>(C::MASK == 0 ? __builtin_fmaf(s[t][r], c, -base) : s[t][r] - base);
+          sum += s[t][r];
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < TV; ++d) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] *= shrink;
+      }
+      // probabilities are rounded to the type of the values for the matrix units (half a step of at most 2^-9 each, of
+      // changing sign; the sum above has them unrounded)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        u32x4 p;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) p[w] = T::pack(s[x >> 1][8 * (x & 1) + 2 * w], s[x >> 1][8 * (x & 1) + 2 * w + 1]);
+#pragma unroll
+        for (int d = 0; d < TV; ++d) acc[d] = T::mma(read_transposed<DV>(vt, 16 * x, d, lane), p, acc[d]);
+      }
+    }
+    if (more) put(buf ^ 1);
+    __syncthreads();
+  }
+
+  sum = add_halves(sum);
+  if (!exists) return;
+  if (SPLIT) {
+    const long slot = (static_cast<long>(split) * heads + head) * rows + row;
+    float *to = ws + slot * padded(DV);
+    if (sum > 0.0f || sum != sum) {
+#pragma unroll
+      for (int d = 0; d < TV; ++d) {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          *reinterpret_cast<f32x4 *>(to + 32 * d + 8 * r4 + 4 * half) =
+            f32x4{acc[d][4 * r4], acc[d][4 * r4 + 1], acc[d][4 * r4 + 2], acc[d][4 * r4 + 3]};
+        }
+      }
+    }
+    if (half == 0) {
+      float *state = ws + static_cast<long>(splits) * heads * rows * padded(DV) + 2 * slot;
+      state[0] = top;
+      state[1] = sum;
+    }
+    return;
+  }
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const RowsOf<C, DV> orows(out, b, hkv, e);
+  char *to = const_cast<char *>(orows.base) + orows.offset(row);
+#pragma unroll
+  for (int d = 0; d < TV; ++d) {
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const int at = 32 * d + 8 * r4 + 4 * half;
+      if (DV % 32 != 0 && at >= DV) continue;
+      u32x2 w;
+      w[0] = T::pack(acc[d][4 * r4] * inverse, acc[d][4 * r4 + 1] * inverse);
+      w[1] = T::pack(acc[d][4 * r4 + 2] * inverse, acc[d][4 * r4 + 3] * inverse);
+      *reinterpret_cast<u32x2 *>(to + 2 * at) = w;
+    }
+  }
+  if (lse != nullptr && half == 0) {
+    lse[(b * C::H + hkv * C::G + g) * e.sq + i] = log_sum<C>(top, sum);
+  }
+}
+
+// The ranges of a split joined: a thread takes four channels of a row.
+template <typename C>
+AKG_DEV void join(const float *ws, void *out, float *lse, Extents e, int splits) {
+  typedef typename C::T T;
+  constexpr int DV = C::DV, kPer = DV / 4;
+  const long rows = e.sq * C::G, heads = e.batch * C::HKV;
+  const long at = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (at >= heads * rows * kPer) return;
+  const long slot = at / kPer, head = slot / rows, row = slot % rows, stride = heads * rows;
+  const int d = static_cast<int>(at % kPer) * 4;
+  const float *state = ws + static_cast<long>(splits) * stride * padded(DV) + 2 * slot;
+  float top = neg_inf();
+  for (int s = 0; s < splits; ++s) top = __builtin_fmaxf(top, state[2 * s * stride]);
+  const float base = top == neg_inf() ? 0.0f : top;
+  float sum = 0.0f;
+  f32x4 acc = {};
+  for (int s = 0; s < splits; ++s) {
+    const float own = state[2 * s * stride + 1];
+    if (own == 0.0f) continue;   // (a range without keys wrote no accumulators)
+    const float w = power<C>(state[2 * s * stride] - base);
+    sum = __builtin_fmaf(own, w, sum);
+    const f32x4 x = *reinterpret_cast<const f32x4 *>(ws + (s * stride + slot) * padded(DV) + d);
+#pragma unroll
+    for (int z = 0; z < 4; ++z) acc[z] = __builtin_fmaf(x[z], w, acc[z]);
+  }
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const long b = head / C::HKV, hkv = head % C::HKV;
+  const RowsOf<C, DV> orows(out, b, hkv, e);
+  u32x2 w;
+  w[0] = T::pack(acc[0] * inverse, acc[1] * inverse);
+  w[1] = T::pack(acc[2] * inverse, acc[3] * inverse);
+  *reinterpret_cast<u32x2 *>(const_cast<char *>(orows.base) + orows.offset(row) + 2 * d) = w;
+  if (lse != nullptr && d == 0) {
+    lse[(b * C::H + hkv * C::G + row % C::G) * e.sq + row / C::G] = log_sum<C>(top, sum);
+  }
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------------
+// float16 holds nothing below 2^-24, and a score's gradient is a probability times a difference: where the largest
+// |dout| of the rows concerned is below 1 the gradients of the scores are computed times the power of two that lifts it
+// there, and the result is scaled back in float32. (bfloat16 has the exponents of float32: factor 1.)
+template <typename T>
+AKG_DEV float lift_of(float largest) {
+  if (!T::kNarrowRange || !(largest < 1.0f) || largest == 0.0f) return 1.0f;
+  const int up = -__builtin_amdgcn_frexp_expf(largest);   // largest = m 2^-up, 1/2 <= m < 1
+  return __builtin_ldexpf(1.0f, up < 100 ? up : 100);
+}
+
+// What the backward kernels know of a row's sum: exp(score - lse) = 2^((score - top) log2 e - rest), rest = 0 where lse says
+// it. Where a mask is added and lse is large (rows whose mask is -1e9 throughout), a float32 lse has lost the log of the
+// sum behind the maximum: the kernel of dq then finds both again.
+constexpr float kLargeLse = 4096.0f;
+
+// Places in the workspace of the backward kernels, in floats: delta of every row, for an added mask top and rest of every
+// row, and the largest |dout| of every workgroup of the first kernel.
+template <typename C>
+struct BackwardSpace {
+  long rows;   // of all key heads
+  AKG_DEV long top(long row) const { return rows + row; }
+  AKG_DEV long rest(long row) const { return 2 * rows + row; }
+  AKG_DEV long largest() const { return C::ADDED ? 3 * rows : rows; }
+};
+
+// dq of 32 rows a wavefront: keys and values pass by in tiles. Leaves in `ws` what the kernel of dk and dv needs.
+template <typename C, int NW>
+AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
+                              const void *mask, const int *qlens, const int *klens, void *dq, float *ws, Extents e, float scale) {
+  typedef typename C::T T;
+  constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, CV = (DV + 15) / 16, TK = padded(DK) / 32, kThreads = 64 * NW;
+  __shared__ __attribute__((aligned(16))) u8 lds[2][kTile * (pitch(DK) + pitch(DV))];
+  __shared__ float largestOf[NW];
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const long rows = e.sq * C::G, tiles = (rows + kRows * NW - 1) / (kRows * NW), heads = e.batch * C::HKV;
+  long head, tile;
+  head_and_tile(blockIdx.x, heads, head, tile);
+  tile = tiles - 1 - tile;
+  const long b = head / C::HKV, hkv = head % C::HKV;
+  const int ql = clamped_length<C>(qlens, b, e.sq), kl = clamped_length<C>(klens, b, e.sk);
+  const long row0 = tile * (kRows * NW), row = row0 + wave * kRows + (lane & 31);
+  const long i = row / C::G, g = row % C::G;
+  const bool exists = row < rows;
+  const int seen = exists ? keys_seen<C>(i, ql, kl) : 0;
+  long last = (row0 + kRows * NW < rows ? row0 + kRows * NW : rows) - 1;
+  long lastI = last / C::G;
+  if (lastI >= ql) lastI = ql - 1;
+  const int end = row0 / C::G < ql ? keys_seen<C>(lastI, ql, kl) : 0;
+
+  const RowsOf<C, DK> qrows(q, b, hkv, e);
+  const RowsOf<C, DV> grows(dout, b, hkv, e), orows(out, b, hkv, e);
+  u32x4 own[CK], grad[CV];
+  load_own<DK>(qrows.base + qrows.offset(exists ? row : 0), seen > 0, lane, own);
+  load_own<DV>(grows.base + grows.offset(exists ? row : 0), seen > 0, lane, grad);
+  float delta = 0.0f, largest = 0.0f;
+  {
+    u32x4 o[CV];
+    load_own<DV>(orows.base + orows.offset(exists ? row : 0), seen > 0, lane, o);
+#pragma unroll
+    for (int x = 0; x < CV; ++x) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        delta = __builtin_fmaf(T::low(o[x][w]), T::low(grad[x][w]), delta);
+        delta = __builtin_fmaf(T::high(o[x][w]), T::high(grad[x][w]), delta);
+        if (T::kNarrowRange) {
+          largest = __builtin_fmaxf(largest, __builtin_fabsf(T::low(grad[x][w])));
+          largest = __builtin_fmaxf(largest, __builtin_fabsf(T::high(grad[x][w])));
+        }
+      }
+    }
+    delta = add_halves(delta);
+  }
+  const BackwardSpace<C> space{heads * rows};
+  if (exists && half == 0) ws[head * rows + row] = delta;
+  float lift = 1.0f;
+  if (T::kNarrowRange) {
+    largest = max_halves(largest);
+    lift = lift_of<T>(largest);
+#pragma unroll
+    for (int step = 1; step < 32; step *= 2) largest = __builtin_fmaxf(largest, __shfl_xor(largest, step));
+    if (lane == 0) largestOf[wave] = largest;
+  }
+  float sums = exists && seen > 0 ? lse[(b * C::H + hkv * C::G + g) * e.sq + i] : neg_inf();
+  // (a row without keys: exp2(s - inf) = 0)
+  const bool lost = C::ADDED && __builtin_fabsf(sums) > kLargeLse && __builtin_fabsf(sums) < __builtin_inff();
+  sums = sums == neg_inf() ? __builtin_inff() : C::ADDED ? sums : sums * kLog2e;
+  float rest = 0.0f;
+  const float c = C::ADDED ? scale : scale * kLog2e;
+
+  f32x16 acc[TK];
+#pragma unroll
+  for (int d = 0; d < TK; ++d) acc[d] = {};
+  const KeysOf<C, DK> keys(k, b, hkv, e);
+  const KeysOf<C, DV> values(v, b, hkv, e);
+  TileLoad<kTile, DK, kThreads> kload;
+  TileLoad<kTile, DV, kThreads> vload;
+  auto fetch = [&](int k0) {
+    const Buffer kb = make_buffer(keys.base + k0 * keys.step, records((kl - k0 - 1) * keys.step + 2 * DK));
+    const Buffer vb = make_buffer(values.base + k0 * values.step, records((kl - k0 - 1) * values.step + 2 * DV));
+    kload.load(kb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(keys.step)); });
+    vload.load(vb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(values.step)); });
+  };
+  auto put = [&](int buf) {
+    kload.store(lds[buf], tid);
+    vload.store(lds[buf] + kTile * pitch(DK), tid);
+  };
+#pragma unroll
+  for (int buf = 0; buf < 2; ++buf) {
+    clear_padding<kTile, DK, kThreads>(lds[buf], tid);
+    clear_padding<kTile, DV, kThreads>(lds[buf] + kTile * pitch(DK), tid);
+  }
+  if (end > 0) {
+    fetch(0);
+    put(0);
+  }
+  __syncthreads();
+  if (T::kNarrowRange && tid == 0) {
+    float all = 0.0f;
+    for (int w = 0; w < NW; ++w) all = __builtin_fmaxf(all, largestOf[w]);
+    ws[space.largest() + head * tiles + tile] = all;
+  }
+  const long maskAt = C::MASK != 0 ? mask_row<C>(b, hkv * C::G + g, exists ? i : 0, e) : 0;
+  if constexpr (C::ADDED) {
+    if (__any(lost)) {   // (by this wavefront alone, keys straight from memory: such rows are rare)
+      float top = neg_inf(), sum = 0.0f;
+      for (int k0 = 0; __any(k0 < seen); k0 += 32) {
+        f32x16 s = {};
+        const int key = k0 + (lane & 31);
+        u32x4 operand[CK];
+        load_own<DK>(keys.base + (key < kl ? key : 0) * keys.step, key < kl, lane, operand);
+#pragma unroll
+        for (int x = 0; x < CK; ++x) s = T::mma(operand[x], own[x], s);
+        float peak = neg_inf();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = k0 + 8 * (r >> 2) + 4 * half + (r & 3);
+          s[r] = j < seen ? with_mask<C>(s[r], c, mask, maskAt + j) : neg_inf();
+          peak = __builtin_fmaxf(peak, s[r]);
+        }
+        const float m = __builtin_fmaxf(top, max_halves(peak)), base = m == neg_inf() ? 0.0f : m;
+        sum *= power<C>(top - base);
+        top = m;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += power<C>(s[r] - base);
+      }
+      sum = add_halves(sum);
+      if (lost && sum > 0.0f) {
+        sums = top;
+        rest = __builtin_amdgcn_logf(sum);
+      }
+    }
+    if (exists && half == 0) {
+      ws[space.top(head * rows + row)] = sums;
+      ws[space.rest(head * rows + row)] = rest;
+    }
+  }
+  int buf = 0;
+  for (int k0 = 0; k0 < end; k0 += kTile, buf ^= 1) {
+    const bool more = k0 + kTile < end;
+    if (more) fetch(k0 + kTile);
+    const u8 *kt = lds[buf], *vt = lds[buf] + kTile * pitch(DK);
+    if (__any(k0 < seen)) {
+      const bool ragged = __any(k0 + kTile > seen);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int x = 0; x < CK; ++x) s = T::mma(read_row<DK>(kt, 32 * t, x, lane), own[x], s);
+#pragma unroll
+        for (int x = 0; x < CV; ++x) dp = T::mma(read_row<DV>(vt, 32 * t, x, lane), grad[x], dp);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = k0 + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
+          float x = s[r];
+          if (C::MASK != 0) {
+            x = j < seen ? with_mask<C>(x, c, mask, maskAt + j) - sums : neg_inf();
+            if (C::ADDED) x = __builtin_fmaf(x, kLog2e, -rest);
+          } else {
+            x = __builtin_fmaf(x, c, -sums);
+            if (ragged) x = j < seen ? x : neg_inf();
+          }
+          s[r] = __builtin_amdgcn_exp2f(x) * ((dp[r] - delta) * lift);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          u32x4 p;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) p[w] = T::pack(s[8 * x + 2 * w], s[8 * x + 2 * w + 1]);
+#pragma unroll
+          for (int d = 0; d < TK; ++d) acc[d] = T::mma(read_transposed<DK>(kt, 32 * t + 16 * x, d, lane), p, acc[d]);
+        }
+      }
+    }
+    if (more) put(buf ^ 1);
+    __syncthreads();
+  }
+  if (!exists || dq == nullptr) return;
+  const float back = scale / lift;
+  const RowsOf<C, DK> drows(dq, b, hkv, e);
+  char *to = const_cast<char *>(drows.base) + drows.offset(row);
+#pragma unroll
+  for (int d = 0; d < TK; ++d) {
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const int at = 32 * d + 8 * r4 + 4 * half;
+      if (DK % 32 != 0 && at >= DK) continue;
+      u32x2 w;
+      w[0] = T::pack(acc[d][4 * r4] * back, acc[d][4 * r4 + 1] * back);
+      w[1] = T::pack(acc[d][4 * r4 + 2] * back, acc[d][4 * r4 + 3] * back);
+      *reinterpret_cast<u32x2 *>(to + 2 * at) = w;
+    }
+  }
+}
+
+// dk and dv of 32 keys a wavefront: the queries of all heads that share them pass by in tiles.
+template <typename C, int NW, int NWQ>
+AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const void *v, const float *lse, const void *mask,
+                           const int *qlens, const int *klens, void *dk, void *dv, const float *ws, Extents e, float scale) {
+  typedef typename C::T T;
+  constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, CV = (DV + 15) / 16, TK = padded(DK) / 32, TV = padded(DV) / 32, kThreads = 64 * NW;
+  __shared__ __attribute__((aligned(16))) u8 lds[2][kTileRows * (pitch(DK) + pitch(DV))];
+  __shared__ __attribute__((aligned(16))) float sumsOf[2][kTileRows], deltaOf[2][kTileRows], restOf[C::ADDED ? 2 : 1][kTileRows];
+  __shared__ __attribute__((aligned(16))) int seenOf[2][kTileRows];
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const long rows = e.sq * C::G, heads = e.batch * C::HKV;
+  long head, tile;
+  head_and_tile(blockIdx.x, heads, head, tile);
+  const long b = head / C::HKV, hkv = head % C::HKV;
+  const int ql = clamped_length<C>(qlens, b, e.sq), kl = clamped_length<C>(klens, b, e.sk);
+  const int key0 = static_cast<int>(tile) * (kRows * NW) + wave * kRows;
+  const int key = key0 + (lane & 31);
+  const bool counts = key < kl;
+  const KeysOf<C, DK> keys(k, b, hkv, e);
+  const KeysOf<C, DV> values(v, b, hkv, e);
+  const BackwardSpace<C> space{heads * rows};
+  u32x4 own[CK], val[CV];
+  load_own<DK>(keys.base + (counts ? key : 0) * keys.step, counts, lane, own);
+  load_own<DV>(values.base + (counts ? key : 0) * values.step, counts, lane, val);
+  float lift = 1.0f;
+  if (T::kNarrowRange) {
+    const long tilesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ);
+    float largest = 0.0f;
+    for (long t = lane; t < tilesQ; t += 64) largest = __builtin_fmaxf(largest, ws[space.largest() + head * tilesQ + t]);
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) largest = __builtin_fmaxf(largest, __shfl_xor(largest, step));
+    lift = lift_of<T>(largest);
+  }
+  const float c = C::ADDED ? scale : scale * kLog2e;
+  f32x16 acck[TK], accv[TV];
+#pragma unroll
+  for (int d = 0; d < TK; ++d) acck[d] = {};
+#pragma unroll
+  for (int d = 0; d < TV; ++d) accv[d] = {};
+
+  // queries that see the first key of the workgroup, up to the last one of the sequence
+  const int first0 = static_cast<int>(tile) * (kRows * NW);
+  long from = 0;
+  if (C::CAUSAL) {
+    const long i = static_cast<long>(first0) - (kl - ql);
+    from = (i > 0 ? i : 0) * C::G / kTileRows * kTileRows;
+  }
+  const long upto = first0 < kl ? static_cast<long>(ql) * C::G : 0;
+
+  const RowsOf<C, DK> qrows(q, b, hkv, e);
+  const RowsOf<C, DV> grows(dout, b, hkv, e);
+  TileLoad<kTileRows, DK, kThreads> qload;
+  TileLoad<kTileRows, DV, kThreads> gload;
+  float sums = 0.0f, delta = 0.0f, rest = 0.0f;
+  int seen = 0;
+  auto fetch = [&](long r0) {
+    const long i0 = r0 / C::G;
+    const Buffer qb = make_buffer(qrows.base + i0 * qrows.stepI, 0x7fffffffL);
+    const Buffer gb = make_buffer(grows.base + i0 * grows.stepI, 0x7fffffffL);
+    auto offsetIn = [&](const auto &of, int r) {
+      const long at = r0 + r;
+      return at < upto ? static_cast<u32>((at / C::G - i0) * of.stepI + at % C::G * of.stepG) : kBeyondEveryBuffer;
+    };
+    qload.load(qb, tid, [&](int r) { return offsetIn(qrows, r); });
+    gload.load(gb, tid, [&](int r) { return offsetIn(grows, r); });
+    if (tid < kTileRows) {
+      const long at = r0 + tid;
+      const bool ok = at < upto;
+      const long i = ok ? at / C::G : 0, g = ok ? at % C::G : 0;
+      if (C::ADDED) {
+        sums = ok ? ws[space.top(head * rows + at)] : __builtin_inff();
+        rest = ok ? ws[space.rest(head * rows + at)] : 0.0f;
+      } else {
+        sums = ok ? lse[(b * C::H + hkv * C::G + g) * e.sq + i] : neg_inf();
+        sums = sums == neg_inf() ? __builtin_inff() : sums * kLog2e;
+      }
+      delta = ok ? ws[head * rows + at] : 0.0f;
+      seen = ok ? keys_seen<C>(i, ql, kl) : 0;
+    }
+  };
+  auto put = [&](int buf) {
+    qload.store(lds[buf], tid);
+    gload.store(lds[buf] + kTileRows * pitch(DK), tid);
+    if (tid < kTileRows) {
+      sumsOf[buf][tid] = sums;
+      if (C::ADDED) restOf[buf][tid] = rest;
+      deltaOf[buf][tid] = delta;
+      seenOf[buf][tid] = seen;
+    }
+  };
+#pragma unroll
+  for (int buf = 0; buf < 2; ++buf) {
+    clear_padding<kTileRows, DK, kThreads>(lds[buf], tid);
+    clear_padding<kTileRows, DV, kThreads>(lds[buf] + kTileRows * pitch(DK), tid);
+  }
+  if (from < upto) {
+    fetch(from);
+    put(0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (long r0 = from; r0 < upto; r0 += kTileRows, buf ^= 1) {
+    const bool more = r0 + kTileRows < upto;
+    if (more) fetch(r0 + kTileRows);
+    const u8 *qt = lds[buf], *gt = lds[buf] + kTileRows * pitch(DK);
+    // the tile's last row sees most keys, its first one least
+    const long lastRow = (r0 + kTileRows < upto ? r0 + kTileRows : upto) - 1;
+    if (key0 < keys_seen<C>(lastRow / C::G, ql, kl)) {
+      const bool ragged = key0 + kRows > keys_seen<C>(r0 / C::G, ql, kl);
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int x = 0; x < CK; ++x) s = T::mma(read_row<DK>(qt, 0, x, lane), own[x], s);
+#pragma unroll
+      for (int x = 0; x < CV; ++x) dp = T::mma(read_row<DV>(gt, 0, x, lane), val[x], dp);
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&sumsOf[buf][8 * r4 + 4 * half]);
+        const f32x4 d4 = *reinterpret_cast<const f32x4 *>(&deltaOf[buf][8 * r4 + 4 * half]);
+        const i32x4 n4 = *reinterpret_cast<const i32x4 *>(&seenOf[buf][8 * r4 + 4 * half]);
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const int r = 4 * r4 + z;
+          float x = s[r];
+          if (C::MASK != 0) {
+            const long at = r0 + 8 * r4 + 4 * half + z;
+            x = key < n4[z] ? with_mask<C>(x, c, mask, mask_row<C>(b, hkv * C::G + at % C::G, at / C::G, e) + key) - l4[z] : neg_inf();
+            if (C::ADDED) x = __builtin_fmaf(x, kLog2e, -restOf[buf][8 * r4 + 4 * half + z]);
+          } else {
+            x = __builtin_fmaf(x, c, -l4[z]);
+            if (ragged) x = key < n4[z] ? x : neg_inf();
+          }
+          const float p = __builtin_amdgcn_exp2f(x);
+          s[r] = p;
+          dp[r] = p * ((dp[r] - d4[z]) * lift);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        u32x4 p, ds;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          p[w] = T::pack(s[8 * x + 2 * w], s[8 * x + 2 * w + 1]);
+          ds[w] = T::pack(dp[8 * x + 2 * w], dp[8 * x + 2 * w + 1]);
+        }
+#pragma unroll
+        for (int d = 0; d < TV; ++d) accv[d] = T::mma(read_transposed<DV>(gt, 16 * x, d, lane), p, accv[d]);
+#pragma unroll
+        for (int d = 0; d < TK; ++d) acck[d] = T::mma(read_transposed<DK>(qt, 16 * x, d, lane), ds, acck[d]);
+      }
+    }
+    if (more) put(buf ^ 1);
+    __syncthreads();
+  }
+  if (key >= e.sk) return;
+  const float back = scale / lift;
+  auto store = [&](char *to, int dim, const f32x16 *acc, int tilesD, float factor) {
+#pragma unroll
+    for (int d = 0; d < tilesD; ++d) {
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int at = 32 * d + 8 * r4 + 4 * half;
+        if (dim % 32 != 0 && at >= dim) continue;
+        u32x2 w;
+        w[0] = T::pack(acc[d][4 * r4] * factor, acc[d][4 * r4 + 1] * factor);
+        w[1] = T::pack(acc[d][4 * r4 + 2] * factor, acc[d][4 * r4 + 3] * factor);
+        *reinterpret_cast<u32x2 *>(to + 2 * at) = w;
+      }
+    }
+  };
+  const KeysOf<C, DK> dkeys(dk, b, hkv, e);
+  const KeysOf<C, DV> dvalues(dv, b, hkv, e);
+  if (dk != nullptr) store(const_cast<char *>(dkeys.base) + key * dkeys.step, DK, acck, TK, back);
+  if (dv != nullptr) store(const_cast<char *>(dvalues.base) + key * dvalues.step, DV, accv, TV, 1.0f);
+}
+
+}  // namespace attn
+}  // namespace akg

@@ -4,7 +4,7 @@ The document layout is the one the reference's translator reads
 (akg-mlir/lib/Target/MindsporeDialect/TranslateToMindsporeDialect.cpp:55-75,295-415): top-level `op`, `process`,
 `input_desc` (a list of single-element lists), `op_desc` (each with `name`, `attr`, `input_desc`, `output_desc`)
 and `output_desc`. Scalar constants are op inputs of shape [1] that carry a numeric `value` (:650-658).
-Only op names of the reference's op table (:417-486) are emitted.
+Only op names of the reference's op table (:417-486) are emitted, and this backend's own operators of an attention layer.
 """
 import json
 import re
@@ -569,6 +569,73 @@ def attention_probabilities(batch, m, k, n, dtype="bfloat16", name=None):
     e = b.unary("Exp", b.sub(s, b.reduce("ReduceMax", s, [2], True)))
     p = b.div(e, b.reduce("ReduceSum", e, [2], True))
     return b.dumps([b.cast(p, dtype)])
+
+
+def _layer(b, name, inputs, outs, attrs):
+    """One op entry with several results: `outs` is a list of (shape, dtype), `attrs` of (name, value)."""
+    kinds = {bool: "bool", float: "float", int: "int", str: "str"}
+    results = []
+    for shape, dtype in outs:
+        results.append(Tensor("output_0_%d" % b._n_out, shape, dtype))
+        b._n_out += 1
+    b.ops.append({
+        "attr": [{"data_type": kinds[type(v)], "name": n, "value": v} for n, v in attrs],
+        "impl_path": "", "input_desc": [[t.desc()] for t in inputs], "name": name,
+        "output_desc": [t.desc(with_value=False) for t in results]})
+    return results
+
+
+def rotary_embedding(b, xs, positions, layout="BSND", base=10000.0, rotary_dims=0, interleaved=False, inverse=False, scaling=None,
+                     magnitude=1.0):
+    """Rotary positions of one or two tensors of heads ([batch, sequence, heads, channels], or "BNSD"; they may differ in
+    their heads only), `positions` int32 / int64 [sequence] or [batch, sequence]. The first `rotary_dims` channels (0: all)
+    are turned in pairs - channel i with i + rotary_dims / 2, or adjacent ones where `interleaved` - by position *
+    base^(-2 i / rotary_dims); `inverse` turns back (the gradient). `scaling`: None, {"kind": "linear", "factor"} or {"kind":
+    "wavelength", "factor", "original_length", "low", "high"} (rates that turn fewer than `low` times over the original
+    length are divided by the factor, those that turn more than `high` times are not, the ones between in part). `magnitude`
+    multiplies the result of the turned channels. Returns one result per tensor."""
+    attrs = [("layout", layout), ("base", float(base)), ("rotary_dims", int(rotary_dims)), ("interleaved", bool(interleaved)),
+             ("inverse", bool(inverse)), ("magnitude", float(magnitude)), ("scaling", scaling["kind"] if scaling else "none")]
+    for key in ("factor", "original_length", "low", "high"):
+        if scaling and key in scaling:
+            attrs.append((key, float(scaling[key])))
+    return _layer(b, "RotaryEmbedding", list(xs) + [positions], [(x.shape, x.dtype) for x in xs], attrs)
+
+
+def _attention_attrs(layout, causal, scale, mask, query_lengths, key_lengths):
+    attrs = [("layout", layout), ("causal", bool(causal)), ("has_mask", mask is not None),
+             ("has_query_lengths", query_lengths is not None), ("has_key_lengths", key_lengths is not None)]
+    if scale is not None:
+        attrs.append(("scale", float(scale)))
+    return attrs, [t for t in (mask, query_lengths, key_lengths) if t is not None]
+
+
+def attention(b, q, k, v, mask=None, query_lengths=None, key_lengths=None, layout="BSND", causal=False, scale=None, lse=True):
+    """softmax(scale q k^T + mask) v without the probabilities in memory; heads of q may share those of k and v. `mask` is
+    bool (true: the pair counts) or float (added), [batch | 1, heads | 1, queries | 1, keys]; `query_lengths`, `key_lengths`
+    int32 [batch]; `causal`: query i of a sequence sees the keys up to i + (keys - queries) of that sequence. A query that
+    sees nothing, and queries behind their length, give zeros. Returns [out, lse] (lse float32 [batch, heads, queries], the
+    log of the sum of exponentials, -inf where a query sees nothing) or [out]."""
+    attrs, more = _attention_attrs(layout, causal, scale, mask, query_lengths, key_lengths)
+    heads, seq = (q.shape[1], q.shape[2]) if layout == "BNSD" else (q.shape[2], q.shape[1])
+    outs = [(q.shape[:3] + v.shape[3:], q.dtype)] + ([([q.shape[0], heads, seq], "float32")] if lse else [])
+    return _layer(b, "Attention", [q, k, v] + more, outs, attrs)
+
+
+def attention_grad(b, dout, q, k, v, out, lse, mask=None, query_lengths=None, key_lengths=None, layout="BSND", causal=False, scale=None):
+    """Gradients [dq, dk, dv] of `attention` from the gradient of its first result and what it returned; the probabilities are
+    computed again. The mask gets none."""
+    attrs, more = _attention_attrs(layout, causal, scale, mask, query_lengths, key_lengths)
+    return _layer(b, "AttentionGrad", [dout, q, k, v, out, lse] + more, [(t.shape, t.dtype) for t in (q, k, v)], attrs)
+
+
+def cache_attention(b, q, key_cache, value_cache, key_scale, value_scale, block_table, lengths, scale=None):
+    """Attention of the last queries of every sequence, q [batch, queries, heads, channels], over a cache in 8 bits: blocks
+    int8 [blocks, key heads, tokens of a block, channels] with float32 scales [blocks, key heads], `block_table` int32
+    [batch, blocks of a sequence], `lengths` int32 [batch] (tokens of a sequence, the queries' own among them: query i sees
+    the first length - queries + 1 + i). Entries of the table outside the pool hold no tokens. Returns the result."""
+    attrs = [] if scale is None else [("scale", float(scale))]
+    return _layer(b, "CacheAttention", [q, key_cache, value_cache, key_scale, value_scale, block_table, lengths], [(q.shape, q.dtype)], attrs)[0]
 
 
 def sgd_clip_by_global_norm(rows, cols, dtype="float32", lr=0.01, clip=1.0, name=None):
