@@ -87,8 +87,9 @@ class LayerEmitter {
     return "// Generated by the akg HIP lowering for gfx950. Op description: " + g_.name + "\n// family: attention, op: " + op_.name +
            "\n#include \"akg_rt.hpp\"\n" + header + "\n";
   }
-  static std::string kernel(const std::string &name, int threads, const std::string &args, const std::string &body) {
-    return "extern \"C\" __global__ __launch_bounds__(" + std::to_string(threads) + ") void " + name + "(" + args + ") {\n" + body + "}\n\n";
+  // `wavesPerSimd`: how many the registers have to leave room for (0: the compiler's choice).
+  static std::string kernel(const std::string &name, int threads, const std::string &args, const std::string &body, int wavesPerSimd = 0) {
+    return "extern \"C\" __global__ __launch_bounds__(" + std::to_string(threads) + (wavesPerSimd ? ", " + std::to_string(wavesPerSimd) : "") + ") void " + name + "(" + args + ") {\n" + body + "}\n\n";
   }
   const char *trait() const { return in(0).dtype == DType::BF16 ? "akg::attn::BF16" : "akg::attn::F16"; }
 
@@ -289,18 +290,18 @@ class LayerEmitter {
     queries << "  akg::attn::backward_queries<akg_C, " << nwq << ">(" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << inName(3) << ", "
             << inName(4) << ", " << inName(5) << ", " << optionals(6) << ", " << outName(0) << ", akg_ws, " << extents << ", " << number(l_.scale) << ");\n";
     keys << "  akg::attn::backward_keys<akg_C, " << nwk << ", " << nwq << ">(" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << inName(3)
-         << ", " << inName(5) << ", " << optionals(6) << ", " << outName(1) << ", " << outName(2) << ", akg_ws, " << extents << ", " << number(l_.scale) << ");\n";
+         << ", " << optionals(6) << ", " << outName(1) << ", " << outName(2) << ", akg_ws, " << extents << ", " << number(l_.scale) << ");\n";
     KernelPhase first;
     first.kernelName = g_.name + "_queries";
     first.grid[0] = checkGrid(s.keyHeads * tilesQ);
     first.block[0] = static_cast<unsigned>(64 * nwq);
     k_.earlierPhases.push_back(first);
-    o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(k_.kernelName, 64 * nwk, args, keys.str());
+    o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(k_.kernelName, 64 * nwk, args, keys.str(), std::max(s.dk, s.dv) > 128 ? 0 : 2);
     k_.grid[0] = checkGrid(s.keyHeads * ceilDiv(s.sk, 32 * nwk));
     k_.block[0] = static_cast<unsigned>(64 * nwk);
-    // per row delta (and, for an added mask, two parts of its log-sum), per workgroup of the first kernel the largest |dout|
+    // per row delta and its log-sum (in two parts for an added mask), per workgroup of the first kernel the largest |dout|
     const bool added = l_.hasMask && in(6).dtype != DType::Bool;
-    k_.workspaceBytes = static_cast<uint64_t>(4 * s.keyHeads * ((added ? 3 : 1) * s.rows + tilesQ));
+    k_.workspaceBytes = static_cast<uint64_t>(4 * s.keyHeads * ((added ? 3 : 2) * s.rows + tilesQ));
     k_.source = o.str();
     k_.family = KernelFamily::Attention;
     k_.scalarArgs = {s.batch, s.sq, s.sk};

@@ -17,7 +17,9 @@
  * (16 bytes of a row per lane) and transposed (ds_read_b64_tr_b16: four rows of 16 columns per sixteen lanes). Rows are an
  * odd multiple of 64 bytes apart, so four neighbouring rows of 64 bytes cover the 256 bytes of the banks (transposed
  * reads), and the 16-byte chunks inside 64 bytes are permuted by (row / 4) % 4, so the sixteen rows that a 128-bit read
- * serves at a time (the lane quads 0, 3, 5, 6 of a half wavefront, then 1, 2, 4, 7) fall into different bank groups.
+ * serves at a time (the lane quads 0, 3, 5, 6 of a half wavefront, then 1, 2, 4, 7) fall into different bank groups. (Rows
+ * without padding and whole units permuted by the row are as free of conflicts, but every read then has an address of its
+ * own instead of an offset: eight to sixteen registers more, which the kernels of 128 channels spill.)
  *
  * Heads that share keys are rows of one problem: row r of a key head is query r / G of head r % G, so the tiles of keys
  * and values are fetched once for the group, and the gradients of keys and values are sums without atomics.
@@ -72,6 +74,13 @@ constexpr int kTileRows = 32;  // queries of a tile (dk, dv)
 
 constexpr int padded(int d) { return (d + 31) / 32 * 32; }
 constexpr int pitch(int d) { return padded(d) / 32 % 2 == 1 ? padded(d) * 2 : padded(d) * 2 + 64; }
+// Byte of chunk `chunk` (16 bytes) of row `row` in a tile of D channels.
+template <int D>
+AKG_DEV int chunk_at(int row, int chunk) {
+  return row * pitch(D) + ((chunk ^ ((row >> 2) & 3)) << 4);
+}
+// Keys that are only read along the row: rows an odd number of chunks apart.
+constexpr int own_pitch(int d) { return padded(d) * 2 + 16; }
 
 AKG_DEV float neg_inf() { return -__builtin_inff(); }
 // The two halves of a row's lane pair (n and n + 32) joined.
@@ -168,37 +177,48 @@ struct TileLoad {
       held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, (kWhole || c < kChunks) ? off : kBeyondEveryBuffer, 0, 0));
     }
   }
+  template <bool OWN = false>
   AKG_DEV void store(u8 *tile, int tid) const {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int c = tid + i * THREADS;
       const int row = c / kPerRow, chunk = c % kPerRow;
-      if (kWhole || c < kChunks) *reinterpret_cast<u32x4 *>(tile + row * pitch(D) + ((chunk ^ ((row >> 2) & 3)) << 4)) = held[i];
+      if (kWhole || c < kChunks) *reinterpret_cast<u32x4 *>(tile + (OWN ? row * own_pitch(D) + chunk * 16 : chunk_at<D>(row, chunk))) = held[i];
     }
   }
 };
 
-// 16 bytes of row `row0 + lane % 32`: channels 16 c + 8 (lane / 32) ... + 7, the operand of 16 contracted channels.
+// A lane's places in a tile of D channels. What differs between the reads of a tile is then a constant offset (left to
+// itself the compiler keeps an address per read).
 template <int D>
-AKG_DEV u32x4 read_row(const u8 *tile, int row0, int c, int lane) {
-  const int row = row0 + (lane & 31);
-  const int chunk = 2 * c + (lane >> 5);
-  return *reinterpret_cast<const u32x4 *>(tile + row * pitch(D) + ((chunk ^ ((row >> 2) & 3)) << 4));
-}
-// Column 32 dt + lane % 32 of the rows row0 + 4 h .. 4 h + 3 and row0 + 8 + 4 h .. (h = lane / 32; row0 a multiple of 16).
+struct Reader {
+  int along[2], across[2];
+  AKG_DEV explicit Reader(int lane) {
+    const int row = lane & 31, h = lane >> 5;
+    along[0] = chunk_at<D>(row, h);
+    along[1] = chunk_at<D>(row, 2 + h);
+    const int i = lane & 15, r = 4 * h + (i >> 2), chunk = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+    across[0] = chunk_at<D>(r, chunk) + (i & 1) * 8;
+    across[1] = chunk_at<D>(r + 8, chunk) + (i & 1) * 8;
+  }
+  // 16 bytes of row `row0 + lane % 32` (row0 a multiple of 32): channels 16 c + 8 (lane / 32) ... + 7, the operand of 16
+  // contracted channels.
+  AKG_DEV u32x4 row(const u8 *tile, int row0, int c) const {
+    return *reinterpret_cast<const u32x4 *>(tile + along[c & 1] + (row0 * pitch(D) + 64 * (c >> 1)));
+  }
+  // Column 32 dt + lane % 32 of the rows row0 + 4 h .. 4 h + 3 and row0 + 8 + 4 h .. (h = lane / 32; row0 a multiple of 16).
+  AKG_DEV u32x4 transposed(const u8 *tile, int row0, int dt) const {
+    const int more = row0 * pitch(D) + 64 * dt;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(tile + across[0] + more));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(tile + across[1] + more));
+    const u32x2 l = __builtin_bit_cast(u32x2, lo), u = __builtin_bit_cast(u32x2, hi);
+    return u32x4{l[0], l[1], u[0], u[1]};
+  }
+};
 template <int D>
-AKG_DEV u32x4 read_transposed(const u8 *tile, int row0, int dt, int lane) {
-  const int i = lane & 15;
-  const int row = row0 + 4 * (lane >> 5) + (i >> 2);
-  const int chunk = 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-  const u8 *p0 = tile + row * pitch(D) + ((chunk ^ ((row >> 2) & 3)) << 4) + (i & 1) * 8;
-  const u8 *p1 = tile + (row + 8) * pitch(D) + ((chunk ^ (((row + 8) >> 2) & 3)) << 4) + (i & 1) * 8;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p0));
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p1));
-  const u32x2 l = __builtin_bit_cast(u32x2, lo), u = __builtin_bit_cast(u32x2, hi);
-  return u32x4{l[0], l[1], u[0], u[1]};
+AKG_DEV u32x4 read_own(const u8 *keys, int row0, int c, int lane) {
+  return *reinterpret_cast<const u32x4 *>(keys + (row0 + (lane & 31)) * own_pitch(D) + ((lane >> 5) << 4) + 32 * c);
 }
-
 // The channels behind D of a tile's rows (D to the next multiple of 32) hold zeros: written once, never again.
 template <int ROWS, int D, int THREADS>
 AKG_DEV void clear_padding(u8 *tile, int tid) {
@@ -206,7 +226,7 @@ AKG_DEV void clear_padding(u8 *tile, int tid) {
     constexpr int kPad = (padded(D) - D) / 8;
     for (int c = tid; c < ROWS * kPad; c += THREADS) {
       const int row = c / kPad, chunk = D / 8 + c % kPad;
-      *reinterpret_cast<u32x4 *>(tile + row * pitch(D) + ((chunk ^ ((row >> 2) & 3)) << 4)) = u32x4{0, 0, 0, 0};
+      *reinterpret_cast<u32x4 *>(tile + chunk_at<D>(row, chunk)) = u32x4{0, 0, 0, 0};
     }
   }
 }
@@ -313,6 +333,8 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
 
   const KeysOf<C, DK> keys(k, b, hkv, e);
   const KeysOf<C, DV> values(v, b, hkv, e);
+  const Reader<DK> kread(lane);
+  const Reader<DV> vread(lane);
   TileLoad<kTile, DK, kThreads> kload;
   TileLoad<kTile, DV, kThreads> vload;
   auto fetch = [&](int k0) {
@@ -349,7 +371,7 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
       for (int t = 0; t < 2; ++t) {
         s[t] = {};
 #pragma unroll
-        for (int x = 0; x < CK; ++x) s[t] = T::mma(read_row<DK>(kt, 32 * t, x, lane), own[x], s[t]);
+        for (int x = 0; x < CK; ++x) s[t] = T::mma(kread.row(kt, 32 * t, x), own[x], s[t]);
       }
       const bool ragged = __any(k0 + kTile > seen);
       if (C::MASK != 0 || ragged) {
@@ -402,7 +424,7 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
 #pragma unroll
         for (int w = 0; w < 4; ++w) p[w] = T::pack(s[x >> 1][8 * (x & 1) + 2 * w], s[x >> 1][8 * (x & 1) + 2 * w + 1]);
 #pragma unroll
-        for (int d = 0; d < TV; ++d) acc[d] = T::mma(read_transposed<DV>(vt, 16 * x, d, lane), p, acc[d]);
+        for (int d = 0; d < TV; ++d) acc[d] = T::mma(vread.transposed(vt, 16 * x, d), p, acc[d]);
       }
     }
     if (more) put(buf ^ 1);
@@ -504,14 +526,15 @@ AKG_DEV float lift_of(float largest) {
 // sum behind the maximum: the kernel of dq then finds both again.
 constexpr float kLargeLse = 4096.0f;
 
-// Places in the workspace of the backward kernels, in floats: delta of every row, for an added mask top and rest of every
-// row, and the largest |dout| of every workgroup of the first kernel.
+// Places in the workspace of the backward kernels, in floats: delta and top of every row (top: times log2 e where no mask is
+// added; infinite for a row without keys, whose probabilities then are 2^-inf = 0), for an added mask the rest, and the
+// largest |dout| of every workgroup of the first kernel.
 template <typename C>
 struct BackwardSpace {
   long rows;   // of all key heads
   AKG_DEV long top(long row) const { return rows + row; }
   AKG_DEV long rest(long row) const { return 2 * rows + row; }
-  AKG_DEV long largest() const { return C::ADDED ? 3 * rows : rows; }
+  AKG_DEV long largest() const { return (C::ADDED ? 3 : 2) * rows; }
 };
 
 // dq of 32 rows a wavefront: keys and values pass by in tiles. Leaves in `ws` what the kernel of dk and dv needs.
@@ -583,6 +606,8 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
   for (int d = 0; d < TK; ++d) acc[d] = {};
   const KeysOf<C, DK> keys(k, b, hkv, e);
   const KeysOf<C, DV> values(v, b, hkv, e);
+  const Reader<DK> kread(lane);
+  const Reader<DV> vread(lane);
   TileLoad<kTile, DK, kThreads> kload;
   TileLoad<kTile, DV, kThreads> vload;
   auto fetch = [&](int k0) {
@@ -640,11 +665,9 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
         rest = __builtin_amdgcn_logf(sum);
       }
     }
-    if (exists && half == 0) {
-      ws[space.top(head * rows + row)] = sums;
-      ws[space.rest(head * rows + row)] = rest;
-    }
+    if (exists && half == 0) ws[space.rest(head * rows + row)] = rest;
   }
+  if (exists && half == 0) ws[space.top(head * rows + row)] = sums;
   int buf = 0;
   for (int k0 = 0; k0 < end; k0 += kTile, buf ^= 1) {
     const bool more = k0 + kTile < end;
@@ -656,9 +679,9 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
       for (int t = 0; t < 2; ++t) {
         f32x16 s = {}, dp = {};
 #pragma unroll
-        for (int x = 0; x < CK; ++x) s = T::mma(read_row<DK>(kt, 32 * t, x, lane), own[x], s);
+        for (int x = 0; x < CK; ++x) s = T::mma(kread.row(kt, 32 * t, x), own[x], s);
 #pragma unroll
-        for (int x = 0; x < CV; ++x) dp = T::mma(read_row<DV>(vt, 32 * t, x, lane), grad[x], dp);
+        for (int x = 0; x < CV; ++x) dp = T::mma(vread.row(vt, 32 * t, x), grad[x], dp);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int j = k0 + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
@@ -678,7 +701,7 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
 #pragma unroll
           for (int w = 0; w < 4; ++w) p[w] = T::pack(s[8 * x + 2 * w], s[8 * x + 2 * w + 1]);
 #pragma unroll
-          for (int d = 0; d < TK; ++d) acc[d] = T::mma(read_transposed<DK>(kt, 32 * t + 16 * x, d, lane), p, acc[d]);
+          for (int d = 0; d < TK; ++d) acc[d] = T::mma(kread.transposed(kt, 32 * t + 16 * x, d), p, acc[d]);
         }
       }
     }
@@ -705,13 +728,17 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
 
 // dk and dv of 32 keys a wavefront: the queries of all heads that share them pass by in tiles.
 template <typename C, int NW, int NWQ>
-AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const void *v, const float *lse, const void *mask,
+AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const void *v, const void *mask,
                            const int *qlens, const int *klens, void *dk, void *dv, const float *ws, Extents e, float scale) {
   typedef typename C::T T;
   constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, CV = (DV + 15) / 16, TK = padded(DK) / 32, TV = padded(DV) / 32, kThreads = 64 * NW;
+  // From 192 channels on (keys and values together) the accumulators and the wavefront's own operands would leave room for
+  // one wavefront per SIMD: its keys lie in LDS then, and two fit.
+  constexpr bool kKeysInLds = padded(DK) + padded(DV) > 192;
   __shared__ __attribute__((aligned(16))) u8 lds[2][kTileRows * (pitch(DK) + pitch(DV))];
-  __shared__ __attribute__((aligned(16))) float sumsOf[2][kTileRows], deltaOf[2][kTileRows], restOf[C::ADDED ? 2 : 1][kTileRows];
-  __shared__ __attribute__((aligned(16))) int seenOf[2][kTileRows];
+  __shared__ __attribute__((aligned(16))) u8 ownKeys[kKeysInLds ? kRows * NW * own_pitch(DK) : 16];
+  constexpr int kStates = C::ADDED ? 3 : 2;   // of a row: delta, top and rest (BackwardSpace)
+  __shared__ __attribute__((aligned(16))) float stateOf[2][kStates][kTileRows];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const long rows = e.sq * C::G, heads = e.batch * C::HKV;
   long head, tile;
@@ -724,8 +751,20 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
   const KeysOf<C, DK> keys(k, b, hkv, e);
   const KeysOf<C, DV> values(v, b, hkv, e);
   const BackwardSpace<C> space{heads * rows};
-  u32x4 own[CK], val[CV];
-  load_own<DK>(keys.base + (counts ? key : 0) * keys.step, counts, lane, own);
+  u32x4 own[kKeysInLds ? 1 : CK], val[CV];
+  if constexpr (kKeysInLds) {
+    const int key00 = static_cast<int>(tile) * (kRows * NW);
+    const Buffer kb = make_buffer(keys.base + key00 * keys.step, records((kl - key00 - 1) * keys.step + 2 * DK));
+    TileLoad<kRows * NW, DK, kThreads> kload;
+    kload.load(kb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(keys.step)); });
+    kload.template store<true>(ownKeys, tid);   // (padding channels meet zeros of the queries, but must be finite)
+    for (int c = tid; DK % 32 != 0 && c < kRows * NW * ((padded(DK) - DK) / 8); c += kThreads) {
+      constexpr int kPad = DK % 32 != 0 ? (padded(DK) - DK) / 8 : 1;
+      *reinterpret_cast<u32x4 *>(ownKeys + c / kPad * own_pitch(DK) + (DK / 8 + c % kPad) * 16) = u32x4{0, 0, 0, 0};
+    }
+  } else {
+    load_own<DK>(keys.base + (counts ? key : 0) * keys.step, counts, lane, own);
+  }
   load_own<DV>(values.base + (counts ? key : 0) * values.step, counts, lane, val);
   float lift = 1.0f;
   if (T::kNarrowRange) {
@@ -745,52 +784,43 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
 
   // queries that see the first key of the workgroup, up to the last one of the sequence
   const int first0 = static_cast<int>(tile) * (kRows * NW);
-  long from = 0;
+  int from = 0;
   if (C::CAUSAL) {
-    const long i = static_cast<long>(first0) - (kl - ql);
-    from = (i > 0 ? i : 0) * C::G / kTileRows * kTileRows;
+    const int i = first0 - (kl - ql);
+    from = (i > 0 ? (i < ql ? i : ql) : 0) * C::G / kTileRows * kTileRows;
   }
-  const long upto = first0 < kl ? static_cast<long>(ql) * C::G : 0;
+  const int upto = first0 < kl ? ql * C::G : 0;
 
   const RowsOf<C, DK> qrows(q, b, hkv, e);
   const RowsOf<C, DV> grows(dout, b, hkv, e);
+  const Reader<DK> qread(lane);
+  const Reader<DV> gread(lane);
   TileLoad<kTileRows, DK, kThreads> qload;
   TileLoad<kTileRows, DV, kThreads> gload;
-  float sums = 0.0f, delta = 0.0f, rest = 0.0f;
-  int seen = 0;
-  auto fetch = [&](long r0) {
-    const long i0 = r0 / C::G;
+  // Rows behind the last one read zeros (nothing is asked of memory): their probabilities are 1 and their products 0.
+  float state[kStates];
+  auto fetch = [&](int r0) {
+    const int i0 = r0 / C::G;
     const Buffer qb = make_buffer(qrows.base + i0 * qrows.stepI, 0x7fffffffL);
     const Buffer gb = make_buffer(grows.base + i0 * grows.stepI, 0x7fffffffL);
+    const int left = upto - r0, lead = r0 - i0 * C::G;
     auto offsetIn = [&](const auto &of, int r) {
-      const long at = r0 + r;
-      return at < upto ? static_cast<u32>((at / C::G - i0) * of.stepI + at % C::G * of.stepG) : kBeyondEveryBuffer;
+      const int at = lead + r;
+      return r < left ? static_cast<u32>(at / C::G * static_cast<int>(of.stepI) + at % C::G * static_cast<int>(of.stepG)) : kBeyondEveryBuffer;
     };
     qload.load(qb, tid, [&](int r) { return offsetIn(qrows, r); });
     gload.load(gb, tid, [&](int r) { return offsetIn(grows, r); });
     if (tid < kTileRows) {
-      const long at = r0 + tid;
-      const bool ok = at < upto;
-      const long i = ok ? at / C::G : 0, g = ok ? at % C::G : 0;
-      if (C::ADDED) {
-        sums = ok ? ws[space.top(head * rows + at)] : __builtin_inff();
-        rest = ok ? ws[space.rest(head * rows + at)] : 0.0f;
-      } else {
-        sums = ok ? lse[(b * C::H + hkv * C::G + g) * e.sq + i] : neg_inf();
-        sums = sums == neg_inf() ? __builtin_inff() : sums * kLog2e;
-      }
-      delta = ok ? ws[head * rows + at] : 0.0f;
-      seen = ok ? keys_seen<C>(i, ql, kl) : 0;
+#pragma unroll
+      for (int x = 0; x < kStates; ++x) state[x] = tid < left ? ws[x * heads * rows + head * rows + r0 + tid] : 0.0f;
     }
   };
   auto put = [&](int buf) {
     qload.store(lds[buf], tid);
     gload.store(lds[buf] + kTileRows * pitch(DK), tid);
     if (tid < kTileRows) {
-      sumsOf[buf][tid] = sums;
-      if (C::ADDED) restOf[buf][tid] = rest;
-      deltaOf[buf][tid] = delta;
-      seenOf[buf][tid] = seen;
+#pragma unroll
+      for (int x = 0; x < kStates; ++x) stateOf[buf][x][tid] = state[x];
     }
   };
 #pragma unroll
@@ -804,56 +834,70 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
   }
   __syncthreads();
   int buf = 0;
-  for (long r0 = from; r0 < upto; r0 += kTileRows, buf ^= 1) {
-    const bool more = r0 + kTileRows < upto;
-    if (more) fetch(r0 + kTileRows);
+  for (int r0 = from; r0 < upto; r0 += kTileRows, buf ^= 1) {
     const u8 *qt = lds[buf], *gt = lds[buf] + kTileRows * pitch(DK);
     // the tile's last row sees most keys, its first one least
-    const long lastRow = (r0 + kTileRows < upto ? r0 + kTileRows : upto) - 1;
-    if (key0 < keys_seen<C>(lastRow / C::G, ql, kl)) {
-      const bool ragged = key0 + kRows > keys_seen<C>(r0 / C::G, ql, kl);
+    const int lastRow = (r0 + kTileRows < upto ? r0 + kTileRows : upto) - 1;
+    const bool active = key0 < keys_seen<C>(lastRow / C::G, ql, kl);
+    u32x4 p[2], ds[2];
+    if (active) {
       f32x16 s = {}, dp = {};
 #pragma unroll
-      for (int x = 0; x < CK; ++x) s = T::mma(read_row<DK>(qt, 0, x, lane), own[x], s);
+      for (int x = 0; x < CK; ++x) s = T::mma(qread.row(qt, 0, x), kKeysInLds ? read_own<DK>(ownKeys, wave * kRows, x, lane) : own[kKeysInLds ? 0 : x], s);
 #pragma unroll
-      for (int x = 0; x < CV; ++x) dp = T::mma(read_row<DV>(gt, 0, x, lane), val[x], dp);
+      for (int x = 0; x < CV; ++x) dp = T::mma(gread.row(gt, 0, x), val[x], dp);
+      if (C::MASK != 0 || key0 + kRows > keys_seen<C>(r0 / C::G, ql, kl)) {
+        __builtin_amdgcn_sched_barrier(0);   // (a branch, not a select for every tile)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int at = r0 + 8 * (r >> 2) + 4 * half + (r & 3), i = at / C::G;
+          const bool ok = key < keys_seen<C>(i, ql, kl);
+          if (C::MASK != 0) {
+            s[r] = ok ? with_mask<C>(s[r], c, mask, mask_row<C>(b, hkv * C::G + at % C::G, i, e) + key) : neg_inf();
+          } else {
+            s[r] = ok ? s[r] : neg_inf();
+          }
+        }
+      }
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&sumsOf[buf][8 * r4 + 4 * half]);
-        const f32x4 d4 = *reinterpret_cast<const f32x4 *>(&deltaOf[buf][8 * r4 + 4 * half]);
-        const i32x4 n4 = *reinterpret_cast<const i32x4 *>(&seenOf[buf][8 * r4 + 4 * half]);
+        const f32x4 d4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][0][8 * r4 + 4 * half]);
+        const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][1][8 * r4 + 4 * half]);
+        f32x4 o4 = {};
+        if (C::ADDED) o4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][kStates - 1][8 * r4 + 4 * half]);
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
           const int r = 4 * r4 + z;
-          float x = s[r];
-          if (C::MASK != 0) {
-            const long at = r0 + 8 * r4 + 4 * half + z;
-            x = key < n4[z] ? with_mask<C>(x, c, mask, mask_row<C>(b, hkv * C::G + at % C::G, at / C::G, e) + key) - l4[z] : neg_inf();
-            if (C::ADDED) x = __builtin_fmaf(x, kLog2e, -restOf[buf][8 * r4 + 4 * half + z]);
-          } else {
-            x = __builtin_fmaf(x, c, -l4[z]);
-            if (ragged) x = key < n4[z] ? x : neg_inf();
-          }
-          const float p = __builtin_amdgcn_exp2f(x);
-          s[r] = p;
-          dp[r] = p * ((dp[r] - d4[z]) * lift);
+          float x = C::MASK != 0 ? s[r] - l4[z] : __builtin_fmaf(s[r], c, -l4[z]);
+          if (C::ADDED) x = __builtin_fmaf(x, kLog2e, -o4[z]);
+          s[r] = __builtin_amdgcn_exp2f(x);
+          dp[r] = s[r] * (T::kNarrowRange ? (dp[r] - d4[z]) * lift : dp[r] - d4[z]);
         }
       }
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        u32x4 p, ds;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          p[w] = T::pack(s[8 * x + 2 * w], s[8 * x + 2 * w + 1]);
-          ds[w] = T::pack(dp[8 * x + 2 * w], dp[8 * x + 2 * w + 1]);
+          p[x][w] = T::pack(s[8 * x + 2 * w], s[8 * x + 2 * w + 1]);
+          ds[x][w] = T::pack(dp[8 * x + 2 * w], dp[8 * x + 2 * w + 1]);
         }
-#pragma unroll
-        for (int d = 0; d < TV; ++d) accv[d] = T::mma(read_transposed<DV>(gt, 16 * x, d, lane), p, accv[d]);
-#pragma unroll
-        for (int d = 0; d < TK; ++d) acck[d] = T::mma(read_transposed<DK>(qt, 16 * x, d, lane), ds, acck[d]);
+        asm volatile("" : "+v"(p[x]), "+v"(ds[x]));   // (the scores end here: their registers hold the next tile's rows)
       }
     }
-    if (more) put(buf ^ 1);
+    fetch(r0 + kTileRows);
+    if (active) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int d = 0; d < TV; ++d) accv[d] = T::mma(gread.transposed(gt, 16 * x, d), p[x], accv[d]);
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int d = 0; d < TK; ++d) acck[d] = T::mma(qread.transposed(qt, 16 * x, d), ds[x], acck[d]);
+      }
+    }
+    put(buf ^ 1);
     __syncthreads();
   }
   if (key >= e.sk) return;
