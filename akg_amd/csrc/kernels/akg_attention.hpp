@@ -286,6 +286,24 @@ AKG_DEV void head_and_tile(long id, long heads, long &head, long &tile) {
   }
 }
 
+// Order of a block of MF matrix instructions fed by RD LDS reads: LEAD reads ahead, then after every matrix instruction its
+// share of the others. (Left to itself the compiler issues a read right in front of its use, and the matrix cores wait.)
+template <int MF, int RD, int LEAD, int M = 0>
+struct FeedOrder {
+  static constexpr int kLead = LEAD < RD ? LEAD : RD;
+  static constexpr int kEach = (RD - kLead + MF - 1) / (MF > 0 ? MF : 1);
+  static constexpr int kFrom = M * kEach < RD - kLead ? M * kEach : RD - kLead;
+  static constexpr int kUpto = (M + 1) * kEach < RD - kLead ? (M + 1) * kEach : RD - kLead;
+  static AKG_DEV void emit() {
+    if constexpr (M == 0) __builtin_amdgcn_sched_group_barrier(0x100, kLead, 0);
+    if constexpr (M < MF) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if constexpr (kUpto > kFrom) __builtin_amdgcn_sched_group_barrier(0x100, kUpto - kFrom, 0);
+      FeedOrder<MF, RD, LEAD, M + 1>::emit();
+    }
+  }
+};
+
 // ---- forward ----------------------------------------------------------------------------------------------------------
 // SPLIT: the workgroup takes one of `splits` ranges of the keys and leaves accumulators, maximum and sum in `ws`.
 template <typename C, int NW, bool SPLIT>
@@ -373,6 +391,7 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
 #pragma unroll
         for (int x = 0; x < CK; ++x) s[t] = T::mma(kread.row(kt, 32 * t, x), own[x], s[t]);
       }
+      FeedOrder<2 * CK, 2 * CK, 6>::emit();
       const bool ragged = __any(k0 + kTile > seen);
       if (C::MASK != 0 || ragged) {
 #pragma unroll
@@ -418,14 +437,19 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
       }
       // probabilities are rounded to the type of the values for the matrix units (half a step of at most 2^-9 each, of
       // changing sign; the sum above has them unrounded)
+      u32x4 p[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        u32x4 p;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) p[w] = T::pack(s[x >> 1][8 * (x & 1) + 2 * w], s[x >> 1][8 * (x & 1) + 2 * w + 1]);
-#pragma unroll
-        for (int d = 0; d < TV; ++d) acc[d] = T::mma(vread.transposed(vt, 16 * x, d), p, acc[d]);
+        for (int w = 0; w < 4; ++w) p[x][w] = T::pack(s[x >> 1][8 * (x & 1) + 2 * w], s[x >> 1][8 * (x & 1) + 2 * w + 1]);
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+#pragma unroll
+        for (int d = 0; d < TV; ++d) acc[d] = T::mma(vread.transposed(vt, 16 * x, d), p[x], acc[d]);
+      }
+      FeedOrder<4 * TV, 8 * TV, 8>::emit();
     }
     if (more) put(buf ^ 1);
     __syncthreads();
@@ -743,6 +767,12 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
   const long rows = e.sq * C::G, heads = e.batch * C::HKV;
   long head, tile;
   head_and_tile(blockIdx.x, heads, head, tile);
+  // The first keys are seen by most queries, and come first. Where every workgroup finds a place at once, two to a CU, the
+  // second half goes by in reverse, so that the CUs with the longest ones get the shortest ones too.
+  if (C::CAUSAL && gridDim.x <= 512u) {
+    const long tiles = (e.sk + kRows * NW - 1) / (kRows * NW), first = (tiles + 1) / 2;
+    if (tile >= first) tile = tiles - 1 - (tile - first);
+  }
   const long b = head / C::HKV, hkv = head % C::HKV;
   const int ql = clamped_length<C>(qlens, b, e.sq), kl = clamped_length<C>(klens, b, e.sk);
   const int key0 = static_cast<int>(tile) * (kRows * NW) + wave * kRows;
@@ -846,6 +876,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
       for (int x = 0; x < CK; ++x) s = T::mma(qread.row(qt, 0, x), kKeysInLds ? read_own<DK>(ownKeys, wave * kRows, x, lane) : own[kKeysInLds ? 0 : x], s);
 #pragma unroll
       for (int x = 0; x < CV; ++x) dp = T::mma(gread.row(gt, 0, x), val[x], dp);
+      FeedOrder<CK + CV, (kKeysInLds ? 2 : 1) * CK + CV, 6>::emit();
       if (C::MASK != 0 || key0 + kRows > keys_seen<C>(r0 / C::G, ql, kl)) {
         __builtin_amdgcn_sched_barrier(0);   // (a branch, not a select for every tile)
 #pragma unroll
@@ -896,6 +927,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
 #pragma unroll
         for (int d = 0; d < TK; ++d) acck[d] = T::mma(qread.transposed(qt, 16 * x, d), ds[x], acck[d]);
       }
+      FeedOrder<2 * (TV + TK), 4 * (TV + TK), 8>::emit();
     }
     put(buf ^ 1);
     __syncthreads();
