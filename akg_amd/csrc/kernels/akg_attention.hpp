@@ -304,6 +304,22 @@ struct FeedOrder {
   }
 };
 
+// The same with other work beside it: after every matrix instruction also VA vector instructions and TR transcendental ones.
+template <int MF, int RD, int LEAD, int VA, int TR, int M = 0>
+struct BesideOrder {
+  typedef FeedOrder<MF, RD, LEAD, M> F;
+  static AKG_DEV void emit() {
+    if constexpr (M == 0) __builtin_amdgcn_sched_group_barrier(0x100, F::kLead, 0);
+    if constexpr (M < MF) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if constexpr (F::kUpto > F::kFrom) __builtin_amdgcn_sched_group_barrier(0x100, F::kUpto - F::kFrom, 0);
+      if constexpr (VA > 0) __builtin_amdgcn_sched_group_barrier(0x002, VA, 0);
+      if constexpr (TR > 0) __builtin_amdgcn_sched_group_barrier(0x400, TR, 0);
+      BesideOrder<MF, RD, LEAD, VA, TR, M + 1>::emit();
+    }
+  }
+};
+
 // ---- forward ----------------------------------------------------------------------------------------------------------
 // SPLIT: the workgroup takes one of `splits` ranges of the keys and leaves accumulators, maximum and sum in `ws`.
 template <typename C, int NW, bool SPLIT>
@@ -311,7 +327,9 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
                      void *out, float *lse, float *ws, Extents e, float scale, int splits) {
   typedef typename C::T T;
   constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, TV = padded(DV) / 32, kThreads = 64 * NW;
-  __shared__ __attribute__((aligned(16))) u8 lds[2][kTile * (pitch(DK) + pitch(DV))];
+  // A third tile of keys, where a CU holds one workgroup anyway, spares a barrier: what is being written no wavefront reads.
+  constexpr int kKeyTiles = NW == 8 && kTile * (3 * pitch(DK) + 2 * pitch(DV)) <= 160 * 1024 ? 3 : 2;
+  __shared__ __attribute__((aligned(16))) u8 ktiles[kKeyTiles][kTile * pitch(DK)], vtiles[2][kTile * pitch(DV)];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const long rows = e.sq * C::G, tiles = (rows + kRows * NW - 1) / (kRows * NW), heads = e.batch * C::HKV;
   long id = blockIdx.x;
@@ -347,7 +365,7 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   f32x16 acc[TV];
 #pragma unroll
   for (int d = 0; d < TV; ++d) acc[d] = {};
-  float top = neg_inf(), sum = 0.0f;   // the row's maximum; the sum over this lane's keys
+  float top = neg_inf(), sum[2] = {0.0f, 0.0f};   // the row's maximum (or a little less); sums over this lane's keys
 
   const KeysOf<C, DK> keys(k, b, hkv, e);
   const KeysOf<C, DV> values(v, b, hkv, e);
@@ -355,112 +373,154 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   const Reader<DV> vread(lane);
   TileLoad<kTile, DK, kThreads> kload;
   TileLoad<kTile, DV, kThreads> vload;
-  auto fetch = [&](int k0) {
-    const Buffer kb = make_buffer(keys.base + k0 * keys.step, records((kl - k0 - 1) * keys.step + 2 * DK));
-    const Buffer vb = make_buffer(values.base + k0 * values.step, records((kl - k0 - 1) * values.step + 2 * DV));
+  // Keys are fetched a tile further ahead than values: while the probabilities of a tile are computed (vector instructions)
+  // the scores of the next one are (matrix instructions), in one stream.
+  auto fetch_keys = [&](int k0) {
     // (rows behind the keys' length lie behind the descriptor and read zeros)
+    const Buffer kb = make_buffer(keys.base + k0 * keys.step, records((kl - k0 - 1) * keys.step + 2 * DK));
     kload.load(kb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(keys.step)); });
+  };
+  auto fetch_values = [&](int k0) {
+    const Buffer vb = make_buffer(values.base + k0 * values.step, records((kl - k0 - 1) * values.step + 2 * DV));
     vload.load(vb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(values.step)); });
   };
-  auto put = [&](int buf) {
-    kload.store(lds[buf], tid);
-    vload.store(lds[buf] + kTile * pitch(DK), tid);
-  };
 #pragma unroll
-  for (int buf = 0; buf < 2; ++buf) {
-    clear_padding<kTile, DK, kThreads>(lds[buf], tid);
-    clear_padding<kTile, DV, kThreads>(lds[buf] + kTile * pitch(DK), tid);
-  }
+  for (int x = 0; x < kKeyTiles; ++x) clear_padding<kTile, DK, kThreads>(ktiles[x], tid);
+#pragma unroll
+  for (int x = 0; x < 2; ++x) clear_padding<kTile, DV, kThreads>(vtiles[x], tid);
   if (first < end) {
-    fetch(first);
-    put(0);
+    fetch_keys(first);
+    fetch_values(first);
+    kload.store(ktiles[0], tid);
+    vload.store(vtiles[0], tid);
+    if (first + kTile < end) {
+      fetch_keys(first + kTile);
+      kload.store(ktiles[1], tid);
+    }
   }
   __syncthreads();
 
   const long maskAt = C::MASK != 0 ? mask_row<C>(b, hkv * C::G + g, exists ? i : 0, e) : 0;
-  int buf = 0;
-  for (int k0 = first; k0 < end; k0 += kTile, buf ^= 1) {
-    const bool more = k0 + kTile < end;
-    if (more) fetch(k0 + kTile);
-    const u8 *kt = lds[buf], *vt = lds[buf] + kTile * pitch(DK);
-    if (__any(k0 < seen)) {   // (wavefronts whose rows see nothing of the tile only help to fetch the next one)
-      f32x16 s[2];
+  f32x16 s;                 // scores of 32 keys
+  float peak = neg_inf();   // the largest of them (of this lane's keys)
+  auto scores = [&](const u8 *kt, int row0) {
+    f32x16 to = {};
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        s[t] = {};
+    for (int x = 0; x < CK; ++x) to = T::mma(kread.row(kt, row0, x), own[x], to);
+    return to;
+  };
+  // What the mask, the lengths and the causal order leave of the scores of the keys from j0 on.
+  auto limit = [&](int j0, f32x16 &x) {
 #pragma unroll
-        for (int x = 0; x < CK; ++x) s[t] = T::mma(kread.row(kt, 32 * t, x), own[x], s[t]);
+    for (int r = 0; r < 16; ++r) {
+      const int j = j0 + 8 * (r >> 2) + 4 * half + (r & 3);
+      if (C::MASK != 0) {
+        x[r] = j < seen ? with_mask<C>(x[r], c, mask, maskAt + j) : neg_inf();
+      } else {
+        x[r] = j < seen ? x[r] : neg_inf();
       }
-      FeedOrder<2 * CK, 2 * CK, 6>::emit();
-      const bool ragged = __any(k0 + kTile > seen);
-      if (C::MASK != 0 || ragged) {
+    }
+  };
+  auto largest = [&](const f32x16 &x) {
+    float m = x[0];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int j = k0 + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
-            if (C::MASK != 0) {
-              s[t][r] = j < seen ? with_mask<C>(s[t][r], c, mask, maskAt + j) : neg_inf();
-            } else {
-              s[t][r] = j < seen ? s[t][r] : neg_inf();
-            }
-          }
-        }
-      }
-      float m = top;
-      {
-        float peak = s[0][0];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) peak = __builtin_fmaxf(peak, s[t][r]);
-        }
-        if (C::MASK == 0) peak *= c;
-        m = __builtin_fmaxf(m, max_halves(peak));
-      }
-      const float base = m == neg_inf() ? 0.0f : m;
-      const float shrink = power<C>(top - base);
+    for (int r = 1; r < 16; ++r) m = __builtin_fmaxf(m, x[r]);
+    return m;
+  };
+  // The keys from j0 on, whose scores are in `s`: their probabilities, while the scores of the 32 keys behind them are
+  // computed (rows `krow` of `kt`; of whatever lies there where no row sees more), and their part of the result. One stream
+  // without branches around it: with the two cases apart the accumulators were held twice.
+  auto step = [&](int j0, const u8 *vt, int vrow, const u8 *kt, int krow) {
+    // The maximum that the exponents are taken against follows the scores only when they are 2^8 above it: sums and
+    // accumulators then have to be rescaled, which most tiles are spared; what is kept is as exact against any maximum.
+    float m = max_halves(peak);
+    if (C::MASK == 0) m *= c;
+    if (__any(m > top + (C::ADDED ? 5.5f : 8.0f))) {
+      m = __builtin_fmaxf(top, m);
+      const float shrink = power<C>(top - (m == neg_inf() ? 0.0f : m));
       top = m;
-      sum *= shrink;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[t][r] = power<C>(C::MASK == 0 ? __builtin_fmaf(s[t][r], c, -base) : s[t][r] - base);
-          sum += s[t][r];
-        }
-      }
+      sum[0] *= shrink;
+      sum[1] *= shrink;
 #pragma unroll
       for (int d = 0; d < TV; ++d) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] *= shrink;
       }
-      // probabilities are rounded to the type of the values for the matrix units (half a step of at most 2^-9 each, of
-      // changing sign; the sum above has them unrounded)
-      u32x4 p[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) p[x][w] = T::pack(s[x >> 1][8 * (x & 1) + 2 * w], s[x >> 1][8 * (x & 1) + 2 * w + 1]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-#pragma unroll
-        for (int d = 0; d < TV; ++d) acc[d] = T::mma(vread.transposed(vt, 16 * x, d), p[x], acc[d]);
-      }
-      FeedOrder<4 * TV, 8 * TV, 8>::emit();
     }
-    if (more) put(buf ^ 1);
+    const float base = top == neg_inf() ? 0.0f : top;
+    // Probabilities are rounded to the type of the values for the matrix units (half a step of at most 2^-9 each, of
+    // changing sign; the sum has them unrounded). A matrix instruction keeps its unit busy for 32 cycles and the issue for
+    // four: a few vector instructions behind each of them, and operands read four ahead. (The barriers keep that order.)
+    constexpr int kLead = 4, kEach = (16 + CK - 1) / CK;
+    u32x4 p[2], a[CK];
+    f32x16 next = {};
+#pragma unroll
+    for (int x = 0; x < kLead && x < CK; ++x) a[x] = kread.row(kt, krow, x);
+#pragma unroll
+    for (int x = 0; x < CK; ++x) {
+      __builtin_amdgcn_sched_barrier(0);
+      next = T::mma(a[x], own[x], next);
+      if (x + kLead < CK) a[x + kLead] = kread.row(kt, krow, x + kLead);
+#pragma unroll
+      for (int r = x * kEach; r < 16 && r < (x + 1) * kEach; ++r) {
+        s[r] = power<C>(C::MASK == 0 ? __builtin_fmaf(s[r], c, -base) : s[r] - base);
+        sum[r & 1] += s[r];
+        if (r & 1) p[r >> 3][(r >> 1) & 3] = T::pack(s[r - 1], s[r]);
+      }
+      asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));
+    }
+    u32x4 t[2 * TV];
+#pragma unroll
+    for (int x = 0; x < kLead && x < 2 * TV; ++x) t[x] = vread.transposed(vt, vrow + 16 * (x / TV), x % TV);
+    peak = neg_inf();
+    constexpr int kMost = (16 + 2 * TV - 1) / (2 * TV);
+#pragma unroll
+    for (int x = 0; x < 2 * TV; ++x) {
+      __builtin_amdgcn_sched_barrier(0);
+      acc[x % TV] = T::mma(t[x], p[x / TV], acc[x % TV]);
+      if (x + kLead < 2 * TV) t[x + kLead] = vread.transposed(vt, vrow + 16 * ((x + kLead) / TV), (x + kLead) % TV);
+#pragma unroll
+      for (int r = x * kMost; r < 16 && r < (x + 1) * kMost; ++r) peak = __builtin_fmaxf(peak, next[r]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (C::MASK != 0 || __any(j0 + 64 > seen)) {
+      __builtin_amdgcn_sched_barrier(0);
+      limit(j0 + 32, next);
+      peak = largest(next);
+    }
+    s = next;
+  };
+  bool active = first < end && __any(first < seen);   // (wavefronts whose rows see nothing of a tile only help to fetch the next one)
+  if (active) {
+    s = scores(ktiles[0], 0);
+    if (C::MASK != 0 || __any(first + 32 > seen)) limit(first, s);
+    peak = largest(s);
+  }
+  int buf = 0, kbuf = 0;
+  for (int k0 = first; k0 < end; k0 += kTile) {
+    const bool more = k0 + kTile < end;
+    const int knext = kbuf + 1 < kKeyTiles ? kbuf + 1 : 0, kthen = kKeyTiles == 2 ? kbuf : knext + 1 < kKeyTiles ? knext + 1 : 0;
+    fetch_keys(k0 + 2 * kTile < end ? k0 + 2 * kTile : kl);   // (none left: zeros)
+    fetch_values(more ? k0 + kTile : kl);
+    if (active) {
+      step(k0, vtiles[buf], 0, ktiles[kbuf], 32);
+      step(k0 + 32, vtiles[buf], 32, ktiles[knext], 0);
+      active = more && __any(k0 + kTile < seen);
+    }
+    if (kKeyTiles == 2) __syncthreads();   // (the tile written now was read in this round)
+    kload.store(ktiles[kthen], tid);
+    vload.store(vtiles[buf ^ 1], tid);
     __syncthreads();
+    kbuf = knext;
+    buf ^= 1;
   }
 
-  sum = add_halves(sum);
+  const float all = add_halves(sum[0] + sum[1]);
   if (!exists) return;
   if (SPLIT) {
     const long slot = (static_cast<long>(split) * heads + head) * rows + row;
     float *to = ws + slot * padded(DV);
-    if (sum > 0.0f || sum != sum) {
+    if (all > 0.0f || all != all) {
 #pragma unroll
       for (int d = 0; d < TV; ++d) {
 #pragma unroll
@@ -473,11 +533,11 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
     if (half == 0) {
       float *state = ws + static_cast<long>(splits) * heads * rows * padded(DV) + 2 * slot;
       state[0] = top;
-      state[1] = sum;
+      state[1] = all;
     }
     return;
   }
-  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
   const RowsOf<C, DV> orows(out, b, hkv, e);
   char *to = const_cast<char *>(orows.base) + orows.offset(row);
 #pragma unroll
@@ -493,7 +553,7 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
     }
   }
   if (lse != nullptr && half == 0) {
-    lse[(b * C::H + hkv * C::G + g) * e.sq + i] = log_sum<C>(top, sum);
+    lse[(b * C::H + hkv * C::G + g) * e.sq + i] = log_sum<C>(top, all);
   }
 }
 
