@@ -243,6 +243,15 @@ AKG_DEV void load_own(const char *row, bool ok, int lane, u32x4 (&own)[(D + 15) 
 
 AKG_DEV u32 records(long bytes) { return static_cast<u32>(bytes < 0 ? 0 : (bytes < 0x7fffffffL ? bytes : 0x7fffffffL)); }
 
+template <bool B, typename X, typename Y>
+struct conditional {
+  typedef X type;
+};
+template <typename X, typename Y>
+struct conditional<false, X, Y> {
+  typedef Y type;
+};
+
 // ---- masks ------------------------------------------------------------------------------------------------------------
 template <typename C>
 AKG_DEV long mask_row(long b, long h, long i, const Extents &e) {
@@ -261,6 +270,39 @@ AKG_DEV float with_mask(float s, float factor, const void *mask, long at) {
   if constexpr (C::MASK == 4) return __builtin_fmaf(s, factor, static_cast<const float *>(mask)[at]);
   return s * factor;
 }
+// The mask's row of one query, 32 keys at a time: a lane holds four groups of four adjacent ones (as of the scores), requested
+// before the scores are computed.
+template <typename C>
+struct MaskRow {
+  typedef conditional<C::MASK == 1, u8, typename conditional<C::MASK == 4, float, u16>::type> Choice;
+  typedef typename Choice::type E;
+  typedef E E4 __attribute__((ext_vector_type(4)));
+  typedef E4 Unaligned __attribute__((aligned(sizeof(E))));
+  const E *row;
+  long keys;
+  struct Part {
+    E4 value[4];
+    AKG_DEV float apply(float s, float factor, int r) const {
+      const E one = value[r >> 2][r & 3];
+      return with_mask<C>(s, factor, &one, 0);
+    }
+  };
+  AKG_DEV MaskRow(const void *mask, long at, long n) : row(static_cast<const E *>(mask) + at), keys(n) {}
+  AKG_DEV Part part(int j0, int half) const {
+    Part p;
+    if (j0 + 32 <= keys) {
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) p.value[r4] = *reinterpret_cast<const Unaligned *>(row + j0 + 8 * r4 + 4 * half);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = j0 + 8 * (r >> 2) + 4 * half + (r & 3);
+        p.value[r >> 2][r & 3] = row[j < keys ? j : keys - 1];   // (what lies behind the keys is not counted)
+      }
+    }
+    return p;
+  }
+};
 // 2^x or e^x of a difference of scores, and a row's log of the sum from its maximum and its sum.
 template <typename C>
 AKG_DEV float power(float x) {
@@ -304,34 +346,18 @@ struct FeedOrder {
   }
 };
 
-// The same with other work beside it: after every matrix instruction also VA vector instructions and TR transcendental ones.
-template <int MF, int RD, int LEAD, int VA, int TR, int M = 0>
-struct BesideOrder {
-  typedef FeedOrder<MF, RD, LEAD, M> F;
-  static AKG_DEV void emit() {
-    if constexpr (M == 0) __builtin_amdgcn_sched_group_barrier(0x100, F::kLead, 0);
-    if constexpr (M < MF) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if constexpr (F::kUpto > F::kFrom) __builtin_amdgcn_sched_group_barrier(0x100, F::kUpto - F::kFrom, 0);
-      if constexpr (VA > 0) __builtin_amdgcn_sched_group_barrier(0x002, VA, 0);
-      if constexpr (TR > 0) __builtin_amdgcn_sched_group_barrier(0x400, TR, 0);
-      BesideOrder<MF, RD, LEAD, VA, TR, M + 1>::emit();
-    }
-  }
-};
-
 // ---- forward ----------------------------------------------------------------------------------------------------------
 // SPLIT: the workgroup takes one of `splits` ranges of the keys and leaves accumulators, maximum and sum in `ws`.
 template <typename C, int NW, bool SPLIT>
 AKG_DEV void forward(const void *q, const void *k, const void *v, const void *mask, const int *qlens, const int *klens,
                      void *out, float *lse, float *ws, Extents e, float scale, int splits) {
   typedef typename C::T T;
-  constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, TV = padded(DV) / 32, kThreads = 64 * NW;
+  constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, TV = padded(DV) / 32, kThreads = 64 * NW, kGroup = kRows * NW;
   // A third tile of keys, where a CU holds one workgroup anyway, spares a barrier: what is being written no wavefront reads.
   constexpr int kKeyTiles = NW == 8 && kTile * (3 * pitch(DK) + 2 * pitch(DV)) <= 160 * 1024 ? 3 : 2;
   __shared__ __attribute__((aligned(16))) u8 ktiles[kKeyTiles][kTile * pitch(DK)], vtiles[2][kTile * pitch(DV)];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-  const long rows = e.sq * C::G, tiles = (rows + kRows * NW - 1) / (kRows * NW), heads = e.batch * C::HKV;
+  const long rows = e.sq * C::G, tiles = (rows + kGroup - 1) / kGroup, heads = e.batch * C::HKV;
   long id = blockIdx.x;
   const int split = SPLIT ? static_cast<int>(id % splits) : 0;
   if (SPLIT) id /= splits;
@@ -341,12 +367,9 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   const long b = head / C::HKV, hkv = head % C::HKV;
   const int ql = clamped_length<C>(qlens, b, e.sq), kl = clamped_length<C>(klens, b, e.sk);
 
-  const long row0 = tile * (kRows * NW), row = row0 + wave * kRows + (lane & 31);
-  const long i = row / C::G, g = row % C::G;
-  const bool exists = row < rows;
-  const int seen = exists ? keys_seen<C>(i, ql, kl) : 0;
+  const long row0 = tile * kGroup;
   // keys of the workgroup: those of its last row that has any
-  long last = (row0 + kRows * NW < rows ? row0 + kRows * NW : rows) - 1;
+  long last = (row0 + kGroup < rows ? row0 + kGroup : rows) - 1;
   long lastI = last / C::G;
   if (lastI >= ql) lastI = ql - 1;
   const int most = row0 / C::G < ql ? keys_seen<C>(lastI, ql, kl) : 0;
@@ -358,14 +381,17 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   }
 
   const RowsOf<C, DK> qrows(q, b, hkv, e);
+  const float c = C::ADDED ? scale : scale * kLog2e;
+  const long row = row0 + wave * kRows + (lane & 31), i = row / C::G;
+  const bool exists = row < rows;
+  const int seen = exists ? keys_seen<C>(i, ql, kl) : 0;
   u32x4 own[CK];
   load_own<DK>(qrows.base + qrows.offset(exists ? row : 0), seen > 0, lane, own);
-  const float c = C::ADDED ? scale : scale * kLog2e;
-
   f32x16 acc[TV];
 #pragma unroll
   for (int d = 0; d < TV; ++d) acc[d] = {};
   float top = neg_inf(), sum[2] = {0.0f, 0.0f};   // the row's maximum (or a little less); sums over this lane's keys
+  const MaskRow<C> maskRow(mask, C::MASK != 0 ? mask_row<C>(b, hkv * C::G + row % C::G, exists ? i : 0, e) : 0, e.sk);
 
   const KeysOf<C, DK> keys(k, b, hkv, e);
   const KeysOf<C, DV> values(v, b, hkv, e);
@@ -400,31 +426,19 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   }
   __syncthreads();
 
-  const long maskAt = C::MASK != 0 ? mask_row<C>(b, hkv * C::G + g, exists ? i : 0, e) : 0;
   f32x16 s;                 // scores of 32 keys
   float peak = neg_inf();   // the largest of them (of this lane's keys)
-  auto scores = [&](const u8 *kt, int row0) {
-    f32x16 to = {};
-#pragma unroll
-    for (int x = 0; x < CK; ++x) to = T::mma(kread.row(kt, row0, x), own[x], to);
-    return to;
-  };
-  // What the mask, the lengths and the causal order leave of the scores of the keys from j0 on.
+  typename MaskRow<C>::Part part, later;   // what the mask says of these 32 keys and the next (requested 64 keys ahead)
+  // What the mask, the lengths and the causal order leave of the scores of the keys from j0 on, and their largest.
   auto limit = [&](int j0, f32x16 &x) {
+    float m = neg_inf();
+    const bool ragged = __any(j0 + 32 > seen);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int j = j0 + 8 * (r >> 2) + 4 * half + (r & 3);
-      if (C::MASK != 0) {
-        x[r] = j < seen ? with_mask<C>(x[r], c, mask, maskAt + j) : neg_inf();
-      } else {
-        x[r] = j < seen ? x[r] : neg_inf();
-      }
+      if (C::MASK != 0) x[r] = part.apply(x[r], c, r);
+      if (ragged) x[r] = j0 + 8 * (r >> 2) + 4 * half + (r & 3) < seen ? x[r] : neg_inf();
+      m = __builtin_fmaxf(m, x[r]);
     }
-  };
-  auto largest = [&](const f32x16 &x) {
-    float m = x[0];
-#pragma unroll
-    for (int r = 1; r < 16; ++r) m = __builtin_fmaxf(m, x[r]);
     return m;
   };
   // The keys from j0 on, whose scores are in `s`: their probabilities, while the scores of the 32 keys behind them are
@@ -448,6 +462,10 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
       }
     }
     const float base = top == neg_inf() ? 0.0f : top;
+    if (C::MASK != 0) {
+      part = later;
+      later = maskRow.part(j0 + 64, half);
+    }
     // Probabilities are rounded to the type of the values for the matrix units (half a step of at most 2^-9 each, of
     // changing sign; the sum has them unrounded). A matrix instruction keeps its unit busy for 32 cycles and the issue for
     // four: a few vector instructions behind each of them, and operands read four ahead. (The barriers keep that order.)
@@ -480,21 +498,25 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
       acc[x % TV] = T::mma(t[x], p[x / TV], acc[x % TV]);
       if (x + kLead < 2 * TV) t[x + kLead] = vread.transposed(vt, vrow + 16 * ((x + kLead) / TV), (x + kLead) % TV);
 #pragma unroll
-      for (int r = x * kMost; r < 16 && r < (x + 1) * kMost; ++r) peak = __builtin_fmaxf(peak, next[r]);
+      for (int r = x * kMost; C::MASK == 0 && r < 16 && r < (x + 1) * kMost; ++r) peak = __builtin_fmaxf(peak, next[r]);
     }
     __builtin_amdgcn_sched_barrier(0);
     if (C::MASK != 0 || __any(j0 + 64 > seen)) {
       __builtin_amdgcn_sched_barrier(0);
-      limit(j0 + 32, next);
-      peak = largest(next);
+      peak = limit(j0 + 32, next);
     }
     s = next;
   };
   bool active = first < end && __any(first < seen);   // (wavefronts whose rows see nothing of a tile only help to fetch the next one)
   if (active) {
-    s = scores(ktiles[0], 0);
-    if (C::MASK != 0 || __any(first + 32 > seen)) limit(first, s);
-    peak = largest(s);
+    if (C::MASK != 0) {
+      part = maskRow.part(first, half);
+      later = maskRow.part(first + 32, half);
+    }
+    s = {};
+#pragma unroll
+    for (int x = 0; x < CK; ++x) s = T::mma(kread.row(ktiles[0], 0, x), own[x], s);
+    peak = limit(first, s);
   }
   int buf = 0, kbuf = 0;
   for (int k0 = first; k0 < end; k0 += kTile) {
@@ -552,9 +574,7 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
       *reinterpret_cast<u32x2 *>(to + 2 * at) = w;
     }
   }
-  if (lse != nullptr && half == 0) {
-    lse[(b * C::H + hkv * C::G + g) * e.sq + i] = log_sum<C>(top, all);
-  }
+  if (lse != nullptr && half == 0) lse[(b * C::H + hkv * C::G + row % C::G) * e.sq + i] = log_sum<C>(top, all);
 }
 
 // The ranges of a split joined: a thread takes four channels of a row.
