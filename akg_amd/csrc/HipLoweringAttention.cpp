@@ -280,7 +280,7 @@ class LayerEmitter {
 
   void attentionGrad() {
     const Sizes s = sizes(in(1), in(2), in(3));
-    const int nwq = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8), nwk = 4;
+    const int nwq = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8), nwk = 4, rg = std::max(s.dk, s.dv) > 128 ? 1 : 2;
     const int64_t tilesQ = ceilDiv(s.rows, 32 * nwq);
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n") << config(s, 6);
@@ -289,16 +289,16 @@ class LayerEmitter {
     std::ostringstream queries, keys;
     queries << "  akg::attn::backward_queries<akg_C, " << nwq << ">(" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << inName(3) << ", "
             << inName(4) << ", " << inName(5) << ", " << optionals(6) << ", " << outName(0) << ", akg_ws, " << extents << ", " << number(l_.scale) << ");\n";
-    keys << "  akg::attn::backward_keys<akg_C, " << nwk << ", " << nwq << ">(" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << inName(3)
+    keys << "  akg::attn::backward_keys<akg_C, " << nwk << ", " << rg << ", " << nwq << ">(" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << inName(3)
          << ", " << optionals(6) << ", " << outName(1) << ", " << outName(2) << ", akg_ws, " << extents << ", " << number(l_.scale) << ");\n";
     KernelPhase first;
     first.kernelName = g_.name + "_queries";
     first.grid[0] = checkGrid(s.keyHeads * tilesQ);
     first.block[0] = static_cast<unsigned>(64 * nwq);
     k_.earlierPhases.push_back(first);
-    o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(k_.kernelName, 64 * nwk, args, keys.str(), std::max(s.dk, s.dv) > 128 ? 0 : 2);
+    o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(k_.kernelName, 64 * nwk * rg, args, keys.str(), std::max(s.dk, s.dv) > 128 ? 0 : 2);
     k_.grid[0] = checkGrid(s.keyHeads * ceilDiv(s.sk, 32 * nwk));
-    k_.block[0] = static_cast<unsigned>(64 * nwk);
+    k_.block[0] = static_cast<unsigned>(64 * nwk * rg);
     // per row delta and its log-sum (in two parts for an added mask), per workgroup of the first kernel the largest |dout|
     const bool added = l_.hasMask && in(6).dtype != DType::Bool;
     k_.workspaceBytes = static_cast<uint64_t>(4 * s.keyHeads * ((added ? 3 : 2) * s.rows + tilesQ));

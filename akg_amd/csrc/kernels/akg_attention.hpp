@@ -830,29 +830,26 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
   }
 }
 
-// dk and dv of 32 keys a wavefront: the queries of all heads that share them pass by in tiles.
-template <typename C, int NW, int NWQ>
+// dk and dv of 32 keys a wavefront: the queries of all heads that share them pass by in tiles. RG groups of wavefronts have
+// the same keys and take the tiles of rows in turns; their sums are joined at the end, in LDS. (Causal: the first keys are
+// seen by all rows, and a workgroup that goes through them alone is the last to end.)
+template <typename C, int NW, int RG, int NWQ>
 AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const void *v, const void *mask,
                            const int *qlens, const int *klens, void *dk, void *dv, const float *ws, Extents e, float scale) {
   typedef typename C::T T;
-  constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, CV = (DV + 15) / 16, TK = padded(DK) / 32, TV = padded(DV) / 32, kThreads = 64 * NW;
+  constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, CV = (DV + 15) / 16, TK = padded(DK) / 32, TV = padded(DV) / 32, kThreads = 64 * NW * RG, kRound = kTileRows * RG;
   // From 192 channels on (keys and values together) the accumulators and the wavefront's own operands would leave room for
   // one wavefront per SIMD: its keys lie in LDS then, and two fit.
   constexpr bool kKeysInLds = padded(DK) + padded(DV) > 192;
-  __shared__ __attribute__((aligned(16))) u8 lds[2][kTileRows * (pitch(DK) + pitch(DV))];
+  __shared__ __attribute__((aligned(16))) u8 lds[2][kRound * (pitch(DK) + pitch(DV))];
   __shared__ __attribute__((aligned(16))) u8 ownKeys[kKeysInLds ? kRows * NW * own_pitch(DK) : 16];
   constexpr int kStates = C::ADDED ? 3 : 2;   // of a row: delta, top and rest (BackwardSpace)
-  __shared__ __attribute__((aligned(16))) float stateOf[2][kStates][kTileRows];
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  __shared__ __attribute__((aligned(16))) float stateOf[2][kStates][kRound];
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, group = __builtin_amdgcn_readfirstlane(tid >> 6) / NW, half = lane >> 5;
   const long rows = e.sq * C::G, heads = e.batch * C::HKV;
   long head, tile;
   head_and_tile(blockIdx.x, heads, head, tile);
-  // The first keys are seen by most queries, and come first. Where every workgroup finds a place at once, two to a CU, the
-  // second half goes by in reverse, so that the CUs with the longest ones get the shortest ones too.
-  if (C::CAUSAL && gridDim.x <= 512u) {
-    const long tiles = (e.sk + kRows * NW - 1) / (kRows * NW), first = (tiles + 1) / 2;
-    if (tile >= first) tile = tiles - 1 - (tile - first);
-  }
+  // (the first keys are seen by most queries, and come first)
   const long b = head / C::HKV, hkv = head % C::HKV;
   const int ql = clamped_length<C>(qlens, b, e.sq), kl = clamped_length<C>(klens, b, e.sk);
   const int key0 = static_cast<int>(tile) * (kRows * NW) + wave * kRows;
@@ -897,7 +894,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
   int from = 0;
   if (C::CAUSAL) {
     const int i = first0 - (kl - ql);
-    from = (i > 0 ? (i < ql ? i : ql) : 0) * C::G / kTileRows * kTileRows;
+    from = (i > 0 ? (i < ql ? i : ql) : 0) * C::G / kRound * kRound;
   }
   const int upto = first0 < kl ? ql * C::G : 0;
 
@@ -905,8 +902,8 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
   const RowsOf<C, DV> grows(dout, b, hkv, e);
   const Reader<DK> qread(lane);
   const Reader<DV> gread(lane);
-  TileLoad<kTileRows, DK, kThreads> qload;
-  TileLoad<kTileRows, DV, kThreads> gload;
+  TileLoad<kRound, DK, kThreads> qload;
+  TileLoad<kRound, DV, kThreads> gload;
   // Rows behind the last one read zeros (nothing is asked of memory): their probabilities are 1 and their products 0.
   float state[kStates];
   auto fetch = [&](int r0) {
@@ -920,23 +917,23 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     };
     qload.load(qb, tid, [&](int r) { return offsetIn(qrows, r); });
     gload.load(gb, tid, [&](int r) { return offsetIn(grows, r); });
-    if (tid < kTileRows) {
+    if (tid < kRound) {
 #pragma unroll
       for (int x = 0; x < kStates; ++x) state[x] = tid < left ? ws[x * heads * rows + head * rows + r0 + tid] : 0.0f;
     }
   };
   auto put = [&](int buf) {
     qload.store(lds[buf], tid);
-    gload.store(lds[buf] + kTileRows * pitch(DK), tid);
-    if (tid < kTileRows) {
+    gload.store(lds[buf] + kRound * pitch(DK), tid);
+    if (tid < kRound) {
 #pragma unroll
       for (int x = 0; x < kStates; ++x) stateOf[buf][x][tid] = state[x];
     }
   };
 #pragma unroll
   for (int buf = 0; buf < 2; ++buf) {
-    clear_padding<kTileRows, DK, kThreads>(lds[buf], tid);
-    clear_padding<kTileRows, DV, kThreads>(lds[buf] + kTileRows * pitch(DK), tid);
+    clear_padding<kRound, DK, kThreads>(lds[buf], tid);
+    clear_padding<kRound, DV, kThreads>(lds[buf] + kRound * pitch(DK), tid);
   }
   if (from < upto) {
     fetch(from);
@@ -944,11 +941,12 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
   }
   __syncthreads();
   int buf = 0;
-  for (int r0 = from; r0 < upto; r0 += kTileRows, buf ^= 1) {
-    const u8 *qt = lds[buf], *gt = lds[buf] + kTileRows * pitch(DK);
+  for (int round = from; round < upto; round += kRound, buf ^= 1) {
+    const int r0 = round + group * kTileRows, at0 = group * kTileRows;   // this group's tile
+    const u8 *qt = lds[buf] + at0 * pitch(DK), *gt = lds[buf] + kRound * pitch(DK) + at0 * pitch(DV);
     // the tile's last row sees most keys, its first one least
     const int lastRow = (r0 + kTileRows < upto ? r0 + kTileRows : upto) - 1;
-    const bool active = key0 < keys_seen<C>(lastRow / C::G, ql, kl);
+    const bool active = r0 < upto && key0 < keys_seen<C>(lastRow / C::G, ql, kl);
     u32x4 p[2], ds[2];
     if (active) {
       f32x16 s = {}, dp = {};
@@ -972,10 +970,10 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
       }
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        const f32x4 d4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][0][8 * r4 + 4 * half]);
-        const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][1][8 * r4 + 4 * half]);
+        const f32x4 d4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][0][at0 + 8 * r4 + 4 * half]);
+        const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][1][at0 + 8 * r4 + 4 * half]);
         f32x4 o4 = {};
-        if (C::ADDED) o4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][kStates - 1][8 * r4 + 4 * half]);
+        if (C::ADDED) o4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][kStates - 1][at0 + 8 * r4 + 4 * half]);
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
           const int r = 4 * r4 + z;
@@ -995,7 +993,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
         asm volatile("" : "+v"(p[x]), "+v"(ds[x]));   // (the scores end here: their registers hold the next tile's rows)
       }
     }
-    fetch(r0 + kTileRows);
+    fetch(round + kRound);
     if (active) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -1011,6 +1009,35 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     }
     put(buf ^ 1);
     __syncthreads();
+  }
+  // the groups' sums joined: group g leaves a few accumulators at a time where the tiles were, group 0 adds them
+  if constexpr (RG > 1) {
+    constexpr int kRegs = 16 * (TK + TV), kPart = sizeof(lds) / (64 * NW * (RG - 1) * 4) / 16 * 16 < kRegs ? sizeof(lds) / (64 * NW * (RG - 1) * 4) / 16 * 16 : kRegs;
+    float *parts = reinterpret_cast<float *>(&lds[0][0]);
+#pragma unroll
+    for (int p0 = 0; p0 < kRegs; p0 += kPart) {
+      __syncthreads();
+#pragma unroll
+      for (int x = p0; x < kRegs && x < p0 + kPart; ++x) {
+        if (group > 0) parts[(((group - 1) * kPart + x - p0) * NW + wave) * 64 + lane] = x < 16 * TK ? acck[x / 16 % TK][x % 16] : accv[(x - 16 * TK) / 16 % TV][x % 16];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int x = p0; x < kRegs && x < p0 + kPart; ++x) {
+        if (group == 0) {
+#pragma unroll
+          for (int g = 0; g < RG - 1; ++g) {
+            const float more = parts[((g * kPart + x - p0) * NW + wave) * 64 + lane];
+            if (x < 16 * TK) {
+              acck[x / 16 % TK][x % 16] += more;
+            } else {
+              accv[(x - 16 * TK) / 16 % TV][x % 16] += more;
+            }
+          }
+        }
+      }
+    }
+    if (group > 0) return;
   }
   if (key >= e.sk) return;
   const float back = scale / lift;
