@@ -231,6 +231,8 @@ class LayerEmitter {
     const int64_t first = s.sk - s.sq + 1, low = std::max<int64_t>(0, 1 - first), n = std::max<int64_t>(0, s.sq - low);
     return n * (first + low) + n * (n - 1) / 2;
   }
+  // Rows of a workgroup of attn::join (join_rows).
+  static int64_t joinRows(int64_t dv) { return 256 / (dv / 4 * (dv / 4 * 8 <= 256 ? 8 : 4)); }
   // Wavefronts of a workgroup that gives 32 rows to each: as many as keep every CU busy (a tile is fetched once for all of them).
   int waves(const Sizes &s, int most) const {
     int w = most;
@@ -263,7 +265,7 @@ class LayerEmitter {
       k_.earlierPhases.push_back(ranges);
       o << kernel(ranges.kernelName, 64 * nw, args, call(true));
       o << kernel(k_.kernelName, 256, args, "  akg::attn::join<akg_C>(akg_ws, " + outs + ", " + extents + ", static_cast<int>(akg_splits));\n");
-      k_.grid[0] = checkGrid(ceilDiv(s.keyHeads * s.rows * (s.dv / 4), 256));
+      k_.grid[0] = checkGrid(ceilDiv(s.keyHeads * s.rows, joinRows(s.dv)));
       k_.block[0] = 256;
       k_.workspaceBytes = static_cast<uint64_t>(splits * s.keyHeads * s.rows * (ceilDiv(s.dv, 32) * 32 + 2) * 4);
     } else {
@@ -330,7 +332,7 @@ class LayerEmitter {
     const std::string args = signature({"akg_batch", "akg_sq", "akg_blocks", "akg_per_sequence", "akg_splits"}, splits > 1);
     auto call = [&](bool split) {
       std::ostringstream c;
-      c << "  akg::attn::over_cache<akg_C, " << page << ", " << rt << ", " << flag(split) << ">(";
+      c << "  akg::attn::over_cache<akg_C, " << page << ", " << rt << ", " << flag(split) << ", " << flag(perSequence * page <= 128 * splits) << ">(";
       for (size_t i = 0; i < 7; ++i) c << inName(i) << ", ";
       c << outName(0) << ", " << (split ? "akg_ws" : "nullptr") << ", akg::attn::CacheExtents{akg_batch, akg_sq, akg_blocks, akg_per_sequence}, "
         << number(l_.scale) << ", static_cast<int>(akg_splits));\n";
@@ -345,7 +347,7 @@ class LayerEmitter {
       o << kernel(ranges.kernelName, 256, args, call(true))
         << kernel(k_.kernelName, 256, args, "  akg::attn::join<akg_C>(akg_ws, " + outName(0) +
                   ", nullptr, akg::attn::Extents{akg_batch, akg_sq, 0}, static_cast<int>(akg_splits));\n");
-      k_.grid[0] = checkGrid(ceilDiv(batch * kvHeads * rows * (dim / 4), 256));
+      k_.grid[0] = checkGrid(ceilDiv(batch * kvHeads * rows, joinRows(dim)));
       k_.workspaceBytes = static_cast<uint64_t>(splits * batch * kvHeads * rows * (ceilDiv(dim, 32) * 32 + 2) * 4);
     } else {
       o << kernel(k_.kernelName, 256, args, call(false));

@@ -62,9 +62,10 @@ struct CacheExtents {
   long batch, sq, pages, perSequence;   // sequences, queries of each, blocks in the pool, blocks of a sequence's table
 };
 
-// T: type of queries and results; RT: tiles of 16 rows of a workgroup; `splits` workgroups share the tokens of a
-// sequence (1: the result is written; more: accumulators, maximum and sum go to `ws` for attn::join).
-template <typename C, int PAGE, int RT, bool SPLIT>
+// RT: tiles of 16 rows of a workgroup; `splits` workgroups share the tokens of a sequence (1: the result is written; more:
+// accumulators, maximum and sum go to `ws` for attn::join). ONCE: every wavefront has a step of its own at most, so which
+// one it is need not wait for the length.
+template <typename C, int PAGE, int RT, bool SPLIT, bool ONCE>
 AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, const float *kscale, const float *vscale,
                         const int *table, const int *lengths, void *out, float *ws, CacheExtents e, float scale, int splits) {
   typedef typename C::T T;
@@ -89,7 +90,9 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
   long end = length - e.sq + lastRow / G + 1;
   if (end > length) end = length;
   long steps = end > 0 ? (end + kStep - 1) / kStep : 0, firstStep = 0;
-  if (SPLIT) {
+  if (ONCE) {
+    firstStep = static_cast<long>(split) * kWaves;
+  } else if (SPLIT) {
     const long each = (steps + splits - 1) / splits;
     firstStep = split * each < steps ? split * each : steps;
     steps = firstStep + each < steps ? firstStep + each : steps;
@@ -161,10 +164,9 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
   };
   // Page of the sixteen tokens from 32 step + 16 x on (-1: none, or outside the pool).
   auto page_of = [&](long step, int x) {
-    const long j = step * kStep + 16 * x;
-    if (step >= steps || j >= end) return -1L;
-    const long p = table[b * e.perSequence + j / PAGE];
-    return p >= 0 && p < e.pages ? p : -1L;
+    const long j = step * kStep + 16 * x, at = j / PAGE;
+    const long p = table[b * e.perSequence + (at < e.perSequence ? at : 0)];   // (asked for before the length is known)
+    return step < steps && j < end && p >= 0 && p < e.pages ? p : -1L;
   };
   auto fetch = [&](Step &s, long step, const long (&page)[2]) {
 #pragma unroll
@@ -206,12 +208,16 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
   Step now, next;
   long page[2] = {page_of(step, 0), page_of(step, 1)};
   if (step < steps) fetch(now, step, page);
-  page[0] = page_of(step + kWaves, 0);
-  page[1] = page_of(step + kWaves, 1);
+  if (!ONCE) {
+    page[0] = page_of(step + kWaves, 0);
+    page[1] = page_of(step + kWaves, 1);
+  }
   for (; step < steps; step += kWaves) {
-    if (step + kWaves < steps) fetch(next, step + kWaves, page);
-    page[0] = page_of(step + 2 * kWaves, 0);
-    page[1] = page_of(step + 2 * kWaves, 1);
+    if (!ONCE) {
+      if (step + kWaves < steps) fetch(next, step + kWaves, page);
+      page[0] = page_of(step + 2 * kWaves, 0);
+      page[1] = page_of(step + 2 * kWaves, 1);
+    }
     // scores of 2 x 16 tokens
     acc4 s[RT][2];
 #pragma unroll
@@ -298,6 +304,7 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
       column(IntTag<2>());
       column(IntTag<3>());
     }
+    if (ONCE) break;
     now = next;
   }
 
