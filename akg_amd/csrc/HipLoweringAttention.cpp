@@ -323,8 +323,13 @@ class LayerEmitter {
     const int64_t units = ceilDiv(dim, 64);
     const int64_t rt = std::min<int64_t>(ceilDiv(rows, 16), std::max<int64_t>(1, std::min<int64_t>(4, 8 / units)));
     const int64_t groups = batch * kvHeads * ceilDiv(rows, 16 * rt);
-    // workgroups that share a sequence: four to a CU, at least one step of 32 tokens for each of their four wavefronts
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({ceilDiv(4 * cus_, groups), ceilDiv(perSequence * page, 128), 64}));
+    // Workgroups that share a sequence: two to a CU, with at least one step of 32 tokens for each of their four wavefronts, and
+    // up to eight where each has 1024 tokens or more. us at two, four, eight to a CU: 16 x 2000 tokens (4 key heads of 64
+    // channels) 10.5, 11.7, 11.8; 32 x 8192 .. 16384 tokens (8 of 128) 180, 195, 174.
+    const int64_t tokens = perSequence * page;
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({std::max(ceilDiv(2 * cus_, groups), std::min(ceilDiv(8 * cus_, groups), tokens / 1024)),
+                                                                   ceilDiv(tokens, 128), 64}));
+    // (registers for three wavefronts a SIMD: 147 instead of 180, 195 -> 175 us in the second of these)
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n#include \"akg_cache_attention.hpp\"\n")
       << "typedef akg::attn::Config<" << trait() << ", " << dim << ", " << dim << ", " << kvHeads << ", " << group
@@ -332,7 +337,7 @@ class LayerEmitter {
     const std::string args = signature({"akg_batch", "akg_sq", "akg_blocks", "akg_per_sequence", "akg_splits"}, splits > 1);
     auto call = [&](bool split) {
       std::ostringstream c;
-      c << "  akg::attn::over_cache<akg_C, " << page << ", " << rt << ", " << flag(split) << ", " << flag(perSequence * page <= 128 * splits) << ">(";
+      c << "  akg::attn::over_cache<akg_C, " << page << ", " << rt << ", " << flag(split) << ", " << flag(tokens <= 128 * splits) << ">(";
       for (size_t i = 0; i < 7; ++i) c << inName(i) << ", ";
       c << outName(0) << ", " << (split ? "akg_ws" : "nullptr") << ", akg::attn::CacheExtents{akg_batch, akg_sq, akg_blocks, akg_per_sequence}, "
         << number(l_.scale) << ", static_cast<int>(akg_splits));\n";
@@ -344,13 +349,13 @@ class LayerEmitter {
       ranges.grid[0] = checkGrid(groups * splits);
       ranges.block[0] = 256;
       k_.earlierPhases.push_back(ranges);
-      o << kernel(ranges.kernelName, 256, args, call(true))
+      o << kernel(ranges.kernelName, 256, args, call(true), rt == 1 ? 3 : 0)
         << kernel(k_.kernelName, 256, args, "  akg::attn::join<akg_C>(akg_ws, " + outName(0) +
                   ", nullptr, akg::attn::Extents{akg_batch, akg_sq, 0}, static_cast<int>(akg_splits));\n");
       k_.grid[0] = checkGrid(ceilDiv(batch * kvHeads * rows, joinRows(dim)));
       k_.workspaceBytes = static_cast<uint64_t>(splits * batch * kvHeads * rows * (ceilDiv(dim, 32) * 32 + 2) * 4);
     } else {
-      o << kernel(k_.kernelName, 256, args, call(false));
+      o << kernel(k_.kernelName, 256, args, call(false), rt == 1 ? 3 : 0);
       k_.grid[0] = checkGrid(groups);
     }
     k_.block[0] = 256;
