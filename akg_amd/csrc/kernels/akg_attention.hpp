@@ -353,9 +353,9 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
                      void *out, float *lse, float *ws, Extents e, float scale, int splits) {
   typedef typename C::T T;
   constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, TV = padded(DV) / 32, kThreads = 64 * NW, kGroup = kRows * NW;
-  // A third tile of keys, where a CU holds one workgroup anyway, spares a barrier: what is being written no wavefront reads.
-  constexpr int kKeyTiles = NW == 8 && kTile * (3 * pitch(DK) + 2 * pitch(DV)) <= 160 * 1024 ? 3 : 2;
-  __shared__ __attribute__((aligned(16))) u8 ktiles[kKeyTiles][kTile * pitch(DK)], vtiles[2][kTile * pitch(DV)];
+  // A third tile, where a CU holds one workgroup anyway, spares a barrier: what is being written no wavefront reads.
+  constexpr int kTiles = NW == 8 && 3 * kTile * (pitch(DK) + pitch(DV)) <= 160 * 1024 ? 3 : 2;
+  __shared__ __attribute__((aligned(16))) u8 ktiles[kTiles][kTile * pitch(DK)], vtiles[kTiles][kTile * pitch(DV)];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const long rows = e.sq * C::G, tiles = (rows + kGroup - 1) / kGroup, heads = e.batch * C::HKV;
   long id = blockIdx.x;
@@ -399,30 +399,27 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   const Reader<DV> vread(lane);
   TileLoad<kTile, DK, kThreads> kload;
   TileLoad<kTile, DV, kThreads> vload;
-  // Keys are fetched a tile further ahead than values: while the probabilities of a tile are computed (vector instructions)
-  // the scores of the next one are (matrix instructions), in one stream.
-  auto fetch_keys = [&](int k0) {
+  auto fetch = [&](int k0) {
     // (rows behind the keys' length lie behind the descriptor and read zeros)
     const Buffer kb = make_buffer(keys.base + k0 * keys.step, records((kl - k0 - 1) * keys.step + 2 * DK));
-    kload.load(kb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(keys.step)); });
-  };
-  auto fetch_values = [&](int k0) {
     const Buffer vb = make_buffer(values.base + k0 * values.step, records((kl - k0 - 1) * values.step + 2 * DV));
+    kload.load(kb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(keys.step)); });
     vload.load(vb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(values.step)); });
   };
 #pragma unroll
-  for (int x = 0; x < kKeyTiles; ++x) clear_padding<kTile, DK, kThreads>(ktiles[x], tid);
-#pragma unroll
-  for (int x = 0; x < 2; ++x) clear_padding<kTile, DV, kThreads>(vtiles[x], tid);
-  if (first < end) {
-    fetch_keys(first);
-    fetch_values(first);
-    kload.store(ktiles[0], tid);
-    vload.store(vtiles[0], tid);
-    if (first + kTile < end) {
-      fetch_keys(first + kTile);
-      kload.store(ktiles[1], tid);
-    }
+  for (int x = 0; x < kTiles; ++x) {
+    clear_padding<kTile, DK, kThreads>(ktiles[x], tid);
+    clear_padding<kTile, DV, kThreads>(vtiles[x], tid);
+  }
+  if (first < end) {   // (two tiles, both asked for before the first is waited for)
+    fetch(first);
+    const TileLoad<kTile, DK, kThreads> know = kload;
+    const TileLoad<kTile, DV, kThreads> vnow = vload;
+    fetch(first + kTile < end ? first + kTile : kl);
+    know.store(ktiles[0], tid);
+    vnow.store(vtiles[0], tid);
+    kload.store(ktiles[1], tid);
+    vload.store(vtiles[1], tid);
   }
   __syncthreads();
 
@@ -518,23 +515,21 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
     for (int x = 0; x < CK; ++x) s = T::mma(kread.row(ktiles[0], 0, x), own[x], s);
     peak = limit(first, s);
   }
-  int buf = 0, kbuf = 0;
+  int buf = 0;
   for (int k0 = first; k0 < end; k0 += kTile) {
-    const bool more = k0 + kTile < end;
-    const int knext = kbuf + 1 < kKeyTiles ? kbuf + 1 : 0, kthen = kKeyTiles == 2 ? kbuf : knext + 1 < kKeyTiles ? knext + 1 : 0;
-    fetch_keys(k0 + 2 * kTile < end ? k0 + 2 * kTile : kl);   // (none left: zeros)
-    fetch_values(more ? k0 + kTile : kl);
+    const int next = buf + 1 < kTiles ? buf + 1 : 0, then = kTiles == 2 ? buf : next + 1 < kTiles ? next + 1 : 0;
+    fetch(k0 + 2 * kTile < end ? k0 + 2 * kTile : kl);   // (none left: zeros, nothing is asked of memory)
     if (active) {
-      step(k0, vtiles[buf], 0, ktiles[kbuf], 32);
-      step(k0 + 32, vtiles[buf], 32, ktiles[knext], 0);
-      active = more && __any(k0 + kTile < seen);
+      step(k0, vtiles[buf], 0, ktiles[buf], 32);
+      step(k0 + 32, vtiles[buf], 32, ktiles[next], 0);
+      active = k0 + kTile < end && __any(k0 + kTile < seen);
     }
-    if (kKeyTiles == 2) __syncthreads();   // (the tile written now was read in this round)
-    kload.store(ktiles[kthen], tid);
-    vload.store(vtiles[buf ^ 1], tid);
+    if (k0 + kTile >= end) break;
+    if (kTiles == 2) __syncthreads();   // (the tile written now was read in this round)
+    kload.store(ktiles[then], tid);
+    vload.store(vtiles[then], tid);
     __syncthreads();
-    kbuf = knext;
-    buf ^= 1;
+    buf = next;
   }
 
   const float all = add_halves(sum[0] + sum[1]);
