@@ -67,6 +67,19 @@ struct F16 {
   static AKG_DEV float high(u32 w) { return static_cast<float>(__builtin_bit_cast(pair, w)[1]); }
 };
 
+template <int N>
+struct IntTag {
+  static constexpr int value = N;
+};
+// f(0) ... f(N - 1) with constants: what a loop that the compiler may decide not to unroll cannot promise.
+template <int N, int I = 0, typename F>
+AKG_DEV void unrolled(F &&f) {
+  if constexpr (I < N) {
+    f(IntTag<I>());
+    unrolled<N, I + 1>(f);
+  }
+}
+
 constexpr float kLog2e = 0x1.715476p+0f, kLn2 = 0x1.62e430p-1f;
 constexpr int kRows = 32;      // rows of a wavefront
 constexpr int kTile = 64;      // keys of a tile (forward, dq)
@@ -678,13 +691,16 @@ struct BackwardSpace {
   AKG_DEV long largest() const { return (C::ADDED ? 3 : 2) * rows; }
 };
 
-// dq of 32 rows a wavefront: keys and values pass by in tiles. Leaves in `ws` what the kernel of dk and dv needs.
+// dq of 32 rows a wavefront: keys and values pass by in tiles, 32 keys a step: the scores and their gradients' products, then
+// the gradients of the scores (vector instructions) between the matrix instructions that multiply those of the step before.
+// Leaves in `ws` what the kernel of dk and dv needs.
 template <typename C, int NW>
 AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
                               const void *mask, const int *qlens, const int *klens, void *dq, float *ws, Extents e, float scale) {
   typedef typename C::T T;
   constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, CV = (DV + 15) / 16, TK = padded(DK) / 32, kThreads = 64 * NW;
-  __shared__ __attribute__((aligned(16))) u8 lds[2][kTile * (pitch(DK) + pitch(DV))];
+  constexpr int kTiles = NW == 8 && 3 * kTile * (pitch(DK) + pitch(DV)) + 64 <= 160 * 1024 ? 3 : 2;   // (as in the forward pass)
+  __shared__ __attribute__((aligned(16))) u8 ktiles[kTiles][kTile * pitch(DK)], vtiles[kTiles][kTile * pitch(DV)];
   __shared__ float largestOf[NW];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const long rows = e.sq * C::G, tiles = (rows + kRows * NW - 1) / (kRows * NW), heads = e.batch * C::HKV;
@@ -757,18 +773,20 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
     kload.load(kb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(keys.step)); });
     vload.load(vb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(values.step)); });
   };
-  auto put = [&](int buf) {
-    kload.store(lds[buf], tid);
-    vload.store(lds[buf] + kTile * pitch(DK), tid);
-  };
 #pragma unroll
-  for (int buf = 0; buf < 2; ++buf) {
-    clear_padding<kTile, DK, kThreads>(lds[buf], tid);
-    clear_padding<kTile, DV, kThreads>(lds[buf] + kTile * pitch(DK), tid);
+  for (int x = 0; x < kTiles; ++x) {
+    clear_padding<kTile, DK, kThreads>(ktiles[x], tid);
+    clear_padding<kTile, DV, kThreads>(vtiles[x], tid);
   }
   if (end > 0) {
     fetch(0);
-    put(0);
+    const TileLoad<kTile, DK, kThreads> know = kload;
+    const TileLoad<kTile, DV, kThreads> vnow = vload;
+    fetch(kTile < end ? kTile : kl);
+    know.store(ktiles[0], tid);
+    vnow.store(vtiles[0], tid);
+    kload.store(ktiles[1], tid);
+    vload.store(vtiles[1], tid);
   }
   __syncthreads();
   if (T::kNarrowRange && tid == 0) {
@@ -809,45 +827,105 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
     if (exists && half == 0) ws[space.rest(head * rows + row)] = rest;
   }
   if (exists && half == 0) ws[space.top(head * rows + row)] = sums;
-  int buf = 0;
-  for (int k0 = 0; k0 < end; k0 += kTile, buf ^= 1) {
-    const bool more = k0 + kTile < end;
-    if (more) fetch(k0 + kTile);
-    const u8 *kt = lds[buf], *vt = lds[buf] + kTile * pitch(DK);
-    if (__any(k0 < seen)) {
-      const bool ragged = __any(k0 + kTile > seen);
+  const MaskRow<C> maskRow(mask, maskAt, e.sk);
+  typename MaskRow<C>::Part part, later;   // what the mask says of 32 keys and the next (requested 64 keys ahead)
+  constexpr int kLead = 4;
+  f32x16 s, dp;
+  u32x4 ds[2];   // gradients of the scores of 32 keys, rounded (half a step of each, of changing sign)
+  // The scores of the keys from j0 on (rows `at` of the tiles) and the products dout v.
+  auto scores = [&](int j0, const u8 *kt, const u8 *vt, int at) {
+    if (C::MASK != 0) {
+      part = later;
+      later = maskRow.part(j0 + 32, half);
+    }
+    s = {};
+    dp = {};
+    u32x4 a[CK + CV];
+    auto operand = [&](auto x) {
+      constexpr int m = decltype(x)::value;
+      if constexpr (m < CK) {
+        return kread.row(kt, at, m);
+      } else {
+        return vread.row(vt, at, m - CK);
+      }
+    };
+    unrolled<(kLead < CK + CV ? kLead : CK + CV)>([&](auto x) { a[decltype(x)::value] = operand(x); });
+    unrolled<CK + CV>([&](auto x) {
+      constexpr int m = decltype(x)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (m < CK) {
+        s = T::mma(a[m], own[m], s);
+      } else {
+        dp = T::mma(a[m], grad[m - CK], dp);
+      }
+      if constexpr (m + kLead < CK + CV) a[m + kLead] = operand(IntTag<m + kLead>());
+    });
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        f32x16 s = {}, dp = {};
+    for (int r = 0; C::MASK != 0 && r < 16; ++r) s[r] = part.apply(s[r], c, r);
+    if (__any(j0 + 32 > seen)) {
+      __builtin_amdgcn_sched_barrier(0);   // (a branch, not a select for every tile)
 #pragma unroll
-        for (int x = 0; x < CK; ++x) s = T::mma(kread.row(kt, 32 * t, x), own[x], s);
-#pragma unroll
-        for (int x = 0; x < CV; ++x) dp = T::mma(vread.row(vt, 32 * t, x), grad[x], dp);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = k0 + 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
-          float x = s[r];
-          if (C::MASK != 0) {
-            x = j < seen ? with_mask<C>(x, c, mask, maskAt + j) - sums : neg_inf();
-            if (C::ADDED) x = __builtin_fmaf(x, kLog2e, -rest);
-          } else {
-            x = __builtin_fmaf(x, c, -sums);
-            if (ragged) x = j < seen ? x : neg_inf();
-          }
-          s[r] = __builtin_amdgcn_exp2f(x) * ((dp[r] - delta) * lift);
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          u32x4 p;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) p[w] = T::pack(s[8 * x + 2 * w], s[8 * x + 2 * w + 1]);
-#pragma unroll
-          for (int d = 0; d < TK; ++d) acc[d] = T::mma(kread.transposed(kt, 32 * t + 16 * x, d), p, acc[d]);
-        }
+      for (int r = 0; r < 16; ++r) {
+        const bool ok = j0 + 8 * (r >> 2) + 4 * half + (r & 3) < seen;
+        s[r] = ok ? s[r] : neg_inf();
+        dp[r] = ok ? dp[r] : 0.0f;
       }
     }
-    if (more) put(buf ^ 1);
+  };
+  auto pair = [&](int r, u32x4 (&to)[2]) {
+    float y[2];
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+      float x = C::MASK != 0 ? s[r + o] - sums : __builtin_fmaf(s[r + o], c, -sums);
+      if (C::ADDED) x = __builtin_fmaf(x, kLog2e, -rest);
+      y[o] = __builtin_amdgcn_exp2f(x) * (T::kNarrowRange ? (dp[r + o] - delta) * lift : dp[r + o] - delta);
+    }
+    u32 w = T::pack(y[0], y[1]);
+    asm volatile("" : "+v"(w));   // (computed here: left to itself the compiler moves it behind the matrix instructions)
+    to[r >> 3][(r >> 1) & 3] = w;
+  };
+  // The products of the step before (rows `at` of `kt`), and between them the gradients of the scores of this one (of whatever
+  // is there behind the last step: one stream without branches, or the accumulators are held twice).
+  auto products = [&](const u8 *kt, int at) {
+    u32x4 a[2 * TK], to[2];
+    auto operand = [&](int m) { return kread.transposed(kt, at + 16 * (m / TK), m % TK); };
+    unrolled<(kLead < 2 * TK ? kLead : 2 * TK)>([&](auto x) { a[decltype(x)::value] = operand(decltype(x)::value); });
+    unrolled<2 * TK>([&](auto x) {
+      constexpr int m = decltype(x)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      acc[m % TK] = T::mma(a[m], ds[m / TK], acc[m % TK]);
+      if constexpr (m + kLead < 2 * TK) a[m + kLead] = operand(m + kLead);
+      constexpr int from = m * 8 / (2 * TK), count = (m + 1) * 8 / (2 * TK) - from;   // of eight pairs
+      unrolled<count>([&](auto y) { pair(2 * (from + decltype(y)::value), to); });
+    });
+    __builtin_amdgcn_sched_barrier(0);
+    ds[0] = to[0];
+    ds[1] = to[1];
+  };
+  bool active = end > 0 && __any(0 < seen);   // (wavefronts whose rows see nothing of a tile only help to fetch the next one)
+  if (active) {
+    if (C::MASK != 0) later = maskRow.part(0, half);
+    scores(0, ktiles[0], vtiles[0], 0);
+    unrolled<8>([&](auto y) { pair(2 * decltype(y)::value, ds); });
+  }
+  int buf = 0;
+  for (int k0 = 0; k0 < end; k0 += kTile) {
+    const int next = buf + 1 < kTiles ? buf + 1 : 0, then = kTiles == 2 ? buf : next + 1 < kTiles ? next + 1 : 0;
+    fetch(k0 + 2 * kTile < end ? k0 + 2 * kTile : kl);   // (none left: zeros, nothing is asked of memory)
+    if (active) {
+      scores(k0 + 32, ktiles[buf], vtiles[buf], 32);
+      products(ktiles[buf], 0);
+      scores(k0 + kTile, ktiles[next], vtiles[next], 0);
+      products(ktiles[buf], 32);
+      active = __any(k0 + kTile < seen);
+    }
+    if (k0 + kTile >= end) break;
+    if (kTiles == 2) __syncthreads();   // (the tile written now was read in this round)
+    kload.store(ktiles[then], tid);
+    vload.store(vtiles[then], tid);
     __syncthreads();
+    buf = next;
   }
   if (!exists || dq == nullptr) return;
   const float back = scale / lift;

@@ -21,10 +21,6 @@ namespace akg {
 namespace attn {
 
 typedef f32x4 acc4;
-template <int N>
-struct IntTag {
-  static constexpr int value = N;
-};
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
 AKG_DEV acc4 mma16(u32x4 a, u32x4 b, acc4 c) {
