@@ -231,8 +231,12 @@ class LayerEmitter {
     const int64_t first = s.sk - s.sq + 1, low = std::max<int64_t>(0, 1 - first), n = std::max<int64_t>(0, s.sq - low);
     return n * (first + low) + n * (n - 1) / 2;
   }
-  // Rows of a workgroup of attn::join (join_rows).
-  static int64_t joinRows(int64_t dv) { return 256 / (dv / 4 * (dv / 4 * 8 <= 256 ? 8 : 4)); }
+  // Workspace of ranges that several workgroups share (attn::Ranges): `groups` counters, `rows` rows over all ranges.
+  static uint64_t rangesBytes(int64_t groups, int64_t rows, int64_t dv) {
+    const int64_t bytes = ceilDiv(groups * 4, 256) * 256 + rows * (ceilDiv(dv, 32) * 128 + 8);
+    if (bytes >= (1LL << 31)) throw LoweringError("the ranges' results take more than 2 GiB");
+    return static_cast<uint64_t>(bytes);
+  }
   // Wavefronts of a workgroup that gives 32 rows to each: as many as keep every CU busy (a tile is fetched once for all of them).
   int waves(const Sizes &s, int most) const {
     int w = most;
@@ -257,22 +261,10 @@ class LayerEmitter {
              optionals(3) + ", " + outs + ", " + (split ? "akg_ws" : "nullptr") + ", " + extents + ", " + number(l_.scale) + ", static_cast<int>(akg_splits));\n";
     };
     if (!wanted(0)) throw LoweringError("op " + op_.name + ": its first result must be an output");
-    if (splits > 1) {
-      KernelPhase ranges;
-      ranges.kernelName = g_.name + "_ranges";
-      ranges.grid[0] = checkGrid(groups * splits);
-      ranges.block[0] = static_cast<unsigned>(64 * nw);
-      k_.earlierPhases.push_back(ranges);
-      o << kernel(ranges.kernelName, 64 * nw, args, call(true));
-      o << kernel(k_.kernelName, 256, args, "  akg::attn::join<akg_C>(akg_ws, " + outs + ", " + extents + ", static_cast<int>(akg_splits));\n");
-      k_.grid[0] = checkGrid(ceilDiv(s.keyHeads * s.rows, joinRows(s.dv)));
-      k_.block[0] = 256;
-      k_.workspaceBytes = static_cast<uint64_t>(splits * s.keyHeads * s.rows * (ceilDiv(s.dv, 32) * 32 + 2) * 4);
-    } else {
-      o << kernel(k_.kernelName, 64 * nw, args, call(false));
-      k_.grid[0] = checkGrid(groups);
-      k_.block[0] = static_cast<unsigned>(64 * nw);
-    }
+    o << kernel(k_.kernelName, 64 * nw, args, call(splits > 1));
+    k_.grid[0] = checkGrid(groups * splits);
+    k_.block[0] = static_cast<unsigned>(64 * nw);
+    if (splits > 1) k_.workspaceBytes = rangesBytes(groups, splits * s.keyHeads * s.rows, s.dv);
     k_.source = o.str();
     k_.family = KernelFamily::Attention;
     k_.scalarArgs = {s.batch, s.sq, s.sk, splits};
@@ -343,21 +335,9 @@ class LayerEmitter {
         << number(l_.scale) << ", static_cast<int>(akg_splits));\n";
       return c.str();
     };
-    if (splits > 1) {
-      KernelPhase ranges;
-      ranges.kernelName = g_.name + "_ranges";
-      ranges.grid[0] = checkGrid(groups * splits);
-      ranges.block[0] = 256;
-      k_.earlierPhases.push_back(ranges);
-      o << kernel(ranges.kernelName, 256, args, call(true), rt == 1 ? 3 : 0)
-        << kernel(k_.kernelName, 256, args, "  akg::attn::join<akg_C>(akg_ws, " + outName(0) +
-                  ", nullptr, akg::attn::Extents{akg_batch, akg_sq, 0}, static_cast<int>(akg_splits));\n");
-      k_.grid[0] = checkGrid(ceilDiv(batch * kvHeads * rows, joinRows(dim)));
-      k_.workspaceBytes = static_cast<uint64_t>(splits * batch * kvHeads * rows * (ceilDiv(dim, 32) * 32 + 2) * 4);
-    } else {
-      o << kernel(k_.kernelName, 256, args, call(false), rt == 1 ? 3 : 0);
-      k_.grid[0] = checkGrid(groups);
-    }
+    o << kernel(k_.kernelName, 256, args, call(splits > 1), rt == 1 ? 3 : 0);
+    k_.grid[0] = checkGrid(groups * splits);
+    if (splits > 1) k_.workspaceBytes = rangesBytes(groups, splits * batch * kvHeads * rows, dim);
     k_.block[0] = 256;
     k_.source = o.str();
     k_.family = KernelFamily::Attention;

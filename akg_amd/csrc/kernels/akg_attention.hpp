@@ -359,8 +359,112 @@ struct FeedOrder {
   }
 };
 
+// ---- ranges of keys that several workgroups share -----------------------------------------------------------------------
+// Every range leaves accumulators, maximum and sum of its rows in the workspace; the workgroup that arrives last at the
+// counter of its rows joins them, in the order of the ranges whoever that is (a second launch cost 3 us more).
+// Workspace: the counters, to the next 256 bytes; accumulators [ranges][rows of all key heads][padded channels]; then
+// (maximum, sum) [ranges][rows].
+template <typename C>
+struct Ranges {
+  Buffer ws;
+  unsigned *counters;
+  long rows;      // of all key heads
+  int splits;
+  u32 accumulators, states;
+  AKG_DEV Ranges(float *workspace, long groups, long all, int n) : counters(reinterpret_cast<unsigned *>(workspace)), rows(all), splits(n) {
+    accumulators = static_cast<u32>((groups * 4 + 255) / 256 * 256);
+    states = accumulators + static_cast<u32>(n * all * padded(C::DV) * 4);
+    ws = make_buffer(workspace, states + n * all * 8L);   // (below 2 GiB: checked by the host)
+  }
+  AKG_DEV u32 accumulator(long s, long row, int d) const { return accumulators + static_cast<u32>(((s * rows + row) * padded(C::DV) + d) * 4); }
+  AKG_DEV u32 state(long s, long row) const { return states + static_cast<u32>((s * rows + row) * 8); }
+};
+
+// Rows row0 .. row0 + count - 1 (of one key head, `at` that of row0 among all) from their ranges. Of a row, a thread takes four
+// channels of every `sharers`-th range, four ranges requested at a time; sharers meet in LDS that the workgroup needs no more.
+template <int THREADS>
+struct Meeting {
+  f32x4 parts[THREADS];
+  float tops[THREADS], sums[THREADS];
+  unsigned flag;   // of last_workgroup
+};
+template <typename C, int THREADS>
+AKG_DEV void join(const Ranges<C> &in, Meeting<THREADS> &meet, long b, long hkv, long row0, long at, int count, void *out, float *lse,
+                  const Extents &e, int tid) {
+  typedef typename C::T T;
+  constexpr int DV = C::DV, kPer = DV / 4, kAtOnce = 4;
+  int sharers = 1;
+  while (sharers < 8 && 2 * sharers * kPer * count <= THREADS && 2 * sharers <= in.splits) sharers *= 2;
+  const int per = kPer * sharers, together = THREADS / per, first = tid % per / kPer, d = tid % kPer * 4;
+  const RowsOf<C, DV> orows(out, b, hkv, e);
+  for (int r0 = 0; r0 < count; r0 += together) {
+    const int r = r0 + tid / per;
+    const bool mine = tid < together * per && r < count;
+    float top = neg_inf(), sum = 0.0f;
+    f32x4 acc = {};
+    for (int s0 = first; mine && s0 < in.splits; s0 += sharers * kAtOnce) {
+      float x[kAtOnce][4], t[kAtOnce][2];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {   // (behind the last range: zeros)
+        const int s = s0 + u * sharers;
+        ws_load_chunk_if<2>(in.ws, s < in.splits, in.state(s, at + r), t[u]);
+        ws_load_chunk_if<4>(in.ws, s < in.splits, in.accumulator(s, at + r, d), x[u]);
+      }
+      float m = top;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (t[u][1] == 0.0f) {   // (a range without keys wrote no accumulators)
+          t[u][0] = neg_inf();
+#pragma unroll
+          for (int z = 0; z < 4; ++z) x[u][z] = 0.0f;
+        }
+        m = __builtin_fmaxf(m, t[u][0]);
+      }
+      const float base = m == neg_inf() ? 0.0f : m, old = power<C>(top - base);
+      top = m;
+      sum *= old;
+      acc *= old;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const float w = power<C>(t[u][0] - base);
+        sum = __builtin_fmaf(t[u][1], w, sum);
+#pragma unroll
+        for (int z = 0; z < 4; ++z) acc[z] = __builtin_fmaf(x[u][z], w, acc[z]);
+      }
+    }
+    if (sharers > 1) {
+      if (r0 > 0) __syncthreads();
+      meet.parts[tid] = acc;
+      meet.tops[tid] = top;
+      meet.sums[tid] = sum;
+      __syncthreads();
+      if (mine && first == 0) {
+        for (int g = 1; g < sharers; ++g) top = __builtin_fmaxf(top, meet.tops[tid + g * kPer]);
+        const float base = top == neg_inf() ? 0.0f : top;
+        sum = 0.0f;
+        acc = f32x4{};
+        for (int g = 0; g < sharers; ++g) {
+          const float w = power<C>(meet.tops[tid + g * kPer] - base);
+          sum = __builtin_fmaf(meet.sums[tid + g * kPer], w, sum);
+          const f32x4 x = meet.parts[tid + g * kPer];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) acc[z] = __builtin_fmaf(x[z], w, acc[z]);
+        }
+      }
+    }
+    if (!mine || first != 0) continue;
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const long row = row0 + r;
+    u32x2 w;
+    w[0] = T::pack(acc[0] * inverse, acc[1] * inverse);
+    w[1] = T::pack(acc[2] * inverse, acc[3] * inverse);
+    *reinterpret_cast<u32x2 *>(const_cast<char *>(orows.base) + orows.offset(row) + 2 * d) = w;
+    if (lse != nullptr && d == 0) lse[(b * C::H + hkv * C::G + row % C::G) * e.sq + row / C::G] = log_sum<C>(top, sum);
+  }
+}
+
 // ---- forward ----------------------------------------------------------------------------------------------------------
-// SPLIT: the workgroup takes one of `splits` ranges of the keys and leaves accumulators, maximum and sum in `ws`.
+// SPLIT: the workgroup takes one of `splits` ranges of the keys (Ranges).
 template <typename C, int NW, bool SPLIT>
 AKG_DEV void forward(const void *q, const void *k, const void *v, const void *mask, const int *qlens, const int *klens,
                      void *out, float *lse, float *ws, Extents e, float scale, int splits) {
@@ -368,7 +472,13 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, TV = padded(DV) / 32, kThreads = 64 * NW, kGroup = kRows * NW;
   // A third tile, where a CU holds one workgroup anyway, spares a barrier: what is being written no wavefront reads.
   constexpr int kTiles = NW == 8 && 3 * kTile * (pitch(DK) + pitch(DV)) <= 160 * 1024 ? 3 : 2;
-  __shared__ __attribute__((aligned(16))) u8 ktiles[kTiles][kTile * pitch(DK)], vtiles[kTiles][kTile * pitch(DV)];
+  struct Lds {
+    u8 ktiles[kTiles][kTile * pitch(DK)], vtiles[kTiles][kTile * pitch(DV)];
+  };
+  __shared__ __attribute__((aligned(16))) Lds lds;
+  static_assert(sizeof(Lds) >= sizeof(Meeting<kThreads>), "the join meets where the tiles were");
+  auto &ktiles = lds.ktiles;
+  auto &vtiles = lds.vtiles;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const long rows = e.sq * C::G, tiles = (rows + kGroup - 1) / kGroup, heads = e.batch * C::HKV;
   long id = blockIdx.x;
@@ -546,27 +656,30 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   }
 
   const float all = add_halves(sum[0] + sum[1]);
-  if (!exists) return;
   if (SPLIT) {
-    const long slot = (static_cast<long>(split) * heads + head) * rows + row;
-    float *to = ws + slot * padded(DV);
-    if (all > 0.0f || all != all) {
+    auto &meet = reinterpret_cast<Meeting<kThreads> &>(lds);
+    const Ranges<C> ranges(ws, heads * tiles, heads * rows, splits);
+    const long slot = head * rows + row;
+    if (exists) {
+      if (all > 0.0f || all != all) {
 #pragma unroll
-      for (int d = 0; d < TV; ++d) {
+        for (int d = 0; d < TV; ++d) {
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          *reinterpret_cast<f32x4 *>(to + 32 * d + 8 * r4 + 4 * half) =
-            f32x4{acc[d][4 * r4], acc[d][4 * r4 + 1], acc[d][4 * r4 + 2], acc[d][4 * r4 + 3]};
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const float x[4] = {acc[d][4 * r4], acc[d][4 * r4 + 1], acc[d][4 * r4 + 2], acc[d][4 * r4 + 3]};
+            ws_store_chunk<4>(ranges.ws, ranges.accumulator(split, slot, 32 * d + 8 * r4 + 4 * half), x);
+          }
         }
       }
+      const float state[2] = {top, all};
+      if (half == 0) ws_store_chunk<2>(ranges.ws, ranges.state(split, slot), state);
     }
-    if (half == 0) {
-      float *state = ws + static_cast<long>(splits) * heads * rows * padded(DV) + 2 * slot;
-      state[0] = top;
-      state[1] = all;
-    }
+    if (!last_workgroup(ranges.counters, id, splits, tid, &meet.flag)) return;
+    const long count = rows - row0 < kGroup ? rows - row0 : kGroup;
+    join<C, kThreads>(ranges, meet, b, hkv, row0, head * rows + row0, static_cast<int>(count), out, lse, e, tid);
     return;
   }
+  if (!exists) return;
   const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
   const RowsOf<C, DV> orows(out, b, hkv, e);
   char *to = const_cast<char *>(orows.base) + orows.offset(row);
@@ -583,85 +696,6 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
     }
   }
   if (lse != nullptr && half == 0) lse[(b * C::H + hkv * C::G + row % C::G) * e.sq + i] = log_sum<C>(top, all);
-}
-
-// The ranges of a split joined. A thread takes four channels of a row in every kSplits-th range, four ranges requested at a
-// time; the threads of a row meet in LDS. (One thread for all ranges waits for memory once per range: 12 us instead of 4 for
-// 15 ranges of 1024 rows.)
-constexpr int join_splits(int dv) { return dv / 4 * 8 <= 256 ? 8 : 4; }
-constexpr int join_rows(int dv) { return 256 / (dv / 4 * join_splits(dv)); }
-template <typename C>
-AKG_DEV void join(const float *ws, void *out, float *lse, Extents e, int splits) {
-  typedef typename C::T T;
-  constexpr int DV = C::DV, kPer = DV / 4, kSplits = join_splits(DV), kRowThreads = kPer * kSplits, kAtOnce = 4;
-  __shared__ __attribute__((aligned(16))) f32x4 parts[256];
-  __shared__ float tops[256], sums[256];
-  const int tid = static_cast<int>(threadIdx.x);
-  const long rows = e.sq * C::G, stride = e.batch * C::HKV * rows;
-  const long slot = static_cast<long>(blockIdx.x) * join_rows(DV) + tid / kRowThreads;
-  const bool mine = tid < join_rows(DV) * kRowThreads && slot < stride;
-  const int first = tid % kRowThreads / kPer, d = tid % kPer * 4;
-  const float *states = ws + static_cast<long>(splits) * stride * padded(DV) + 2 * slot, *from = ws + slot * padded(DV) + d;
-  float top = neg_inf(), sum = 0.0f;
-  f32x4 acc = {};
-  for (int s0 = first; mine && s0 < splits; s0 += kSplits * kAtOnce) {
-    f32x4 x[kAtOnce];
-    float t[kAtOnce], n[kAtOnce];
-#pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const int s = s0 + u * kSplits < splits ? s0 + u * kSplits : s0;
-      t[u] = states[2 * s * stride];
-      n[u] = states[2 * s * stride + 1];
-      x[u] = *reinterpret_cast<const f32x4 *>(from + s * stride * padded(DV));
-    }
-    float m = top;
-#pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      if (s0 + u * kSplits >= splits) n[u] = 0.0f;
-      if (n[u] == 0.0f) {   // (a range without keys wrote no accumulators)
-        t[u] = neg_inf();
-        x[u] = f32x4{};
-      }
-      m = __builtin_fmaxf(m, t[u]);
-    }
-    const float base = m == neg_inf() ? 0.0f : m, old = power<C>(top - base);
-    top = m;
-    sum *= old;
-    acc *= old;
-#pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const float w = power<C>(t[u] - base);
-      sum = __builtin_fmaf(n[u], w, sum);
-#pragma unroll
-      for (int z = 0; z < 4; ++z) acc[z] = __builtin_fmaf(x[u][z], w, acc[z]);
-    }
-  }
-  parts[tid] = acc;
-  tops[tid] = top;
-  sums[tid] = sum;
-  __syncthreads();
-  if (!mine || first != 0) return;
-#pragma unroll
-  for (int g = 1; g < kSplits; ++g) top = __builtin_fmaxf(top, tops[tid + g * kPer]);
-  const float base = top == neg_inf() ? 0.0f : top;
-  float all = 0.0f;
-  f32x4 y = {};
-#pragma unroll
-  for (int g = 0; g < kSplits; ++g) {
-    const float w = power<C>(tops[tid + g * kPer] - base);
-    all = __builtin_fmaf(sums[tid + g * kPer], w, all);
-    const f32x4 x = parts[tid + g * kPer];
-#pragma unroll
-    for (int z = 0; z < 4; ++z) y[z] = __builtin_fmaf(x[z], w, y[z]);
-  }
-  const float inverse = all == 0.0f ? 0.0f : 1.0f / all;
-  const long head = slot / rows, row = slot % rows, b = head / C::HKV, hkv = head % C::HKV;
-  const RowsOf<C, DV> orows(out, b, hkv, e);
-  u32x2 w;
-  w[0] = T::pack(y[0] * inverse, y[1] * inverse);
-  w[1] = T::pack(y[2] * inverse, y[3] * inverse);
-  *reinterpret_cast<u32x2 *>(const_cast<char *>(orows.base) + orows.offset(row) + 2 * d) = w;
-  if (lse != nullptr && d == 0) lse[(b * C::H + hkv * C::G + row % C::G) * e.sq + row / C::G] = log_sum<C>(top, all);
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------

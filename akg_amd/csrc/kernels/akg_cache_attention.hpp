@@ -59,7 +59,7 @@ struct CacheExtents {
 };
 
 // RT: tiles of 16 rows of a workgroup; `splits` workgroups share the tokens of a sequence (1: the result is written; more:
-// accumulators, maximum and sum go to `ws` for attn::join). ONCE: every wavefront has a step of its own at most, so which
+// Ranges). ONCE: every wavefront has a step of its own at most, so which
 // one it is need not wait for the length.
 template <typename C, int PAGE, int RT, bool SPLIT, bool ONCE>
 AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, const float *kscale, const float *vscale,
@@ -305,6 +305,7 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
   }
 
   // the four wavefronts joined, one tile of rows at a time; then thread (row, channels) writes
+  const Ranges<C> ranges(ws, e.batch * HKV * blocks, e.batch * HKV * rows, splits);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const float own = add_groups(sum[rt]);
@@ -334,7 +335,7 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
     }
     if (row < rows) {
       const long i = row / G, h = hkv * G + row % G;
-      const long slot = (static_cast<long>(split) * e.batch * HKV + head) * rows + row;
+      const long slot = head * rows + row;
       const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
       // 16 channel positions x 4 NU tiles: position m of tile 4 u + t is channel 4 NU m + 4 u + t (64 u + 4 m + t)
       for (int c = tid >> 4; c < 16 * NU; c += 16) {
@@ -349,18 +350,24 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
           for (int w = 0; w < kWaves; ++w) y[t] = __builtin_fmaf(parts[w][4 * u + t][m16][row16], weight[w], y[t]);
         }
         if (SPLIT) {
-          *reinterpret_cast<f32x4 *>(ws + slot * padded(D) + d) = f32x4{y[0], y[1], y[2], y[3]};
+          ws_store_chunk<4>(ranges.ws, ranges.accumulator(split, slot, d), y);
         } else {
           const u32x2 two = {T::pack(y[0] * inverse, y[1] * inverse), T::pack(y[2] * inverse, y[3] * inverse)};
           *reinterpret_cast<u32x2 *>(static_cast<char *>(out) + ((b * e.sq + i) * C::H + h) * (2L * D) + 2 * d) = two;
         }
       }
       if (SPLIT && tid < 16) {
-        float *state = ws + static_cast<long>(splits) * e.batch * HKV * rows * padded(D) + 2 * slot;
-        state[0] = m;
-        state[1] = total;
+        const float state[2] = {m, total};
+        ws_store_chunk<2>(ranges.ws, ranges.state(split, slot), state);
       }
     }
+  }
+  if (SPLIT) {
+    static_assert(sizeof(parts) >= sizeof(Meeting<64 * kWaves>), "the join meets where the wavefronts did");
+    auto &meet = reinterpret_cast<Meeting<64 * kWaves> &>(parts);
+    if (!last_workgroup(ranges.counters, id, splits, tid, &meet.flag)) return;
+    const long count = rows - row0 < 16 * RT ? rows - row0 : 16 * RT;
+    join<C, 64 * kWaves>(ranges, meet, b, hkv, row0, head * rows + row0, static_cast<int>(count), out, nullptr, Extents{e.batch, e.sq, 0}, tid);
   }
 }
 
