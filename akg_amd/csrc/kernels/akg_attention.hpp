@@ -552,13 +552,18 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   // What the mask, the lengths and the causal order leave of the scores of the keys from j0 on, and their largest.
   auto limit = [&](int j0, f32x16 &x) {
     float m = neg_inf();
-    const bool ragged = __any(j0 + 32 > seen);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      if (C::MASK != 0) x[r] = part.apply(x[r], c, r);
-      if (ragged) x[r] = j0 + 8 * (r >> 2) + 4 * half + (r & 3) < seen ? x[r] : neg_inf();
-      m = __builtin_fmaxf(m, x[r]);
+    for (int r = 0; C::MASK != 0 && r < 16; ++r) x[r] = part.apply(x[r], c, r);
+    if (__any(j0 + 32 > seen)) {
+      const int left = seen - j0 - 4 * half;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        x[r] = 8 * (r >> 2) + (r & 3) < left ? x[r] : neg_inf();
+        asm volatile("" : "+v"(x[r]));   // (a branch: the compiler would compare and select for every tile)
+      }
     }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m = __builtin_fmaxf(m, x[r]);
     return m;
   };
   // The keys from j0 on, whose scores are in `s`: their probabilities, while the scores of the 32 keys behind them are
