@@ -1122,6 +1122,16 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     u32x4 p[2], ds[2];
     if (active) {
       f32x16 s = {}, dp = {};
+      // (what the mask says is asked for before the scores are computed)
+      typename MaskRow<C>::E said[16];
+      if (C::MASK != 0) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int x = r0 + 8 * (r >> 2) + 4 * half + (r & 3), at = x < upto ? x : upto - 1;
+          said[r] = static_cast<const typename MaskRow<C>::E *>(mask)[mask_row<C>(b, hkv * C::G + at % C::G, at / C::G, e) + (counts ? key : 0)];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int x = 0; x < CK; ++x) s = T::mma(qread.row(qt, 0, x), kKeysInLds ? read_own<DK>(ownKeys, wave * kRows, x, lane) : own[kKeysInLds ? 0 : x], s);
 #pragma unroll
@@ -1134,7 +1144,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
           const int at = r0 + 8 * (r >> 2) + 4 * half + (r & 3), i = at / C::G;
           const bool ok = key < keys_seen<C>(i, ql, kl);
           if (C::MASK != 0) {
-            s[r] = ok ? with_mask<C>(s[r], c, mask, mask_row<C>(b, hkv * C::G + at % C::G, i, e) + key) : neg_inf();
+            s[r] = ok ? with_mask<C>(s[r], c, said, r) : neg_inf();
           } else {
             s[r] = ok ? s[r] : neg_inf();
           }
@@ -1182,33 +1192,34 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     put(buf ^ 1);
     __syncthreads();
   }
-  // the groups' sums joined: group g leaves a few accumulators at a time where the tiles were, group 0 adds them
+  // the groups' sums joined: group g leaves as many accumulators as fit where the tiles were, group 0 adds them
   if constexpr (RG > 1) {
-    constexpr int kRegs = 16 * (TK + TV), kPart = sizeof(lds) / (64 * NW * (RG - 1) * 4) / 16 * 16 < kRegs ? sizeof(lds) / (64 * NW * (RG - 1) * 4) / 16 * 16 : kRegs;
-    float *parts = reinterpret_cast<float *>(&lds[0][0]);
-#pragma unroll
-    for (int p0 = 0; p0 < kRegs; p0 += kPart) {
+    constexpr int kFit = static_cast<int>(sizeof(lds)) / (64 * NW * (RG - 1) * 16), kFours = 4 * (TK + TV), kPart = kFit < kFours ? kFit : kFours;
+    f32x4 *parts = reinterpret_cast<f32x4 *>(&lds[0][0]);
+    unrolled<(kFours + kPart - 1) / kPart>([&](auto pass) {
+      constexpr int p0 = decltype(pass)::value * kPart, kCount = kFours - p0 < kPart ? kFours - p0 : kPart;
       __syncthreads();
-#pragma unroll
-      for (int x = p0; x < kRegs && x < p0 + kPart; ++x) {
-        if (group > 0) parts[(((group - 1) * kPart + x - p0) * NW + wave) * 64 + lane] = x < 16 * TK ? acck[x / 16 % TK][x % 16] : accv[(x - 16 * TK) / 16 % TV][x % 16];
+      if (group > 0) {
+        unrolled<kCount>([&](auto y) {
+          constexpr int x = p0 + decltype(y)::value, r = 4 * (x % 4);
+          const f32x16 &acc = x < 4 * TK ? acck[x / 4 % TK] : accv[(x - 4 * TK) / 4 % TV];
+          parts[(((group - 1) * kPart + x - p0) * NW + wave) * 64 + lane] = f32x4{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]};
+        });
       }
       __syncthreads();
-#pragma unroll
-      for (int x = p0; x < kRegs && x < p0 + kPart; ++x) {
-        if (group == 0) {
+      if (group == 0) {
+        unrolled<kCount>([&](auto y) {
+          constexpr int x = p0 + decltype(y)::value, r = 4 * (x % 4);
+          f32x16 &acc = x < 4 * TK ? acck[x / 4 % TK] : accv[(x - 4 * TK) / 4 % TV];
 #pragma unroll
           for (int g = 0; g < RG - 1; ++g) {
-            const float more = parts[((g * kPart + x - p0) * NW + wave) * 64 + lane];
-            if (x < 16 * TK) {
-              acck[x / 16 % TK][x % 16] += more;
-            } else {
-              accv[(x - 16 * TK) / 16 % TV][x % 16] += more;
-            }
+            const f32x4 more = parts[((g * kPart + x - p0) * NW + wave) * 64 + lane];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) acc[r + z] += more[z];
           }
-        }
+        });
       }
-    }
+    });
     if (group > 0) return;
   }
   if (key >= e.sk) return;
