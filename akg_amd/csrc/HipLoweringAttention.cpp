@@ -274,7 +274,8 @@ class LayerEmitter {
 
   void attentionGrad() {
     const Sizes s = sizes(in(1), in(2), in(3));
-    const int nwq = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8), nwk = 4, rg = std::max(s.dk, s.dv) > 128 ? 1 : 2;
+    const int nwq = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8), rg = std::max(s.dk, s.dv) > 128 ? 1 : 2;
+    const int nwk = s.keyHeads * ceilDiv(s.sk, 128) < cus_ ? 2 : 4;
     const int64_t tilesQ = ceilDiv(s.rows, 32 * nwq);
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n") << config(s, 6);
@@ -290,7 +291,7 @@ class LayerEmitter {
     first.grid[0] = checkGrid(s.keyHeads * tilesQ);
     first.block[0] = static_cast<unsigned>(64 * nwq);
     k_.earlierPhases.push_back(first);
-    o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(k_.kernelName, 64 * nwk * rg, args, keys.str(), std::max(s.dk, s.dv) > 128 ? 0 : 2);
+    o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(k_.kernelName, 64 * nwk * rg, args, keys.str(), std::max(s.dk, s.dv) > 128 || nwk == 2 ? 0 : 2);
     k_.grid[0] = checkGrid(s.keyHeads * ceilDiv(s.sk, 32 * nwk));
     k_.block[0] = static_cast<unsigned>(64 * nwk * rg);
     // per row delta and its log-sum (in two parts for an added mask), per workgroup of the first kernel the largest |dout|
