@@ -884,15 +884,18 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
   }
   if (exists && half == 0) ws[space.top(head * rows + row)] = sums;
   const MaskRow<C> maskRow(mask, maskAt, e);
-  typename MaskRow<C>::Part part, later;   // what the mask says of 32 keys and the next (requested 64 keys ahead)
+  // What the mask says of 32 keys and the next, where registers allow.
+  constexpr bool kAhead = padded(DK) + padded(DV) <= 192 || sizeof(typename MaskRow<C>::E) < 4;
+  typename MaskRow<C>::Part part, later;
   constexpr int kLead = 4;
   f32x16 s, dp;
   u32x4 ds[2];   // gradients of the scores of 32 keys, rounded (half a step of each, of changing sign)
   // The scores of the keys from j0 on (rows `at` of the tiles) and the products dout v.
   auto scores = [&](int j0, const u8 *kt, const u8 *vt, int at) {
     if (C::MASK != 0) {
-      part = later;
-      later = maskRow.part(j0 + 32, half);
+      if (kAhead) part = later;
+      (kAhead ? later : part) = maskRow.part(kAhead ? j0 + 32 : j0, half);
+      if (!kAhead) __builtin_amdgcn_sched_barrier(0);
     }
     s = {};
     dp = {};
@@ -962,7 +965,7 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
   };
   bool active = end > 0 && __any(0 < seen);   // (wavefronts whose rows see nothing of a tile only help to fetch the next one)
   if (active) {
-    if (C::MASK != 0) later = maskRow.part(0, half);
+    if (C::MASK != 0 && kAhead) later = maskRow.part(0, half);
     scores(0, ktiles[0], vtiles[0], 0);
     unrolled<8>([&](auto y) { pair(2 * decltype(y)::value, ds); });
   }
