@@ -237,10 +237,37 @@ class LayerEmitter {
     if (bytes >= (1LL << 31)) throw LoweringError("the ranges' results take more than 2 GiB");
     return static_cast<uint64_t>(bytes);
   }
+  // The kernel `body` whose workgroups (`groups` of `groupRows` rows, times `splits`) share the keys' axis, and what joins
+  // their results: the last workgroup of a group, which saves a launch (attention of one query of 8 x 32/8 heads of 128 over 512
+  // keys 11.8 instead of 12.3 us), or, where that one would read more than 16 KiB alone, a launch of its own (2 x 16 queries
+  // over 8192 keys, 1 MiB a group: 27 instead of 87 us; 4 x 4 over 4096, 128 KiB: 21 instead of 28).
+  static constexpr int64_t kJoinInside = 16 << 10;
+  static bool joinsInside(int64_t groupRows, int64_t splits, int64_t dv) { return 4 * groupRows * splits * dv <= kJoinInside; }
+  void ranges(std::ostringstream &o, const std::string &args, const std::string &body, int threads, int hint, const std::string &joinExtents, const std::string &outs,
+              int64_t groups, int64_t groupRows, int64_t splits, int64_t keyHeads, int64_t rows, int64_t dv) {
+    k_.workspaceBytes = rangesBytes(groups, splits * keyHeads * rows, dv);
+    if (joinsInside(std::min(groupRows, rows), splits, dv)) {
+      o << kernel(k_.kernelName, threads, args, body, hint);
+      k_.grid[0] = checkGrid(groups * splits);
+      k_.block[0] = static_cast<unsigned>(threads);
+      return;
+    }
+    KernelPhase first;
+    first.kernelName = g_.name + "_ranges";
+    first.grid[0] = checkGrid(groups * splits);
+    first.block[0] = static_cast<unsigned>(threads);
+    k_.earlierPhases.push_back(first);
+    const int64_t joinRows = std::max<int64_t>(1, 256 / dv);
+    o << kernel(first.kernelName, threads, args, body, hint)
+      << kernel(k_.kernelName, 256, args, "  akg::attn::join_rows<akg_C, " + std::to_string(joinRows) + ", " + std::to_string(groupRows) + ">(akg_ws, " + outs + ", " +
+                joinExtents + ", static_cast<int>(akg_splits));\n");
+    k_.grid[0] = checkGrid(keyHeads * ceilDiv(rows, joinRows));
+    k_.block[0] = 256;
+  }
   // Wavefronts of a workgroup that gives 32 rows to each: as many as keep every CU busy (a tile is fetched once for all of them).
   int waves(const Sizes &s, int most) const {
     int w = most;
-    while (w > 1 && (s.rows <= 32 * (w / 2) || s.keyHeads * ceilDiv(s.rows, 32 * w) < cus_)) w /= 2;
+    while (w > 2 && (s.rows <= 32 * (w / 2) || s.keyHeads * ceilDiv(s.rows, 32 * w) < cus_)) w /= 2;
     return w;
   }
 
@@ -248,23 +275,26 @@ class LayerEmitter {
     const Sizes s = sizes(in(0), in(1), in(2));
     const int nw = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8);
     const int64_t groups = s.keyHeads * ceilDiv(s.rows, 32 * nw);
-    // few rows and a long axis of keys: several workgroups share it, at least four tiles of 64 each
+    // few rows and a long axis of keys: several workgroups share it, at least two tiles of 64 each
     int64_t splits = 1;
-    if (groups < cus_) splits = std::max<int64_t>(1, std::min<int64_t>({ceilDiv(2 * cus_, groups), s.sk / 256, 64}));
+    if (groups < cus_) splits = std::max<int64_t>(1, std::min<int64_t>({ceilDiv(2 * cus_, groups), s.sk / 128, 64}));
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n") << config(s, 3);
     const std::string args = signature({"akg_batch", "akg_sq", "akg_sk", "akg_splits"}, splits > 1);
     const std::string extents = "akg::attn::Extents{akg_batch, akg_sq, akg_sk}";
     const std::string outs = outName(0) + ", " + outName(1);
     auto call = [&](bool split) {
-      return "  akg::attn::forward<akg_C, " + std::to_string(nw) + ", " + flag(split) + ">(" + inName(0) + ", " + inName(1) + ", " + inName(2) + ", " +
-             optionals(3) + ", " + outs + ", " + (split ? "akg_ws" : "nullptr") + ", " + extents + ", " + number(l_.scale) + ", static_cast<int>(akg_splits));\n";
+      return "  akg::attn::forward<akg_C, " + std::to_string(nw) + ", " + flag(split) + ", " +
+             flag(split && joinsInside(std::min<int64_t>(32 * nw, s.rows), splits, s.dv)) + ">(" + inName(0) + ", " + inName(1) + ", " + inName(2) + ", " + optionals(3) + ", " + outs + ", " + (split ? "akg_ws" : "nullptr") + ", " + extents + ", " + number(l_.scale) + ", static_cast<int>(akg_splits));\n";
     };
     if (!wanted(0)) throw LoweringError("op " + op_.name + ": its first result must be an output");
-    o << kernel(k_.kernelName, 64 * nw, args, call(splits > 1));
-    k_.grid[0] = checkGrid(groups * splits);
-    k_.block[0] = static_cast<unsigned>(64 * nw);
-    if (splits > 1) k_.workspaceBytes = rangesBytes(groups, splits * s.keyHeads * s.rows, s.dv);
+    if (splits > 1) {
+      ranges(o, args, call(true), 64 * nw, 0, extents, outs, groups, 32 * nw, splits, s.keyHeads, s.rows, s.dv);
+    } else {
+      o << kernel(k_.kernelName, 64 * nw, args, call(false));
+      k_.grid[0] = checkGrid(groups);
+      k_.block[0] = static_cast<unsigned>(64 * nw);
+    }
     k_.source = o.str();
     k_.family = KernelFamily::Attention;
     k_.scalarArgs = {s.batch, s.sq, s.sk, splits};
@@ -330,16 +360,21 @@ class LayerEmitter {
     const std::string args = signature({"akg_batch", "akg_sq", "akg_blocks", "akg_per_sequence", "akg_splits"}, splits > 1);
     auto call = [&](bool split) {
       std::ostringstream c;
-      c << "  akg::attn::over_cache<akg_C, " << page << ", " << rt << ", " << flag(split) << ", " << flag(tokens <= 128 * splits) << ">(";
+      c << "  akg::attn::over_cache<akg_C, " << page << ", " << rt << ", " << flag(split) << ", " << flag(split && joinsInside(std::min(16 * rt, rows), splits, dim)) << ", "
+        << flag(tokens <= 128 * splits) << ">(";
       for (size_t i = 0; i < 7; ++i) c << inName(i) << ", ";
       c << outName(0) << ", " << (split ? "akg_ws" : "nullptr") << ", akg::attn::CacheExtents{akg_batch, akg_sq, akg_blocks, akg_per_sequence}, "
         << number(l_.scale) << ", static_cast<int>(akg_splits));\n";
       return c.str();
     };
-    o << kernel(k_.kernelName, 256, args, call(splits > 1), rt == 1 ? 3 : 0);
-    k_.grid[0] = checkGrid(groups * splits);
-    if (splits > 1) k_.workspaceBytes = rangesBytes(groups, splits * batch * kvHeads * rows, dim);
-    k_.block[0] = 256;
+    const int hint = rt == 1 ? 3 : 0;
+    if (splits > 1) {
+      ranges(o, args, call(true), 256, hint, "akg::attn::Extents{akg_batch, akg_sq, 0}", outName(0) + ", nullptr", groups, 16 * rt, splits, batch * kvHeads, rows, dim);
+    } else {
+      o << kernel(k_.kernelName, 256, args, call(false), hint);
+      k_.grid[0] = checkGrid(groups);
+      k_.block[0] = 256;
+    }
     k_.source = o.str();
     k_.family = KernelFamily::Attention;
     k_.scalarArgs = {batch, sq, blocks, perSequence, splits};

@@ -479,9 +479,18 @@ AKG_DEV void join(const Ranges<C> &in, Meeting<THREADS> &meet, long b, long hkv,
   }
 }
 
+// A launch of its own that joins, ROWS rows of a key head a workgroup; the ranges' workgroups had GROUP rows each.
+template <typename C, int ROWS, int GROUP>
+AKG_DEV void join_rows(float *ws, void *out, float *lse, const Extents &e, int splits) {
+  __shared__ Meeting<256> meet;
+  const long rows = e.sq * C::G, tiles = (rows + ROWS - 1) / ROWS, head = blockIdx.x / tiles, row0 = blockIdx.x % tiles * ROWS;
+  const Ranges<C> ranges(ws, e.batch * C::HKV * ((rows + GROUP - 1) / GROUP), e.batch * C::HKV * rows, splits);
+  join<C, 256>(ranges, meet, head / C::HKV, head % C::HKV, row0, head * rows + row0, static_cast<int>(rows - row0 < ROWS ? rows - row0 : ROWS), out, lse, e, static_cast<int>(threadIdx.x));
+}
+
 // ---- forward ----------------------------------------------------------------------------------------------------------
-// SPLIT: the workgroup takes one of `splits` ranges of the keys (Ranges).
-template <typename C, int NW, bool SPLIT>
+// SPLIT: the workgroup takes one of `splits` ranges of the keys (Ranges). JOIN: the last one joins them.
+template <typename C, int NW, bool SPLIT, bool JOIN>
 AKG_DEV void forward(const void *q, const void *k, const void *v, const void *mask, const int *qlens, const int *klens,
                      void *out, float *lse, float *ws, Extents e, float scale, int splits) {
   typedef typename C::T T;
@@ -696,7 +705,7 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
       const float state[2] = {top, all};
       if (half == 0) ws_store_chunk<2>(ranges.ws, ranges.state(split, slot), state);
     }
-    if (!last_workgroup(ranges.counters, id, splits, tid, &meet.flag)) return;
+    if (!JOIN || !last_workgroup(ranges.counters, id, splits, tid, &meet.flag)) return;
     const long count = rows - row0 < kGroup ? rows - row0 : kGroup;
     join<C, kThreads>(ranges, meet, b, hkv, row0, head * rows + row0, static_cast<int>(count), out, lse, e, tid);
     return;

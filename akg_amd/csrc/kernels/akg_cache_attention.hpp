@@ -59,9 +59,9 @@ struct CacheExtents {
 };
 
 // RT: tiles of 16 rows of a workgroup; `splits` workgroups share the tokens of a sequence (1: the result is written; more:
-// Ranges). ONCE: every wavefront has a step of its own at most, so which
-// one it is need not wait for the length.
-template <typename C, int PAGE, int RT, bool SPLIT, bool ONCE>
+// Ranges), and the last of them joins them (JOIN). ONCE: every wavefront has a step of its own at most, so which one it is
+// need not wait for the length.
+template <typename C, int PAGE, int RT, bool SPLIT, bool JOIN, bool ONCE>
 AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, const float *kscale, const float *vscale,
                         const int *table, const int *lengths, void *out, float *ws, CacheExtents e, float scale, int splits) {
   typedef typename C::T T;
@@ -365,7 +365,7 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
   if (SPLIT) {
     static_assert(sizeof(parts) >= sizeof(Meeting<64 * kWaves>), "the join meets where the wavefronts did");
     auto &meet = reinterpret_cast<Meeting<64 * kWaves> &>(parts);
-    if (!last_workgroup(ranges.counters, id, splits, tid, &meet.flag)) return;
+    if (!JOIN || !last_workgroup(ranges.counters, id, splits, tid, &meet.flag)) return;
     const long count = rows - row0 < 16 * RT ? rows - row0 : 16 * RT;
     join<C, 64 * kWaves>(ranges, meet, b, hkv, row0, head * rows + row0, static_cast<int>(count), out, nullptr, Extents{e.batch, e.sq, 0}, tid);
   }
