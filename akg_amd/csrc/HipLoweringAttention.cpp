@@ -305,33 +305,57 @@ class LayerEmitter {
   void attentionGrad() {
     const Sizes s = sizes(in(1), in(2), in(3));
     const int nwq = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8), rg = std::max(s.dk, s.dv) > 128 ? 1 : 2;
-    const int nwk = s.keyHeads * ceilDiv(s.sk, 128) < cus_ ? 2 : 4;
+    // A workgroup of the kernel of dk and dv has 128 keys. Where that leaves CUs idle it shares the rows with others, 512 of
+    // them each at least (causal: two to a CU, since the first keys have most rows), or has 64. us of the gradient unshared,
+    // shared: 1 x 1024 x 16/4 heads of 128, causal, 129, 75; 1 x 4096 x 32/4 918, 583; 8 x 200 x 12 heads of 64 with 128 keys
+    // and 64: 24.9, 23.7.
+    const int64_t groups128 = s.keyHeads * ceilDiv(s.sk, 128);
+    const int64_t splits = std::max<int64_t>(1, std::min((l_.causal ? 2 : 1) * cus_ / groups128, s.rows / 512));
+    const int nwk = splits > 1 || groups128 >= cus_ ? 4 : 2;
     const int64_t tilesQ = ceilDiv(s.rows, 32 * nwq);
+    const int64_t groups = s.keyHeads * ceilDiv(s.sk, 32 * nwk);
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n") << config(s, 6);
-    const std::string args = signature({"akg_batch", "akg_sq", "akg_sk"}, true);
-    const std::string extents = "akg::attn::Extents{akg_batch, akg_sq, akg_sk}";
+    std::vector<std::string> scalars = {"akg_batch", "akg_sq", "akg_sk"};
+    if (splits > 1) scalars.push_back("akg_splits");
+    const std::string args = signature(scalars, true);
+    const std::string extents = "akg::attn::Extents{akg_batch, akg_sq, akg_sk}", ranges = splits > 1 ? "static_cast<int>(akg_splits)" : "1";
     std::ostringstream queries, keys;
     queries << "  akg::attn::backward_queries<akg_C, " << nwq << ">(" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << inName(3) << ", "
             << inName(4) << ", " << inName(5) << ", " << optionals(6) << ", " << outName(0) << ", akg_ws, " << extents << ", " << number(l_.scale) << ");\n";
-    keys << "  akg::attn::backward_keys<akg_C, " << nwk << ", " << rg << ", " << nwq << ">(" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << inName(3)
-         << ", " << optionals(6) << ", " << outName(1) << ", " << outName(2) << ", akg_ws, " << extents << ", " << number(l_.scale) << ");\n";
+    keys << "  akg::attn::backward_keys<akg_C, " << nwk << ", " << rg << ", " << nwq << ", " << flag(splits > 1) << ">(" << inName(0) << ", " << inName(1) << ", "
+         << inName(2) << ", " << inName(3) << ", " << optionals(6) << ", " << outName(1) << ", " << outName(2) << ", akg_ws, " << extents << ", " << number(l_.scale) << ", "
+         << ranges << ");\n";
     KernelPhase first;
     first.kernelName = g_.name + "_queries";
     first.grid[0] = checkGrid(s.keyHeads * tilesQ);
     first.block[0] = static_cast<unsigned>(64 * nwq);
     k_.earlierPhases.push_back(first);
-    o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(k_.kernelName, 64 * nwk * rg, args, keys.str(), std::max(s.dk, s.dv) > 128 || nwk == 2 ? 0 : 2);
-    k_.grid[0] = checkGrid(s.keyHeads * ceilDiv(s.sk, 32 * nwk));
-    k_.block[0] = static_cast<unsigned>(64 * nwk * rg);
+    const std::string keysName = splits > 1 ? g_.name + "_keys" : k_.kernelName;
+    o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(keysName, 64 * nwk * rg, args, keys.str(), std::max(s.dk, s.dv) > 128 || nwk == 2 ? 0 : 2);
+    KernelPhase last;
+    last.grid[0] = checkGrid(groups * splits);
+    last.block[0] = static_cast<unsigned>(64 * nwk * rg);
     // per row delta and its log-sum (in two parts for an added mask), per workgroup of the first kernel the largest |dout|
     const bool added = l_.hasMask && in(6).dtype != DType::Bool;
     k_.workspaceBytes = static_cast<uint64_t>(4 * s.keyHeads * ((added ? 3 : 2) * s.rows + tilesQ));
+    if (splits > 1) {
+      last.kernelName = keysName;
+      k_.earlierPhases.push_back(last);
+      o << kernel(k_.kernelName, 256, args, "  akg::attn::backward_join<akg_C, " + std::to_string(nwq) + ">(akg_ws, " + outName(1) + ", " + outName(2) + ", " + extents +
+                  ", " + ranges + ");\n");
+      last.grid[0] = checkGrid(ceilDiv(s.keyHeads * s.sk * ((s.dk + s.dv) / 4), 256));
+      last.block[0] = 256;
+      k_.workspaceBytes = (k_.workspaceBytes + 255) / 256 * 256 + static_cast<uint64_t>(4 * splits * s.keyHeads * s.sk * 32 * (ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32)));
+    }
+    std::copy(last.grid, last.grid + 3, k_.grid);
+    std::copy(last.block, last.block + 3, k_.block);
     k_.source = o.str();
     k_.family = KernelFamily::Attention;
     k_.scalarArgs = {s.batch, s.sq, s.sk};
+    if (splits > 1) k_.scalarArgs.push_back(splits);
     k_.algorithmicOps = static_cast<uint64_t>((6 * s.dk + 4 * s.dv) * s.batch * s.heads * pairs(s, l_.causal));
-    k_.scheduleNote = "32 rows per wavefront, wavefronts " + std::to_string(nwq) + " (dq), " + std::to_string(nwk) + " (dk, dv)";
+    k_.scheduleNote = "32 rows per wavefront, wavefronts " + std::to_string(nwq) + " (dq), " + std::to_string(nwk) + " (dk, dv), row ranges " + std::to_string(splits);
   }
 
   // ---- CacheAttention -------------------------------------------------------------------------------------------------

@@ -754,6 +754,9 @@ struct BackwardSpace {
   AKG_DEV long top(long row) const { return rows + row; }
   AKG_DEV long rest(long row) const { return 2 * rows + row; }
   AKG_DEV long largest() const { return (C::ADDED ? 3 : 2) * rows; }
+  // behind them, to the next 256 bytes: sums of dk and dv over ranges of rows, [ranges][key heads][keys][padded channels of both]
+  static constexpr int kSums = padded(C::DK) + padded(C::DV);
+  AKG_DEV long sums(long workgroups) const { return (largest() + workgroups + 63) / 64 * 64; }
 };
 
 // dq of 32 rows a wavefront: keys and values pass by in tiles, 32 keys a step: the scores and their gradients' products, then
@@ -1017,9 +1020,11 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
 // dk and dv of 32 keys a wavefront: the queries of all heads that share them pass by in tiles. RG groups of wavefronts have
 // the same keys and take the tiles of rows in turns; their sums are joined at the end, in LDS. (Causal: the first keys are
 // seen by all rows, and a workgroup that goes through them alone is the last to end.)
-template <typename C, int NW, int RG, int NWQ>
+// SPLIT: where the tiles of keys are fewer than the CUs, `splits` workgroups take a range of the rows each and leave their
+// sums in `ws` for backward_join.
+template <typename C, int NW, int RG, int NWQ, bool SPLIT>
 AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const void *v, const void *mask,
-                           const int *qlens, const int *klens, void *dk, void *dv, const float *ws, Extents e, float scale) {
+                           const int *qlens, const int *klens, void *dk, void *dv, float *ws, Extents e, float scale, int splits) {
   typedef typename C::T T;
   constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, CV = (DV + 15) / 16, TK = padded(DK) / 32, TV = padded(DV) / 32, kThreads = 64 * NW * RG, kRound = kTileRows * RG;
   // From 192 channels on (keys and values together) the accumulators and the wavefront's own operands would leave room for
@@ -1031,8 +1036,10 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
   __shared__ __attribute__((aligned(16))) float stateOf[2][kStates][kRound];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, group = __builtin_amdgcn_readfirstlane(tid >> 6) / NW, half = lane >> 5;
   const long rows = e.sq * C::G, heads = e.batch * C::HKV;
+  const long id = SPLIT ? blockIdx.x / splits : blockIdx.x;
+  const int split = SPLIT ? static_cast<int>(blockIdx.x % splits) : 0;
   long head, tile;
-  head_and_tile(blockIdx.x, heads, head, tile);
+  head_and_tile(id, heads, head, tile);
   // (the first keys are seen by most queries, and come first)
   const long b = head / C::HKV, hkv = head % C::HKV;
   const int ql = clamped_length<C>(qlens, b, e.sq), kl = clamped_length<C>(klens, b, e.sk);
@@ -1080,7 +1087,13 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     const int i = first0 - (kl - ql);
     from = (i > 0 ? (i < ql ? i : ql) : 0) * C::G / kRound * kRound;
   }
-  const int upto = first0 < kl ? ql * C::G : 0;
+  int upto = first0 < kl ? ql * C::G : 0;
+  if (SPLIT && from < upto) {
+    const int rounds = (upto - from + kRound - 1) / kRound, each = (rounds + splits - 1) / splits * kRound;
+    const long start = from + static_cast<long>(split) * each;
+    from = start < upto ? static_cast<int>(start) : upto;
+    upto = from + each < upto ? from + each : upto;
+  }
 
   const RowsOf<C, DK> qrows(q, b, hkv, e);
   const RowsOf<C, DV> grows(dout, b, hkv, e);
@@ -1236,6 +1249,21 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
   }
   if (key >= e.sk) return;
   const float back = scale / lift;
+  if constexpr (SPLIT) {
+    const long tilesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ);
+    float *to = ws + space.sums(heads * tilesQ) + ((split * heads + head) * e.sk + key) * BackwardSpace<C>::kSums;
+#pragma unroll
+    for (int d = 0; d < TK + TV; ++d) {
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        f32x4 x;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) x[z] = d < TK ? acck[d % TK][4 * r4 + z] * back : accv[d < TK ? 0 : d - TK][4 * r4 + z];
+        *reinterpret_cast<f32x4 *>(to + 32 * d + 8 * r4 + 4 * half) = x;
+      }
+    }
+    return;
+  }
   auto store = [&](char *to, int dim, const f32x16 *acc, int tilesD, float factor) {
 #pragma unroll
     for (int d = 0; d < tilesD; ++d) {
@@ -1254,6 +1282,27 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
   const KeysOf<C, DV> dvalues(dv, b, hkv, e);
   if (dk != nullptr) store(const_cast<char *>(dkeys.base) + key * dkeys.step, DK, acck, TK, back);
   if (dv != nullptr) store(const_cast<char *>(dvalues.base) + key * dvalues.step, DV, accv, TV, 1.0f);
+}
+
+// dk and dv from the sums over ranges of rows, in their order: four channels a thread.
+template <typename C, int NWQ>
+AKG_DEV void backward_join(const float *ws, void *dk, void *dv, Extents e, int splits) {
+  typedef typename C::T T;
+  constexpr int DK = C::DK, DV = C::DV, kFours = (DK + DV) / 4, kSums = BackwardSpace<C>::kSums;
+  const long rows = e.sq * C::G, heads = e.batch * C::HKV, tilesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ);
+  const long at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x, row = at / kFours;
+  if (row >= heads * e.sk) return;
+  const int c = static_cast<int>(at % kFours) * 4;
+  const bool isK = c < DK;
+  const float *from = ws + BackwardSpace<C>{heads * rows}.sums(heads * tilesQ) + row * kSums + (isK ? c : padded(DK) + c - DK);
+  f32x4 sum = {};
+  for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const f32x4 *>(from + s * heads * e.sk * kSums);
+  const long head = row / e.sk, key = row % e.sk, b = head / C::HKV, hkv = head % C::HKV;
+  const KeysOf<C, DK> dkeys(dk, b, hkv, e);
+  const KeysOf<C, DV> dvalues(dv, b, hkv, e);
+  if ((isK ? dk : dv) == nullptr) return;
+  char *to = isK ? const_cast<char *>(dkeys.base) + key * dkeys.step + 2 * c : const_cast<char *>(dvalues.base) + key * dvalues.step + 2 * (c - DK);
+  *reinterpret_cast<u32x2 *>(to) = u32x2{T::pack(sum[0], sum[1]), T::pack(sum[2], sum[3])};
 }
 
 }  // namespace attn
