@@ -127,17 +127,8 @@ class LayerEmitter {
     std::vector<int64_t> heads;
     int64_t all = 0;
     for (size_t t = 0; t < tensors; ++t) {
-      heads.push_back(in(t).shape[headDim]);
+      heads.push_back(wanted(t) ? in(t).shape[headDim] : 0);
       all += heads.back();
-    }
-    // heads of a thread: the angles are computed once for them, as long as that leaves enough threads
-    int64_t each = 8;
-    while (each > 1 && batch * seq * chunks * ceilDiv(all, each) < static_cast<int64_t>(cus_) * 512) each /= 2;
-    std::vector<int64_t> groups;
-    int64_t allGroups = 0;
-    for (int64_t h : heads) {
-      groups.push_back(wanted(groups.size()) ? ceilDiv(h, each) : 0);
-      allGroups += groups.back();
     }
     const std::vector<uint64_t> rate = rates();
     std::ostringstream o;
@@ -147,10 +138,10 @@ class LayerEmitter {
     o << "};\n\n";
     std::ostringstream b;
     const bool perBatch = positions.shape.size() == 2 && positions.shape[0] == batch;
-    b << "  constexpr int P = " << pairs << ", CHUNKS = " << chunks << ", GROUPS = " << allGroups << ";\n"
+    b << "  constexpr int P = " << pairs << ", CHUNKS = " << chunks << ", HEADS = " << all << ";\n"
       << "  const long at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;\n"
-      << "  const long token = at / (CHUNKS * GROUPS);\n  if (token >= akg_batch * akg_seq) return;\n"
-      << "  const int rest = static_cast<int>(at % (CHUNKS * GROUPS)), chunk = rest % CHUNKS, group = rest / CHUNKS;\n"
+      << "  const long token = at / (CHUNKS * HEADS);\n  if (token >= akg_batch * akg_seq) return;\n"
+      << "  const int rest = static_cast<int>(at % (CHUNKS * HEADS)), chunk = rest % CHUNKS, head = rest / CHUNKS;\n"
       << "  const long b = token / akg_seq, s = token % akg_seq;\n"
       << "  const akg::u64 position = static_cast<akg::u64>(static_cast<long long>(" << inName(tensors) << "[" << (perBatch ? "token" : "s") << "]));\n"
       << "  float sine[P], cosine[P];\n#pragma unroll\n  for (int e = 0; e < P; ++e) {\n"
@@ -159,19 +150,19 @@ class LayerEmitter {
       << "    sine[e] *= " << number(l_.inverse ? -l_.magnitude : l_.magnitude) << ";\n    cosine[e] *= " << number(l_.magnitude) << ";\n  }\n";
     int64_t before = 0;
     for (size_t t = 0; t < tensors; ++t) {
-      if (groups[t] == 0) continue;
-      b << "  " << (before ? "else " : "") << "if (group < " << before + groups[t] << ") akg::rotary::turn<" << dtypeTag(x.dtype) << ", " << dim << ", " << r
-        << ", " << heads[t] << ", P, " << each << ", " << flag(l_.headsFirst) << ", " << flag(l_.interleaved) << ">(" << inName(t) << ", " << outName(t)
-        << ", b, s, akg_seq, (group - " << before << ") * " << each << ", chunk, sine, cosine);\n";
-      before += groups[t];
+      if (heads[t] == 0) continue;
+      b << "  " << (before ? "else " : "") << "if (head < " << before + heads[t] << ") akg::rotary::turn<" << dtypeTag(x.dtype) << ", " << dim << ", " << r
+        << ", " << heads[t] << ", P, " << flag(l_.headsFirst) << ", " << flag(l_.interleaved) << ">(" << inName(t) << ", " << outName(t)
+        << ", b, s, akg_seq, head - " << before << ", chunk, sine, cosine);\n";
+      before += heads[t];
     }
     o << kernel(k_.kernelName, 256, signature({"akg_batch", "akg_seq"}, false), b.str());
     k_.source = o.str();
     k_.family = KernelFamily::Rotary;
     k_.scalarArgs = {batch, seq};
-    k_.grid[0] = checkGrid(ceilDiv(batch * seq * chunks * allGroups, 256));
+    k_.grid[0] = checkGrid(ceilDiv(batch * seq * chunks * all, 256));
     k_.block[0] = 256;
-    k_.scheduleNote = "pairs per thread " + std::to_string(pairs) + ", heads per thread " + std::to_string(each);
+    k_.scheduleNote = "pairs per thread " + std::to_string(pairs);
   }
 
   // ---- Attention and its gradient -------------------------------------------------------------------------------------
