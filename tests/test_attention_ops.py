@@ -331,6 +331,45 @@ def test_cache_attention(case, tmp_path):
     close(got, r["out"], ref.cache_bound(r, case[0]), "cache attention")
 
 
+# ---- axes that several workgroups share, and masks of a few elements ----------------------------------------------------
+SHARED = [
+    ("bfloat16", "BSND", 1, 20, 1500, 16, 2, 128, 128, True, None, "padded"),   # 64 rows times 11 ranges of keys: joined by a launch of its own
+    ("float16", "BNSD", 2, 3, 700, 4, 4, 64, 64, False, "rows", None),          # 3 rows times 5 ranges: by the last workgroup
+    ("float16", "BSND", 1, 40, 900, 8, 1, 256, 256, False, "float32", None),
+    ("bfloat16", "BSND", 1, 33, 640, 6, 1, 8, 24, False, None, None),
+    ("bfloat16", "BSND", 1, 600, 600, 8, 2, 64, 64, True, None, "padded"),      # the gradients of keys and values: 2400 rows in 4 ranges
+    ("float16", "BNSD", 2, 520, 300, 4, 1, 96, 40, False, "bool", None),
+    ("float16", "BSND", 4, 300, 70, 8, 1, 256, 128, True, None, "zero"),
+    ("float16", "BSND", 1, 3, 5, 1, 1, 64, 64, False, "bool", None),            # a mask of 15 bytes
+    ("bfloat16", "BSND", 1, 1, 7, 2, 1, 16, 16, False, "float32", None),
+    ("float16", "BSND", 1, 2, 45, 1, 1, 64, 64, False, "float16", None),
+    ("bfloat16", "BSND", 2, 40, 33, 2, 2, 64, 64, False, "bool", None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SHARED, ids=lambda c: "-".join(str(x) for x in c))
+def test_shared_axes(case, tmp_path):
+    test_attention(case, tmp_path / "forward")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SHARED, ids=lambda c: "-".join(str(x) for x in c))
+def test_shared_axes_gradient(case, tmp_path):
+    test_attention_gradient(case, tmp_path / "gradient")
+
+
+@pytest.mark.gpu
+def test_a_shared_axis_gives_the_same_bits_every_time(tmp_path):
+    """The ranges are joined in their order, whichever workgroup ends last."""
+    for case in (SHARED[0], SHARED[1]):
+        t, extra, options, m, ql, kl = attention_case(case)
+        text, inputs = describe_attention(t, extra, options)
+        first = launch(text, inputs, tmp_path)
+        for _ in range(3):
+            assert all(torch.equal(x, y) for x, y in zip(first, launch(text, inputs, tmp_path)))
+
+
 # ---- refusals and what is chosen, without a GPU -----------------------------------------------------------------------
 def refused(text, code, part):
     with pytest.raises(driver.AkgHipError) as e:
