@@ -255,7 +255,10 @@ class LayerEmitter {
     k_.grid[0] = checkGrid(keyHeads * ceilDiv(rows, joinRows));
     k_.block[0] = 256;
   }
-  // Wavefronts of a workgroup that gives 32 rows to each: as many as keep every CU busy (a tile is fetched once for all of them).
+  // Wavefronts of a workgroup that gives 32 rows to each: as many as leave a workgroup for every CU (a tile is fetched once for
+  // all of them), two at least (the second one fetches even where it has no rows). us with eight, four, two, one: 2 x 4096 x
+  // 32/8 heads of 128 360, 384, -, -; 4 x 1000 x 1003 x 16 of 64 with a mask 49, 50, 68, 85; 1 x 1024 x 16 of 128 35, 35,
+  // 29, 35; 8 x 200 x 12 of 64 9.7, 9.1, 9.4, 10.4; one query over 8192 keys 56, 45, 45, 46.
   int waves(const Sizes &s, int most) const {
     int w = most;
     while (w > 2 && (s.rows <= 32 * (w / 2) || s.keyHeads * ceilDiv(s.rows, 32 * w) < cus_)) w /= 2;
@@ -266,7 +269,8 @@ class LayerEmitter {
     const Sizes s = sizes(in(0), in(1), in(2));
     const int nw = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8);
     const int64_t groups = s.keyHeads * ceilDiv(s.rows, 32 * nw);
-    // few rows and a long axis of keys: several workgroups share it, at least two tiles of 64 each
+    // Few rows and a long axis of keys: several workgroups share it, two to a CU (8 sequences over 8192 keys: 44 us; one to
+    // a CU 61), at least two tiles of 64 each (one query over 512 keys: 10.2 us; four tiles 13.1, one 11.4).
     int64_t splits = 1;
     if (groups < cus_) splits = std::max<int64_t>(1, std::min<int64_t>({ceilDiv(2 * cus_, groups), s.sk / 128, 64}));
     std::ostringstream o;
@@ -276,7 +280,8 @@ class LayerEmitter {
     const std::string outs = outName(0) + ", " + outName(1);
     auto call = [&](bool split) {
       return "  akg::attn::forward<akg_C, " + std::to_string(nw) + ", " + flag(split) + ", " +
-             flag(split && joinsInside(std::min<int64_t>(32 * nw, s.rows), splits, s.dv)) + ">(" + inName(0) + ", " + inName(1) + ", " + inName(2) + ", " + optionals(3) + ", " + outs + ", " + (split ? "akg_ws" : "nullptr") + ", " + extents + ", " + number(l_.scale) + ", static_cast<int>(akg_splits));\n";
+             flag(split && joinsInside(std::min<int64_t>(32 * nw, s.rows), splits, s.dv)) + ">(" + inName(0) + ", " + inName(1) + ", " + inName(2) + ", " +
+             optionals(3) + ", " + outs + ", " + (split ? "akg_ws" : "nullptr") + ", " + extents + ", " + number(l_.scale) + ", static_cast<int>(akg_splits));\n";
     };
     if (!wanted(0)) throw LoweringError("op " + op_.name + ": its first result must be an output");
     if (splits > 1) {

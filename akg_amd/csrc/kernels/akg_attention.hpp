@@ -490,6 +490,13 @@ AKG_DEV void join_rows(float *ws, void *out, float *lse, const Extents &e, int s
 
 // ---- forward ----------------------------------------------------------------------------------------------------------
 // SPLIT: the workgroup takes one of `splits` ranges of the keys (Ranges). JOIN: the last one joins them.
+//
+// Many rows are bound by the matrix units and by the issue of what stands beside them: 2 x 4096 queries and keys, 32 heads over
+// 8 of 128 channels, causal, bfloat16, take 299 us, 0.92 PFLOP/s (a matrix product of 8192 each way reaches 1.36); the
+// matrix instructions alone would take 215, the vector instructions alone 151. Few rows are bound by the keys and values from
+// memory: one query of 8 sequences over 8192 keys takes 51 us, 4.0 TB/s, and 44 where the last level cache still holds part
+// of them. Tried for both and left out: a second set of tiles under way (token 54, training unchanged), 64 rows a wavefront,
+// four wavefronts a workgroup and two workgroups a CU (training 382), raised wave priority around the matrix instructions.
 template <typename C, int NW, bool SPLIT, bool JOIN>
 AKG_DEV void forward(const void *q, const void *k, const void *v, const void *mask, const int *qlens, const int *klens,
                      void *out, float *lse, float *ws, Extents e, float scale, int splits) {
@@ -761,7 +768,8 @@ struct BackwardSpace {
 
 // dq of 32 rows a wavefront: keys and values pass by in tiles, 32 keys a step: the scores and their gradients' products, then
 // the gradients of the scores (vector instructions) between the matrix instructions that multiply those of the step before.
-// Leaves in `ws` what the kernel of dk and dv needs.
+// Leaves in `ws` what the kernel of dk and dv needs. Bound as the forward pass is: the training case there takes 417 us, 0.99
+// PFLOP/s of its three products (425 with the gradients of a step computed in front of its own products).
 template <typename C, int NW>
 AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
                               const void *mask, const int *qlens, const int *klens, void *dq, float *ws, Extents e, float scale) {
@@ -1021,7 +1029,8 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
 // the same keys and take the tiles of rows in turns; their sums are joined at the end, in LDS. (Causal: the first keys are
 // seen by all rows, and a workgroup that goes through them alone is the last to end.)
 // SPLIT: where the tiles of keys are fewer than the CUs, `splits` workgroups take a range of the rows each and leave their
-// sums in `ws` for backward_join.
+// sums in `ws` for backward_join. Two groups of wavefronts hide each other's vector instructions behind matrix instructions:
+// the training case of the forward pass takes 567 us, 0.97 PFLOP/s of its four products (one group: 930).
 template <typename C, int NW, int RG, int NWQ, bool SPLIT>
 AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const void *v, const void *mask,
                            const int *qlens, const int *klens, void *dk, void *dv, float *ws, Extents e, float scale, int splits) {

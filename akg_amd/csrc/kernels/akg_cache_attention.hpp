@@ -14,6 +14,10 @@
  * The scale of a key block multiplies the scores in float32. That of a value block multiplies the probabilities, which
  * are rounded to float16 behind it: relative to the power of two above the largest scale so far, so that they stay in
  * [0, 1] however small the scales are (the accumulators follow by exact powers of two).
+ *
+ * 32 sequences of 8192 to 16384 tokens, one query of 32 heads over 8 of 128 channels, take 168 us: 4.8 TB/s of the 5.2 that
+ * a copy reaches. Short ones wait for what depends on one another (length, block numbers, blocks, the other wavefronts, the
+ * other workgroups): 512 tokens of one sequence take 7.6 us, 16 x 2000 tokens 10.5.
  */
 #pragma once
 

@@ -5,8 +5,8 @@
  * Angles are counted in turns as 64-bit binary fractions: position * rate modulo 2^64 drops the whole turns exactly, so
  * an angle at position 2^31 is as good as one at 1 (a float32 product is off by hundredths of a turn from a million on).
  * What is left of a quarter turn goes through the Taylor series of sine and cosine on [-pi / 4, pi / 4], whose first
- * dropped terms are below 2^-28 there. Bound by memory: a thread turns the pairs of 16-byte accesses of one head (2 x 4096
- * tokens of 32 + 8 heads of 128 channels in bfloat16 take 60.5 us, 5.5 TB/s; with the angles computed once for two, four
+ * dropped terms are below 2^-28 there. Bound by memory: a thread turns the pairs of 16-byte accesses of one head (4 x 4096
+ * tokens of 32 + 8 heads of 128 channels in bfloat16 take 60 us, 5.6 TB/s; with the angles computed once for two, four
  * and eight heads a thread 61, 64 and 65 us: the arithmetic hides behind the accesses, the longer chains do not).
  */
 #pragma once
