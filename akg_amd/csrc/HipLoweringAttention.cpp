@@ -35,7 +35,6 @@ class LayerEmitter {
       case OpKind::AttentionGrad: attentionGrad(); break;
       default: cacheAttention(); break;
     }
-    for (const KernelPhase &p : k_.earlierPhases) checkGrid(p.grid[0]);
     k_.shapeArgs = lowering::buildShapeArgs(g_);
     if (k_.algorithmicBytes == 0) k_.algorithmicBytes = lowering::countAlgorithmicBytes(g_);
     return k_;
@@ -58,8 +57,9 @@ class LayerEmitter {
   }
   bool wanted(size_t j) const { return outName(j) != "nullptr"; }
 
-  static unsigned checkGrid(int64_t n) {
-    if (n <= 0 || n >= (1LL << 31)) throw LoweringError("more workgroups than a launch holds");
+  // (a launch has fewer than 2^32 threads)
+  static unsigned checkGrid(int64_t n, int64_t threads) {
+    if (n <= 0 || n * threads >= (1LL << 32)) throw LoweringError("more threads than a launch holds");
     return static_cast<unsigned>(n);
   }
   static std::string number(double v) {
@@ -160,7 +160,7 @@ class LayerEmitter {
     k_.source = o.str();
     k_.family = KernelFamily::Rotary;
     k_.scalarArgs = {batch, seq};
-    k_.grid[0] = checkGrid(ceilDiv(batch * seq * chunks * all, 256));
+    k_.grid[0] = checkGrid(ceilDiv(batch * seq * chunks * all, 256), 256);
     k_.block[0] = 256;
     k_.scheduleNote = "pairs per thread " + std::to_string(pairs);
   }
@@ -239,20 +239,20 @@ class LayerEmitter {
     k_.workspaceBytes = rangesBytes(groups, splits * keyHeads * rows, dv);
     if (joinsInside(std::min(groupRows, rows), splits, dv)) {
       o << kernel(k_.kernelName, threads, args, body, hint);
-      k_.grid[0] = checkGrid(groups * splits);
+      k_.grid[0] = checkGrid(groups * splits, threads);
       k_.block[0] = static_cast<unsigned>(threads);
       return;
     }
     KernelPhase first;
     first.kernelName = g_.name + "_ranges";
-    first.grid[0] = checkGrid(groups * splits);
+    first.grid[0] = checkGrid(groups * splits, threads);
     first.block[0] = static_cast<unsigned>(threads);
     k_.earlierPhases.push_back(first);
     const int64_t joinRows = std::max<int64_t>(1, 256 / dv);
     o << kernel(first.kernelName, threads, args, body, hint)
       << kernel(k_.kernelName, 256, args, "  akg::attn::join_rows<akg_C, " + std::to_string(joinRows) + ", " + std::to_string(groupRows) + ">(akg_ws, " + outs + ", " +
                 joinExtents + ", static_cast<int>(akg_splits));\n");
-    k_.grid[0] = checkGrid(keyHeads * ceilDiv(rows, joinRows));
+    k_.grid[0] = checkGrid(keyHeads * ceilDiv(rows, joinRows), 256);
     k_.block[0] = 256;
   }
   // Wavefronts of a workgroup that gives 32 rows to each: as many as leave a workgroup for every CU (a tile is fetched once for
@@ -288,7 +288,7 @@ class LayerEmitter {
       ranges(o, args, call(true), 64 * nw, 0, extents, outs, groups, 32 * nw, splits, s.keyHeads, s.rows, s.dv);
     } else {
       o << kernel(k_.kernelName, 64 * nw, args, call(false));
-      k_.grid[0] = checkGrid(groups);
+      k_.grid[0] = checkGrid(groups, 64 * nw);
       k_.block[0] = static_cast<unsigned>(64 * nw);
     }
     k_.source = o.str();
@@ -324,13 +324,13 @@ class LayerEmitter {
          << ranges << ");\n";
     KernelPhase first;
     first.kernelName = g_.name + "_queries";
-    first.grid[0] = checkGrid(s.keyHeads * tilesQ);
+    first.grid[0] = checkGrid(s.keyHeads * tilesQ, 64 * nwq);
     first.block[0] = static_cast<unsigned>(64 * nwq);
     k_.earlierPhases.push_back(first);
     const std::string keysName = splits > 1 ? g_.name + "_keys" : k_.kernelName;
     o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(keysName, 64 * nwk * rg, args, keys.str(), std::max(s.dk, s.dv) > 128 || nwk == 2 ? 0 : 2);
     KernelPhase last;
-    last.grid[0] = checkGrid(groups * splits);
+    last.grid[0] = checkGrid(groups * splits, 64 * nwk * rg);
     last.block[0] = static_cast<unsigned>(64 * nwk * rg);
     // per row delta and its log-sum (in two parts for an added mask), per workgroup of the first kernel the largest |dout|
     const bool added = l_.hasMask && in(6).dtype != DType::Bool;
@@ -340,7 +340,7 @@ class LayerEmitter {
       k_.earlierPhases.push_back(last);
       o << kernel(k_.kernelName, 256, args, "  akg::attn::backward_join<akg_C, " + std::to_string(nwq) + ">(akg_ws, " + outName(1) + ", " + outName(2) + ", " + extents +
                   ", " + ranges + ");\n");
-      last.grid[0] = checkGrid(ceilDiv(s.keyHeads * s.sk * ((s.dk + s.dv) / 4), 256));
+      last.grid[0] = checkGrid(ceilDiv(s.keyHeads * s.sk * ((s.dk + s.dv) / 4), 256), 256);
       last.block[0] = 256;
       k_.workspaceBytes = (k_.workspaceBytes + 255) / 256 * 256 + static_cast<uint64_t>(4 * splits * s.keyHeads * s.sk * 32 * (ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32)));
     }
@@ -392,7 +392,7 @@ class LayerEmitter {
       ranges(o, args, call(true), 256, hint, "akg::attn::Extents{akg_batch, akg_sq, 0}", outName(0) + ", nullptr", groups, 16 * rt, splits, batch * kvHeads, rows, dim);
     } else {
       o << kernel(k_.kernelName, 256, args, call(false), hint);
-      k_.grid[0] = checkGrid(groups);
+      k_.grid[0] = checkGrid(groups, 256);
       k_.block[0] = 256;
     }
     k_.source = o.str();

@@ -482,3 +482,19 @@ def test_few_rows_over_many_keys_are_split(tmp_path):
     def kernel(q, k):
         return driver.HipKernel(attention_text(q=(1, q, 4, 64), k=(1, k, 2, 64), v=(1, k, 2, 64)), out_dir=str(tmp_path))
     assert kernel(1, 8192).workspace_bytes > 0 and kernel(1, 200).workspace_bytes == 0
+
+
+def test_launches_of_too_many_threads_are_refused():
+    b = builder()
+    refused(b.dumps(op_desc.rotary_embedding(b, [b.input([1, 1 << 27, 32, 16], "float16")], b.input([1 << 27], "int32"))), -4, "more threads")
+    refused(attention_text(q=(1 << 22, 1, 16, 64), k=(1 << 22, 1, 16, 64), v=(1 << 22, 1, 16, 64)), -4, "more threads")
+
+
+def test_rows_of_the_gradient_are_shared_where_keys_are_few(tmp_path):
+    def kernel(s, h, hkv, batch=1):
+        b = builder()
+        dout, q, out = (b.input([batch, s, h, 64], "float16") for _ in range(3))
+        k, v = (b.input([batch, s, hkv, 64], "float16") for _ in range(2))
+        return driver.HipKernel(b.dumps(op_desc.attention_grad(b, dout, q, k, v, out, b.input([batch, h, s], "float32"))), out_dir=str(tmp_path))
+    assert "backward_join" in kernel(512, 8, 2).source
+    assert "backward_join" not in kernel(200, 4, 4).source and "backward_join" not in kernel(2048, 16, 16, 2).source
