@@ -82,8 +82,8 @@ struct KernelPhase {
 
 struct LoweredKernel {
   std::string kernelName;  // "<op>_kernel", as the reference names its outlined gpu.func
-  // Kernels of the same code object that run before `kernelName`, in this order (empty for all families but the
-  // grouped segment sum). Grid, block and name of the kernel proper stay in the fields below.
+  // Kernels of the same code object that run before `kernelName`, in this order (empty but for the grouped
+  // segment sum, attention's gradient and attention whose ranges of keys a launch of its own joins). Grid, block and name of the kernel proper stay in the fields below.
   std::vector<KernelPhase> earlierPhases;
   std::string source;      // HIP translation unit
   KernelFamily family = KernelFamily::Elementwise;

@@ -59,19 +59,23 @@ typedef struct akg_hip_tensor_desc {
 typedef struct akg_hip_kernel_info {
   char kernel_name[256];              /* "<op>_kernel" (KernelOutliningExt.cpp:433) */
   char family[32];                    /* "elementwise" | "row_reduce" | "stream_reduce" | "gemm_epilogue" | "indexed" | "segment_sum" |
+                                         "column_reduce" | "plane_reduce" | "gemm_rows" | "rotary" | "attention" |
                                          "staged" (a sequence of kernels of the other families; kernel_name, grid and
                                          block are those of the last one) */
   char operator_type[32];             /* fusion class, OperatorIdentify.cpp:51-93 */
   uint32_t grid[3];                   /* blockIdx.x/y/z extents, as written to <k>.json (of the kernel proper when
-                                         earlier launches precede it: segment sums over many positions) */
+                                         earlier launches precede it: segment sums over many positions,
+                                         attention's gradient, ranges of keys joined by a launch) */
   uint32_t block[3];                  /* threadIdx.x/y/z extents */
   uint64_t algorithmic_bytes;         /* bytes of every input and output, each counted once (an input that is only
                                          sliced or gathered from: the bytes taken out of it) */
-  uint64_t algorithmic_ops;           /* 2*M*N*K of the contraction, 0 for bandwidth-bound families */
+  uint64_t algorithmic_ops;           /* 2*M*N*K of the contraction (attention: of the products of all pairs of query
+                                         and key that full lengths leave), 0 for bandwidth-bound families */
   int32_t cache_hit;                  /* 1 if no device compilation was needed: the code object came from the
                                          artifact directory or from this process's memory (same source digest) */
   uint64_t workspace_bytes;           /* device scratch the handle owns per device (streaming reductions, GEMMs
-                                         with K split over workgroups, grouped segment sums), else 0 */
+                                         with K split over workgroups, grouped segment sums, attention's gradient and
+                                         attention whose keys several workgroups share), else 0 */
   double build_ms;                    /* wall time it took to make this handle: translation, lowering and, unless
                                          cache_hit, device compilation (a new shape set of a dynamic description that
                                          shares a code object costs about a millisecond, a device compilation ~0.5 s) */
