@@ -255,13 +255,23 @@ class LayerEmitter {
     k_.grid[0] = checkGrid(keyHeads * ceilDiv(rows, joinRows), 256);
     k_.block[0] = 256;
   }
-  // Wavefronts of a workgroup that gives 32 rows to each: as many as leave a workgroup for every CU (a tile is fetched once for
-  // all of them), two at least (the second one fetches even where it has no rows). us with eight, four, two, one: 2 x 4096 x
-  // 32/8 heads of 128 360, 384, -, -; 4 x 1000 x 1003 x 16 of 64 with a mask 49, 50, 68, 85; 1 x 1024 x 16 of 128 35, 35,
-  // 29, 35; 8 x 200 x 12 of 64 9.7, 9.1, 9.4, 10.4; one query over 8192 keys 56, 45, 45, 46.
+  // Wavefronts of a workgroup that gives 32 rows to each (a tile is fetched once for all of them), two at least: the second
+  // one fetches even where it has no rows (one query over 8192 keys with one wavefront 46 us, with two 44).
+  // Causal: as many as leave a workgroup for every CU, since rows differ in their keys and many small workgroups even that out
+  // (2 x 4096 x 32/8 heads of 128 with eight 360 us, four 384; 1 x 1024 x 16 of 128 with eight, four, two 35, 35, 29).
+  // Else the number that puts the fewest on the busiest SIMD: of equals the largest, or the smallest where that is one, which
+  // spreads them over most CUs (gradient of 8 x 5792 x 1 of 128: 184 workgroups of eight 536 us, 368 of four 640; of 4 x 2638 x
+  // 8/4 of 40: four 333, eight 347; attention of 3 x 478 x 8 of 40: two 17.0, four 16.5, eight 17.2).
   int waves(const Sizes &s, int most) const {
     int w = most;
-    while (w > 2 && (s.rows <= 32 * (w / 2) || s.keyHeads * ceilDiv(s.rows, 32 * w) < cus_)) w /= 2;
+    if (l_.causal) {
+      while (w > 2 && (s.rows <= 32 * (w / 2) || s.keyHeads * ceilDiv(s.rows, 32 * w) < cus_)) w /= 2;
+      return w;
+    }
+    auto load = [&](int n) { return ceilDiv(ceilDiv(s.keyHeads * ceilDiv(s.rows, 32 * n), cus_) * n, 4); };
+    for (int n = most / 2; n >= 2; n /= 2) {
+      if (load(n) < load(w) || load(n) == 1) w = n;
+    }
     return w;
   }
 
@@ -269,10 +279,13 @@ class LayerEmitter {
     const Sizes s = sizes(in(0), in(1), in(2));
     const int nw = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8);
     const int64_t groups = s.keyHeads * ceilDiv(s.rows, 32 * nw);
-    // Few rows and a long axis of keys: several workgroups share it, two to a CU (8 sequences over 8192 keys: 44 us; one to
-    // a CU 61), at least two tiles of 64 each (one query over 512 keys: 10.2 us; four tiles 13.1, one 11.4).
+    // Few rows and a long axis of keys: several workgroups share it, as many as two to a CU, or one of eight
+    // wavefronts (8 sequences over 8192 keys: 44 us; one to a CU 61), at least two tiles of 64 each (one query over 512 keys: 10.2 us; four tiles 13.1, one 11.4). A launch
+    // that joins has to be worth it (4 x 439 queries and keys of 8/4 heads of 96: 15.8 us, in two ranges 24.5; 2 x 5 queries
+    // over 759 keys of 32/4 of 64: 14.9 in two, 11.3 in five).
     int64_t splits = 1;
-    if (groups < cus_) splits = std::max<int64_t>(1, std::min<int64_t>({ceilDiv(2 * cus_, groups), s.sk / 128, 64}));
+    if (groups < cus_) splits = std::max<int64_t>(1, std::min<int64_t>({(nw == 8 ? 1 : 2) * cus_ / groups, s.sk / 128, 64}));
+    if (!joinsInside(std::min<int64_t>(32 * nw, s.rows), splits, s.dv) && s.sk - s.sk / splits < 512) splits = 1;
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n") << config(s, 3);
     const std::string args = signature({"akg_batch", "akg_sq", "akg_sk", "akg_splits"}, splits > 1);
@@ -303,11 +316,13 @@ class LayerEmitter {
     const int nwq = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8), rg = std::max(s.dk, s.dv) > 128 ? 1 : 2;
     // A workgroup of the kernel of dk and dv has 128 keys. Where that leaves CUs idle it shares the rows with others, 512 of
     // them each at least (causal: two to a CU, since the first keys have most rows), or has 64. us of the gradient unshared,
-    // shared: 1 x 1024 x 16/4 heads of 128, causal, 129, 75; 1 x 4096 x 32/4 918, 583; 8 x 200 x 12 heads of 64 with 128 keys
-    // and 64: 24.9, 23.7.
-    const int64_t groups128 = s.keyHeads * ceilDiv(s.sk, 128);
-    const int64_t splits = std::max<int64_t>(1, std::min((l_.causal ? 2 : 1) * cus_ / groups128, s.rows / 512));
-    const int nwk = splits > 1 || groups128 >= cus_ ? 4 : 2;
+    // shared: 1 x 1024 x 16/4 heads of 128, causal, 129, 75; 1 x 4096 x 32/4 918, 568; 8 x 200 x 12 heads of 64 with 128 keys
+    // and 64: 24.9, 23.7. A mask beside more than 64 channels leaves the registers of two wavefronts a SIMD too few: 64 keys
+    // and one (5 x 1773 x 8/4 heads of 96, causal, with a mask: 312, 240).
+    const bool crowded = l_.hasMask && ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32) > 4;
+    const int64_t whole = s.keyHeads * ceilDiv(s.sk, crowded ? 64 : 128);
+    const int64_t splits = std::max<int64_t>(1, std::min((l_.causal ? 2 : 1) * cus_ / whole, s.rows / 512));
+    const int nwk = !crowded && (splits > 1 || whole >= cus_) ? 4 : 2;
     const int64_t tilesQ = ceilDiv(s.rows, 32 * nwq);
     const int64_t groups = s.keyHeads * ceilDiv(s.sk, 32 * nwk);
     std::ostringstream o;
