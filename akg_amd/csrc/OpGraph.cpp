@@ -594,7 +594,7 @@ class GraphBuilder {
   static double numberAttr(const json::Value &attrs, const char *name, double otherwise) {
     const json::Value *a = findAttr(attrs, name);
     if (a == nullptr) return otherwise;
-    if (!a->isNumber()) throw TranslateError(std::string("attribute ") + name + " must be a number");
+    if (!a->isNumber() || !std::isfinite(a->asDouble())) throw TranslateError(std::string("attribute ") + name + " must be a finite number");
     return a->asDouble();
   }
   static bool boolAttr(const json::Value &attrs, const char *name) {
@@ -620,7 +620,10 @@ class GraphBuilder {
     if (node->kind == OpKind::RotaryEmbedding) {
       l.base = numberAttr(attrs, "base", 10000.0);
       l.magnitude = numberAttr(attrs, "magnitude", 1.0);
-      l.rotaryDims = static_cast<int64_t>(numberAttr(attrs, "rotary_dims", 0.0));
+      const double dims = numberAttr(attrs, "rotary_dims", 0.0);
+      if (!(dims >= 0.0 && dims < 2147483648.0) || dims != std::floor(dims)) throw TranslateError(at + "rotary_dims must be a whole number");
+      l.rotaryDims = static_cast<int64_t>(dims);
+      if (std::fabs(l.magnitude) > 0x1p100) throw TranslateError(at + "magnitude must be at most 2^100");
       l.interleaved = boolAttr(attrs, "interleaved");
       l.inverse = boolAttr(attrs, "inverse");
       const std::string scaling = textAttr(attrs, "scaling", "none");
@@ -643,7 +646,9 @@ class GraphBuilder {
       return node->inputs.size();
     }
     l.scale = numberAttr(attrs, "scale", 0.0);
-    if (findAttr(attrs, "scale") != nullptr && !(l.scale > 0.0)) throw TranslateError(at + "scale must be above 0");
+    if (findAttr(attrs, "scale") != nullptr && !(l.scale >= 0x1p-100 && l.scale <= 0x1p100)) {   // (in float32 neither 0 nor infinite)
+      throw TranslateError(at + "scale must be above 0, from 2^-100 to 2^100");
+    }
     if (node->kind == OpKind::CacheAttention) {
       if (l.headsFirst) throw TranslateError(at + "layout must be BSND");
       return 7;

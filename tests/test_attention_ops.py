@@ -498,3 +498,20 @@ def test_rows_of_the_gradient_are_shared_where_keys_are_few(tmp_path):
         return driver.HipKernel(b.dumps(op_desc.attention_grad(b, dout, q, k, v, out, b.input([batch, h, s], "float32"))), out_dir=str(tmp_path))
     assert "backward_join" in kernel(512, 8, 2).source
     assert "backward_join" not in kernel(200, 4, 4).source and "backward_join" not in kernel(2048, 16, 16, 2).source
+
+
+def test_attributes_that_no_float_holds_are_refused():
+    def turned(**changes):
+        b = builder()
+        doc = json.loads(b.dumps(op_desc.rotary_embedding(b, [b.input([2, 5, 4, 64], "float16")], b.input([5], "int32"),
+                                                         scaling={"kind": "linear", "factor": 2.0})))
+        for a in doc["op_desc"][0]["attr"]:
+            a["value"] = changes.get(a["name"], a["value"])
+        return json.dumps(doc)
+    driver.translate(turned())
+    for name, value in (("rotary_dims", 62.5), ("rotary_dims", 1e30), ("rotary_dims", -2), ("magnitude", 1e300), ("magnitude", -1e39), ("base", math.inf),
+                        ("base", math.nan), ("factor", math.inf)):
+        refused(turned(**{name: value}), -3, name)
+    for scale in (1e300, 1e-60, 0.0, -1.0, math.inf, math.nan):
+        refused(attention_text(scale=scale), -3, "scale")
+    driver.translate(attention_text(scale=2.0 ** -100))
