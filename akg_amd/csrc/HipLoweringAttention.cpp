@@ -320,6 +320,7 @@ class LayerEmitter {
     // and 64: 24.9, 23.7. A mask beside more than 64 channels leaves the registers of two wavefronts a SIMD too few: 64 keys
     // and one (5 x 1773 x 8/4 heads of 96, causal, with a mask: 312, 240).
     const bool crowded = l_.hasMask && ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32) > 4;
+    const bool apart = ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32) > 8;   // (dk and dv by workgroups of their own)
     const int64_t whole = s.keyHeads * ceilDiv(s.sk, crowded ? 64 : 128);
     const int64_t splits = std::max<int64_t>(1, std::min((l_.causal ? 2 : 1) * cus_ / whole, s.rows / 512));
     const int nwk = !crowded && (splits > 1 || whole >= cus_) ? 4 : 2;
@@ -334,7 +335,7 @@ class LayerEmitter {
     std::ostringstream queries, keys;
     queries << "  akg::attn::backward_queries<akg_C, " << nwq << ">(" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << inName(3) << ", "
             << inName(4) << ", " << inName(5) << ", " << optionals(6) << ", " << outName(0) << ", akg_ws, " << extents << ", " << number(l_.scale) << ");\n";
-    keys << "  akg::attn::backward_keys<akg_C, " << nwk << ", " << rg << ", " << nwq << ", " << flag(splits > 1) << ">(" << inName(0) << ", " << inName(1) << ", "
+    keys << "  akg::attn::backward_keys<akg_C, " << nwk << ", " << rg << ", " << nwq << ", " << flag(splits > 1) << ", " << flag(apart) << ">(" << inName(0) << ", " << inName(1) << ", "
          << inName(2) << ", " << inName(3) << ", " << optionals(6) << ", " << outName(1) << ", " << outName(2) << ", akg_ws, " << extents << ", " << number(l_.scale) << ", "
          << ranges << ");\n";
     KernelPhase first;
@@ -345,7 +346,7 @@ class LayerEmitter {
     const std::string keysName = splits > 1 ? g_.name + "_keys" : k_.kernelName;
     o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(keysName, 64 * nwk * rg, args, keys.str(), std::max(s.dk, s.dv) > 128 || nwk == 2 ? 0 : 2);
     KernelPhase last;
-    last.grid[0] = checkGrid(groups * splits, 64 * nwk * rg);
+    last.grid[0] = checkGrid((apart ? 2 : 1) * groups * splits, 64 * nwk * rg);
     last.block[0] = static_cast<unsigned>(64 * nwk * rg);
     // per row delta and its log-sum (in two parts for an added mask), per workgroup of the first kernel the largest |dout|
     const bool added = l_.hasMask && in(6).dtype != DType::Bool;

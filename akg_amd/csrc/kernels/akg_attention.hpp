@@ -1031,7 +1031,10 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
 // SPLIT: where the tiles of keys are fewer than the CUs, `splits` workgroups take a range of the rows each and leave their
 // sums in `ws` for backward_join. Two groups of wavefronts hide each other's vector instructions behind matrix instructions:
 // the training case of the forward pass takes 550 us, 1.0 PFLOP/s of its four products (one group: 930).
-template <typename C, int NW, int RG, int NWQ, bool SPLIT>
+// APART: above 256 channels (keys and values together) the accumulators of both leave too little room for the operands: a
+// workgroup computes dk or dv, and the scores are computed twice (gradient of 2 x 2048, 32/8 heads of 256, causal: 941 us
+// instead of 2481; of 192: 765 instead of 795).
+template <typename C, int NW, int RG, int NWQ, bool SPLIT, bool APART>
 AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const void *v, const void *mask,
                            const int *qlens, const int *klens, void *dk, void *dv, float *ws, Extents e, float scale, int splits) {
   typedef typename C::T T;
@@ -1043,257 +1046,270 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
   __shared__ __attribute__((aligned(16))) u8 ownKeys[kKeysInLds ? kRows * NW * own_pitch(DK) : 16];
   constexpr int kStates = C::ADDED ? 3 : 2;   // of a row: delta, top and rest (BackwardSpace)
   __shared__ __attribute__((aligned(16))) float stateOf[2][kStates][kRound];
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, group = __builtin_amdgcn_readfirstlane(tid >> 6) / NW, half = lane >> 5;
-  const long rows = e.sq * C::G, heads = e.batch * C::HKV;
-  const long id = SPLIT ? blockIdx.x / splits : blockIdx.x;
-  const int split = SPLIT ? static_cast<int>(blockIdx.x % splits) : 0;
-  long head, tile;
-  head_and_tile(id, heads, head, tile);
-  // (the first keys are seen by most queries, and come first)
-  const long b = head / C::HKV, hkv = head % C::HKV;
-  const int ql = clamped_length<C>(qlens, b, e.sq), kl = clamped_length<C>(klens, b, e.sk);
-  const int key0 = static_cast<int>(tile) * (kRows * NW) + wave * kRows;
-  const int key = key0 + (lane & 31);
-  const bool counts = key < kl;
-  const KeysOf<C, DK> keys(k, b, hkv, e);
-  const KeysOf<C, DV> values(v, b, hkv, e);
-  const BackwardSpace<C> space{heads * rows};
-  u32x4 own[kKeysInLds ? 1 : CK], val[CV];
-  if constexpr (kKeysInLds) {
-    const int key00 = static_cast<int>(tile) * (kRows * NW);
-    const Buffer kb = make_buffer(keys.base + key00 * keys.step, records((kl - key00 - 1) * keys.step + 2 * DK));
-    TileLoad<kRows * NW, DK, kThreads> kload;
-    kload.load(kb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(keys.step)); });
-    kload.template store<true>(ownKeys, tid);   // (padding channels meet zeros of the queries, but must be finite)
-    for (int c = tid; DK % 32 != 0 && c < kRows * NW * ((padded(DK) - DK) / 8); c += kThreads) {
-      constexpr int kPad = DK % 32 != 0 ? (padded(DK) - DK) / 8 : 1;
-      *reinterpret_cast<u32x4 *>(ownKeys + c / kPad * own_pitch(DK) + (DK / 8 + c % kPad) * 16) = u32x4{0, 0, 0, 0};
+  auto run = [&](auto which) __attribute__((always_inline)) {
+    constexpr bool kDk = decltype(which)::value != 2, kDv = decltype(which)::value != 1;
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, group = __builtin_amdgcn_readfirstlane(tid >> 6) / NW, half = lane >> 5;
+    const long rows = e.sq * C::G, heads = e.batch * C::HKV;
+    const long block = APART ? blockIdx.x / 2 : blockIdx.x, id = SPLIT ? block / splits : block;
+    const int split = SPLIT ? static_cast<int>(block % splits) : 0;
+    long head, tile;
+    head_and_tile(id, heads, head, tile);
+    // (the first keys are seen by most queries, and come first)
+    const long b = head / C::HKV, hkv = head % C::HKV;
+    const int ql = clamped_length<C>(qlens, b, e.sq), kl = clamped_length<C>(klens, b, e.sk);
+    const int key0 = static_cast<int>(tile) * (kRows * NW) + wave * kRows;
+    const int key = key0 + (lane & 31);
+    const bool counts = key < kl;
+    const KeysOf<C, DK> keys(k, b, hkv, e);
+    const KeysOf<C, DV> values(v, b, hkv, e);
+    const BackwardSpace<C> space{heads * rows};
+    u32x4 own[kKeysInLds ? 1 : CK], val[CV] = {};
+    if constexpr (kKeysInLds) {
+      const int key00 = static_cast<int>(tile) * (kRows * NW);
+      const Buffer kb = make_buffer(keys.base + key00 * keys.step, records((kl - key00 - 1) * keys.step + 2 * DK));
+      TileLoad<kRows * NW, DK, kThreads> kload;
+      kload.load(kb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(keys.step)); });
+      kload.template store<true>(ownKeys, tid);   // (padding channels meet zeros of the queries, but must be finite)
+      for (int c = tid; DK % 32 != 0 && c < kRows * NW * ((padded(DK) - DK) / 8); c += kThreads) {
+        constexpr int kPad = DK % 32 != 0 ? (padded(DK) - DK) / 8 : 1;
+        *reinterpret_cast<u32x4 *>(ownKeys + c / kPad * own_pitch(DK) + (DK / 8 + c % kPad) * 16) = u32x4{0, 0, 0, 0};
+      }
+    } else {
+      load_own<DK>(keys.base + (counts ? key : 0) * keys.step, counts, lane, own);
+    }
+    if (kDk) load_own<DV>(values.base + (counts ? key : 0) * values.step, counts, lane, val);
+    float lift = 1.0f;
+    if (T::kNarrowRange) {
+      const long tilesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ);
+      float largest = 0.0f;
+      for (long t = lane; t < tilesQ; t += 64) largest = __builtin_fmaxf(largest, ws[space.largest() + head * tilesQ + t]);
+#pragma unroll
+      for (int step = 1; step < 64; step *= 2) largest = __builtin_fmaxf(largest, __shfl_xor(largest, step));
+      lift = lift_of<T>(largest);
+    }
+    const float c = C::ADDED ? scale : scale * kLog2e;
+    f32x16 acck[kDk ? TK : 1], accv[kDv ? TV : 1];
+#pragma unroll
+    for (int d = 0; kDk && d < TK; ++d) acck[d] = {};
+#pragma unroll
+    for (int d = 0; kDv && d < TV; ++d) accv[d] = {};
+
+    // queries that see the first key of the workgroup, up to the last one of the sequence
+    const int first0 = static_cast<int>(tile) * (kRows * NW);
+    int from = 0;
+    if (C::CAUSAL) {
+      const int i = first0 - (kl - ql);
+      from = (i > 0 ? (i < ql ? i : ql) : 0) * C::G / kRound * kRound;
+    }
+    int upto = first0 < kl ? ql * C::G : 0;
+    if (SPLIT && from < upto) {
+      const int rounds = (upto - from + kRound - 1) / kRound, each = (rounds + splits - 1) / splits * kRound;
+      const long start = from + static_cast<long>(split) * each;
+      from = start < upto ? static_cast<int>(start) : upto;
+      upto = from + each < upto ? from + each : upto;
+    }
+
+    const RowsOf<C, DK> qrows(q, b, hkv, e);
+    const RowsOf<C, DV> grows(dout, b, hkv, e);
+    const Reader<DK> qread(lane);
+    const Reader<DV> gread(lane);
+    TileLoad<kRound, DK, kThreads> qload;
+    TileLoad<kRound, DV, kThreads> gload;
+    // Rows behind the last one read zeros (nothing is asked of memory): their probabilities are 1 and their products 0.
+    float state[kStates];
+    auto fetch = [&](int r0, bool any) {
+      const int i0 = r0 / C::G;
+      const Buffer qb = make_buffer(qrows.base + i0 * qrows.stepI, 0x7fffffffL);
+      const Buffer gb = make_buffer(grows.base + i0 * grows.stepI, 0x7fffffffL);
+      const int left = any ? upto - r0 : 0, lead = r0 - i0 * C::G;
+      auto offsetIn = [&](const auto &of, int r) {
+        const int at = lead + r;
+        return r < left ? static_cast<u32>(at / C::G * static_cast<int>(of.stepI) + at % C::G * static_cast<int>(of.stepG)) : kBeyondEveryBuffer;
+      };
+      qload.load(qb, tid, [&](int r) { return offsetIn(qrows, r); });
+      gload.load(gb, tid, [&](int r) { return offsetIn(grows, r); });
+      if (tid < kRound) {
+#pragma unroll
+        for (int x = 0; x < kStates; ++x) state[x] = tid < left ? ws[x * heads * rows + head * rows + r0 + tid] : 0.0f;
+      }
+    };
+    auto put = [&](int buf) {
+      qload.store(lds[buf], tid);
+      gload.store(lds[buf] + kRound * pitch(DK), tid);
+      if (tid < kRound) {
+#pragma unroll
+        for (int x = 0; x < kStates; ++x) stateOf[buf][x][tid] = state[x];
+      }
+    };
+#pragma unroll
+    for (int buf = 0; buf < 2; ++buf) {
+      clear_padding<kRound, DK, kThreads>(lds[buf], tid);
+      clear_padding<kRound, DV, kThreads>(lds[buf] + kRound * pitch(DK), tid);
+    }
+    // The last rows first: all tiles of a key head then pass the same rows at the same time, whatever row their first is, and
+    // find them in the L2 (2 x 4096, 32/8 heads of 128, causal: 0.46 GB from memory; the first rows first 1.7 GB, 10 us more).
+    const int start = from + (upto - from - 1) / kRound * kRound;
+    if (from < upto) {
+      fetch(start, true);
+      put(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int round = start; from < upto && round >= from; round -= kRound, buf ^= 1) {
+      const int r0 = round + group * kTileRows, at0 = group * kTileRows;   // this group's tile
+      const u8 *qt = lds[buf] + at0 * pitch(DK), *gt = lds[buf] + kRound * pitch(DK) + at0 * pitch(DV);
+      // the tile's last row sees most keys, its first one least
+      const int lastRow = (r0 + kTileRows < upto ? r0 + kTileRows : upto) - 1;
+      const bool active = r0 < upto && key0 < keys_seen<C>(lastRow / C::G, ql, kl);
+      u32x4 p[2], ds[2];
+      if (active) {
+        f32x16 s = {}, dp = {};
+        // (what the mask says is asked for before the scores are computed)
+        typename MaskRow<C>::E said[16];
+        if (C::MASK != 0) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int x = r0 + 8 * (r >> 2) + 4 * half + (r & 3), at = x < upto ? x : upto - 1;
+            said[r] = static_cast<const typename MaskRow<C>::E *>(mask)[mask_row<C>(b, hkv * C::G + at % C::G, at / C::G, e) + (counts ? key : 0)];
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int x = 0; x < CK; ++x) s = T::mma(qread.row(qt, 0, x), kKeysInLds ? read_own<DK>(ownKeys, wave * kRows, x, lane) : own[kKeysInLds ? 0 : x], s);
+#pragma unroll
+        for (int x = 0; kDk && x < CV; ++x) dp = T::mma(gread.row(gt, 0, x), val[x], dp);
+        FeedOrder<CK + (kDk ? CV : 0), (kKeysInLds ? 2 : 1) * CK + (kDk ? CV : 0), 6>::emit();
+        if (C::MASK != 0 || key0 + kRows > keys_seen<C>(r0 / C::G, ql, kl)) {
+          __builtin_amdgcn_sched_barrier(0);   // (a branch, not a select for every tile)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int at = r0 + 8 * (r >> 2) + 4 * half + (r & 3), i = at / C::G;
+            const bool ok = key < keys_seen<C>(i, ql, kl);
+            if (C::MASK != 0) {
+              s[r] = ok ? with_mask<C>(s[r], c, said, r) : neg_inf();
+            } else {
+              s[r] = ok ? s[r] : neg_inf();
+            }
+          }
+        }
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 d4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][0][at0 + 8 * r4 + 4 * half]);
+          const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][1][at0 + 8 * r4 + 4 * half]);
+          f32x4 o4 = {};
+          if (C::ADDED) o4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][kStates - 1][at0 + 8 * r4 + 4 * half]);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            const int r = 4 * r4 + z;
+            float x = C::MASK != 0 ? s[r] - l4[z] : __builtin_fmaf(s[r], c, -l4[z]);
+            if (C::ADDED) x = __builtin_fmaf(x, kLog2e, -o4[z]);
+            s[r] = __builtin_amdgcn_exp2f(x);
+            if (kDk) dp[r] = s[r] * (T::kNarrowRange ? (dp[r] - d4[z]) * lift : dp[r] - d4[z]);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            p[x][w] = T::pack(s[8 * x + 2 * w], s[8 * x + 2 * w + 1]);
+            ds[x][w] = T::pack(dp[8 * x + 2 * w], dp[8 * x + 2 * w + 1]);
+          }
+          asm volatile("" : "+v"(p[x]), "+v"(ds[x]));   // (the scores end here: their registers hold the next tile's rows)
+        }
+      }
+      fetch(round > from ? round - kRound : from, round > from);   // (none left: zeros, nothing is asked of memory)
+      if (active) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int d = 0; kDv && d < TV; ++d) accv[d] = T::mma(gread.transposed(gt, 16 * x, d), p[x], accv[d]);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int d = 0; kDk && d < TK; ++d) acck[d] = T::mma(qread.transposed(qt, 16 * x, d), ds[x], acck[d]);
+        }
+        FeedOrder<2 * ((kDv ? TV : 0) + (kDk ? TK : 0)), 4 * ((kDv ? TV : 0) + (kDk ? TK : 0)), 8>::emit();
+      }
+      put(buf ^ 1);
+      __syncthreads();
+    }
+    // the groups' sums joined: group g leaves as many accumulators as fit where the tiles were, group 0 adds them
+    static_assert(RG == 1 || !APART, "groups join both");
+    if constexpr (RG > 1) {
+      constexpr int kFit = static_cast<int>(sizeof(lds)) / (64 * NW * (RG - 1) * 16), kFours = 4 * (TK + TV), kPart = kFit < kFours ? kFit : kFours;
+      f32x4 *parts = reinterpret_cast<f32x4 *>(&lds[0][0]);
+      unrolled<(kFours + kPart - 1) / kPart>([&](auto pass) {
+        constexpr int p0 = decltype(pass)::value * kPart, kCount = kFours - p0 < kPart ? kFours - p0 : kPart;
+        __syncthreads();
+        if (group > 0) {
+          unrolled<kCount>([&](auto y) {
+            constexpr int x = p0 + decltype(y)::value, r = 4 * (x % 4);
+            const f32x16 &acc = x < 4 * TK ? acck[x / 4 % TK] : accv[(x - 4 * TK) / 4 % TV];
+            parts[(((group - 1) * kPart + x - p0) * NW + wave) * 64 + lane] = f32x4{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]};
+          });
+        }
+        __syncthreads();
+        if (group == 0) {
+          unrolled<kCount>([&](auto y) {
+            constexpr int x = p0 + decltype(y)::value, r = 4 * (x % 4);
+            f32x16 &acc = x < 4 * TK ? acck[x / 4 % TK] : accv[(x - 4 * TK) / 4 % TV];
+#pragma unroll
+            for (int g = 0; g < RG - 1; ++g) {
+              const f32x4 more = parts[((g * kPart + x - p0) * NW + wave) * 64 + lane];
+#pragma unroll
+              for (int z = 0; z < 4; ++z) acc[r + z] += more[z];
+            }
+          });
+        }
+      });
+      if (group > 0) return;
+    }
+    if (key >= e.sk) return;
+    const float back = scale / lift;
+    if constexpr (SPLIT) {
+      const long tilesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ);
+      float *to = ws + space.sums(heads * tilesQ) + ((split * heads + head) * e.sk + key) * BackwardSpace<C>::kSums;
+#pragma unroll
+      for (int d = kDk ? 0 : TK; d < (kDv ? TK + TV : TK); ++d) {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          f32x4 x;
+#pragma unroll
+          for (int z = 0; z < 4; ++z) x[z] = d < TK ? acck[kDk ? d % TK : 0][4 * r4 + z] * back : accv[kDv && d >= TK ? d - TK : 0][4 * r4 + z];
+          *reinterpret_cast<f32x4 *>(to + 32 * d + 8 * r4 + 4 * half) = x;
+        }
+      }
+      return;
+    }
+    auto store = [&](char *to, int dim, const f32x16 *acc, int tilesD, float factor) {
+#pragma unroll
+      for (int d = 0; d < tilesD; ++d) {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int at = 32 * d + 8 * r4 + 4 * half;
+          if (dim % 32 != 0 && at >= dim) continue;
+          u32x2 w;
+          w[0] = T::pack(acc[d][4 * r4] * factor, acc[d][4 * r4 + 1] * factor);
+          w[1] = T::pack(acc[d][4 * r4 + 2] * factor, acc[d][4 * r4 + 3] * factor);
+          *reinterpret_cast<u32x2 *>(to + 2 * at) = w;
+        }
+      }
+    };
+    const KeysOf<C, DK> dkeys(dk, b, hkv, e);
+    const KeysOf<C, DV> dvalues(dv, b, hkv, e);
+    if (kDk && dk != nullptr) store(const_cast<char *>(dkeys.base) + key * dkeys.step, DK, acck, TK, back);
+    if (kDv && dv != nullptr) store(const_cast<char *>(dvalues.base) + key * dvalues.step, DV, accv, TV, 1.0f);
+  };
+  if constexpr (APART) {
+    if (blockIdx.x % 2 == 0) {
+      run(IntTag<1>());
+    } else {
+      run(IntTag<2>());
     }
   } else {
-    load_own<DK>(keys.base + (counts ? key : 0) * keys.step, counts, lane, own);
+    run(IntTag<0>());
   }
-  load_own<DV>(values.base + (counts ? key : 0) * values.step, counts, lane, val);
-  float lift = 1.0f;
-  if (T::kNarrowRange) {
-    const long tilesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ);
-    float largest = 0.0f;
-    for (long t = lane; t < tilesQ; t += 64) largest = __builtin_fmaxf(largest, ws[space.largest() + head * tilesQ + t]);
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) largest = __builtin_fmaxf(largest, __shfl_xor(largest, step));
-    lift = lift_of<T>(largest);
-  }
-  const float c = C::ADDED ? scale : scale * kLog2e;
-  f32x16 acck[TK], accv[TV];
-#pragma unroll
-  for (int d = 0; d < TK; ++d) acck[d] = {};
-#pragma unroll
-  for (int d = 0; d < TV; ++d) accv[d] = {};
-
-  // queries that see the first key of the workgroup, up to the last one of the sequence
-  const int first0 = static_cast<int>(tile) * (kRows * NW);
-  int from = 0;
-  if (C::CAUSAL) {
-    const int i = first0 - (kl - ql);
-    from = (i > 0 ? (i < ql ? i : ql) : 0) * C::G / kRound * kRound;
-  }
-  int upto = first0 < kl ? ql * C::G : 0;
-  if (SPLIT && from < upto) {
-    const int rounds = (upto - from + kRound - 1) / kRound, each = (rounds + splits - 1) / splits * kRound;
-    const long start = from + static_cast<long>(split) * each;
-    from = start < upto ? static_cast<int>(start) : upto;
-    upto = from + each < upto ? from + each : upto;
-  }
-
-  const RowsOf<C, DK> qrows(q, b, hkv, e);
-  const RowsOf<C, DV> grows(dout, b, hkv, e);
-  const Reader<DK> qread(lane);
-  const Reader<DV> gread(lane);
-  TileLoad<kRound, DK, kThreads> qload;
-  TileLoad<kRound, DV, kThreads> gload;
-  // Rows behind the last one read zeros (nothing is asked of memory): their probabilities are 1 and their products 0.
-  float state[kStates];
-  auto fetch = [&](int r0, bool any) {
-    const int i0 = r0 / C::G;
-    const Buffer qb = make_buffer(qrows.base + i0 * qrows.stepI, 0x7fffffffL);
-    const Buffer gb = make_buffer(grows.base + i0 * grows.stepI, 0x7fffffffL);
-    const int left = any ? upto - r0 : 0, lead = r0 - i0 * C::G;
-    auto offsetIn = [&](const auto &of, int r) {
-      const int at = lead + r;
-      return r < left ? static_cast<u32>(at / C::G * static_cast<int>(of.stepI) + at % C::G * static_cast<int>(of.stepG)) : kBeyondEveryBuffer;
-    };
-    qload.load(qb, tid, [&](int r) { return offsetIn(qrows, r); });
-    gload.load(gb, tid, [&](int r) { return offsetIn(grows, r); });
-    if (tid < kRound) {
-#pragma unroll
-      for (int x = 0; x < kStates; ++x) state[x] = tid < left ? ws[x * heads * rows + head * rows + r0 + tid] : 0.0f;
-    }
-  };
-  auto put = [&](int buf) {
-    qload.store(lds[buf], tid);
-    gload.store(lds[buf] + kRound * pitch(DK), tid);
-    if (tid < kRound) {
-#pragma unroll
-      for (int x = 0; x < kStates; ++x) stateOf[buf][x][tid] = state[x];
-    }
-  };
-#pragma unroll
-  for (int buf = 0; buf < 2; ++buf) {
-    clear_padding<kRound, DK, kThreads>(lds[buf], tid);
-    clear_padding<kRound, DV, kThreads>(lds[buf] + kRound * pitch(DK), tid);
-  }
-  // The last rows first: all tiles of a key head then pass the same rows at the same time, whatever row their first is, and
-  // find them in the L2 (2 x 4096, 32/8 heads of 128, causal: 0.46 GB from memory; the first rows first 1.7 GB, 10 us more).
-  const int start = from + (upto - from - 1) / kRound * kRound;
-  if (from < upto) {
-    fetch(start, true);
-    put(0);
-  }
-  __syncthreads();
-  int buf = 0;
-  for (int round = start; from < upto && round >= from; round -= kRound, buf ^= 1) {
-    const int r0 = round + group * kTileRows, at0 = group * kTileRows;   // this group's tile
-    const u8 *qt = lds[buf] + at0 * pitch(DK), *gt = lds[buf] + kRound * pitch(DK) + at0 * pitch(DV);
-    // the tile's last row sees most keys, its first one least
-    const int lastRow = (r0 + kTileRows < upto ? r0 + kTileRows : upto) - 1;
-    const bool active = r0 < upto && key0 < keys_seen<C>(lastRow / C::G, ql, kl);
-    u32x4 p[2], ds[2];
-    if (active) {
-      f32x16 s = {}, dp = {};
-      // (what the mask says is asked for before the scores are computed)
-      typename MaskRow<C>::E said[16];
-      if (C::MASK != 0) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int x = r0 + 8 * (r >> 2) + 4 * half + (r & 3), at = x < upto ? x : upto - 1;
-          said[r] = static_cast<const typename MaskRow<C>::E *>(mask)[mask_row<C>(b, hkv * C::G + at % C::G, at / C::G, e) + (counts ? key : 0)];
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-#pragma unroll
-      for (int x = 0; x < CK; ++x) s = T::mma(qread.row(qt, 0, x), kKeysInLds ? read_own<DK>(ownKeys, wave * kRows, x, lane) : own[kKeysInLds ? 0 : x], s);
-#pragma unroll
-      for (int x = 0; x < CV; ++x) dp = T::mma(gread.row(gt, 0, x), val[x], dp);
-      FeedOrder<CK + CV, (kKeysInLds ? 2 : 1) * CK + CV, 6>::emit();
-      if (C::MASK != 0 || key0 + kRows > keys_seen<C>(r0 / C::G, ql, kl)) {
-        __builtin_amdgcn_sched_barrier(0);   // (a branch, not a select for every tile)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int at = r0 + 8 * (r >> 2) + 4 * half + (r & 3), i = at / C::G;
-          const bool ok = key < keys_seen<C>(i, ql, kl);
-          if (C::MASK != 0) {
-            s[r] = ok ? with_mask<C>(s[r], c, said, r) : neg_inf();
-          } else {
-            s[r] = ok ? s[r] : neg_inf();
-          }
-        }
-      }
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const f32x4 d4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][0][at0 + 8 * r4 + 4 * half]);
-        const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][1][at0 + 8 * r4 + 4 * half]);
-        f32x4 o4 = {};
-        if (C::ADDED) o4 = *reinterpret_cast<const f32x4 *>(&stateOf[buf][kStates - 1][at0 + 8 * r4 + 4 * half]);
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const int r = 4 * r4 + z;
-          float x = C::MASK != 0 ? s[r] - l4[z] : __builtin_fmaf(s[r], c, -l4[z]);
-          if (C::ADDED) x = __builtin_fmaf(x, kLog2e, -o4[z]);
-          s[r] = __builtin_amdgcn_exp2f(x);
-          dp[r] = s[r] * (T::kNarrowRange ? (dp[r] - d4[z]) * lift : dp[r] - d4[z]);
-        }
-      }
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          p[x][w] = T::pack(s[8 * x + 2 * w], s[8 * x + 2 * w + 1]);
-          ds[x][w] = T::pack(dp[8 * x + 2 * w], dp[8 * x + 2 * w + 1]);
-        }
-        asm volatile("" : "+v"(p[x]), "+v"(ds[x]));   // (the scores end here: their registers hold the next tile's rows)
-      }
-    }
-    fetch(round > from ? round - kRound : from, round > from);   // (none left: zeros, nothing is asked of memory)
-    if (active) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-#pragma unroll
-        for (int d = 0; d < TV; ++d) accv[d] = T::mma(gread.transposed(gt, 16 * x, d), p[x], accv[d]);
-      }
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-#pragma unroll
-        for (int d = 0; d < TK; ++d) acck[d] = T::mma(qread.transposed(qt, 16 * x, d), ds[x], acck[d]);
-      }
-      FeedOrder<2 * (TV + TK), 4 * (TV + TK), 8>::emit();
-    }
-    put(buf ^ 1);
-    __syncthreads();
-  }
-  // the groups' sums joined: group g leaves as many accumulators as fit where the tiles were, group 0 adds them
-  if constexpr (RG > 1) {
-    constexpr int kFit = static_cast<int>(sizeof(lds)) / (64 * NW * (RG - 1) * 16), kFours = 4 * (TK + TV), kPart = kFit < kFours ? kFit : kFours;
-    f32x4 *parts = reinterpret_cast<f32x4 *>(&lds[0][0]);
-    unrolled<(kFours + kPart - 1) / kPart>([&](auto pass) {
-      constexpr int p0 = decltype(pass)::value * kPart, kCount = kFours - p0 < kPart ? kFours - p0 : kPart;
-      __syncthreads();
-      if (group > 0) {
-        unrolled<kCount>([&](auto y) {
-          constexpr int x = p0 + decltype(y)::value, r = 4 * (x % 4);
-          const f32x16 &acc = x < 4 * TK ? acck[x / 4 % TK] : accv[(x - 4 * TK) / 4 % TV];
-          parts[(((group - 1) * kPart + x - p0) * NW + wave) * 64 + lane] = f32x4{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]};
-        });
-      }
-      __syncthreads();
-      if (group == 0) {
-        unrolled<kCount>([&](auto y) {
-          constexpr int x = p0 + decltype(y)::value, r = 4 * (x % 4);
-          f32x16 &acc = x < 4 * TK ? acck[x / 4 % TK] : accv[(x - 4 * TK) / 4 % TV];
-#pragma unroll
-          for (int g = 0; g < RG - 1; ++g) {
-            const f32x4 more = parts[((g * kPart + x - p0) * NW + wave) * 64 + lane];
-#pragma unroll
-            for (int z = 0; z < 4; ++z) acc[r + z] += more[z];
-          }
-        });
-      }
-    });
-    if (group > 0) return;
-  }
-  if (key >= e.sk) return;
-  const float back = scale / lift;
-  if constexpr (SPLIT) {
-    const long tilesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ);
-    float *to = ws + space.sums(heads * tilesQ) + ((split * heads + head) * e.sk + key) * BackwardSpace<C>::kSums;
-#pragma unroll
-    for (int d = 0; d < TK + TV; ++d) {
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        f32x4 x;
-#pragma unroll
-        for (int z = 0; z < 4; ++z) x[z] = d < TK ? acck[d % TK][4 * r4 + z] * back : accv[d < TK ? 0 : d - TK][4 * r4 + z];
-        *reinterpret_cast<f32x4 *>(to + 32 * d + 8 * r4 + 4 * half) = x;
-      }
-    }
-    return;
-  }
-  auto store = [&](char *to, int dim, const f32x16 *acc, int tilesD, float factor) {
-#pragma unroll
-    for (int d = 0; d < tilesD; ++d) {
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const int at = 32 * d + 8 * r4 + 4 * half;
-        if (dim % 32 != 0 && at >= dim) continue;
-        u32x2 w;
-        w[0] = T::pack(acc[d][4 * r4] * factor, acc[d][4 * r4 + 1] * factor);
-        w[1] = T::pack(acc[d][4 * r4 + 2] * factor, acc[d][4 * r4 + 3] * factor);
-        *reinterpret_cast<u32x2 *>(to + 2 * at) = w;
-      }
-    }
-  };
-  const KeysOf<C, DK> dkeys(dk, b, hkv, e);
-  const KeysOf<C, DV> dvalues(dv, b, hkv, e);
-  if (dk != nullptr) store(const_cast<char *>(dkeys.base) + key * dkeys.step, DK, acck, TK, back);
-  if (dv != nullptr) store(const_cast<char *>(dvalues.base) + key * dvalues.step, DV, accv, TV, 1.0f);
 }
 
 // dk and dv from the sums over ranges of rows, in their order: four channels a thread.

@@ -347,6 +347,21 @@ SHARED = [
 ]
 
 
+WIDE = [
+    ("bfloat16", "BSND", 1, 700, 90, 4, 2, 192, 192, True, None, "padded"),     # dk and dv by workgroups of their own, rows in two ranges
+    ("float16", "BNSD", 2, 65, 130, 2, 2, 256, 8, False, "float32", None),
+    ("float16", "BSND", 1, 40, 33, 2, 1, 40, 256, True, "bool", "padded"),
+    ("bfloat16", "BNSD", 2, 96, 96, 3, 3, 136, 136, False, None, None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", WIDE, ids=lambda c: "-".join(str(x) for x in c))
+def test_wide_heads(case, tmp_path):
+    test_attention(case, tmp_path / "forward")
+    test_attention_gradient(case, tmp_path / "gradient")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("case", SHARED, ids=lambda c: "-".join(str(x) for x in c))
 def test_shared_axes(case, tmp_path):
