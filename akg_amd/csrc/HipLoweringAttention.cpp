@@ -388,7 +388,8 @@ class LayerEmitter {
     const int64_t tokens = perSequence * page;
     const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({std::max(ceilDiv(2 * cus_, groups), std::min(ceilDiv(8 * cus_, groups), tokens / 1024)),
                                                                    ceilDiv(tokens, 128), 64}));
-    // (registers for three wavefronts a SIMD: 147 instead of 180, 195 -> 175 us in the second of these)
+    // Registers for three wavefronts a SIMD, two above 128 channels: 175 us instead of 195 in the second of these; 16 x 8192
+    // tokens, 8 key heads of 192 and 256: 67 and 91 us, with the compiler's choice 69 and 124, with three 156 (spilled) and 124.
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n#include \"akg_cache_attention.hpp\"\n")
       << "typedef akg::attn::Config<" << trait() << ", " << dim << ", " << dim << ", " << kvHeads << ", " << group
@@ -403,7 +404,7 @@ class LayerEmitter {
         << number(l_.scale) << ", static_cast<int>(akg_splits));\n";
       return c.str();
     };
-    const int hint = rt == 1 ? 3 : 0;
+    const int hint = rt == 1 ? (units <= 2 ? 3 : 2) : 0;
     if (splits > 1) {
       ranges(o, args, call(true), 256, hint, "akg::attn::Extents{akg_batch, akg_sq, 0}", outName(0) + ", nullptr", groups, 16 * rt, splits, batch * kvHeads, rows, dim);
     } else {
