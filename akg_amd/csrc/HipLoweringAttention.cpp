@@ -380,7 +380,9 @@ class LayerEmitter {
     if (page % 16 != 0) throw LoweringError("op " + op_.name + ": the tokens of a block must be a multiple of 16");
     if (rows >= (1LL << 30) || perSequence * page >= (1LL << 30)) throw LoweringError("op " + op_.name + ": more than 2^30 tokens or rows");
     const int64_t units = ceilDiv(dim, 64);
-    const int64_t rt = std::min<int64_t>(ceilDiv(rows, 16), std::max<int64_t>(1, std::min<int64_t>(4, 8 / units)));
+    // Tiles of 16 rows a workgroup: as many as registers of two wavefronts a SIMD hold (16 sequences of 4096 tokens, 4 key heads of
+    // 128, 64 rows each: two tiles 39 us, four tiles and one wavefront 56; of 256: one tile 72, two 84).
+    const int64_t rt = std::min<int64_t>(ceilDiv(rows, 16), std::max<int64_t>(1, 4 / units));
     const int64_t groups = batch * kvHeads * ceilDiv(rows, 16 * rt);
     // Workgroups that share a sequence: two to a CU, with at least one step of 32 tokens for each of their four wavefronts, and
     // up to eight where each has 1024 tokens or more. us at two, four, eight to a CU: 16 x 2000 tokens (4 key heads of 64
@@ -388,8 +390,9 @@ class LayerEmitter {
     const int64_t tokens = perSequence * page;
     const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({std::max(ceilDiv(2 * cus_, groups), std::min(ceilDiv(8 * cus_, groups), tokens / 1024)),
                                                                    ceilDiv(tokens, 128), 64}));
-    // Registers for three wavefronts a SIMD, two above 128 channels: 175 us instead of 195 in the second of these; 16 x 8192
-    // tokens, 8 key heads of 192 and 256: 67 and 91 us, with the compiler's choice 69 and 124, with three 156 (spilled) and 124.
+    // Registers for two wavefronts a SIMD, three for one tile of up to 128 channels: 175 us instead of 195 in the second of these;
+    // 32 rows over 16 x 4096 tokens, 4 key heads of 128, 26 instead of 36; one query over 16 x 8192, 8 key heads of 192 and 256,
+    // 67 and 91 instead of 69 and 124 (with three 156, spilled, and 124).
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n#include \"akg_cache_attention.hpp\"\n")
       << "typedef akg::attn::Config<" << trait() << ", " << dim << ", " << dim << ", " << kvHeads << ", " << group
@@ -404,7 +407,7 @@ class LayerEmitter {
         << number(l_.scale) << ", static_cast<int>(akg_splits));\n";
       return c.str();
     };
-    const int hint = rt == 1 ? (units <= 2 ? 3 : 2) : 0;
+    const int hint = rt == 1 && units <= 2 ? 3 : 2;
     if (splits > 1) {
       ranges(o, args, call(true), 256, hint, "akg::attn::Extents{akg_batch, akg_sq, 0}", outName(0) + ", nullptr", groups, 16 * rt, splits, batch * kvHeads, rows, dim);
     } else {
