@@ -492,7 +492,7 @@ AKG_DEV void join_rows(float *ws, void *out, float *lse, const Extents &e, int s
 // SPLIT: the workgroup takes one of `splits` ranges of the keys (Ranges). JOIN: the last one joins them.
 //
 // Many rows are bound by the matrix units and by the issue of what stands beside them: 2 x 4096 queries and keys, 32 heads over
-// 8 of 128 channels, causal, bfloat16, take 299 us, 0.92 PFLOP/s (a matrix product of 8192 each way reaches 1.36); the
+// 8 of 128 channels, causal, bfloat16, take 294 us, 0.94 PFLOP/s (a matrix product of 8192 each way reaches 1.36); the
 // matrix instructions alone would take 215, the vector instructions alone 151. Few rows are bound by the keys and values from
 // memory: one query of 8 sequences over 8192 keys takes 51 us, 4.0 TB/s, and 44 where the last level cache still holds part
 // of them. Tried for both and left out: a second set of tiles under way (token 54, training unchanged), 64 rows a wavefront,
