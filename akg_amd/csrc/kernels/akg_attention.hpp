@@ -686,7 +686,7 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
       active = k0 + kTile < end && __any(k0 + kTile < seen);
     }
     if (k0 + kTile >= end) break;
-    if (kTiles == 2) __syncthreads();   // (the tile written now was read in this round)
+    if (kTiles == 2) __syncthreads();   // (the tile written now has been read until here)
     kload.store(ktiles[then], tid);
     vload.store(vtiles[then], tid);
     __syncthreads();
@@ -1001,7 +1001,7 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
       active = __any(k0 + kTile < seen);
     }
     if (k0 + kTile >= end) break;
-    if (kTiles == 2) __syncthreads();   // (the tile written now was read in this round)
+    if (kTiles == 2) __syncthreads();   // (the tile written now has been read until here)
     kload.store(ktiles[then], tid);
     vload.store(vtiles[then], tid);
     __syncthreads();
