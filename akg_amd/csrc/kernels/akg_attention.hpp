@@ -160,7 +160,7 @@ template <typename C>
 AKG_DEV int keys_seen(long i, int ql, int kl) {
   if (i >= ql) return 0;
   if (!C::CAUSAL) return kl;
-  const int n = static_cast<int>(i) + kl - ql + 1;
+  const int n = kl - (ql - 1 - static_cast<int>(i));
   return n < 0 ? 0 : (n < kl ? n : kl);
 }
 
@@ -530,9 +530,9 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   const int most = row0 / C::G < ql ? keys_seen<C>(lastI, ql, kl) : 0;
   int first = 0, end = most;
   if (SPLIT) {
-    const int all = (most + kTile - 1) / kTile, each = (all + splits - 1) / splits;
-    first = split * each * kTile < most ? split * each * kTile : most;
-    end = first + each * kTile < most ? first + each * kTile : most;
+    const long all = (most + kTile - 1) / kTile, each = (all + splits - 1) / splits * kTile, start = split * each;
+    first = start < most ? static_cast<int>(start) : most;
+    if (each < most - first) end = first + static_cast<int>(each);
   }
 
   const RowsOf<C, DK> qrows(q, b, hkv, e);
@@ -1098,15 +1098,15 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     const int first0 = static_cast<int>(tile) * (kRows * NW);
     int from = 0;
     if (C::CAUSAL) {
-      const int i = first0 - (kl - ql);
-      from = (i > 0 ? (i < ql ? i : ql) : 0) * C::G / kRound * kRound;
+      const long i = static_cast<long>(first0) - kl + ql;
+      from = static_cast<int>((i > 0 ? (i < ql ? i : ql) : 0) * C::G / kRound * kRound);
     }
     int upto = first0 < kl ? ql * C::G : 0;
     if (SPLIT && from < upto) {
       const int rounds = (upto - from + kRound - 1) / kRound, each = (rounds + splits - 1) / splits * kRound;
       const long start = from + static_cast<long>(split) * each;
       from = start < upto ? static_cast<int>(start) : upto;
-      upto = from + each < upto ? from + each : upto;
+      if (each < upto - from) upto = from + each;
     }
 
     const RowsOf<C, DK> qrows(q, b, hkv, e);
