@@ -313,7 +313,7 @@ class LayerEmitter {
 
   void attentionGrad() {
     const Sizes s = sizes(in(1), in(2), in(3));
-    const int nwq = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8), rg = std::max(s.dk, s.dv) > 128 ? 1 : 2;
+    const int rg = std::max(s.dk, s.dv) > 128 ? 1 : 2;
     // A workgroup of the kernel of dk and dv has 128 keys. Where that leaves CUs idle it shares the rows with others, 512 of
     // them each at least (causal: two to a CU, since the first keys have most rows), or has 64. us of the gradient unshared,
     // shared: 1 x 1024 x 16/4 heads of 128, causal, 129, 75; 1 x 4096 x 32/4 918, 568; 8 x 200 x 12 heads of 64 with 128 keys
@@ -324,33 +324,54 @@ class LayerEmitter {
     const int64_t whole = s.keyHeads * ceilDiv(s.sk, crowded ? 64 : 128);
     const int64_t splits = std::max<int64_t>(1, std::min((l_.causal ? 2 : 1) * cus_ / whole, s.rows / 512));
     const int nwk = !crowded && (splits > 1 || whole >= cus_) ? 4 : 2;
-    const int64_t tilesQ = ceilDiv(s.rows, 32 * nwq);
     const int64_t groups = s.keyHeads * ceilDiv(s.sk, 32 * nwk);
+    // Small problems: what both kernels need of the rows in a launch of its own, then both in one launch, side by side, while
+    // neither fills the card (8 x 200 x 12 heads of 64: 18.8 us instead of 24.0, 2 x 512 x 12 of 64 19.6 instead of 28.5; with
+    // three workgroups a CU 2 x 2000 x 2001 x 16/4 of 128 with a mask takes 551 instead of 497).
+    const bool together = splits == 1 && nwk * rg == 4 && !apart && 2 * (groups + s.keyHeads * ceilDiv(s.rows, 128)) <= 5 * cus_;
+    const int nwq = together ? 4 : waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8);
+    const int64_t tilesQ = ceilDiv(s.rows, 32 * nwq);
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n") << config(s, 6);
     std::vector<std::string> scalars = {"akg_batch", "akg_sq", "akg_sk"};
     if (splits > 1) scalars.push_back("akg_splits");
     const std::string args = signature(scalars, true);
     const std::string extents = "akg::attn::Extents{akg_batch, akg_sq, akg_sk}", ranges = splits > 1 ? "static_cast<int>(akg_splits)" : "1";
-    std::ostringstream queries, keys;
-    queries << "  akg::attn::backward_queries<akg_C, " << nwq << ">(" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << inName(3) << ", "
-            << inName(4) << ", " << inName(5) << ", " << optionals(6) << ", " << outName(0) << ", akg_ws, " << extents << ", " << number(l_.scale) << ");\n";
-    keys << "  akg::attn::backward_keys<akg_C, " << nwk << ", " << rg << ", " << nwq << ", " << flag(splits > 1) << ", " << flag(apart) << ">(" << inName(0) << ", " << inName(1) << ", "
-         << inName(2) << ", " << inName(3) << ", " << optionals(6) << ", " << outName(1) << ", " << outName(2) << ", akg_ws, " << extents << ", " << number(l_.scale) << ", "
-         << ranges << ");\n";
-    KernelPhase first;
-    first.kernelName = g_.name + "_queries";
+    auto queries = [&](int part, const std::string &block, const std::string &lds) {
+      return "  akg::attn::backward_queries<akg_C, " + std::to_string(nwq) + ", " + std::to_string(part) + ">(" + inName(0) + ", " + inName(1) + ", " + inName(2) + ", " +
+             inName(3) + ", " + inName(4) + ", " + inName(5) + ", " + optionals(6) + ", " + outName(0) + ", akg_ws, " + extents + ", " + number(l_.scale) + ", " + block + ", " +
+             lds + ");\n";
+    };
+    auto keys = [&](const std::string &block, const std::string &lds) {
+      return "  akg::attn::backward_keys<akg_C, " + std::to_string(nwk) + ", " + std::to_string(rg) + ", " + std::to_string(nwq) + ", " + flag(splits > 1) + ", " + flag(apart) +
+             ">(" + inName(0) + ", " + inName(1) + ", " + inName(2) + ", " + inName(3) + ", " + optionals(6) + ", " + outName(1) + ", " + outName(2) + ", akg_ws, " + extents + ", " +
+             number(l_.scale) + ", " + ranges + ", " + block + ", " + lds + ");\n";
+    };
+    auto queriesLds = [&](int part) { return "akg::attn::QueriesLds<akg_C, " + std::to_string(nwq) + ", " + std::to_string(part) + ">"; };
+    const std::string keysLds = "akg::attn::KeysLds<akg_C, " + std::to_string(nwk) + ", " + std::to_string(rg) + ">", keysName = splits > 1 ? g_.name + "_keys" : k_.kernelName;
+    const int hint = std::max(s.dk, s.dv) > 128 || nwk == 2 ? 0 : 2, part = together ? 1 : 0;
+    KernelPhase first, last;
+    first.kernelName = g_.name + (together ? "_rows" : "_queries");
     first.grid[0] = checkGrid(s.keyHeads * tilesQ, 64 * nwq);
     first.block[0] = static_cast<unsigned>(64 * nwq);
     k_.earlierPhases.push_back(first);
-    const std::string keysName = splits > 1 ? g_.name + "_keys" : k_.kernelName;
-    o << kernel(first.kernelName, 64 * nwq, args, queries.str()) << kernel(keysName, 64 * nwk * rg, args, keys.str(), std::max(s.dk, s.dv) > 128 || nwk == 2 ? 0 : 2);
-    KernelPhase last;
-    last.grid[0] = checkGrid((apart ? 2 : 1) * groups * splits, 64 * nwk * rg);
+    o << kernel(first.kernelName, 64 * nwq, args, "  __shared__ " + queriesLds(part) + " akg_lds;\n" + queries(part, "blockIdx.x", "akg_lds"));
+    if (together) {
+      o << kernel(keysName, 256, args,
+                  "  typedef " + queriesLds(2) + " akg_Q;\n  typedef " + keysLds + " akg_K;\n" +
+                      "  __shared__ __attribute__((aligned(16))) akg::u8 akg_lds[sizeof(akg_Q) > sizeof(akg_K) ? sizeof(akg_Q) : sizeof(akg_K)];\n" +
+                      "  const long akg_keys = akg_batch * akg_C::HKV * ((akg_sk + " + std::to_string(32 * nwk - 1) + ") / " + std::to_string(32 * nwk) + ");\n" +
+                      "  if (blockIdx.x < akg_keys) {\n" + keys("blockIdx.x", "*reinterpret_cast<akg_K *>(akg_lds)") + "  } else {\n" +
+                      queries(2, "blockIdx.x - akg_keys", "*reinterpret_cast<akg_Q *>(akg_lds)") + "  }\n");
+      last.grid[0] = checkGrid(groups + s.keyHeads * tilesQ, 256);
+    } else {
+      o << kernel(keysName, 64 * nwk * rg, args, "  __shared__ " + keysLds + " akg_lds;\n" + keys("blockIdx.x", "akg_lds"), hint);
+      last.grid[0] = checkGrid((apart ? 2 : 1) * groups * splits, 64 * nwk * rg);
+    }
     last.block[0] = static_cast<unsigned>(64 * nwk * rg);
-    // per row delta and its log-sum (in two parts for an added mask), per workgroup of the first kernel the largest |dout|
+    // per row delta and its log-sum (in two parts for an added mask), per wavefront of the first kernel the largest |dout|
     const bool added = l_.hasMask && in(6).dtype != DType::Bool;
-    k_.workspaceBytes = static_cast<uint64_t>(4 * s.keyHeads * ((added ? 3 : 2) * s.rows + tilesQ));
+    k_.workspaceBytes = static_cast<uint64_t>(4 * s.keyHeads * ((added ? 3 : 2) * s.rows + tilesQ * nwq));
     if (splits > 1) {
       last.kernelName = keysName;
       k_.earlierPhases.push_back(last);

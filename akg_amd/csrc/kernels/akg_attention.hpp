@@ -754,7 +754,7 @@ constexpr float kLargeLse = 4096.0f;
 
 // Places in the workspace of the backward kernels, in floats: delta and top of every row (top: times log2 e where no mask is
 // added; infinite for a row without keys, whose probabilities then are 2^-inf = 0), for an added mask the rest, and the
-// largest |dout| of every workgroup of the first kernel.
+// largest |dout| of every wavefront of the first kernel.
 template <typename C>
 struct BackwardSpace {
   long rows;   // of all key heads
@@ -763,25 +763,32 @@ struct BackwardSpace {
   AKG_DEV long largest() const { return (C::ADDED ? 3 : 2) * rows; }
   // behind them, to the next 256 bytes: sums of dk and dv over ranges of rows, [ranges][key heads][keys][padded channels of both]
   static constexpr int kSums = padded(C::DK) + padded(C::DV);
-  AKG_DEV long sums(long workgroups) const { return (largest() + workgroups + 63) / 64 * 64; }
+  AKG_DEV long sums(long wavefronts) const { return (largest() + wavefronts + 63) / 64 * 64; }
 };
 
 // dq of 32 rows a wavefront: keys and values pass by in tiles, 32 keys a step: the scores and their gradients' products, then
 // the gradients of the scores (vector instructions) between the matrix instructions that multiply those of the step before.
 // Leaves in `ws` what the kernel of dk and dv needs. Bound as the forward pass is: the training case there takes 417 us, 0.99
 // PFLOP/s of its three products (425 with the gradients of a step computed in front of its own products).
-template <typename C, int NW>
+// PART: 0 all of it; 1 only what it leaves in `ws`; 2 only dq, from that.
+template <typename C, int NW, int PART>
+struct QueriesLds {
+  static constexpr int kTiles = NW == 8 && 3 * kTile * (pitch(C::DK) + pitch(C::DV)) <= 160 * 1024 ? 3 : 2;   // (as in the forward pass)
+  __attribute__((aligned(16))) u8 ktiles[kTiles][PART == 1 ? 16 : kTile * pitch(C::DK)], vtiles[kTiles][PART == 1 ? 16 : kTile * pitch(C::DV)];
+};
+template <typename C, int NW, int PART>
 AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
-                              const void *mask, const int *qlens, const int *klens, void *dq, float *ws, Extents e, float scale) {
+                              const void *mask, const int *qlens, const int *klens, void *dq, float *ws, Extents e, float scale, long block,
+                              QueriesLds<C, NW, PART> &lds) {
   typedef typename C::T T;
   constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, CV = (DV + 15) / 16, TK = padded(DK) / 32, kThreads = 64 * NW;
-  constexpr int kTiles = NW == 8 && 3 * kTile * (pitch(DK) + pitch(DV)) + 64 <= 160 * 1024 ? 3 : 2;   // (as in the forward pass)
-  __shared__ __attribute__((aligned(16))) u8 ktiles[kTiles][kTile * pitch(DK)], vtiles[kTiles][kTile * pitch(DV)];
-  __shared__ float largestOf[NW];
+  constexpr int kTiles = QueriesLds<C, NW, PART>::kTiles;
+  auto &ktiles = lds.ktiles;
+  auto &vtiles = lds.vtiles;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   const long rows = e.sq * C::G, tiles = (rows + kRows * NW - 1) / (kRows * NW), heads = e.batch * C::HKV;
   long head, tile;
-  head_and_tile(blockIdx.x, heads, head, tile);
+  head_and_tile(block, heads, head, tile);
   tile = tiles - 1 - tile;
   const long b = head / C::HKV, hkv = head % C::HKV;
   const int ql = clamped_length<C>(qlens, b, e.sq), kl = clamped_length<C>(klens, b, e.sk);
@@ -801,14 +808,14 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
   load_own<DV>(grows.base + grows.offset(exists ? row : 0), seen > 0, lane, grad);
   float delta = 0.0f, largest = 0.0f;
   {
-    u32x4 o[CV];
-    load_own<DV>(orows.base + orows.offset(exists ? row : 0), seen > 0, lane, o);
+    u32x4 o[CV] = {};
+    if (PART != 2) load_own<DV>(orows.base + orows.offset(exists ? row : 0), seen > 0, lane, o);
 #pragma unroll
     for (int x = 0; x < CV; ++x) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        delta = __builtin_fmaf(T::low(o[x][w]), T::low(grad[x][w]), delta);
-        delta = __builtin_fmaf(T::high(o[x][w]), T::high(grad[x][w]), delta);
+        if (PART != 2) delta = __builtin_fmaf(T::low(o[x][w]), T::low(grad[x][w]), delta);
+        if (PART != 2) delta = __builtin_fmaf(T::high(o[x][w]), T::high(grad[x][w]), delta);
         if (T::kNarrowRange) {
           largest = __builtin_fmaxf(largest, __builtin_fabsf(T::low(grad[x][w])));
           largest = __builtin_fmaxf(largest, __builtin_fabsf(T::high(grad[x][w])));
@@ -818,20 +825,23 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
     delta = add_halves(delta);
   }
   const BackwardSpace<C> space{heads * rows};
-  if (exists && half == 0) ws[head * rows + row] = delta;
+  if (PART != 2 && exists && half == 0) ws[head * rows + row] = delta;
+  if (PART == 2 && exists) delta = ws[head * rows + row];
   float lift = 1.0f;
   if (T::kNarrowRange) {
     largest = max_halves(largest);
     lift = lift_of<T>(largest);
 #pragma unroll
     for (int step = 1; step < 32; step *= 2) largest = __builtin_fmaxf(largest, __shfl_xor(largest, step));
-    if (lane == 0) largestOf[wave] = largest;
+    if (PART != 2 && lane == 0) ws[space.largest() + (head * tiles + tile) * NW + wave] = largest;
   }
-  float sums = exists && seen > 0 ? lse[(b * C::H + hkv * C::G + g) * e.sq + i] : neg_inf();
+  float sums = PART != 2 && exists && seen > 0 ? lse[(b * C::H + hkv * C::G + g) * e.sq + i] : neg_inf();
   // (a row without keys: exp2(s - inf) = 0)
   const bool lost = C::ADDED && __builtin_fabsf(sums) > kLargeLse && __builtin_fabsf(sums) < __builtin_inff();
   sums = sums == neg_inf() ? __builtin_inff() : C::ADDED ? sums : sums * kLog2e;
   float rest = 0.0f;
+  if (PART == 2 && exists) sums = ws[space.top(head * rows + row)];
+  if (PART == 2 && C::ADDED && exists) rest = ws[space.rest(head * rows + row)];
   const float c = C::ADDED ? scale : scale * kLog2e;
 
   f32x16 acc[TK];
@@ -850,11 +860,11 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
     vload.load(vb, tid, [&](int r) { return static_cast<u32>(r * static_cast<int>(values.step)); });
   };
 #pragma unroll
-  for (int x = 0; x < kTiles; ++x) {
+  for (int x = 0; PART != 1 && x < kTiles; ++x) {
     clear_padding<kTile, DK, kThreads>(ktiles[x], tid);
     clear_padding<kTile, DV, kThreads>(vtiles[x], tid);
   }
-  if (end > 0) {
+  if (PART != 1 && end > 0) {
     fetch(0);
     const TileLoad<kTile, DK, kThreads> know = kload;
     const TileLoad<kTile, DV, kThreads> vnow = vload;
@@ -865,13 +875,8 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
     vload.store(vtiles[1], tid);
   }
   __syncthreads();
-  if (T::kNarrowRange && tid == 0) {
-    float all = 0.0f;
-    for (int w = 0; w < NW; ++w) all = __builtin_fmaxf(all, largestOf[w]);
-    ws[space.largest() + head * tiles + tile] = all;
-  }
   const long maskAt = C::MASK != 0 ? mask_row<C>(b, hkv * C::G + g, exists ? i : 0, e) : 0;
-  if constexpr (C::ADDED) {
+  if constexpr (C::ADDED && PART != 2) {
     if (__any(lost)) {   // (by this wavefront alone, keys straight from memory: such rows are rare)
       float top = neg_inf(), sum = 0.0f;
       for (int k0 = 0; __any(k0 < seen); k0 += 32) {
@@ -902,7 +907,8 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
     }
     if (exists && half == 0) ws[space.rest(head * rows + row)] = rest;
   }
-  if (exists && half == 0) ws[space.top(head * rows + row)] = sums;
+  if (PART != 2 && exists && half == 0) ws[space.top(head * rows + row)] = sums;
+  if (PART == 1) return;
   const MaskRow<C> maskRow(mask, maskAt, e);
   // What the mask says of 32 keys and the next, where registers allow.
   constexpr bool kAhead = padded(DK) + padded(DV) <= 192 || sizeof(typename MaskRow<C>::E) < 4;
@@ -1034,23 +1040,32 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
 // APART: above 256 channels (keys and values together) the accumulators of both leave too little room for the operands: a
 // workgroup computes dk or dv, and the scores are computed twice (gradient of 2 x 2048, 32/8 heads of 256, causal: 941 us
 // instead of 2481; of 192: 765 instead of 795).
-template <typename C, int NW, int RG, int NWQ, bool SPLIT, bool APART>
-AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const void *v, const void *mask,
-                           const int *qlens, const int *klens, void *dk, void *dv, float *ws, Extents e, float scale, int splits) {
-  typedef typename C::T T;
-  constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, CV = (DV + 15) / 16, TK = padded(DK) / 32, TV = padded(DV) / 32, kThreads = 64 * NW * RG, kRound = kTileRows * RG;
+template <typename C, int NW, int RG>
+struct KeysLds {
   // From 192 channels on (keys and values together) the accumulators and the wavefront's own operands would leave room for
   // one wavefront per SIMD: its keys lie in LDS then, and two fit.
-  constexpr bool kKeysInLds = padded(DK) + padded(DV) > 192;
-  __shared__ __attribute__((aligned(16))) u8 lds[2][kRound * (pitch(DK) + pitch(DV))];
-  __shared__ __attribute__((aligned(16))) u8 ownKeys[kKeysInLds ? kRows * NW * own_pitch(DK) : 16];
-  constexpr int kStates = C::ADDED ? 3 : 2;   // of a row: delta, top and rest (BackwardSpace)
-  __shared__ __attribute__((aligned(16))) float stateOf[2][kStates][kRound];
+  static constexpr bool kKeysInLds = padded(C::DK) + padded(C::DV) > 192;
+  static constexpr int kRound = kTileRows * RG, kStates = C::ADDED ? 3 : 2;   // states of a row: delta, top and rest (BackwardSpace)
+  __attribute__((aligned(16))) u8 rows[2][kRound * (pitch(C::DK) + pitch(C::DV))];
+  __attribute__((aligned(16))) u8 own[kKeysInLds ? kRows * NW * own_pitch(C::DK) : 16];
+  __attribute__((aligned(16))) float states[2][kStates][kRound];
+};
+template <typename C, int NW, int RG, int NWQ, bool SPLIT, bool APART>
+AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const void *v, const void *mask,
+                           const int *qlens, const int *klens, void *dk, void *dv, float *ws, Extents e, float scale, int splits, long blockId, KeysLds<C, NW, RG> &memory) {
+  typedef typename C::T T;
+  constexpr int DK = C::DK, DV = C::DV, CK = (DK + 15) / 16, CV = (DV + 15) / 16, TK = padded(DK) / 32, TV = padded(DV) / 32, kThreads = 64 * NW * RG, kRound = kTileRows * RG;
+  typedef KeysLds<C, NW, RG> Memory;
+  constexpr bool kKeysInLds = Memory::kKeysInLds;
+  constexpr int kStates = Memory::kStates;
+  auto &lds = memory.rows;
+  auto &ownKeys = memory.own;
+  auto &stateOf = memory.states;
   auto run = [&](auto which) __attribute__((always_inline)) {
     constexpr bool kDk = decltype(which)::value != 2, kDv = decltype(which)::value != 1;
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, group = __builtin_amdgcn_readfirstlane(tid >> 6) / NW, half = lane >> 5;
     const long rows = e.sq * C::G, heads = e.batch * C::HKV;
-    const long block = APART ? blockIdx.x / 2 : blockIdx.x, id = SPLIT ? block / splits : block;
+    const long block = APART ? blockId / 2 : blockId, id = SPLIT ? block / splits : block;
     const int split = SPLIT ? static_cast<int>(block % splits) : 0;
     long head, tile;
     head_and_tile(id, heads, head, tile);
@@ -1080,9 +1095,9 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     if (kDk) load_own<DV>(values.base + (counts ? key : 0) * values.step, counts, lane, val);
     float lift = 1.0f;
     if (T::kNarrowRange) {
-      const long tilesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ);
+      const long wavesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ) * NWQ;
       float largest = 0.0f;
-      for (long t = lane; t < tilesQ; t += 64) largest = __builtin_fmaxf(largest, ws[space.largest() + head * tilesQ + t]);
+      for (long t = lane; t < wavesQ; t += 64) largest = __builtin_fmaxf(largest, ws[space.largest() + head * wavesQ + t]);
 #pragma unroll
       for (int step = 1; step < 64; step *= 2) largest = __builtin_fmaxf(largest, __shfl_xor(largest, step));
       lift = lift_of<T>(largest);
@@ -1268,8 +1283,8 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     if (key >= e.sk) return;
     const float back = scale / lift;
     if constexpr (SPLIT) {
-      const long tilesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ);
-      float *to = ws + space.sums(heads * tilesQ) + ((split * heads + head) * e.sk + key) * BackwardSpace<C>::kSums;
+      const long wavesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ) * NWQ;
+      float *to = ws + space.sums(heads * wavesQ) + ((split * heads + head) * e.sk + key) * BackwardSpace<C>::kSums;
 #pragma unroll
       for (int d = kDk ? 0 : TK; d < (kDv ? TK + TV : TK); ++d) {
 #pragma unroll
@@ -1302,7 +1317,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     if (kDv && dv != nullptr) store(const_cast<char *>(dvalues.base) + key * dvalues.step, DV, accv, TV, 1.0f);
   };
   if constexpr (APART) {
-    if (blockIdx.x % 2 == 0) {
+    if (blockId % 2 == 0) {
       run(IntTag<1>());
     } else {
       run(IntTag<2>());
@@ -1317,12 +1332,12 @@ template <typename C, int NWQ>
 AKG_DEV void backward_join(const float *ws, void *dk, void *dv, Extents e, int splits) {
   typedef typename C::T T;
   constexpr int DK = C::DK, DV = C::DV, kFours = (DK + DV) / 4, kSums = BackwardSpace<C>::kSums;
-  const long rows = e.sq * C::G, heads = e.batch * C::HKV, tilesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ);
+  const long rows = e.sq * C::G, heads = e.batch * C::HKV, wavesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ) * NWQ;
   const long at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x, row = at / kFours;
   if (row >= heads * e.sk) return;
   const int c = static_cast<int>(at % kFours) * 4;
   const bool isK = c < DK;
-  const float *from = ws + BackwardSpace<C>{heads * rows}.sums(heads * tilesQ) + row * kSums + (isK ? c : padded(DK) + c - DK);
+  const float *from = ws + BackwardSpace<C>{heads * rows}.sums(heads * wavesQ) + row * kSums + (isK ? c : padded(DK) + c - DK);
   f32x4 sum = {};
   for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const f32x4 *>(from + s * heads * e.sk * kSums);
   const long head = row / e.sk, key = row % e.sk, b = head / C::HKV, hkv = head % C::HKV;
