@@ -185,8 +185,8 @@ class LayerEmitter {
     if (s.dk % 8 != 0 || s.dv % 8 != 0 || s.dk > 256 || s.dv > 256) {
       throw LoweringError("op " + op_.name + ": the channels of a head must be a multiple of 8 up to 256");
     }
-    // row numbers and key numbers are 32-bit values, and so are byte offsets between the heads that share a tile of rows
-    if (s.rows >= (1LL << 31) - 512 || s.sk >= (1LL << 31) - 512) throw LoweringError("op " + op_.name + ": more than 2^31 rows");
+    // row numbers, key numbers and their sums are 32-bit values, and so are byte offsets between the heads that share a tile of rows
+    if (s.rows >= (1LL << 31) - 512 || s.sq + s.sk >= (1LL << 31) - 512) throw LoweringError("op " + op_.name + ": more than 2^31 rows");
     const int64_t widest = 2 * std::max(s.dk, s.dv);
     if ((l_.headsFirst ? s.group * s.sq * widest : 64 * s.heads * widest) >= (1LL << 31) - 65536 || 64 * s.kvHeads * widest >= (1LL << 31) - 65536) {
       throw LoweringError("op " + op_.name + ": the rows of a tile lie more than 2 GiB apart");

@@ -160,7 +160,7 @@ template <typename C>
 AKG_DEV int keys_seen(long i, int ql, int kl) {
   if (i >= ql) return 0;
   if (!C::CAUSAL) return kl;
-  const int n = kl - (ql - 1 - static_cast<int>(i));
+  const int n = static_cast<int>(i) + kl - ql + 1;
   return n < 0 ? 0 : (n < kl ? n : kl);
 }
 

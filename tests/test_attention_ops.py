@@ -505,6 +505,20 @@ def test_launches_of_too_many_threads_are_refused():
     refused(attention_text(q=(1 << 22, 1, 16, 64), k=(1 << 22, 1, 16, 64), v=(1 << 22, 1, 16, 64)), -4, "more threads")
 
 
+def test_rows_and_keys_whose_numbers_pass_32_bits_are_refused():
+    n = 1 << 30
+    refused(attention_text(q=(1, n, 1, 8), k=(1, n, 1, 8), v=(1, n, 1, 8)), -4, "2^31 rows")
+    refused(attention_text(q=(1, n, 2, 8), k=(1, 8, 1, 8), v=(1, 8, 1, 8)), -4, "2^31 rows")
+
+
+def test_small_gradients_are_one_launch_beside_the_rows_own(tmp_path):
+    def kernel(s):
+        b = builder()
+        dout, q, k, v, out = (b.input([2, s, 4, 64], "float16") for _ in range(5))
+        return driver.HipKernel(b.dumps(op_desc.attention_grad(b, dout, q, k, v, out, b.input([2, 4, s], "float32"))), out_dir=str(tmp_path))
+    assert "akg_K" in kernel(200).source and "akg_K" not in kernel(8192).source
+
+
 def test_rows_of_the_gradient_are_shared_where_keys_are_few(tmp_path):
     def kernel(s, h, hkv, batch=1):
         b = builder()
