@@ -186,7 +186,7 @@ class LayerEmitter {
       throw LoweringError("op " + op_.name + ": the channels of a head must be a multiple of 8 up to 256");
     }
     // row numbers, key numbers and their sums are 32-bit values, and so are byte offsets between the heads that share a tile of rows
-    if (s.rows >= (1LL << 31) - 512 || s.sq + s.sk >= (1LL << 31) - 512) throw LoweringError("op " + op_.name + ": more than 2^31 rows");
+    if (s.rows >= (1LL << 31) - 512 || s.sq + s.sk >= (1LL << 31) - 8192) throw LoweringError("op " + op_.name + ": more than 2^31 rows");
     const int64_t widest = 2 * std::max(s.dk, s.dv);
     if ((l_.headsFirst ? s.group * s.sq * widest : 64 * s.heads * widest) >= (1LL << 31) - 65536 || 64 * s.kvHeads * widest >= (1LL << 31) - 65536) {
       throw LoweringError("op " + op_.name + ": the rows of a tile lie more than 2 GiB apart");

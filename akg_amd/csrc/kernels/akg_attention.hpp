@@ -530,9 +530,9 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   const int most = row0 / C::G < ql ? keys_seen<C>(lastI, ql, kl) : 0;
   int first = 0, end = most;
   if (SPLIT) {
-    const long all = (most + kTile - 1) / kTile, each = (all + splits - 1) / splits * kTile, start = split * each;
-    first = start < most ? static_cast<int>(start) : most;
-    if (each < most - first) end = first + static_cast<int>(each);
+    const int all = (most + kTile - 1) / kTile, each = (all + splits - 1) / splits;
+    first = split * each * kTile < most ? split * each * kTile : most;   // (most + 64 kTile stays below 2^31: checked by the host)
+    end = first + each * kTile < most ? first + each * kTile : most;
   }
 
   const RowsOf<C, DK> qrows(q, b, hkv, e);
