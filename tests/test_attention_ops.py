@@ -352,6 +352,8 @@ WIDE = [
     ("float16", "BNSD", 2, 65, 130, 2, 2, 256, 8, False, "float32", None),
     ("float16", "BSND", 1, 40, 33, 2, 1, 40, 256, True, "bool", "padded"),
     ("bfloat16", "BNSD", 2, 96, 96, 3, 3, 136, 136, False, None, None),
+    ("bfloat16", "BSND", 4, 70, 200, 40, 40, 136, 64, True, None, None),        # one group of wavefronts, in one launch with dq
+    ("float16", "BSND", 2, 33, 257, 40, 10, 64, 136, False, "bool", "padded"),
 ]
 
 
