@@ -350,12 +350,35 @@ class LayerEmitter {
     auto queriesLds = [&](int part) { return "akg::attn::QueriesLds<akg_C, " + std::to_string(nwq) + ", " + std::to_string(part) + ">"; };
     const std::string keysLds = "akg::attn::KeysLds<akg_C, " + std::to_string(nwk) + ", " + std::to_string(rg) + ">", keysName = splits > 1 ? g_.name + "_keys" : k_.kernelName;
     const int hint = std::max(s.dk, s.dv) > 128 || nwk == 2 ? 0 : 2, part = together ? 1 : 0;
+    // float16: the largest value of every key head first, beside the rows' own launch or in one of its own
+    const bool bounds = in(0).dtype == DType::F16;
+    const int64_t slices = bounds ? std::min<int64_t>(ceilDiv(s.sk, 128), 256) : 0, rowGroups = s.keyHeads * tilesQ;
+    auto values = [&](const std::string &block) {
+      return "  akg::attn::slice_of_values<akg_C>(" + inName(3) + ", " + (l_.hasKeyLengths ? inName(6 + (l_.hasMask ? 1 : 0) + (l_.hasQueryLengths ? 1 : 0)) : std::string("nullptr")) +
+             ", akg_ws, " + extents + ", akg_batch * akg_C::HKV * ((akg_sq * akg_C::G + " + std::to_string(32 * nwq - 1) + ") / " + std::to_string(32 * nwq) + ") * " +
+             std::to_string(nwq) + ", " + block + ");\n";
+    };
     KernelPhase first, last;
+    if (bounds && !together) {
+      KernelPhase before;
+      before.kernelName = g_.name + "_values";
+      before.grid[0] = checkGrid(s.keyHeads * slices, 256);
+      before.block[0] = 256;
+      k_.earlierPhases.push_back(before);
+      o << kernel(before.kernelName, 256, args, values("blockIdx.x"));
+    }
     first.kernelName = g_.name + (together ? "_rows" : "_queries");
-    first.grid[0] = checkGrid(s.keyHeads * tilesQ, 64 * nwq);
+    first.grid[0] = checkGrid(rowGroups + (together ? s.keyHeads * slices : 0), 64 * nwq);
     first.block[0] = static_cast<unsigned>(64 * nwq);
     k_.earlierPhases.push_back(first);
-    o << kernel(first.kernelName, 64 * nwq, args, "  __shared__ " + queriesLds(part) + " akg_lds;\n" + queries(part, "blockIdx.x", "akg_lds"));
+    std::string rowsBody = "  __shared__ " + queriesLds(part) + " akg_lds;\n";
+    if (bounds && together) {
+      rowsBody += "  const long akg_rows = akg_batch * akg_C::HKV * ((akg_sq * akg_C::G + " + std::to_string(32 * nwq - 1) + ") / " + std::to_string(32 * nwq) + ");\n" +
+                  "  if (blockIdx.x < akg_rows) {\n" + queries(part, "blockIdx.x", "akg_lds") + "  } else {\n" + values("blockIdx.x - akg_rows") + "  }\n";
+    } else {
+      rowsBody += queries(part, "blockIdx.x", "akg_lds");
+    }
+    o << kernel(first.kernelName, 64 * nwq, args, rowsBody);
     if (together) {
       o << kernel(keysName, 256, args,
                   "  typedef " + queriesLds(2) + " akg_Q;\n  typedef " + keysLds + " akg_K;\n" +
@@ -363,15 +386,16 @@ class LayerEmitter {
                       "  const long akg_keys = akg_batch * akg_C::HKV * ((akg_sk + " + std::to_string(32 * nwk - 1) + ") / " + std::to_string(32 * nwk) + ");\n" +
                       "  if (blockIdx.x < akg_keys) {\n" + keys("blockIdx.x", "*reinterpret_cast<akg_K *>(akg_lds)") + "  } else {\n" +
                       queries(2, "blockIdx.x - akg_keys", "*reinterpret_cast<akg_Q *>(akg_lds)") + "  }\n");
-      last.grid[0] = checkGrid(groups + s.keyHeads * tilesQ, 256);
+      last.grid[0] = checkGrid(groups + rowGroups, 256);
     } else {
       o << kernel(keysName, 64 * nwk * rg, args, "  __shared__ " + keysLds + " akg_lds;\n" + keys("blockIdx.x", "akg_lds"), hint);
       last.grid[0] = checkGrid((apart ? 2 : 1) * groups * splits, 64 * nwk * rg);
     }
     last.block[0] = static_cast<unsigned>(64 * nwk * rg);
-    // per row delta and its log-sum (in two parts for an added mask), per wavefront of the first kernel the largest |dout|
+    // per row delta and its log-sum (in two parts for an added mask); float16: what bounds the gradients of the scores
+    // (attn::BackwardSpace)
     const bool added = l_.hasMask && in(6).dtype != DType::Bool;
-    k_.workspaceBytes = static_cast<uint64_t>(4 * s.keyHeads * ((added ? 3 : 2) * s.rows + tilesQ * nwq));
+    k_.workspaceBytes = static_cast<uint64_t>(4 * s.keyHeads * ((added ? 3 : 2) * s.rows + (bounds ? 2 * tilesQ * nwq + slices : 0)));
     if (splits > 1) {
       last.kernelName = keysName;
       k_.earlierPhases.push_back(last);

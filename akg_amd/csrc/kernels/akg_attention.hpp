@@ -737,14 +737,23 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------
-// float16 holds nothing below 2^-24, and a score's gradient is a probability times a difference: where the largest
-// |dout| of the rows concerned is below 1 the gradients of the scores are computed times the power of two that lifts it
-// there, and the result is scaled back in float32. (bfloat16 has the exponents of float32: factor 1.)
+// float16 ends at 65504 and has no digits left below 2^-24, and what the matrix units take as float16 is a probability, at
+// most 1 and over a long axis arbitrarily small, and a score's gradient, that probability times a difference with
+//   |dp - delta| <= B = sum |dout| max |v| + |delta|   (sums over the row's channels, the maximum over the keys of its key head).
+// The gradients of the scores are therefore computed times the power of two that puts B into [2^13, 2^14) (dq: B of the row; dk:
+// the largest of the key head), and the probabilities of dv times 2^13: a probability that float32 puts a little above 1 still
+// fits, normal numbers reach down to 2^-27 of the largest. The results are scaled back in float32. (bfloat16 has the
+// exponents of float32: factor 1.)
+constexpr float kProbabilityLift = 13.0f;   // exponent of 2
 template <typename T>
-AKG_DEV float lift_of(float largest) {
-  if (!T::kNarrowRange || !(largest < 1.0f) || largest == 0.0f) return 1.0f;
-  const int up = -__builtin_amdgcn_frexp_expf(largest);   // largest = m 2^-up, 1/2 <= m < 1
-  return __builtin_ldexpf(1.0f, up < 100 ? up : 100);
+AKG_DEV float lift_of(float bound) {
+  if (!T::kNarrowRange || !(bound > 0.0f && bound < __builtin_inff())) return 1.0f;
+  return __builtin_ldexpf(1.0f, 14 - __builtin_amdgcn_frexp_expf(bound));   // bound = m 2^exponent, 1/2 <= m < 1; lifts from 2^-27 to 2^62
+}
+AKG_DEV float max_lanes(float v) {
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) v = __builtin_fmaxf(v, __shfl_xor(v, step));
+  return v;
 }
 
 // What the backward kernels know of a row's sum: exp(score - lse) = 2^((score - top) log2 e - rest), rest = 0 where lse says
@@ -753,18 +762,62 @@ AKG_DEV float lift_of(float largest) {
 constexpr float kLargeLse = 4096.0f;
 
 // Places in the workspace of the backward kernels, in floats: delta and top of every row (top: times log2 e where no mask is
-// added; infinite for a row without keys, whose probabilities then are 2^-inf = 0), for an added mask the rest, and the
-// largest |dout| of every wavefront of the first kernel.
+// added; infinite for a row without keys, whose probabilities then are 2^-inf = 0), for an added mask the rest; for float16
+// what bounds the gradients of the scores: the largest sum |dout| and |delta| of every wavefront of the first kernel, and the
+// largest |v| of every slice of a key head's keys.
 template <typename C>
 struct BackwardSpace {
-  long rows;   // of all key heads
+  long rows;         // of all key heads
+  long wavefronts;   // of the first kernel, over all key heads
+  static constexpr bool kBounds = C::T::kNarrowRange;
   AKG_DEV long top(long row) const { return rows + row; }
   AKG_DEV long rest(long row) const { return 2 * rows + row; }
-  AKG_DEV long largest() const { return (C::ADDED ? 3 : 2) * rows; }
+  AKG_DEV long sizes(long wavefront) const { return (C::ADDED ? 3 : 2) * rows + 2 * wavefront; }
+  AKG_DEV long values(long slice) const { return sizes(wavefronts) + slice; }
   // behind them, to the next 256 bytes: sums of dk and dv over ranges of rows, [ranges][key heads][keys][padded channels of both]
   static constexpr int kSums = padded(C::DK) + padded(C::DV);
-  AKG_DEV long sums(long wavefronts) const { return (largest() + wavefronts + 63) / 64 * 64; }
+  AKG_DEV long sums(long heads, long sk) const { return ((kBounds ? values(heads * value_slices(sk)) : sizes(0)) + 63) / 64 * 64; }
+  // Slices of a key head's keys, 128 keys each or more.
+  AKG_DEV static long value_slices(long sk) { return sk <= 128 * 256 ? (sk + 127) / 128 : 256; }
+  // The largest |v| of key head `head`, in every lane.
+  AKG_DEV float largest_value(const float *ws, long head, long sk, int lane) const {
+    const long slices = value_slices(sk);
+    float largest = 0.0f;
+    for (long t = lane; t < slices; t += 64) largest = __builtin_fmaxf(largest, ws[values(head * slices + t)]);
+    return max_lanes(largest);
+  }
 };
+
+// The largest |v| of one slice of the keys of a key head, by a workgroup of 256 threads: a launch of its own, or workgroups
+// beside those that find what else the rows need. It reads the values once more: float16 gradients of 8 x 200 x 12 heads of 64
+// take 20.9 us with it and 19.7 without, of 1 x 1024 x 16/4 of 128 79.3 and 75.2, of 2 x 4096 x 32/8 of 128 1068 and 1060.
+template <typename C>
+AKG_DEV void slice_of_values(const void *v, const int *klens, float *ws, Extents e, long wavefronts, long block) {
+  typedef typename C::T T;
+  __shared__ float tops[4];
+  const long heads = e.batch * C::HKV, slices = BackwardSpace<C>::value_slices(e.sk), head = block / slices, slice = block % slices;
+  const long b = head / C::HKV, hkv = head % C::HKV, each = (e.sk + slices - 1) / slices;
+  const int kl = clamped_length<C>(klens, b, e.sk), tid = static_cast<int>(threadIdx.x);
+  const KeysOf<C, C::DV> values(v, b, hkv, e);
+  const long first = slice * each, left = kl - first < each ? kl - first : each;
+  constexpr int kPerRow = C::DV / 8;
+  float largest = 0.0f;
+#pragma unroll 4
+  for (long c = tid; c < left * kPerRow; c += 256) {
+    const u32x4 x = *reinterpret_cast<const u32x4 *>(values.base + (first + c / kPerRow) * values.step + c % kPerRow * 16);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      largest = __builtin_fmaxf(largest, __builtin_fmaxf(__builtin_fabsf(T::low(x[w])), __builtin_fabsf(T::high(x[w]))));
+    }
+  }
+  largest = max_lanes(largest);
+  if ((tid & 63) == 0) tops[tid >> 6] = largest;
+  __syncthreads();
+  if (tid == 0) {
+    const BackwardSpace<C> space{heads * e.sq * C::G, wavefronts};
+    ws[space.values(head * slices + slice)] = __builtin_fmaxf(__builtin_fmaxf(tops[0], tops[1]), __builtin_fmaxf(tops[2], tops[3]));
+  }
+}
 
 // dq of 32 rows a wavefront: keys and values pass by in tiles, 32 keys a step: the scores and their gradients' products, then
 // the gradients of the scores (vector instructions) between the matrix instructions that multiply those of the step before.
@@ -806,7 +859,9 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
   u32x4 own[CK], grad[CV];
   load_own<DK>(qrows.base + qrows.offset(exists ? row : 0), seen > 0, lane, own);
   load_own<DV>(grows.base + grows.offset(exists ? row : 0), seen > 0, lane, grad);
-  float delta = 0.0f, largest = 0.0f;
+  const BackwardSpace<C> space{heads * rows, heads * tiles * NW};
+  const float topValue = T::kNarrowRange && PART != 1 ? space.largest_value(ws, head, e.sk, lane) : 0.0f;
+  float delta = 0.0f, spread = 0.0f;   // spread: sum |dout|
   {
     u32x4 o[CV] = {};
     if (PART != 2) load_own<DV>(orows.base + orows.offset(exists ? row : 0), seen > 0, lane, o);
@@ -816,24 +871,23 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
       for (int w = 0; w < 4; ++w) {
         if (PART != 2) delta = __builtin_fmaf(T::low(o[x][w]), T::low(grad[x][w]), delta);
         if (PART != 2) delta = __builtin_fmaf(T::high(o[x][w]), T::high(grad[x][w]), delta);
-        if (T::kNarrowRange) {
-          largest = __builtin_fmaxf(largest, __builtin_fabsf(T::low(grad[x][w])));
-          largest = __builtin_fmaxf(largest, __builtin_fabsf(T::high(grad[x][w])));
-        }
+        if (T::kNarrowRange) spread += __builtin_fabsf(T::low(grad[x][w])) + __builtin_fabsf(T::high(grad[x][w]));
       }
     }
     delta = add_halves(delta);
   }
-  const BackwardSpace<C> space{heads * rows};
   if (PART != 2 && exists && half == 0) ws[head * rows + row] = delta;
   if (PART == 2 && exists) delta = ws[head * rows + row];
   float lift = 1.0f;
   if (T::kNarrowRange) {
-    largest = max_halves(largest);
-    lift = lift_of<T>(largest);
-#pragma unroll
-    for (int step = 1; step < 32; step *= 2) largest = __builtin_fmaxf(largest, __shfl_xor(largest, step));
-    if (PART != 2 && lane == 0) ws[space.largest() + (head * tiles + tile) * NW + wave] = largest;
+    spread = add_halves(spread);
+    if (PART != 1) lift = lift_of<T>(__builtin_fmaf(spread, topValue, __builtin_fabsf(delta)));
+    if (PART != 2) {
+      const float largest = max_lanes(spread), largestDelta = max_lanes(__builtin_fabsf(delta));
+      const long at = space.sizes((head * tiles + tile) * NW + wave);
+      if (lane == 0) ws[at] = largest;
+      if (lane == 0) ws[at + 1] = largestDelta;
+    }
   }
   float sums = PART != 2 && exists && seen > 0 ? lse[(b * C::H + hkv * C::G + g) * e.sq + i] : neg_inf();
   // (a row without keys: exp2(s - inf) = 0)
@@ -1077,7 +1131,8 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     const bool counts = key < kl;
     const KeysOf<C, DK> keys(k, b, hkv, e);
     const KeysOf<C, DV> values(v, b, hkv, e);
-    const BackwardSpace<C> space{heads * rows};
+    const long wavesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ) * NWQ;
+    const BackwardSpace<C> space{heads * rows, heads * wavesQ};
     u32x4 own[kKeysInLds ? 1 : CK], val[CV] = {};
     if constexpr (kKeysInLds) {
       const int key00 = static_cast<int>(tile) * (kRows * NW);
@@ -1094,14 +1149,18 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     }
     if (kDk) load_own<DV>(values.base + (counts ? key : 0) * values.step, counts, lane, val);
     float lift = 1.0f;
-    if (T::kNarrowRange) {
-      const long wavesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ) * NWQ;
-      float largest = 0.0f;
-      for (long t = lane; t < wavesQ; t += 64) largest = __builtin_fmaxf(largest, ws[space.largest() + head * wavesQ + t]);
-#pragma unroll
-      for (int step = 1; step < 64; step *= 2) largest = __builtin_fmaxf(largest, __shfl_xor(largest, step));
-      lift = lift_of<T>(largest);
+    if (kDk && T::kNarrowRange) {
+      float largest = 0.0f, largestDelta = 0.0f;
+      for (long t = lane; t < wavesQ; t += 64) {
+        const long at = space.sizes(head * wavesQ + t);
+        largest = __builtin_fmaxf(largest, ws[at]);
+        largestDelta = __builtin_fmaxf(largestDelta, ws[at + 1]);
+      }
+      lift = lift_of<T>(__builtin_fmaf(max_lanes(largest), space.largest_value(ws, head, e.sk, lane), max_lanes(largestDelta)));
     }
+    // probabilities leave their exponential lifted: the gradients of the scores take that out of their own factor
+    constexpr float kLift = T::kNarrowRange ? kProbabilityLift : 0.0f, kUnlift = T::kNarrowRange ? 0x1p-13f : 1.0f;
+    const float liftBehind = lift * kUnlift;
     const float c = C::ADDED ? scale : scale * kLog2e;
     f32x16 acck[kDk ? TK : 1], accv[kDv ? TV : 1];
 #pragma unroll
@@ -1130,7 +1189,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     const Reader<DV> gread(lane);
     TileLoad<kRound, DK, kThreads> qload;
     TileLoad<kRound, DV, kThreads> gload;
-    // Rows behind the last one read zeros (nothing is asked of memory): their probabilities are 1 and their products 0.
+    // Rows behind the last one read zeros (nothing is asked of memory): their probabilities are 1 (lifted), their products 0.
     float state[kStates];
     auto fetch = [&](int r0, bool any) {
       const int i0 = r0 / C::G;
@@ -1153,7 +1212,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
       gload.store(lds[buf] + kRound * pitch(DK), tid);
       if (tid < kRound) {
 #pragma unroll
-        for (int x = 0; x < kStates; ++x) stateOf[buf][x][tid] = state[x];
+        for (int x = 0; x < kStates; ++x) stateOf[buf][x][tid] = x == kStates - 1 ? state[x] - kLift : state[x];
       }
     };
 #pragma unroll
@@ -1219,7 +1278,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
             float x = C::MASK != 0 ? s[r] - l4[z] : __builtin_fmaf(s[r], c, -l4[z]);
             if (C::ADDED) x = __builtin_fmaf(x, kLog2e, -o4[z]);
             s[r] = __builtin_amdgcn_exp2f(x);
-            if (kDk) dp[r] = s[r] * (T::kNarrowRange ? (dp[r] - d4[z]) * lift : dp[r] - d4[z]);
+            if (kDk) dp[r] = s[r] * (T::kNarrowRange ? (dp[r] - d4[z]) * liftBehind : dp[r] - d4[z]);
           }
         }
 #pragma unroll
@@ -1283,15 +1342,14 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     if (key >= e.sk) return;
     const float back = scale / lift;
     if constexpr (SPLIT) {
-      const long wavesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ) * NWQ;
-      float *to = ws + space.sums(heads * wavesQ) + ((split * heads + head) * e.sk + key) * BackwardSpace<C>::kSums;
+      float *to = ws + space.sums(heads, e.sk) + ((split * heads + head) * e.sk + key) * BackwardSpace<C>::kSums;
 #pragma unroll
       for (int d = kDk ? 0 : TK; d < (kDv ? TK + TV : TK); ++d) {
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
           f32x4 x;
 #pragma unroll
-          for (int z = 0; z < 4; ++z) x[z] = d < TK ? acck[kDk ? d % TK : 0][4 * r4 + z] * back : accv[kDv && d >= TK ? d - TK : 0][4 * r4 + z];
+          for (int z = 0; z < 4; ++z) x[z] = d < TK ? acck[kDk ? d % TK : 0][4 * r4 + z] * back : accv[kDv && d >= TK ? d - TK : 0][4 * r4 + z] * kUnlift;
           *reinterpret_cast<f32x4 *>(to + 32 * d + 8 * r4 + 4 * half) = x;
         }
       }
@@ -1314,7 +1372,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     const KeysOf<C, DK> dkeys(dk, b, hkv, e);
     const KeysOf<C, DV> dvalues(dv, b, hkv, e);
     if (kDk && dk != nullptr) store(const_cast<char *>(dkeys.base) + key * dkeys.step, DK, acck, TK, back);
-    if (kDv && dv != nullptr) store(const_cast<char *>(dvalues.base) + key * dvalues.step, DV, accv, TV, 1.0f);
+    if (kDv && dv != nullptr) store(const_cast<char *>(dvalues.base) + key * dvalues.step, DV, accv, TV, kUnlift);
   };
   if constexpr (APART) {
     if (blockId % 2 == 0) {
@@ -1337,7 +1395,7 @@ AKG_DEV void backward_join(const float *ws, void *dk, void *dv, Extents e, int s
   if (row >= heads * e.sk) return;
   const int c = static_cast<int>(at % kFours) * 4;
   const bool isK = c < DK;
-  const float *from = ws + BackwardSpace<C>{heads * rows}.sums(heads * wavesQ) + row * kSums + (isK ? c : padded(DK) + c - DK);
+  const float *from = ws + BackwardSpace<C>{heads * rows, heads * wavesQ}.sums(heads, e.sk) + row * kSums + (isK ? c : padded(DK) + c - DK);
   f32x4 sum = {};
   for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const f32x4 *>(from + s * heads * e.sk * kSums);
   const long head = row / e.sk, key = row % e.sk, b = head / C::HKV, hkv = head % C::HKV;
