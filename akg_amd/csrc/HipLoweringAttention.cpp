@@ -321,9 +321,12 @@ class LayerEmitter {
     // and one (5 x 1773 x 8/4 heads of 96, causal, with a mask: 312, 240).
     const bool crowded = l_.hasMask && ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32) > 4;
     const bool apart = ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32) > 8;   // (dk and dv by workgroups of their own)
-    const int64_t whole = s.keyHeads * ceilDiv(s.sk, crowded ? 64 : 128);
+    // (64 keys also where 128 rows of keys or values lie too far apart for 32-bit offsets)
+    const bool far = !l_.headsFirst && 128 * s.kvHeads * 2 * std::max(s.dk, s.dv) >= (1LL << 31) - 65536;
+    const bool few = crowded || far;
+    const int64_t whole = s.keyHeads * ceilDiv(s.sk, few ? 64 : 128);
     const int64_t splits = std::max<int64_t>(1, std::min((l_.causal ? 2 : 1) * cus_ / whole, s.rows / 512));
-    const int nwk = !crowded && (splits > 1 || whole >= cus_) ? 4 : 2;
+    const int nwk = !few && (splits > 1 || whole >= cus_) ? 4 : 2;
     const int64_t groups = s.keyHeads * ceilDiv(s.sk, 32 * nwk);
     // Small problems: what both kernels need of the rows in a launch of its own, then both in one launch, side by side, while
     // neither fills the card (8 x 200 x 12 heads of 64: 18.8 us instead of 24.0, 2 x 512 x 12 of 64 19.6 instead of 28.5; with
