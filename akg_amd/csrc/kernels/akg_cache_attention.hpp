@@ -12,8 +12,10 @@
  *   scores: lane (token l % 16, g = l / 16) reads the 16 channels 64 u + 16 g ... of its token
  *   output: lane (l % 16, g) reads a few adjacent channels of the tokens 4 g .. 4 g + 3 of both blocks of sixteen
  * The scale of a key block multiplies the scores in float32. That of a value block multiplies the probabilities, which
- * are rounded to float16 behind it: relative to the power of two above the largest scale so far, so that they stay in
- * [0, 1] however small the scales are (the accumulators follow by exact powers of two).
+ * are rounded to float16 behind it (2^-11 of each): relative to a power of two that is within a factor of two of the row's
+ * heaviest product of both so far, so that they stay below 2 and the heaviest keep their digits, whatever scales lie on
+ * blocks that the row does not attend to. That power is the row's own, found from a second running maximum, of score + log2
+ * of the scale, and the accumulators follow it exactly.
  *
  * 32 sequences of 8192 to 16384 tokens, one query of 32 heads over 8 of 128 channels, take 168 us: 4.8 TB/s of the 5.2 that
  * a copy reaches. Short ones wait for what depends on one another (length, block numbers, blocks, the other wavefronts, the
@@ -147,14 +149,18 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
 
   acc4 acc[RT][4 * NU];
   float top[RT], sum[RT];
+  float heaviest[RT];    // maximum of score + exponent of the value scale (2^exponent is above the scale, at most twice it)
+  int reference[RT];     // accumulators are in units of 2^reference (behind the maximum)
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     top[rt] = neg_inf();
     sum[rt] = 0.0f;
+    heaviest[rt] = neg_inf();
+    reference[rt] = 0;
 #pragma unroll
     for (int d = 0; d < 4 * NU; ++d) acc[rt][d] = {};
   }
-  int reference = -1000;   // accumulators are in units of 2^reference
+  int lowest = -250;   // of the references: 2^-120 of the largest scale so far, so that scales over references stay finite
 
   struct Step {
     u32x4 k[2][NU];
@@ -234,21 +240,20 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
         }
       }
     }
-    // the scales of the values, relative to a power of two that only grows
-    const float larger = __builtin_fmaxf(__builtin_fabsf(now.vs[0]), __builtin_fabsf(now.vs[1]));
-    int down = 0;
-    if (larger > 0.0f && larger < __builtin_inff()) {
-      const int exponent = __builtin_amdgcn_frexp_expf(larger);
-      if (exponent > reference) {
-        down = reference - exponent;
-        reference = exponent;
-      }
+    // exponents of the scales of the values (zero, and what is no number, weighs nothing)
+    float exponent[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float size = __builtin_fabsf(now.vs[x]);
+      const bool weighs = size > 0.0f && size < __builtin_inff();
+      const int e = __builtin_amdgcn_readfirstlane(weighs ? __builtin_amdgcn_frexp_expf(size) : -1000);   // (the same in all lanes)
+      exponent[x] = e > -1000 ? static_cast<float>(e) : neg_inf();
+      lowest = e - 120 > lowest ? e - 120 : lowest;
     }
-    const float w[2] = {__builtin_ldexpf(now.vs[0], -reference), __builtin_ldexpf(now.vs[1], -reference)};
     u32x4 p[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float peak = neg_inf();
+      float peaks[2] = {neg_inf(), neg_inf()};
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const float f = factor[rt] * now.ks[x];
@@ -256,15 +261,27 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
         for (int r = 0; r < 4; ++r) {
           const long j = step * kStep + 16 * x + 4 * g + r;
           s[rt][x][r] = now.ok[x] && j < seen[rt] ? s[rt][x][r] * f : neg_inf();
-          peak = __builtin_fmaxf(peak, s[rt][x][r]);
+          peaks[x] = __builtin_fmaxf(peaks[x], s[rt][x][r]);
         }
       }
-      const float m = __builtin_fmaxf(top[rt], max_groups(peak));
+      const float peak = max_groups(__builtin_fmaxf(peaks[0], peaks[1]));
+      // (32 tokens of one block have one scale)
+      const float heavy = PAGE % kStep == 0 ? peak + exponent[0] : max_groups(__builtin_fmaxf(peaks[0] + exponent[0], peaks[1] + exponent[1]));
+      const float m = __builtin_fmaxf(top[rt], peak);
       const float base = m == neg_inf() ? 0.0f : m;
       const float shrink = __builtin_amdgcn_exp2f(top[rt] - base);
       top[rt] = m;
       sum[rt] *= shrink;
-      const float all = __builtin_ldexpf(shrink, down);
+      const float before = heaviest[rt];
+      heaviest[rt] = __builtin_fmaxf(before, heavy);
+      int unit = reference[rt];
+      if (heaviest[rt] > neg_inf()) {
+        unit = static_cast<int>(__builtin_floorf(__builtin_fmaxf(heaviest[rt] - base, -250.0f)));   // (at most 128)
+        unit = unit > lowest ? unit : lowest;
+      }
+      const float all = __builtin_ldexpf(shrink, before > neg_inf() ? reference[rt] - unit : 0);   // (at most 2)
+      reference[rt] = unit;
+      const float w[2] = {__builtin_ldexpf(now.vs[0], -unit), __builtin_ldexpf(now.vs[1], -unit)};
 #pragma unroll
       for (int d = 0; d < 4 * NU; ++d) {
 #pragma unroll
@@ -318,7 +335,7 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
       tops[wave][n] = top[rt];
       sums[wave][n] = own;
     }
-    const float unit = reference > -1000 ? __builtin_ldexpf(1.0f, reference) : 0.0f;
+    const float unit = __builtin_ldexpf(1.0f, reference[rt]);
 #pragma unroll
     for (int d = 0; d < 4 * NU; ++d) {
 #pragma unroll
