@@ -281,7 +281,11 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
       }
       const float all = __builtin_ldexpf(shrink, before > neg_inf() ? reference[rt] - unit : 0);   // (at most 2)
       reference[rt] = unit;
-      const float w[2] = {__builtin_ldexpf(now.vs[0], -unit), __builtin_ldexpf(now.vs[1], -unit)};
+      float w[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {   // (a block that the row does not see may have any scale: 0 NaN is no number)
+        w[x] = step * kStep + 16 * x < seen[rt] ? __builtin_ldexpf(now.vs[x], -unit) : 0.0f;
+      }
 #pragma unroll
       for (int d = 0; d < 4 * NU; ++d) {
 #pragma unroll

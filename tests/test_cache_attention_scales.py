@@ -117,3 +117,21 @@ def test_the_bound_sees_a_result_rounded_to_fewer_bits(case):
     bound = tight_bound(t, r, "float16")
     assert ((r["out"].to(torch.bfloat16).double() - r["out"]).abs() > bound).any()
     assert ((r["out"].to(torch.float16).double() - r["out"]).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("page,queries,per", [(16, 3, 3), (64, 2, 2), (32, 4, 40)])
+def test_scales_of_a_block_that_a_query_does_not_see(page, queries, per, bad, tmp_path):
+    """The last query's own token opens a block whose scales are no numbers: the queries before it never see that block."""
+    case = ("float16", 1, queries, 8, 2, 64, page, per, [(per - 1) * page + 1], None)
+    t = cache_case(case)
+    t = {n: t[n] for n in CACHE_ORDER}
+    last = int(t["block_table"][0, per - 1])
+    r = ref.cache_attention(**as_reference(t))
+    bound = tight_bound(t, r, "float16")
+    t["key_scale"][last] = bad
+    t["value_scale"][last] = bad
+    got = launch(describe_cache(t), list(t.values()), tmp_path)[0]
+    close(got[:, :-1], r["out"][:, :-1], bound[:, :-1], "queries before the last")
+    assert not torch.isfinite(got[:, -1]).any()
