@@ -313,6 +313,10 @@ class LayerEmitter {
 
   void attentionGrad() {
     const Sizes s = sizes(in(1), in(2), in(3));
+    // What nobody asks for is not computed: dk and dv need only the rows' values of the kernel of dq, and one of them alone
+    // not the products of the other.
+    const bool wantDq = wanted(0), wantKeys = wanted(1) || wanted(2);
+    const int which = wanted(1) && wanted(2) ? 0 : wanted(1) ? 1 : 2;
     const int rg = std::max(s.dk, s.dv) > 128 ? 1 : 2;
     // A workgroup of the kernel of dk and dv has 128 keys. Where that leaves CUs idle it shares the rows with others, 512 of
     // them each at least (causal: two to a CU, since the first keys have most rows), or has 64. us of the gradient unshared,
@@ -320,19 +324,20 @@ class LayerEmitter {
     // and 64: 24.9, 23.7. A mask beside more than 64 channels leaves the registers of two wavefronts a SIMD too few: 64 keys
     // and one (5 x 1773 x 8/4 heads of 96, causal, with a mask: 312, 240).
     const bool crowded = l_.hasMask && ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32) > 4;
-    const bool apart = ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32) > 8;   // (dk and dv by workgroups of their own)
+    const bool apart = which == 0 && ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32) > 8;   // (dk and dv by workgroups of their own)
     // (64 keys also where 128 rows of keys or values lie too far apart for 32-bit offsets)
     const bool far = !l_.headsFirst && 128 * s.kvHeads * 2 * std::max(s.dk, s.dv) >= (1LL << 31) - 65536;
     const bool few = crowded || far;
     const int64_t whole = s.keyHeads * ceilDiv(s.sk, few ? 64 : 128);
-    const int64_t splits = std::max<int64_t>(1, std::min((l_.causal ? 2 : 1) * cus_ / whole, s.rows / 512));
+    const int64_t splits = wantKeys ? std::max<int64_t>(1, std::min((l_.causal ? 2 : 1) * cus_ / whole, s.rows / 512)) : 1;
     const int nwk = !few && (splits > 1 || whole >= cus_) ? 4 : 2;
     const int64_t groups = s.keyHeads * ceilDiv(s.sk, 32 * nwk);
     // Small problems: what both kernels need of the rows in a launch of its own, then both in one launch, side by side, while
     // neither fills the card (8 x 200 x 12 heads of 64: 18.8 us instead of 24.0, 2 x 512 x 12 of 64 19.6 instead of 28.5; with
     // three workgroups a CU 2 x 2000 x 2001 x 16/4 of 128 with a mask takes 551 instead of 497).
-    const bool together = splits == 1 && nwk * rg == 4 && !apart && 2 * (groups + s.keyHeads * ceilDiv(s.rows, 128)) <= 5 * cus_;
-    const int nwq = together ? 4 : waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8);
+    const bool together = wantDq && wantKeys && splits == 1 && nwk * rg == 4 && !apart && 2 * (groups + s.keyHeads * ceilDiv(s.rows, 128)) <= 5 * cus_;
+    const bool rowsFirst = together || !wantDq;   // (the first launch leaves the rows' values only)
+    const int nwq = rowsFirst ? 4 : waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8);
     const int64_t tilesQ = ceilDiv(s.rows, 32 * nwq);
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n") << config(s, 6);
@@ -346,76 +351,75 @@ class LayerEmitter {
              lds + ");\n";
     };
     auto keys = [&](const std::string &block, const std::string &lds) {
-      return "  akg::attn::backward_keys<akg_C, " + std::to_string(nwk) + ", " + std::to_string(rg) + ", " + std::to_string(nwq) + ", " + flag(splits > 1) + ", " + flag(apart) +
-             ">(" + inName(0) + ", " + inName(1) + ", " + inName(2) + ", " + inName(3) + ", " + optionals(6) + ", " + outName(1) + ", " + outName(2) + ", akg_ws, " + extents + ", " +
-             number(l_.scale) + ", " + ranges + ", " + block + ", " + lds + ");\n";
+      return "  akg::attn::backward_keys<akg_C, " + std::to_string(nwk) + ", " + std::to_string(rg) + ", " + std::to_string(nwq) + ", " + flag(splits > 1) + ", " + flag(apart) + ", " +
+             std::to_string(which) + ">(" + inName(0) + ", " + inName(1) + ", " + inName(2) + ", " + inName(3) + ", " + optionals(6) + ", " + outName(1) + ", " + outName(2) + ", akg_ws, " +
+             extents + ", " + number(l_.scale) + ", " + ranges + ", " + block + ", " + lds + ");\n";
     };
     auto queriesLds = [&](int part) { return "akg::attn::QueriesLds<akg_C, " + std::to_string(nwq) + ", " + std::to_string(part) + ">"; };
-    const std::string keysLds = "akg::attn::KeysLds<akg_C, " + std::to_string(nwk) + ", " + std::to_string(rg) + ">", keysName = splits > 1 ? g_.name + "_keys" : k_.kernelName;
-    const int hint = std::max(s.dk, s.dv) > 128 || nwk == 2 ? 0 : 2, part = together ? 1 : 0;
-    // float16: the largest value of every key head first, beside the rows' own launch or in one of its own
-    const bool bounds = in(0).dtype == DType::F16;
-    const int64_t slices = bounds ? std::min<int64_t>(ceilDiv(s.sk, 128), 256) : 0, rowGroups = s.keyHeads * tilesQ;
-    auto values = [&](const std::string &block) {
+    const std::string keysLds = "akg::attn::KeysLds<akg_C, " + std::to_string(nwk) + ", " + std::to_string(rg) + ">";
+    const int64_t rowGroups = s.keyHeads * tilesQ;
+    // float16: the largest value of every key head first, beside the rows' own launch or in one of its own (dv alone needs none)
+    const bool bounds = in(0).dtype == DType::F16, values = bounds && (wantDq || wanted(1));
+    const int64_t slices = bounds ? std::min<int64_t>(ceilDiv(s.sk, 128), 256) : 0;
+    auto slicesOfValues = [&](const std::string &block) {
       return "  akg::attn::slice_of_values<akg_C>(" + inName(3) + ", " + (l_.hasKeyLengths ? inName(6 + (l_.hasMask ? 1 : 0) + (l_.hasQueryLengths ? 1 : 0)) : std::string("nullptr")) +
              ", akg_ws, " + extents + ", akg_batch * akg_C::HKV * ((akg_sq * akg_C::G + " + std::to_string(32 * nwq - 1) + ") / " + std::to_string(32 * nwq) + ") * " +
              std::to_string(nwq) + ", " + block + ");\n";
     };
-    KernelPhase first, last;
-    if (bounds && !together) {
-      KernelPhase before;
-      before.kernelName = g_.name + "_values";
-      before.grid[0] = checkGrid(s.keyHeads * slices, 256);
-      before.block[0] = 256;
-      k_.earlierPhases.push_back(before);
-      o << kernel(before.kernelName, 256, args, values("blockIdx.x"));
-    }
-    first.kernelName = g_.name + (together ? "_rows" : "_queries");
-    first.grid[0] = checkGrid(rowGroups + (together ? s.keyHeads * slices : 0), 64 * nwq);
-    first.block[0] = static_cast<unsigned>(64 * nwq);
-    k_.earlierPhases.push_back(first);
+    // The launches in their order; the last one is the kernel proper.
+    std::vector<KernelPhase> phases;
+    auto launch = [&](const char *suffix, bool last, int64_t grid, int threads, const std::string &body, int wavesPerSimd = 0) {
+      KernelPhase p;
+      p.kernelName = last ? k_.kernelName : g_.name + suffix;
+      p.grid[0] = checkGrid(grid, threads);
+      p.block[0] = static_cast<unsigned>(threads);
+      phases.push_back(p);
+      o << kernel(p.kernelName, threads, args, body, wavesPerSimd);
+    };
+    if (values && !rowsFirst) launch("_values", false, s.keyHeads * slices, 256, slicesOfValues("blockIdx.x"));
+    const int part = rowsFirst ? 1 : 0;
     std::string rowsBody = "  __shared__ " + queriesLds(part) + " akg_lds;\n";
-    if (bounds && together) {
+    if (values && rowsFirst) {
       rowsBody += "  const long akg_rows = akg_batch * akg_C::HKV * ((akg_sq * akg_C::G + " + std::to_string(32 * nwq - 1) + ") / " + std::to_string(32 * nwq) + ");\n" +
-                  "  if (blockIdx.x < akg_rows) {\n" + queries(part, "blockIdx.x", "akg_lds") + "  } else {\n" + values("blockIdx.x - akg_rows") + "  }\n";
+                  "  if (blockIdx.x < akg_rows) {\n" + queries(part, "blockIdx.x", "akg_lds") + "  } else {\n" + slicesOfValues("blockIdx.x - akg_rows") + "  }\n";
     } else {
       rowsBody += queries(part, "blockIdx.x", "akg_lds");
     }
-    o << kernel(first.kernelName, 64 * nwq, args, rowsBody);
-    if (together) {
-      o << kernel(keysName, 256, args,
-                  "  typedef " + queriesLds(2) + " akg_Q;\n  typedef " + keysLds + " akg_K;\n" +
-                      "  __shared__ __attribute__((aligned(16))) akg::u8 akg_lds[sizeof(akg_Q) > sizeof(akg_K) ? sizeof(akg_Q) : sizeof(akg_K)];\n" +
-                      "  const long akg_keys = akg_batch * akg_C::HKV * ((akg_sk + " + std::to_string(32 * nwk - 1) + ") / " + std::to_string(32 * nwk) + ");\n" +
-                      "  if (blockIdx.x < akg_keys) {\n" + keys("blockIdx.x", "*reinterpret_cast<akg_K *>(akg_lds)") + "  } else {\n" +
-                      queries(2, "blockIdx.x - akg_keys", "*reinterpret_cast<akg_Q *>(akg_lds)") + "  }\n");
-      last.grid[0] = checkGrid(groups + rowGroups, 256);
-    } else {
-      o << kernel(keysName, 64 * nwk * rg, args, "  __shared__ " + keysLds + " akg_lds;\n" + keys("blockIdx.x", "akg_lds"), hint);
-      last.grid[0] = checkGrid((apart ? 2 : 1) * groups * splits, 64 * nwk * rg);
-    }
-    last.block[0] = static_cast<unsigned>(64 * nwk * rg);
+    launch(rowsFirst ? "_rows" : "_queries", !wantKeys, rowGroups + (values && rowsFirst ? s.keyHeads * slices : 0), 64 * nwq, rowsBody);
     // per row delta and its log-sum (in two parts for an added mask); float16: what bounds the gradients of the scores
     // (attn::BackwardSpace)
     const bool added = l_.hasMask && in(6).dtype != DType::Bool;
     k_.workspaceBytes = static_cast<uint64_t>(4 * s.keyHeads * ((added ? 3 : 2) * s.rows + (bounds ? 2 * tilesQ * nwq + slices : 0)));
+    if (together) {
+      launch("_keys", true, groups + rowGroups, 256,
+             "  typedef " + queriesLds(2) + " akg_Q;\n  typedef " + keysLds + " akg_K;\n" +
+                 "  __shared__ __attribute__((aligned(16))) akg::u8 akg_lds[sizeof(akg_Q) > sizeof(akg_K) ? sizeof(akg_Q) : sizeof(akg_K)];\n" +
+                 "  const long akg_keys = akg_batch * akg_C::HKV * ((akg_sk + " + std::to_string(32 * nwk - 1) + ") / " + std::to_string(32 * nwk) + ");\n" +
+                 "  if (blockIdx.x < akg_keys) {\n" + keys("blockIdx.x", "*reinterpret_cast<akg_K *>(akg_lds)") + "  } else {\n" +
+                 queries(2, "blockIdx.x - akg_keys", "*reinterpret_cast<akg_Q *>(akg_lds)") + "  }\n");
+    } else if (wantKeys) {
+      launch("_keys", splits == 1, (apart ? 2 : 1) * groups * splits, 64 * nwk * rg, "  __shared__ " + keysLds + " akg_lds;\n" + keys("blockIdx.x", "akg_lds"),
+             std::max(s.dk, s.dv) > 128 || nwk == 2 ? 0 : 2);
+    }
     if (splits > 1) {
-      last.kernelName = keysName;
-      k_.earlierPhases.push_back(last);
-      o << kernel(k_.kernelName, 256, args, "  akg::attn::backward_join<akg_C, " + std::to_string(nwq) + ">(akg_ws, " + outName(1) + ", " + outName(2) + ", " + extents +
-                  ", " + ranges + ");\n");
-      last.grid[0] = checkGrid(ceilDiv(s.keyHeads * s.sk * ((s.dk + s.dv) / 4), 256), 256);
-      last.block[0] = 256;
+      const int64_t channels = (wanted(1) ? s.dk : 0) + (wanted(2) ? s.dv : 0);
+      launch("_join", true, ceilDiv(s.keyHeads * s.sk * (channels / 4), 256), 256,
+             "  akg::attn::backward_join<akg_C, " + std::to_string(nwq) + ", " + std::to_string(which) + ">(akg_ws, " + outName(1) + ", " + outName(2) + ", " + extents + ", " + ranges + ");\n");
       k_.workspaceBytes = (k_.workspaceBytes + 255) / 256 * 256 + static_cast<uint64_t>(4 * splits * s.keyHeads * s.sk * 32 * (ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32)));
     }
-    std::copy(last.grid, last.grid + 3, k_.grid);
-    std::copy(last.block, last.block + 3, k_.block);
+    std::copy(phases.back().grid, phases.back().grid + 3, k_.grid);
+    std::copy(phases.back().block, phases.back().block + 3, k_.block);
+    phases.pop_back();
+    k_.earlierPhases = phases;
     k_.source = o.str();
     k_.family = KernelFamily::Attention;
     k_.scalarArgs = {s.batch, s.sq, s.sk};
     if (splits > 1) k_.scalarArgs.push_back(splits);
-    k_.algorithmicOps = static_cast<uint64_t>((6 * s.dk + 4 * s.dv) * s.batch * s.heads * pairs(s, l_.causal));
-    k_.scheduleNote = "32 rows per wavefront, wavefronts " + std::to_string(nwq) + " (dq), " + std::to_string(nwk) + " (dk, dv), row ranges " + std::to_string(splits);
+    // scores, dout v (but for dv alone), and a product for each result
+    const int64_t channels = (2 + (wantDq ? 2 : 0) + (wanted(1) ? 2 : 0)) * s.dk + ((wantDq || wanted(1) ? 2 : 0) + (wanted(2) ? 2 : 0)) * s.dv;
+    k_.algorithmicOps = static_cast<uint64_t>(channels * s.batch * s.heads * pairs(s, l_.causal));
+    k_.scheduleNote = "32 rows per wavefront, wavefronts " + std::to_string(nwq) + (wantDq ? " (dq)" : " (rows)");
+    if (wantKeys) k_.scheduleNote += ", " + std::to_string(nwk) + (which == 0 ? " (dk, dv)" : which == 1 ? " (dk)" : " (dv)") + ", row ranges " + std::to_string(splits);
   }
 
   // ---- CacheAttention -------------------------------------------------------------------------------------------------

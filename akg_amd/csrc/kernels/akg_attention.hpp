@@ -1067,7 +1067,7 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
     __syncthreads();
     buf = next;
   }
-  if (!exists || dq == nullptr) return;
+  if (!exists) return;
   const float back = scale / lift;
   const RowsOf<C, DK> drows(dq, b, hkv, e);
   char *to = const_cast<char *>(drows.base) + drows.offset(row);
@@ -1094,6 +1094,7 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
 // APART: above 256 channels (keys and values together) the accumulators of both leave too little room for the operands: a
 // workgroup computes dk or dv, and the scores are computed twice (gradient of 2 x 2048, 32/8 heads of 256, causal: 941 us
 // instead of 2481; of 192: 765 instead of 795).
+// WHICH: 0 both (or, APART, one a workgroup), 1 dk, 2 dv.
 template <typename C, int NW, int RG>
 struct KeysLds {
   // From 192 channels on (keys and values together) the accumulators and the wavefront's own operands would leave room for
@@ -1104,7 +1105,7 @@ struct KeysLds {
   __attribute__((aligned(16))) u8 own[kKeysInLds ? kRows * NW * own_pitch(C::DK) : 16];
   __attribute__((aligned(16))) float states[2][kStates][kRound];
 };
-template <typename C, int NW, int RG, int NWQ, bool SPLIT, bool APART>
+template <typename C, int NW, int RG, int NWQ, bool SPLIT, bool APART, int WHICH>
 AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const void *v, const void *mask,
                            const int *qlens, const int *klens, void *dk, void *dv, float *ws, Extents e, float scale, int splits, long blockId, KeysLds<C, NW, RG> &memory) {
   typedef typename C::T T;
@@ -1309,9 +1310,8 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
       __syncthreads();
     }
     // the groups' sums joined: group g leaves as many accumulators as fit where the tiles were, group 0 adds them
-    static_assert(RG == 1 || !APART, "groups join both");
     if constexpr (RG > 1) {
-      constexpr int kFit = static_cast<int>(sizeof(lds)) / (64 * NW * (RG - 1) * 16), kFours = 4 * (TK + TV), kPart = kFit < kFours ? kFit : kFours;
+      constexpr int kFit = static_cast<int>(sizeof(lds)) / (64 * NW * (RG - 1) * 16), kFoursK = kDk ? 4 * TK : 0, kFours = kFoursK + (kDv ? 4 * TV : 0), kPart = kFit < kFours ? kFit : kFours;
       f32x4 *parts = reinterpret_cast<f32x4 *>(&lds[0][0]);
       unrolled<(kFours + kPart - 1) / kPart>([&](auto pass) {
         constexpr int p0 = decltype(pass)::value * kPart, kCount = kFours - p0 < kPart ? kFours - p0 : kPart;
@@ -1319,7 +1319,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
         if (group > 0) {
           unrolled<kCount>([&](auto y) {
             constexpr int x = p0 + decltype(y)::value, r = 4 * (x % 4);
-            const f32x16 &acc = x < 4 * TK ? acck[x / 4 % TK] : accv[(x - 4 * TK) / 4 % TV];
+            const f32x16 &acc = x < kFoursK ? acck[x < kFoursK ? x / 4 : 0] : accv[x < kFoursK ? 0 : (x - kFoursK) / 4];
             parts[(((group - 1) * kPart + x - p0) * NW + wave) * 64 + lane] = f32x4{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]};
           });
         }
@@ -1327,7 +1327,7 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
         if (group == 0) {
           unrolled<kCount>([&](auto y) {
             constexpr int x = p0 + decltype(y)::value, r = 4 * (x % 4);
-            f32x16 &acc = x < 4 * TK ? acck[x / 4 % TK] : accv[(x - 4 * TK) / 4 % TV];
+            f32x16 &acc = x < kFoursK ? acck[x < kFoursK ? x / 4 : 0] : accv[x < kFoursK ? 0 : (x - kFoursK) / 4];
 #pragma unroll
             for (int g = 0; g < RG - 1; ++g) {
               const f32x4 more = parts[((g * kPart + x - p0) * NW + wave) * 64 + lane];
@@ -1371,8 +1371,8 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
     };
     const KeysOf<C, DK> dkeys(dk, b, hkv, e);
     const KeysOf<C, DV> dvalues(dv, b, hkv, e);
-    if (kDk && dk != nullptr) store(const_cast<char *>(dkeys.base) + key * dkeys.step, DK, acck, TK, back);
-    if (kDv && dv != nullptr) store(const_cast<char *>(dvalues.base) + key * dvalues.step, DV, accv, TV, kUnlift);
+    if (kDk) store(const_cast<char *>(dkeys.base) + key * dkeys.step, DK, acck, TK, back);
+    if (kDv) store(const_cast<char *>(dvalues.base) + key * dvalues.step, DV, accv, TV, kUnlift);
   };
   if constexpr (APART) {
     if (blockId % 2 == 0) {
@@ -1381,27 +1381,26 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
       run(IntTag<2>());
     }
   } else {
-    run(IntTag<0>());
+    run(IntTag<WHICH>());
   }
 }
 
 // dk and dv from the sums over ranges of rows, in their order: four channels a thread.
-template <typename C, int NWQ>
+template <typename C, int NWQ, int WHICH>
 AKG_DEV void backward_join(const float *ws, void *dk, void *dv, Extents e, int splits) {
   typedef typename C::T T;
-  constexpr int DK = C::DK, DV = C::DV, kFours = (DK + DV) / 4, kSums = BackwardSpace<C>::kSums;
+  constexpr int DK = WHICH != 2 ? C::DK : 0, DV = WHICH != 1 ? C::DV : 0, kFours = (DK + DV) / 4, kSums = BackwardSpace<C>::kSums;
   const long rows = e.sq * C::G, heads = e.batch * C::HKV, wavesQ = (rows + kRows * NWQ - 1) / (kRows * NWQ) * NWQ;
   const long at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x, row = at / kFours;
   if (row >= heads * e.sk) return;
   const int c = static_cast<int>(at % kFours) * 4;
   const bool isK = c < DK;
-  const float *from = ws + BackwardSpace<C>{heads * rows, heads * wavesQ}.sums(heads, e.sk) + row * kSums + (isK ? c : padded(DK) + c - DK);
+  const float *from = ws + BackwardSpace<C>{heads * rows, heads * wavesQ}.sums(heads, e.sk) + row * kSums + (isK ? c : padded(C::DK) + c - DK);
   f32x4 sum = {};
   for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const f32x4 *>(from + s * heads * e.sk * kSums);
   const long head = row / e.sk, key = row % e.sk, b = head / C::HKV, hkv = head % C::HKV;
-  const KeysOf<C, DK> dkeys(dk, b, hkv, e);
-  const KeysOf<C, DV> dvalues(dv, b, hkv, e);
-  if ((isK ? dk : dv) == nullptr) return;
+  const KeysOf<C, C::DK> dkeys(dk, b, hkv, e);
+  const KeysOf<C, C::DV> dvalues(dv, b, hkv, e);
   char *to = isK ? const_cast<char *>(dkeys.base) + key * dkeys.step + 2 * c : const_cast<char *>(dvalues.base) + key * dvalues.step + 2 * (c - DK);
   *reinterpret_cast<u32x2 *>(to) = u32x2{T::pack(sum[0], sum[1]), T::pack(sum[2], sum[3])};
 }
