@@ -99,6 +99,11 @@ struct LoweredKernel {
   // Device workspace the kernel takes as one extra trailing pointer argument (0: none). The runtime allocates it
   // per kernel handle and device and zero-fills it once; the kernel leaves it zeroed where it must be.
   uint64_t workspaceBytes = 0;
+  // Where that is more than a launch without allocations has: the same results within it, by other launches of the same code
+  // object, in their order (empty: there is no such schedule, or no need for one).
+  std::vector<KernelPhase> withinPhases;
+  std::vector<int64_t> withinScalarArgs;
+  uint64_t withinWorkspaceBytes = 0;
 };
 
 LoweredKernel lowerToHip(const OpGraph &graph, const LoweringOptions &options);

@@ -20,7 +20,9 @@ int64_t ceilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 class LayerEmitter {
  public:
-  LayerEmitter(const OpGraph &g, const LoweringOptions &options) : g_(g), op_(g.ops[0]), l_(op_.layer), cus_(options.computeUnits) {}
+  // `limit`: bytes of workspace that ranges of an axis may take (0: any number).
+  LayerEmitter(const OpGraph &g, const LoweringOptions &options, int64_t limit = 0)
+      : g_(g), op_(g.ops[0]), l_(op_.layer), cus_(options.computeUnits), limit_(limit), name_(g.name + (limit > 0 ? "_within" : "")) {}
 
   LoweredKernel run() {
     for (size_t i = 0; i < g_.outputs.size(); ++i) {
@@ -28,7 +30,7 @@ class LayerEmitter {
         if (g_.outputs[i] == g_.outputs[j]) throw LoweringError("op " + op_.name + ": a result is listed twice among the outputs");
       }
     }
-    k_.kernelName = g_.name + "_kernel";
+    k_.kernelName = name_ + "_kernel";
     switch (op_.kind) {
       case OpKind::RotaryEmbedding: rotary(); break;
       case OpKind::Attention: attention(); break;
@@ -45,6 +47,8 @@ class LayerEmitter {
   const OpNode &op_;
   const LayerAttributes &l_;
   const int cus_;
+  const int64_t limit_;
+  const std::string name_;   // of the kernels
   LoweredKernel k_;
 
   const TensorValue &in(size_t i) const { return g_.tensor(op_.inputs[i]); }
@@ -223,8 +227,14 @@ class LayerEmitter {
     return n * (first + low) + n * (n - 1) / 2;
   }
   // Workspace of ranges that several workgroups share (attn::Ranges): `groups` counters, `rows` rows over all ranges.
+  static int64_t bytesOfRanges(int64_t groups, int64_t rows, int64_t dv) { return ceilDiv(groups * 4, 256) * 256 + rows * (ceilDiv(dv, 32) * 128 + 8); }
+  // As many of `splits` ranges as the limit holds.
+  int64_t rangesWithin(int64_t splits, int64_t groups, int64_t rows, int64_t dv) const {
+    while (limit_ > 0 && splits > 1 && bytesOfRanges(groups, splits * rows, dv) > limit_) --splits;
+    return splits;
+  }
   static uint64_t rangesBytes(int64_t groups, int64_t rows, int64_t dv) {
-    const int64_t bytes = ceilDiv(groups * 4, 256) * 256 + rows * (ceilDiv(dv, 32) * 128 + 8);
+    const int64_t bytes = bytesOfRanges(groups, rows, dv);
     if (bytes >= (1LL << 31)) throw LoweringError("the ranges' results take more than 2 GiB");
     return static_cast<uint64_t>(bytes);
   }
@@ -244,7 +254,7 @@ class LayerEmitter {
       return;
     }
     KernelPhase first;
-    first.kernelName = g_.name + "_ranges";
+    first.kernelName = name_ + "_ranges";
     first.grid[0] = checkGrid(groups * splits, threads);
     first.block[0] = static_cast<unsigned>(threads);
     k_.earlierPhases.push_back(first);
@@ -285,6 +295,7 @@ class LayerEmitter {
     // over 759 keys of 32/4 of 64: 14.9 in two, 11.3 in five).
     int64_t splits = 1;
     if (groups < cus_) splits = std::max<int64_t>(1, std::min<int64_t>({(nw == 8 ? 1 : 2) * cus_ / groups, s.sk / 128, 64}));
+    splits = rangesWithin(splits, groups, s.keyHeads * s.rows, s.dv);
     if (!joinsInside(std::min<int64_t>(32 * nw, s.rows), splits, s.dv) && s.sk - s.sk / splits < 512) splits = 1;
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n") << config(s, 3);
@@ -329,7 +340,10 @@ class LayerEmitter {
     const bool far = !l_.headsFirst && 128 * s.kvHeads * 2 * std::max(s.dk, s.dv) >= (1LL << 31) - 65536;
     const bool few = crowded || far;
     const int64_t whole = s.keyHeads * ceilDiv(s.sk, few ? 64 : 128);
-    const int64_t splits = wantKeys ? std::max<int64_t>(1, std::min((l_.causal ? 2 : 1) * cus_ / whole, s.rows / 512)) : 1;
+    int64_t splits = wantKeys ? std::max<int64_t>(1, std::min((l_.causal ? 2 : 1) * cus_ / whole, s.rows / 512)) : 1;
+    const int64_t sumsBytes = 4 * s.keyHeads * s.sk * 32 * (ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32));   // of a range
+    // (rows' values and bounds of at most eight wavefronts a workgroup, as below)
+    while (limit_ > 0 && splits > 1 && splits * sumsBytes + 4 * s.keyHeads * (3 * s.rows + 2 * (ceilDiv(s.rows, 32) + 8) + 256) + 256 > limit_) --splits;
     const int nwk = !few && (splits > 1 || whole >= cus_) ? 4 : 2;
     const int64_t groups = s.keyHeads * ceilDiv(s.sk, 32 * nwk);
     // Small problems: what both kernels need of the rows in a launch of its own, then both in one launch, side by side, while
@@ -370,7 +384,7 @@ class LayerEmitter {
     std::vector<KernelPhase> phases;
     auto launch = [&](const char *suffix, bool last, int64_t grid, int threads, const std::string &body, int wavesPerSimd = 0) {
       KernelPhase p;
-      p.kernelName = last ? k_.kernelName : g_.name + suffix;
+      p.kernelName = last ? k_.kernelName : name_ + suffix;
       p.grid[0] = checkGrid(grid, threads);
       p.block[0] = static_cast<unsigned>(threads);
       phases.push_back(p);
@@ -405,7 +419,7 @@ class LayerEmitter {
       const int64_t channels = (wanted(1) ? s.dk : 0) + (wanted(2) ? s.dv : 0);
       launch("_join", true, ceilDiv(s.keyHeads * s.sk * (channels / 4), 256), 256,
              "  akg::attn::backward_join<akg_C, " + std::to_string(nwq) + ", " + std::to_string(which) + ">(akg_ws, " + outName(1) + ", " + outName(2) + ", " + extents + ", " + ranges + ");\n");
-      k_.workspaceBytes = (k_.workspaceBytes + 255) / 256 * 256 + static_cast<uint64_t>(4 * splits * s.keyHeads * s.sk * 32 * (ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32)));
+      k_.workspaceBytes = (k_.workspaceBytes + 255) / 256 * 256 + static_cast<uint64_t>(splits * sumsBytes);
     }
     std::copy(phases.back().grid, phases.back().grid + 3, k_.grid);
     std::copy(phases.back().block, phases.back().block + 3, k_.block);
@@ -440,8 +454,9 @@ class LayerEmitter {
     // up to eight where each has 1024 tokens or more. us at two, four, eight to a CU: 16 x 2000 tokens (4 key heads of 64
     // channels) 10.5, 11.7, 11.8; 32 x 8192 .. 16384 tokens (8 of 128) 180, 195, 174.
     const int64_t tokens = perSequence * page;
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({std::max(ceilDiv(2 * cus_, groups), std::min(ceilDiv(8 * cus_, groups), tokens / 1024)),
-                                                                   ceilDiv(tokens, 128), 64}));
+    const int64_t splits = rangesWithin(std::max<int64_t>(1, std::min<int64_t>({std::max(ceilDiv(2 * cus_, groups), std::min(ceilDiv(8 * cus_, groups), tokens / 1024)),
+                                                                                ceilDiv(tokens, 128), 64})),
+                                        groups, batch * kvHeads * rows, dim);
     // Registers for two wavefronts a SIMD, three for one tile of up to 128 channels: 175 us instead of 195 in the second of these;
     // 32 rows over 16 x 4096 tokens, 4 key heads of 128, 26 instead of 36; one query over 16 x 8192, 8 key heads of 192 and 256,
     // 67 and 91 instead of 69 and 124 (with three 156, spilled, and 124).
@@ -484,8 +499,23 @@ class LayerEmitter {
 LoweredKernel lowerLayerToHip(const OpGraph &graph, const LoweringOptions &options) {
   // (operands that other ops compute lie in memory first: the description is cut there)
   if (graph.ops.size() != 1) throw LoweringError("op " + graph.ops[0].name + ": operators of an attention layer are kernels of their own");
-  LayerEmitter emitter(graph, options);
-  return emitter.run();
+  LoweredKernel k = LayerEmitter(graph, options).run();
+  const int64_t fixed = 16 << 20;   // what a launch without allocations has
+  if (k.workspaceBytes > static_cast<uint64_t>(fixed)) {
+    LoweredKernel within = LayerEmitter(graph, options, fixed).run();
+    if (within.workspaceBytes <= static_cast<uint64_t>(fixed)) {
+      k.source += "\n" + within.source;
+      k.withinPhases = within.earlierPhases;
+      KernelPhase last;
+      last.kernelName = within.kernelName;
+      std::copy(within.grid, within.grid + 3, last.grid);
+      std::copy(within.block, within.block + 3, last.block);
+      k.withinPhases.push_back(last);
+      k.withinScalarArgs = within.scalarArgs;
+      k.withinWorkspaceBytes = within.workspaceBytes;
+    }
+  }
+  return k;
 }
 
 }  // namespace akg

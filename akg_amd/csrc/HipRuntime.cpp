@@ -55,6 +55,7 @@ struct akg_hip_kernel {
     hipModule_t module = nullptr;
     hipFunction_t function = nullptr;
     std::vector<hipFunction_t> earlier;  // lowered.earlierPhases, in their order
+    std::vector<hipFunction_t> within;   // lowered.withinPhases
     void *workspace = nullptr;  // lowered.workspaceBytes of zero-filled device memory, or NULL
     // Launches of one handle share its workspace. They are ordered on the device by the library: a launch that goes to
     // another stream than the last one first waits (through this event) for what that stream holds.
@@ -697,14 +698,16 @@ int ensureLoaded(akg_hip_kernel *k, akg_hip_kernel::Loaded **out) {
       return fail(AKG_HIP_ERR_RUNTIME, "hipModuleGetFunction(" + k->lowered.kernelName + "): " + hipErr(e));
     }
   }
-  for (const akg::KernelPhase &ph : k->lowered.earlierPhases) {
-    hipFunction_t f = nullptr;
-    e = hipModuleGetFunction(&f, l.module, ph.kernelName.c_str());
-    if (e != hipSuccess) {
-      releaseModule(k->codeSha256, device);
-      return fail(AKG_HIP_ERR_RUNTIME, "hipModuleGetFunction(" + ph.kernelName + "): " + hipErr(e));
+  for (const bool within : {false, true}) {
+    for (const akg::KernelPhase &ph : within ? k->lowered.withinPhases : k->lowered.earlierPhases) {
+      hipFunction_t f = nullptr;
+      e = hipModuleGetFunction(&f, l.module, ph.kernelName.c_str());
+      if (e != hipSuccess) {
+        releaseModule(k->codeSha256, device);
+        return fail(AKG_HIP_ERR_RUNTIME, "hipModuleGetFunction(" + ph.kernelName + "): " + hipErr(e));
+      }
+      (within ? l.within : l.earlier).push_back(f);
     }
-    l.earlier.push_back(f);
   }
   if (k->lowered.workspaceBytes > 0) {
     // Zero-filled once; every launch leaves the arrival counters at zero again. Launches of one handle share the
@@ -747,10 +750,10 @@ const akg::TensorValue &tensorAt(const akg_hip_kernel *k, int index) {
 
 uint64_t alignScratch(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// Device memory beyond inputs and outputs that one launch of `k` uses: its own workspace (for a staged description the
-// tensors between its kernels) followed by the workspaces of its stages, each piece a multiple of 256 bytes.
+// Device memory beyond inputs and outputs that one launch of `k` without allocations uses: its own workspace (for a staged
+// description the tensors between its kernels) followed by the workspaces of its stages, each piece a multiple of 256 bytes.
 uint64_t scratchBytesNeeded(const akg_hip_kernel *k) {
-  uint64_t total = alignScratch(k->lowered.workspaceBytes);
+  uint64_t total = alignScratch(k->lowered.withinPhases.empty() ? k->lowered.workspaceBytes : k->lowered.withinWorkspaceBytes);
   for (const auto &st : k->stages) total += scratchBytesNeeded(st.kernel);
   return total;
 }
@@ -858,7 +861,10 @@ int launchOn(akg_hip_kernel *k, akg_hip_kernel::Loaded *l, void *const *devicePt
 
 int launchSequence(akg_hip_kernel *k, akg_hip_kernel::Loaded &l, void *const *devicePtrs, hipStream_t stream,
                    char *scratchBase) {
-  void *const workspace = scratchBase != nullptr ? (k->lowered.workspaceBytes > 0 ? scratchBase : nullptr) : l.workspace;
+  // (a launch without allocations of a kernel whose usual schedule needs more has launches of its own)
+  const bool within = scratchBase != nullptr && !k->lowered.withinPhases.empty();
+  const uint64_t workspaceBytes = within ? k->lowered.withinWorkspaceBytes : k->lowered.workspaceBytes;
+  void *const workspace = scratchBase != nullptr ? (workspaceBytes > 0 ? scratchBase : nullptr) : l.workspace;
   if (!k->stages.empty()) {
     const size_t nin = k->graph.inputs.size();
     char *stageScratch = scratchBase != nullptr ? scratchBase + alignScratch(k->lowered.workspaceBytes) : nullptr;
@@ -890,7 +896,8 @@ int launchSequence(akg_hip_kernel *k, akg_hip_kernel::Loaded &l, void *const *de
   }
   // kernel arguments: the tensor pointers, then the 64-bit scalars of the lowering, then the workspace
   const int n = numTensors(k);
-  const int nscalar = static_cast<int>(k->lowered.scalarArgs.size());
+  const std::vector<int64_t> &scalars = within ? k->lowered.withinScalarArgs : k->lowered.scalarArgs;
+  const int nscalar = static_cast<int>(scalars.size());
   const int nargs = n + nscalar + (workspace ? 1 : 0);
   std::vector<void *> slots(static_cast<size_t>(nargs));
   std::vector<void *> params(static_cast<size_t>(nargs));
@@ -899,18 +906,20 @@ int launchSequence(akg_hip_kernel *k, akg_hip_kernel::Loaded &l, void *const *de
       slots[static_cast<size_t>(i)] = devicePtrs[i];
       params[static_cast<size_t>(i)] = &slots[static_cast<size_t>(i)];
     } else if (i < n + nscalar) {
-      params[static_cast<size_t>(i)] = const_cast<int64_t *>(&k->lowered.scalarArgs[static_cast<size_t>(i - n)]);
+      params[static_cast<size_t>(i)] = const_cast<int64_t *>(&scalars[static_cast<size_t>(i - n)]);
     } else {
       slots[static_cast<size_t>(i)] = workspace;
       params[static_cast<size_t>(i)] = &slots[static_cast<size_t>(i)];
     }
   }
-  for (size_t i = 0; i < l.earlier.size(); ++i) {
-    const akg::KernelPhase &ph = k->lowered.earlierPhases[i];
-    hipError_t pe = hipModuleLaunchKernel(l.earlier[i], ph.grid[0], ph.grid[1], ph.grid[2], ph.block[0], ph.block[1],
+  const std::vector<hipFunction_t> &earlier = within ? l.within : l.earlier;
+  for (size_t i = 0; i < earlier.size(); ++i) {
+    const akg::KernelPhase &ph = within ? k->lowered.withinPhases[i] : k->lowered.earlierPhases[i];
+    hipError_t pe = hipModuleLaunchKernel(earlier[i], ph.grid[0], ph.grid[1], ph.grid[2], ph.block[0], ph.block[1],
                                           ph.block[2], 0, stream, params.data(), nullptr);
     if (pe != hipSuccess) return fail(AKG_HIP_ERR_RUNTIME, "hipModuleLaunchKernel(" + ph.kernelName + "): " + hipErr(pe));
   }
+  if (within) return AKG_HIP_OK;
   hipError_t e = hipModuleLaunchKernel(l.function, k->lowered.grid[0], k->lowered.grid[1], k->lowered.grid[2],
                                        k->lowered.block[0], k->lowered.block[1], k->lowered.block[2], 0, stream,
                                        params.data(), nullptr);

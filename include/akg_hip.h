@@ -152,7 +152,9 @@ int akg_hip_launch(akg_hip_kernel_t *kernel, void *const *device_ptrs, int n_ptr
  * workspace, and the call allocates, loads and frees nothing:
  *  - akg_hip_kernel_prepare must have been called for this handle on the current device (it loads the code objects);
  *    otherwise AKG_HIP_ERR_INVALID_ARGUMENT;
- *  - a handle that needs more than AKG_HIP_STATIC_SCRATCH_MAX bytes is refused with AKG_HIP_ERR_UNSUPPORTED;
+ *  - a handle that needs more than AKG_HIP_STATIC_SCRATCH_MAX bytes is refused with AKG_HIP_ERR_UNSUPPORTED; attention, its
+ *    gradient and cache attention run here with fewer ranges of an axis (or none) where their usual schedule shares it
+ *    through more than that: sums of float32 in another order than akg_hip_launch;
  *  - the part of the array the handle uses is cleared by a fill kernel on `stream` in front of the launch;
  *  - every call on a device shares that device's array, whatever the handle: calls that overlap on one device race.
  *    Order them on one stream or with events.
