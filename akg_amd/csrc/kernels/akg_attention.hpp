@@ -605,8 +605,11 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
   auto step = [&](int j0, const u8 *vt, int vrow, const u8 *kt, int krow) {
     // The maximum that the exponents are taken against follows the scores only when they are 2^8 above it: sums and
     // accumulators then have to be rescaled, which most tiles are spared; what is kept is as exact against any maximum.
+    // float16 takes probabilities up to 2^15 (2^7 at the maximum found, 2^8 above that): the weights of a long tail, each a
+    // small part of the largest, then have their digits down to 2^-21 of it.
+    constexpr float kUnder = !T::kNarrowRange ? 0.0f : C::ADDED ? 7.0f * kLn2 : 7.0f;
     float m = max_halves(peak);
-    if (C::MASK == 0) m *= c;
+    m = C::MASK == 0 ? __builtin_fmaf(m, c, -kUnder) : m - kUnder;
     if (__any(m > top + (C::ADDED ? 5.5f : 8.0f))) {
       m = __builtin_fmaxf(top, m);
       const float shrink = power<C>(top - (m == neg_inf() ? 0.0f : m));
