@@ -12,10 +12,10 @@
  *   scores: lane (token l % 16, g = l / 16) reads the 16 channels 64 u + 16 g ... of its token
  *   output: lane (l % 16, g) reads a few adjacent channels of the tokens 4 g .. 4 g + 3 of both blocks of sixteen
  * The scale of a key block multiplies the scores in float32. That of a value block multiplies the probabilities, which
- * are rounded to float16 behind it (2^-11 of each): relative to a power of two that is within a factor of two of the row's
- * heaviest product of both so far, so that they stay below 2 and the heaviest keep their digits, whatever scales lie on
- * blocks that the row does not attend to. That power is the row's own, found from a second running maximum, of score + log2
- * of the scale, and the accumulators follow it exactly.
+ * are rounded to float16 behind it (2^-11 of each), relative to a power of two that puts the row's heaviest product of both so
+ * far between 2^12 and 2^14: those of a long tail keep their digits down to 2^-26 of the heaviest, whatever scales lie on blocks
+ * that the row does not attend to. That power is the row's own, found from a second running maximum, of score + exponent of the
+ * scale, and the accumulators follow it exactly.
  *
  * 32 sequences of 8192 to 16384 tokens, one query of 32 heads over 8 of 128 channels, take 168 us: 4.8 TB/s of the 5.2 that
  * a copy reaches. Short ones wait for what depends on one another (length, block numbers, blocks, the other wavefronts, the
@@ -276,7 +276,7 @@ AKG_DEV void over_cache(const void *q, const void *kcache, const void *vcache, c
       heaviest[rt] = __builtin_fmaxf(before, heavy);
       int unit = reference[rt];
       if (heaviest[rt] > neg_inf()) {
-        unit = static_cast<int>(__builtin_floorf(__builtin_fmaxf(heaviest[rt] - base, -250.0f)));   // (at most 128)
+        unit = static_cast<int>(__builtin_floorf(__builtin_fmaxf(heaviest[rt] - base - 13.0f, -250.0f)));   // (at most 115)
         unit = unit > lowest ? unit : lowest;
       }
       const float all = __builtin_ldexpf(shrink, before > neg_inf() ? reference[rt] - unit : 0);   // (at most 2)
