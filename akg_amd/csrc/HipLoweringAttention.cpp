@@ -3,6 +3,9 @@
  * become an instance of the hand-written kernels in kernels/akg_rotary.hpp, akg_attention.hpp and akg_cache_attention.hpp.
  * Types, channels, heads, layout and which operands there are go into the source; batch, sequence lengths and the number
  * of blocks are kernel arguments (LoweredKernel::scalarArgs), so calls that differ there share a code object.
+ *
+ * Times in the comments are of launches one behind another on inputs that no cache holds (copies of 640 MB in turn), with
+ * the rule as it is and with the other choice forced; causal and bfloat16 where nothing else is said.
  */
 #include <algorithm>
 #include <cmath>
@@ -93,7 +96,8 @@ class LayerEmitter {
   }
   // `wavesPerSimd`: how many the registers have to leave room for (0: the compiler's choice).
   static std::string kernel(const std::string &name, int threads, const std::string &args, const std::string &body, int wavesPerSimd = 0) {
-    return "extern \"C\" __global__ __launch_bounds__(" + std::to_string(threads) + (wavesPerSimd ? ", " + std::to_string(wavesPerSimd) : "") + ") void " + name + "(" + args + ") {\n" + body + "}\n\n";
+    return "extern \"C\" __global__ __launch_bounds__(" + std::to_string(threads) + (wavesPerSimd ? ", " + std::to_string(wavesPerSimd) : "") + ") void " + name +
+           "(" + args + ") {\n" + body + "}\n\n";
   }
   const char *trait() const { return in(0).dtype == DType::BF16 ? "akg::attn::BF16" : "akg::attn::F16"; }
 
@@ -240,8 +244,8 @@ class LayerEmitter {
   }
   // The kernel `body` whose workgroups (`groups` of `groupRows` rows, times `splits`) share the keys' axis, and what joins
   // their results: the last workgroup of a group, which saves a launch (attention of one query of 8 x 32/8 heads of 128 over 512
-  // keys 11.8 instead of 12.3 us), or, where that one would read more than 16 KiB alone, a launch of its own (2 x 16 queries
-  // over 8192 keys, 1 MiB a group: 27 instead of 87 us; 4 x 4 over 4096, 128 KiB: 21 instead of 28).
+  // keys 12.7 instead of 18.3 us), or, where that one would read more than 16 KiB alone, a launch of its own (2 x 16 queries
+  // over 8192 keys, 1 MiB a group: 29 instead of 87 us; 4 x 4 over 4096, 128 KiB: 23 instead of 29).
   static constexpr int64_t kJoinInside = 16 << 10;
   static bool joinsInside(int64_t groupRows, int64_t splits, int64_t dv) { return 4 * groupRows * splits * dv <= kJoinInside; }
   void ranges(std::ostringstream &o, const std::string &args, const std::string &body, int threads, int hint, const std::string &joinExtents, const std::string &outs,
@@ -266,12 +270,12 @@ class LayerEmitter {
     k_.block[0] = 256;
   }
   // Wavefronts of a workgroup that gives 32 rows to each (a tile is fetched once for all of them), two at least: the second
-  // one fetches even where it has no rows (one query over 8192 keys with one wavefront 46 us, with two 44).
+  // one fetches even where it has no rows (one query of 8 sequences over 8192 keys with one wavefront 56 us, with two 51).
   // Causal: as many as leave a workgroup for every CU, since rows differ in their keys and many small workgroups even that out
-  // (2 x 4096 x 32/8 heads of 128 with eight 360 us, four 384; 1 x 1024 x 16 of 128 with eight, four, two 35, 35, 29).
+  // (2 x 4096 x 32/8 heads of 128 with eight 313 us, four 328; 1 x 1024 x 16 of 128 with eight, four, two 41, 37, 30).
   // Else the number that puts the fewest on the busiest SIMD: of equals the largest, or the smallest where that is one, which
-  // spreads them over most CUs (gradient of 8 x 5792 x 1 of 128: 184 workgroups of eight 536 us, 368 of four 640; of 4 x 2638 x
-  // 8/4 of 40: four 333, eight 347; attention of 3 x 478 x 8 of 40: two 17.0, four 16.5, eight 17.2).
+  // spreads them over most CUs (gradient of 8 x 5792 x 1 of 128: 184 workgroups of eight 526 us, 368 of four 631; of 4 x 2638 x
+  // 8/4 of 40: four 303, eight 318; attention of 3 x 478 x 8 of 40: two 15.0, four 15.1, eight 16.4; none of them causal).
   int waves(const Sizes &s, int most) const {
     int w = most;
     if (l_.causal) {
@@ -290,9 +294,10 @@ class LayerEmitter {
     const int nw = waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8);
     const int64_t groups = s.keyHeads * ceilDiv(s.rows, 32 * nw);
     // Few rows and a long axis of keys: several workgroups share it, as many as two to a CU, or one of eight
-    // wavefronts (8 sequences over 8192 keys: 44 us; one to a CU 61), at least two tiles of 64 each (one query over 512 keys: 10.2 us; four tiles 13.1, one 11.4). A launch
-    // that joins has to be worth it (4 x 439 queries and keys of 8/4 heads of 96: 15.8 us, in two ranges 24.5; 2 x 5 queries
-    // over 759 keys of 32/4 of 64: 14.9 in two, 11.3 in five).
+    // wavefronts (8 sequences over 8192 keys: 51 us; one to a CU 61), at least two tiles of 64 each (one query of 8 sequences
+    // over 512 keys: 12.7 us; four tiles 15.0, one 13.0). A launch that joins has to be worth it (4 x 439 queries and keys of
+    // 8/4 heads of 96, not causal: 16.4 us, in two ranges 27.6; 2 x 5 queries over 759 keys of 32/4 of 64, not causal: 19.8
+    // in one, 15.0 in two, 12.0 in five).
     int64_t splits = 1;
     if (groups < cus_) splits = std::max<int64_t>(1, std::min<int64_t>({(nw == 8 ? 1 : 2) * cus_ / groups, s.sk / 128, 64}));
     splits = rangesWithin(splits, groups, s.keyHeads * s.rows, s.dv);
@@ -331,9 +336,12 @@ class LayerEmitter {
     const int rg = std::max(s.dk, s.dv) > 128 ? 1 : 2;
     // A workgroup of the kernel of dk and dv has 128 keys. Where that leaves CUs idle it shares the rows with others, 512 of
     // them each at least (causal: two to a CU, since the first keys have most rows), or has 64. us of the gradient unshared,
-    // shared: 1 x 1024 x 16/4 heads of 128, causal, 129, 75; 1 x 4096 x 32/4 918, 568; 8 x 200 x 12 heads of 64 with 128 keys
-    // and 64: 24.9, 23.7. A mask beside more than 64 channels leaves the registers of two wavefronts a SIMD too few: 64 keys
-    // and one (5 x 1773 x 8/4 heads of 96, causal, with a mask: 312, 240).
+    // shared: 1 x 1024 x 16/4 heads of 128 101, 73; 1 x 4096 x 32/4 887, 508. With 128 keys and 64, float16 in launches of
+    // their own: 8 x 200 x 12 heads of 64 33.0, 32.0. A mask beside more than 64 channels leaves the registers of two wavefronts
+    // a SIMD too few: 64 keys and one (5 x 1773 x 8/4 heads of 96, float16, with a mask: 311, 294).
+    // Above 256 channels, where dk and dv are workgroups of their own, this makes twice as many workgroups: 1 x 1024 x 16/4 heads
+    // of 256 150 us, with half as many ranges 164, unshared 370; 1 x 2048 x 32/8 529, 489, 761; 2 x 2048 x 32/8 952, 857
+    // unshared; 2 x 1024 x 16/8 of 192, not causal, 244, 325 unshared. (No one count of them is best.)
     const bool crowded = l_.hasMask && ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32) > 4;
     const bool apart = which == 0 && ceilDiv(s.dk, 32) + ceilDiv(s.dv, 32) > 8;   // (dk and dv by workgroups of their own)
     // (64 keys also where 128 rows of keys or values lie too far apart for 32-bit offsets)
@@ -347,8 +355,8 @@ class LayerEmitter {
     const int nwk = !few && (splits > 1 || whole >= cus_) ? 4 : 2;
     const int64_t groups = s.keyHeads * ceilDiv(s.sk, 32 * nwk);
     // Small problems: what both kernels need of the rows in a launch of its own, then both in one launch, side by side, while
-    // neither fills the card (8 x 200 x 12 heads of 64: 18.8 us instead of 24.0, 2 x 512 x 12 of 64 19.6 instead of 28.5; with
-    // three workgroups a CU 2 x 2000 x 2001 x 16/4 of 128 with a mask takes 551 instead of 497).
+    // neither fills the card (float16: 8 x 200 x 12 heads of 64 22.4 us instead of 32.0, 2 x 512 x 12 of 64 22.5 instead of 35.7;
+    // with three workgroups a CU 2 x 2000 x 2001 x 16/4 of 128 with a mask, not causal, takes 518 instead of 471).
     const bool together = wantDq && wantKeys && splits == 1 && nwk * rg == 4 && !apart && 2 * (groups + s.keyHeads * ceilDiv(s.rows, 128)) <= 5 * cus_;
     const bool rowsFirst = together || !wantDq;   // (the first launch leaves the rows' values only)
     const int nwq = rowsFirst ? 4 : waves(s, std::max(s.dk, s.dv) > 128 ? 4 : 8);
@@ -447,19 +455,21 @@ class LayerEmitter {
     if (rows >= (1LL << 30) || perSequence * page >= (1LL << 30)) throw LoweringError("op " + op_.name + ": more than 2^30 tokens or rows");
     const int64_t units = ceilDiv(dim, 64);
     // Tiles of 16 rows a workgroup: as many as registers of two wavefronts a SIMD hold (16 sequences of 4096 tokens, 4 key heads of
-    // 128, 64 rows each: two tiles 39 us, four tiles and one wavefront 56; of 256: one tile 72, two 84).
+    // 128, 64 rows each: two tiles 42 us, four tiles and one wavefront 62; of 256: one tile 81, two 91).
     const int64_t rt = std::min<int64_t>(ceilDiv(rows, 16), std::max<int64_t>(1, 4 / units));
     const int64_t groups = batch * kvHeads * ceilDiv(rows, 16 * rt);
     // Workgroups that share a sequence: two to a CU, with at least one step of 32 tokens for each of their four wavefronts, and
-    // up to eight where each has 1024 tokens or more. us at two, four, eight to a CU: 16 x 2000 tokens (4 key heads of 64
-    // channels) 10.5, 11.7, 11.8; 32 x 8192 .. 16384 tokens (8 of 128) 180, 195, 174.
+    // up to eight where each has 1024 tokens or more. us at one, two, four, eight to a CU: 4 queries over 16 x 2000 tokens
+    // (16/4 heads of 64 channels) 12.5, 13.4, 15.3, 14.7; one over 32 x 8192 .. 16384 tokens (32/8 of 128) 240, 175, 195, 169.
+    // (One to a CU is faster where its ranges can be joined without a second launch, and leaves half of the bandwidth unused
+    // where tokens are many.)
     const int64_t tokens = perSequence * page;
     const int64_t splits = rangesWithin(std::max<int64_t>(1, std::min<int64_t>({std::max(ceilDiv(2 * cus_, groups), std::min(ceilDiv(8 * cus_, groups), tokens / 1024)),
                                                                                 ceilDiv(tokens, 128), 64})),
                                         groups, batch * kvHeads * rows, dim);
-    // Registers for two wavefronts a SIMD, three for one tile of up to 128 channels: 175 us instead of 195 in the second of these;
-    // 32 rows over 16 x 4096 tokens, 4 key heads of 128, 26 instead of 36; one query over 16 x 8192, 8 key heads of 192 and 256,
-    // 67 and 91 instead of 69 and 124 (with three 156, spilled, and 124).
+    // Registers for two wavefronts a SIMD: 32 rows over 16 x 4096 tokens, 4 key heads of 128, 29 us instead of 40; one query over 16
+    // x 8192, 8 key heads of 192 and 256, 76 and 94 instead of 79 and 126 (with three 158, spilled, and 125). Up to 128 channels
+    // one tile leaves room for three as it is (asked for, nothing changes).
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n#include \"akg_cache_attention.hpp\"\n")
       << "typedef akg::attn::Config<" << trait() << ", " << dim << ", " << dim << ", " << kvHeads << ", " << group
@@ -474,7 +484,7 @@ class LayerEmitter {
         << number(l_.scale) << ", static_cast<int>(akg_splits));\n";
       return c.str();
     };
-    const int hint = rt == 1 && units <= 2 ? 3 : 2;
+    const int hint = 2;
     if (splits > 1) {
       ranges(o, args, call(true), 256, hint, "akg::attn::Extents{akg_batch, akg_sq, 0}", outName(0) + ", nullptr", groups, 16 * rt, splits, batch * kvHeads, rows, dim);
     } else {

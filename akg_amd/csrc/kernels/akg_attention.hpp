@@ -287,7 +287,7 @@ AKG_DEV float with_mask(float s, float factor, const void *mask, long at) {
 // before the scores are computed, in wide loads that run on into the next row (no score takes what they find there). Where
 // they would pass the end of the mask they are moved back instead, and `fix` loads one element at a time: in a branch that
 // waits for itself, where the scores are. (With loads in two branches the compiler waited for those of the keys ahead at
-// every use: 4 x 1000 x 1003 x 16 x 64 took 54 us instead of 49.)
+// every use: 4 x 1000 x 1003 x 16 x 64, inputs in the last cache, took 54 us instead of 49 when that was tried.)
 __device__ const u32 kNothing[32] = {};
 template <typename C>
 struct MaskRow {
@@ -377,7 +377,7 @@ struct FeedOrder {
 
 // ---- ranges of keys that several workgroups share -----------------------------------------------------------------------
 // Every range leaves accumulators, maximum and sum of its rows in the workspace; the workgroup that arrives last at the
-// counter of its rows joins them, in the order of the ranges whoever that is (a second launch cost 3 us more).
+// counter of its rows joins them, in the order of the ranges whoever that is (a second launch costs 3 to 6 us more).
 // Workspace: the counters, to the next 256 bytes; accumulators [ranges][rows of all key heads][padded channels]; then
 // (maximum, sum) [ranges][rows].
 template <typename C>
@@ -492,7 +492,7 @@ AKG_DEV void join_rows(float *ws, void *out, float *lse, const Extents &e, int s
 // SPLIT: the workgroup takes one of `splits` ranges of the keys (Ranges). JOIN: the last one joins them.
 //
 // Many rows are bound by the matrix units and by the issue of what stands beside them: 2 x 4096 queries and keys, 32 heads over
-// 8 of 128 channels, causal, bfloat16, take 294 us, 0.94 PFLOP/s (a matrix product of 8192 each way reaches 1.36); the
+// 8 of 128 channels, causal, bfloat16, take 301 us, 0.91 PFLOP/s (a matrix product of 8192 each way reaches 1.36); the
 // matrix instructions alone would take 215, the vector instructions alone 151. Few rows are bound by the keys and values from
 // memory: one query of 8 sequences over 8192 keys takes 51 us, 4.0 TB/s, and 44 where the last level cache still holds part
 // of them. Tried for both and left out: a second set of tiles under way (token 54, training unchanged), 64 rows a wavefront,
@@ -824,8 +824,9 @@ AKG_DEV void slice_of_values(const void *v, const int *klens, float *ws, Extents
 
 // dq of 32 rows a wavefront: keys and values pass by in tiles, 32 keys a step: the scores and their gradients' products, then
 // the gradients of the scores (vector instructions) between the matrix instructions that multiply those of the step before.
-// Leaves in `ws` what the kernel of dk and dv needs. Bound as the forward pass is: the training case there takes 417 us, 0.99
-// PFLOP/s of its three products (425 with the gradients of a step computed in front of its own products).
+// Leaves in `ws` what the kernel of dk and dv needs. Bound as the forward pass is: the training case there takes 390 to 412 us,
+// 1.0 to 1.06 PFLOP/s of its three products, by the card, once that holds its clock, and up to 530 in the milliseconds behind a
+// pause (2 % more with the gradients of a step computed in front of its own products).
 // PART: 0 all of it; 1 only what it leaves in `ws`; 2 only dq, from that.
 template <typename C, int NW, int PART>
 struct QueriesLds {
@@ -1093,10 +1094,11 @@ AKG_DEV void backward_queries(const void *dout, const void *q, const void *k, co
 // seen by all rows, and a workgroup that goes through them alone is the last to end.)
 // SPLIT: where the tiles of keys are fewer than the CUs, `splits` workgroups take a range of the rows each and leave their
 // sums in `ws` for backward_join. Two groups of wavefronts hide each other's vector instructions behind matrix instructions:
-// the training case of the forward pass takes 550 us, 1.0 PFLOP/s of its four products (one group: 930).
+// the training case of the forward pass takes 520 to 557 us, 0.99 to 1.06 PFLOP/s of its four products, by the card, once
+// that holds its clock (the whole gradient 918 us, with one group 1074).
 // APART: above 256 channels (keys and values together) the accumulators of both leave too little room for the operands: a
-// workgroup computes dk or dv, and the scores are computed twice (gradient of 2 x 2048, 32/8 heads of 256, causal: 941 us
-// instead of 2481; of 192: 765 instead of 795).
+// workgroup computes dk or dv, and the scores are computed twice (gradient of 2 x 2048, 32/8 heads of 256, causal: 952 us
+// instead of 2423; of 192: 770 instead of 809).
 // WHICH: 0 both (or, APART, one a workgroup), 1 dk, 2 dv.
 template <typename C, int NW, int RG>
 struct KeysLds {

@@ -17,9 +17,9 @@
  * that the row does not attend to. That power is the row's own, found from a second running maximum, of score + exponent of the
  * scale, and the accumulators follow it exactly.
  *
- * 32 sequences of 8192 to 16384 tokens, one query of 32 heads over 8 of 128 channels, take 168 us: 4.8 TB/s of the 5.2 that
+ * 32 sequences of 8192 to 16384 tokens, one query of 32 heads over 8 of 128 channels, take 169 us: 4.8 TB/s of the 5.2 that
  * a copy reaches. Short ones wait for what depends on one another (length, block numbers, blocks, the other wavefronts, the
- * other workgroups): 512 tokens of one sequence take 7.6 us, 16 x 2000 tokens 10.5.
+ * other workgroups): 512 tokens of one sequence take 7.5 us, 4 queries over 16 x 2000 tokens, in two launches, 11.0.
  */
 #pragma once
 
