@@ -744,7 +744,7 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
 // most 1 and over a long axis arbitrarily small, and a score's gradient, that probability times a difference with
 //   |dp - delta| <= B = sum |dout| max |v| + |delta|   (sums over the row's channels, the maximum over the keys of its key head).
 // The gradients of the scores are therefore computed times the power of two that puts B into [2^13, 2^14) (dq: B of the row; dk:
-// the largest of the key head), and the probabilities of dv times 2^13: a probability that float32 puts a little above 1 still
+// the largest of the rows that a workgroup takes), and the probabilities of dv times 2^13: a probability that float32 puts a little above 1 still
 // fits, normal numbers reach down to 2^-27 of the largest. The results are scaled back in float32. (bfloat16 has the
 // exponents of float32: factor 1.)
 constexpr float kProbabilityLift = 13.0f;   // exponent of 2
@@ -793,7 +793,7 @@ struct BackwardSpace {
 
 // The largest |v| of one slice of the keys of a key head, by a workgroup of 256 threads: a launch of its own, or workgroups
 // beside those that find what else the rows need. It reads the values once more: float16 gradients of 8 x 200 x 12 heads of 64
-// take 20.9 us with it and 19.7 without, of 1 x 1024 x 16/4 of 128 79.3 and 75.2, of 2 x 4096 x 32/8 of 128 1068 and 1060.
+// take 20.4 us with it and 19.4 without, of 1 x 1024 x 16/4 of 128 78 and 75, of 2 x 4096 x 32/8 of 128 983 and 975.
 template <typename C>
 AKG_DEV void slice_of_values(const void *v, const int *klens, float *ws, Extents e, long wavefronts, long block) {
   typedef typename C::T T;
@@ -1154,19 +1154,6 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
       load_own<DK>(keys.base + (counts ? key : 0) * keys.step, counts, lane, own);
     }
     if (kDk) load_own<DV>(values.base + (counts ? key : 0) * values.step, counts, lane, val);
-    float lift = 1.0f;
-    if (kDk && T::kNarrowRange) {
-      float largest = 0.0f, largestDelta = 0.0f;
-      for (long t = lane; t < wavesQ; t += 64) {
-        const long at = space.sizes(head * wavesQ + t);
-        largest = __builtin_fmaxf(largest, ws[at]);
-        largestDelta = __builtin_fmaxf(largestDelta, ws[at + 1]);
-      }
-      lift = lift_of<T>(__builtin_fmaf(max_lanes(largest), space.largest_value(ws, head, e.sk, lane), max_lanes(largestDelta)));
-    }
-    // probabilities leave their exponential lifted: the gradients of the scores take that out of their own factor
-    constexpr float kLift = T::kNarrowRange ? kProbabilityLift : 0.0f, kUnlift = T::kNarrowRange ? 0x1p-13f : 1.0f;
-    const float liftBehind = lift * kUnlift;
     const float c = C::ADDED ? scale : scale * kLog2e;
     f32x16 acck[kDk ? TK : 1], accv[kDv ? TV : 1];
 #pragma unroll
@@ -1188,6 +1175,21 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
       from = start < upto ? static_cast<int>(start) : upto;
       if (each < upto - from) upto = from + each;
     }
+
+    // (of the rows that this workgroup takes: what others have costs its keys no digits)
+    float lift = 1.0f;
+    if (kDk && T::kNarrowRange) {
+      float largest = 0.0f, largestDelta = 0.0f;
+      for (long t = from / kRows + lane; t * kRows < upto; t += 64) {
+        const long at = space.sizes(head * wavesQ + t);
+        largest = __builtin_fmaxf(largest, ws[at]);
+        largestDelta = __builtin_fmaxf(largestDelta, ws[at + 1]);
+      }
+      lift = lift_of<T>(__builtin_fmaf(max_lanes(largest), space.largest_value(ws, head, e.sk, lane), max_lanes(largestDelta)));
+    }
+    // probabilities leave their exponential lifted: the gradients of the scores take that out of their own factor
+    constexpr float kLift = T::kNarrowRange ? kProbabilityLift : 0.0f, kUnlift = T::kNarrowRange ? 0x1p-13f : 1.0f;
+    const float liftBehind = lift * kUnlift;
 
     const RowsOf<C, DK> qrows(q, b, hkv, e);
     const RowsOf<C, DV> grows(dout, b, hkv, e);

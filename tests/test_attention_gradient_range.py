@@ -108,3 +108,39 @@ def test_float16_gradients_over_many_keys(dout_size, tmp_path):
     keys = 296941
     case = ("float16", "BSND", 1, 1, keys, 1, 1, 64, 64, False, None, None)
     check(*large_case(case, dout_size, 1.0, 2.0 ** -5), tmp_path)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout,seq,heads,hkv,dim,lengths", [("BSND", 600, 1, 1, 64, None), ("BNSD", 700, 4, 4, 128, [640]), ("BSND", 520, 40, 40, 64, None),
+                                                              ("BNSD", 520, 2, 2, 192, None)])
+def test_float16_gradients_of_keys_that_the_large_rows_do_not_see(layout, seq, heads, hkv, dim, lengths, tmp_path):
+    """The first 64 queries have gradients of some 2^13, the others of 2^-10. Keys from 128 on are seen by the others alone and keep the
+    digits of what those leave: dk there is bounded by the rows from 64 below the key's tile of 128 on."""
+    case = ("float16", layout, 1, seq, seq, heads, hkv, dim, dim, True, None, None)
+    t, _, options, _, _, _ = attention_case(case)
+    extra, ql, kl = {}, lengths, lengths
+    if lengths:
+        extra = {n: torch.tensor(lengths, dtype=torch.int32) for n in ("query_lengths", "key_lengths")}
+    r = ref.forward(t["q"], t["k"], t["v"], qlens=ql, klens=kl, **options)
+    dout = ref.heads_of(normal(r["out"].shape, "float32", 8), layout)
+    dout[:, :, :64] *= 2.0 ** 13
+    dout[:, :, 64:] *= 2.0 ** -10
+    dout = ref.back(dout, layout).contiguous().to(torch.float16)
+    tensors = [dout, t["q"], t["k"], t["v"], r["out"].to(torch.float16), r["lse"].float()]
+    b = builder()
+    grads = op_desc.attention_grad(b, *[given(b, x) for x in tensors], **{n: given(b, x) for n, x in extra.items()}, **options)
+    got = launch(b.dumps(grads), [x.contiguous() for x in tensors] + list(extra.values()), tmp_path)
+    exact, size = ref.gradient(*tensors, qlens=ql, klens=kl, **options)
+    clean = {n: behind_lengths(x, lengths, layout, 0.0) for n, x in t.items()}
+    dout, out = (behind_lengths(x, lengths, layout, 0.0) for x in (dout, r["out"].to(torch.float16)))
+    whole = range_bounds(exact, clean, dout, out, options, size, seq, seq)
+    late = dout.clone()
+    (late if layout == "BNSD" else late.transpose(1, 2))[:, :, :64] = 0
+    tight = range_bounds(exact, clean, late, out, options, size, seq, seq)
+    for n, x in zip(("dq", "dk", "dv"), got):
+        bound = whole[n]
+        if n == "dk":
+            # (what the first rows leave in the exact value and its sums stays; their steps do not)
+            keys = torch.arange(seq).view(1, 1, -1, 1) if layout == "BNSD" else torch.arange(seq).view(1, -1, 1, 1)
+            bound = torch.where(keys >= 128, tight[n], whole[n])
+        close(x, exact[n]["exact"], bound, n)
