@@ -380,8 +380,8 @@ class LayerEmitter {
     auto queriesLds = [&](int part) { return "akg::attn::QueriesLds<akg_C, " + std::to_string(nwq) + ", " + std::to_string(part) + ">"; };
     const std::string keysLds = "akg::attn::KeysLds<akg_C, " + std::to_string(nwk) + ", " + std::to_string(rg) + ">";
     const int64_t rowGroups = s.keyHeads * tilesQ;
-    // float16: the largest value of every key head first, beside the rows' own launch or in one of its own (dv alone needs none)
-    const bool bounds = in(0).dtype == DType::F16, values = bounds && (wantDq || wanted(1));
+    // float16: dq needs the largest value of every key head first, beside the rows' own launch or in one of its own
+    const bool bounds = in(0).dtype == DType::F16, values = bounds && wantDq;
     const int64_t slices = bounds ? std::min<int64_t>(ceilDiv(s.sk, 128), 256) : 0;
     auto slicesOfValues = [&](const std::string &block) {
       return "  akg::attn::slice_of_values<akg_C>(" + inName(3) + ", " + (l_.hasKeyLengths ? inName(6 + (l_.hasMask ? 1 : 0) + (l_.hasQueryLengths ? 1 : 0)) : std::string("nullptr")) +

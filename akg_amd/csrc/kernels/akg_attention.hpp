@@ -742,9 +742,9 @@ AKG_DEV void forward(const void *q, const void *k, const void *v, const void *ma
 // ---- backward ---------------------------------------------------------------------------------------------------------
 // float16 ends at 65504 and has no digits left below 2^-24, and what the matrix units take as float16 is a probability, at
 // most 1 and over a long axis arbitrarily small, and a score's gradient, that probability times a difference with
-//   |dp - delta| <= B = sum |dout| max |v| + |delta|   (sums over the row's channels, the maximum over the keys of its key head).
-// The gradients of the scores are therefore computed times the power of two that puts B into [2^13, 2^14) (dq: B of the row; dk:
-// the largest of the rows that a workgroup takes), and the probabilities of dv times 2^13: a probability that float32 puts a little above 1 still
+//   |dp - delta| <= B = sum |dout| max |v| + |delta|   (sums over the row's channels).
+// The gradients of the scores are therefore computed times the power of two that puts B into [2^13, 2^14) (dq: B of the row and
+// all keys of its key head; dk: the largest of the rows that a workgroup takes and the keys of a wavefront), and the probabilities of dv times 2^13: a probability that float32 puts a little above 1 still
 // fits, normal numbers reach down to 2^-27 of the largest. The results are scaled back in float32. (bfloat16 has the
 // exponents of float32: factor 1.)
 constexpr float kProbabilityLift = 13.0f;   // exponent of 2
@@ -792,7 +792,7 @@ struct BackwardSpace {
 };
 
 // The largest |v| of one slice of the keys of a key head, by a workgroup of 256 threads: a launch of its own, or workgroups
-// beside those that find what else the rows need. It reads the values once more: float16 gradients of 8 x 200 x 12 heads of 64
+// beside those that find what else the rows need, for dq. It reads the values once more: float16 gradients of 8 x 200 x 12 heads of 64
 // take 20.4 us with it and 19.4 without, of 1 x 1024 x 16/4 of 128 78 and 75, of 2 x 4096 x 32/8 of 128 983 and 975.
 template <typename C>
 AKG_DEV void slice_of_values(const void *v, const int *klens, float *ws, Extents e, long wavefronts, long block) {
@@ -1176,16 +1176,23 @@ AKG_DEV void backward_keys(const void *dout, const void *q, const void *k, const
       if (each < upto - from) upto = from + each;
     }
 
-    // (of the rows that this workgroup takes: what others have costs its keys no digits)
+    // (of the rows that this workgroup takes and the wavefront's own keys: what others have costs these no digits)
     float lift = 1.0f;
     if (kDk && T::kNarrowRange) {
-      float largest = 0.0f, largestDelta = 0.0f;
+      float largest = 0.0f, largestDelta = 0.0f, largestValue = 0.0f;
+#pragma unroll
+      for (int x = 0; x < CV; ++x) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          largestValue = __builtin_fmaxf(largestValue, __builtin_fmaxf(__builtin_fabsf(T::low(val[x][w])), __builtin_fabsf(T::high(val[x][w]))));
+        }
+      }
       for (long t = from / kRows + lane; t * kRows < upto; t += 64) {
         const long at = space.sizes(head * wavesQ + t);
         largest = __builtin_fmaxf(largest, ws[at]);
         largestDelta = __builtin_fmaxf(largestDelta, ws[at + 1]);
       }
-      lift = lift_of<T>(__builtin_fmaf(max_lanes(largest), space.largest_value(ws, head, e.sk, lane), max_lanes(largestDelta)));
+      lift = lift_of<T>(__builtin_fmaf(max_lanes(largest), max_lanes(largestValue), max_lanes(largestDelta)));
     }
     // probabilities leave their exponential lifted: the gradients of the scores take that out of their own factor
     constexpr float kLift = T::kNarrowRange ? kProbabilityLift : 0.0f, kUnlift = T::kNarrowRange ? 0x1p-13f : 1.0f;
