@@ -22,6 +22,7 @@ const char *kernelFamilyName(KernelFamily f) {
     case KernelFamily::GemmRows: return "gemm_rows";
     case KernelFamily::Rotary: return "rotary";
     case KernelFamily::Attention: return "attention";
+    case KernelFamily::LinearAttention: return "linear_attention";
     case KernelFamily::Staged: return "staged";
   }
   return "?";

@@ -31,7 +31,7 @@ class LoweringError : public std::runtime_error {
   explicit LoweringError(const std::string &msg) : std::runtime_error(msg) {}
 };
 
-enum class KernelFamily { Elementwise, RowReduce, GemmEpilogue, StreamReduce, Indexed, SegmentSum, Staged, ColumnReduce, GemmRows, PlaneReduce, Rotary, Attention };
+enum class KernelFamily { Elementwise, RowReduce, GemmEpilogue, StreamReduce, Indexed, SegmentSum, Staged, ColumnReduce, GemmRows, PlaneReduce, Rotary, Attention, LinearAttention };
 const char *kernelFamilyName(KernelFamily f);
 
 // Tuning knobs; 0 means "let the heuristic decide". They can be set through the environment
@@ -83,7 +83,7 @@ struct KernelPhase {
 struct LoweredKernel {
   std::string kernelName;  // "<op>_kernel", as the reference names its outlined gpu.func
   // Kernels of the same code object that run before `kernelName`, in this order (empty but for the grouped
-  // segment sum, attention's gradient and attention whose ranges of keys a launch of its own joins). Grid, block and name of the kernel proper stay in the fields below.
+  // segment sum, attention's gradient, attention whose ranges of keys a launch of its own joins and linear attention in segments). Grid, block and name of the kernel proper stay in the fields below.
   std::vector<KernelPhase> earlierPhases;
   std::string source;      // HIP translation unit
   KernelFamily family = KernelFamily::Elementwise;

@@ -1,6 +1,7 @@
 /**
- * The operators of an attention layer (RotaryEmbedding, Attention, AttentionGrad, CacheAttention): descriptions of one op
- * become an instance of the hand-written kernels in kernels/akg_rotary.hpp, akg_attention.hpp and akg_cache_attention.hpp.
+ * The operators of an attention layer (RotaryEmbedding, Attention, AttentionGrad, CacheAttention, LinearAttention,
+ * LinearAttentionGrad): descriptions of one op become an instance of the hand-written kernels in kernels/akg_rotary.hpp,
+ * akg_attention.hpp, akg_cache_attention.hpp and akg_linear_attention.hpp.
  * Types, channels, heads, layout and which operands there are go into the source; batch, sequence lengths and the number
  * of blocks are kernel arguments (LoweredKernel::scalarArgs), so calls that differ there share a code object.
  *
@@ -11,6 +12,7 @@
 #include <cmath>
 #include <cstdio>
 #include <sstream>
+#include <utility>
 
 #include "HipLowering.h"
 
@@ -20,6 +22,7 @@ namespace {
 using lowering::dtypeTag;
 
 int64_t ceilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+constexpr int64_t kFewTokens = 8;   // up to which linear attention goes token after token
 
 class LayerEmitter {
  public:
@@ -38,6 +41,8 @@ class LayerEmitter {
       case OpKind::RotaryEmbedding: rotary(); break;
       case OpKind::Attention: attention(); break;
       case OpKind::AttentionGrad: attentionGrad(); break;
+      case OpKind::LinearAttention: linearAttention(); break;
+      case OpKind::LinearAttentionGrad: linearAttentionGrad(); break;
       default: cacheAttention(); break;
     }
     k_.shapeArgs = lowering::buildShapeArgs(g_);
@@ -102,12 +107,31 @@ class LayerEmitter {
   const char *trait() const { return in(0).dtype == DType::BF16 ? "akg::attn::BF16" : "akg::attn::F16"; }
 
   // ---- RotaryEmbedding ------------------------------------------------------------------------------------------------
+  // Which axis every pair turns by, and the how many-th pair of that axis it is.
+  std::vector<std::pair<int64_t, int64_t>> axes() const {
+    std::vector<std::pair<int64_t, int64_t>> out;
+    if (l_.sections.empty()) {
+      for (int64_t i = 0; i < l_.rotaryDims / 2; ++i) out.push_back({0, i});
+      return out;
+    }
+    std::vector<int64_t> used(l_.sections.size(), 0);
+    size_t a = 0;
+    for (int64_t i = 0; i < l_.rotaryDims / 2; ++i) {
+      if (l_.axisCycle && i > 0) a = (a + 1) % used.size();
+      while (used[a] == l_.sections[a]) a = (a + 1) % used.size();   // (the sections add up to the pairs)
+      out.push_back({static_cast<int64_t>(a), used[a]++});
+    }
+    return out;
+  }
   // Turns per position of every pair, as fractions of 2^64.
   std::vector<uint64_t> rates() const {
     std::vector<uint64_t> out;
     const long double twoPi = 6.283185307179586476925286766559005768L;
-    for (int64_t i = 0; i < l_.rotaryDims / 2; ++i) {
-      long double w = std::pow(static_cast<long double>(l_.base), -2.0L * static_cast<long double>(i) / static_cast<long double>(l_.rotaryDims));
+    for (const std::pair<int64_t, int64_t> &p : axes()) {
+      const bool own = l_.axisOwnRates;
+      const long double i = static_cast<long double>(own ? p.second : static_cast<int64_t>(out.size()));
+      const long double dims = static_cast<long double>(own ? 2 * l_.sections[static_cast<size_t>(p.first)] : l_.rotaryDims);
+      long double w = std::pow(static_cast<long double>(l_.base), -2.0L * i / dims);
       if (l_.scaling == LayerAttributes::Scaling::Linear) {
         w /= static_cast<long double>(l_.factor);
       } else if (l_.scaling == LayerAttributes::Scaling::Wavelength) {
@@ -144,17 +168,35 @@ class LayerEmitter {
     o << "__device__ const akg::u64 akg_rates[" << rate.size() << "] = {";
     for (size_t i = 0; i < rate.size(); ++i) o << (i ? ", " : "") << rate[i] << "ull";
     o << "};\n\n";
+    // Axes: that of every pair, unless the pairs of a thread all have one (their first pair's).
+    const std::vector<std::pair<int64_t, int64_t>> axis = axes();
+    const bool several = !l_.sections.empty();
+    bool mixed = false;
+    for (size_t i = 0; several && i < axis.size(); ++i) mixed = mixed || axis[i].first != axis[i / static_cast<size_t>(pairs) * static_cast<size_t>(pairs)].first;
+    if (several) {
+      o << "__device__ const akg::u8 akg_axes[" << axis.size() << "] = {";
+      for (size_t i = 0; i < axis.size(); ++i) o << (i ? ", " : "") << axis[i].first;
+      o << "};\n\n";
+    }
     std::ostringstream b;
-    const bool perBatch = positions.shape.size() == 2 && positions.shape[0] == batch;
+    const size_t positionRank = positions.shape.size() - (several ? 1 : 0);
+    const bool perBatch = positionRank == 2 && positions.shape[positions.shape.size() - 2] == batch;
     b << "  constexpr int P = " << pairs << ", CHUNKS = " << chunks << ", HEADS = " << all << ";\n"
       << "  const long at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;\n"
       << "  const long token = at / (CHUNKS * HEADS);\n  if (token >= akg_batch * akg_seq) return;\n"
       << "  const int rest = static_cast<int>(at % (CHUNKS * HEADS)), chunk = rest % CHUNKS, head = rest / CHUNKS;\n"
       << "  const long b = token / akg_seq, s = token % akg_seq;\n"
-      << "  const akg::u64 position = static_cast<akg::u64>(static_cast<long long>(" << inName(tensors) << "[" << (perBatch ? "token" : "s") << "]));\n"
-      << "  float sine[P], cosine[P];\n#pragma unroll\n  for (int e = 0; e < P; ++e) {\n"
-      << "    const int pair = P * chunk + e;\n"
-      << "    akg::rotary::sine_cosine(position * akg_rates[pair < " << r / 2 << " ? pair : 0], sine[e], cosine[e]);\n"
+      << "  float sine[P], cosine[P];\n";
+    const std::string stride = perBatch ? "akg_batch * akg_seq" : "akg_seq", place = perBatch ? "token" : "s";
+    auto position = [&](const std::string &axisOf) {
+      return "const akg::u64 position = static_cast<akg::u64>(static_cast<long long>(" + inName(tensors) + "[" + (several ? axisOf + " * (" + stride + ") + " : "") + place + "]));\n";
+    };
+    const std::string last = std::to_string(r / 2 - 1);
+    if (!mixed) b << "  " << position("static_cast<long>(akg_axes[P * chunk < " + last + " ? P * chunk : " + last + "])");
+    b << "#pragma unroll\n  for (int e = 0; e < P; ++e) {\n"
+      << "    const int pair = P * chunk + e;\n";
+    if (mixed) b << "    " << position("static_cast<long>(akg_axes[pair < " + last + " ? pair : " + last + "])");
+    b << "    akg::rotary::sine_cosine(position * akg_rates[pair < " << r / 2 << " ? pair : 0], sine[e], cosine[e]);\n"
       << "    sine[e] *= " << number(l_.inverse ? -l_.magnitude : l_.magnitude) << ";\n    cosine[e] *= " << number(l_.magnitude) << ";\n  }\n";
     int64_t before = 0;
     for (size_t t = 0; t < tensors; ++t) {
@@ -501,6 +543,238 @@ class LayerEmitter {
                           2 * 2 * static_cast<uint64_t>(q.numel());
     k_.algorithmicOps = static_cast<uint64_t>(4 * dim * batch * heads * sq * perSequence * page);
     k_.scheduleNote = "row tiles " + std::to_string(rt) + ", workgroups per sequence and key head " + std::to_string(splits);
+  }
+
+  // ---- LinearAttention and its gradient -------------------------------------------------------------------------------
+  // One walk over the tokens (linear::Config): which operands are a, b and c, and what becomes of its result.
+  struct WalkOf {
+    std::string a, b, c, out, first, last;
+    int64_t d, e, ha, hb, hc;
+    bool back, turned;
+    const char *result;   // of linear::Result
+    int64_t tiles = 1;
+  };
+  struct LinearSizes {
+    int64_t batch, seq, heads, kvHeads, dk, dv, states;
+  };
+  LinearSizes linearSizes(const TensorValue &q, const TensorValue &v) const {
+    const size_t seqDim = l_.headsFirst ? 2 : 1, headDim = l_.headsFirst ? 1 : 2;
+    LinearSizes s;
+    s.batch = q.shape[0];
+    s.seq = q.shape[seqDim];
+    s.heads = q.shape[headDim];
+    s.kvHeads = v.shape[headDim];
+    s.dk = q.shape[3];
+    s.dv = v.shape[3];
+    s.states = s.batch * s.heads;
+    if (s.dk % 8 != 0 || s.dv % 8 != 0 || s.dk > 256 || s.dv > 256) {
+      throw LoweringError("op " + op_.name + ": the channels of a head must be a multiple of 8 up to 256");
+    }
+    // (byte offsets inside a chunk are 32-bit values; tokens of a segment and their exponents too)
+    if (64 * s.heads * 2 * std::max(s.dk, s.dv) >= (1LL << 31) - 65536) throw LoweringError("op " + op_.name + ": the tokens of a chunk lie more than 2 GiB apart");
+    if (s.seq >= (1LL << 31) - 8192) throw LoweringError("op " + op_.name + ": more than 2^31 tokens");
+    return s;
+  }
+  std::string walkConfig(const WalkOf &w, const LinearSizes &s, int ct, int64_t nw) const {
+    std::ostringstream o;
+    o << "akg::linear::Config<" << trait() << ", " << w.d << ", " << w.e << ", " << ct << ", " << nw << ", " << s.heads << ", " << w.ha << ", " << w.hb << ", " << w.hc
+      << ", " << flag(l_.headsFirst) << ", " << flag(w.back) << ", " << flag(w.turned) << ", akg::linear::Result::" << w.result << ">";
+    return o.str();
+  }
+  // The launches of walks that belong together, the last of them the kernel proper unless `more` follow: with several
+  // segments what each adds to the states, the states in front of each, then the walks themselves. `space`: bytes of the
+  // workspace in front of theirs. The workspace's bytes are returned.
+  int64_t walks(std::ostringstream &o, std::vector<KernelPhase> &phases, std::vector<WalkOf> &all, const LinearSizes &s, const std::string &args, const std::string &decay,
+                const std::string &lengths, const std::string &slots, int64_t space, bool more) {
+    int64_t widest = 0, deepest = 0;
+    for (const WalkOf &w : all) {
+      widest = std::max(widest, w.e);
+      deepest = std::max(deepest, std::max(w.d, w.e));
+    }
+    const bool pairsOfParts = in(0).dtype == DType::F16;
+    const int ct = pairsOfParts ? 1 : 2;
+    const int64_t units = ceilDiv(widest, 32), nw = std::max<int64_t>(2, ceilDiv(units, ceilDiv(units, 4)));
+    int64_t groups = 0, values = 0;
+    for (WalkOf &w : all) {
+      w.tiles = ceilDiv(w.e, 32 * nw);
+      groups += s.states * w.tiles;
+      values += w.d * w.e;
+    }
+    int64_t segments = std::max<int64_t>(1, std::min<int64_t>(2 * cus_ / groups, s.seq / 256));
+    while (limit_ > 0 && segments > 1 && space + 4 * s.states * segments * values > limit_) --segments;
+    const int64_t chunk = 32 * ct, segment = ceilDiv(ceilDiv(s.seq, segments), chunk) * chunk;
+    segments = ceilDiv(s.seq, segment);
+    k_.scalarArgs = {s.batch, s.seq, segment, segments};
+    if (l_.hasSlots) k_.scalarArgs.push_back(in(4).shape[0]);
+    std::vector<std::string> names;
+    o << "typedef " << walkConfig(all[0], s, ct, nw) << " akg_C0;\n";
+    for (size_t i = 1; i < all.size(); ++i) o << "typedef " << walkConfig(all[i], s, ct, nw) << " akg_C" << i << ";\n";
+    o << "\n";
+    int64_t before = space;
+    std::vector<std::string> structs;
+    for (const WalkOf &w : all) {
+      std::ostringstream b;
+      b << "{" << w.a << ", " << w.b << ", " << w.c << ", " << w.out << ", " << decay << ", " << w.first << ", " << w.last << ", " << lengths << ", " << slots << ", ";
+      if (segments > 1) b << "akg_ws + (" << space / 4 << "L + " << (before - space) / 4 << "L * akg_batch * akg_segments)";
+      else b << "nullptr";
+      b << ", akg_seq, " << (l_.hasSlots ? "akg_pool" : "akg_batch") << ", static_cast<int>(akg_segment), static_cast<int>(akg_segments), " << number(l_.scale) << "}";
+      structs.push_back(b.str());
+      before += 4 * s.heads * w.d * w.e;
+    }
+    const int threads = static_cast<int>(64 * nw);
+    const int hint = deepest <= 128 ? 2 : 0;
+    // every walk has the workgroups from `from` on; a head's are on one XCD (attn::head_and_tile)
+    auto body = [&](bool states) {
+      std::ostringstream b;
+      const char *kind = states ? "StateLds" : "Lds";
+      b << "  __shared__ __attribute__((aligned(16))) akg::u8 akg_lds[";
+      std::string size = std::string("sizeof(akg::linear::") + kind + "<akg_C0>)";
+      for (size_t i = 1; i < all.size(); ++i) {
+        const std::string other = std::string("sizeof(akg::linear::") + kind + "<akg_C" + std::to_string(i) + ">)";
+        size = "(" + size + " > " + other + " ? " + size + " : " + other + ")";
+      }
+      b << size << "];\n  long akg_id = blockIdx.x, akg_head, akg_rest;\n  const long akg_heads = akg_batch * " << s.heads << ", akg_parts = " << (states ? "akg_segments - 1" : "akg_segments") << ";\n";
+      for (size_t i = 0; i < all.size(); ++i) {
+        const std::string n = std::to_string(i);
+        b << "  if (akg_id < akg_heads * akg_parts * akg_C" << n << "::kTiles) {\n    const akg::linear::Walk akg_w = " << structs[i] << ";\n"
+          << "    akg::attn::head_and_tile(akg_id, akg_heads, akg_head, akg_rest);\n"
+          << "    akg::linear::walk<akg_C" << n << ", " << flag(states) << ">(akg_w, *reinterpret_cast<akg::linear::" << kind << "<akg_C" << n
+          << "> *>(akg_lds), akg_head, static_cast<int>(akg_rest % akg_C" << n << "::kTiles), static_cast<int>(akg_rest / akg_C" << n << "::kTiles));\n    return;\n  }\n"
+          << "  akg_id -= akg_heads * akg_parts * akg_C" << n << "::kTiles;\n";
+      }
+      return b.str();
+    };
+    auto launch = [&](const std::string &name, int64_t grid, int n, const std::string &text, int wavesPerSimd) {
+      KernelPhase p;
+      p.kernelName = name;
+      p.grid[0] = checkGrid(grid, n);
+      p.block[0] = static_cast<unsigned>(n);
+      phases.push_back(p);
+      o << kernel(name, n, args, text, wavesPerSimd);
+    };
+    if (segments > 1) {
+      launch(name_ + "_states", groups * (segments - 1), threads, body(true), hint);
+      std::ostringstream b;
+      b << "  long akg_at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;\n  const long akg_heads = akg_batch * " << s.heads << ";\n";
+      for (size_t i = 0; i < all.size(); ++i) {
+        b << "  if (akg_at < akg_heads * " << all[i].d * all[i].e / 4 << ") {\n    const akg::linear::Walk akg_w = " << structs[i] << ";\n    akg::linear::scan<akg_C" << i
+          << ">(akg_w, akg_heads, akg_at);\n    return;\n  }\n  akg_at -= akg_heads * " << all[i].d * all[i].e / 4 << ";\n";
+      }
+      launch(name_ + "_starts", ceilDiv(s.states * values / 4, 256), 256, b.str(), 0);
+    }
+    launch(more ? name_ + "_walks" : k_.kernelName, groups * segments, threads, body(false), hint);
+    k_.family = KernelFamily::LinearAttention;
+    k_.scheduleNote = "tokens of a chunk " + std::to_string(chunk) + ", wavefronts " + std::to_string(nw) + ", segments " + std::to_string(segments);
+    return segments > 1 ? space + 4 * s.states * segments * values : space;
+  }
+  void lastPhase(std::vector<KernelPhase> phases) {
+    std::copy(phases.back().grid, phases.back().grid + 3, k_.grid);
+    std::copy(phases.back().block, phases.back().block + 3, k_.block);
+    phases.pop_back();
+    k_.earlierPhases = phases;
+  }
+
+  void linearAttention() {
+    const LinearSizes s = linearSizes(in(0), in(2));
+    size_t next = 4;
+    const std::string state = l_.hasState ? inName(next++) : "nullptr", slots = l_.hasSlots ? inName(next++) : "nullptr";
+    const std::string lengths = l_.hasLengths ? inName(next++) : "nullptr";
+    std::ostringstream o;
+    o << head("#include \"akg_attention.hpp\"\n#include \"akg_linear_attention.hpp\"\n");
+    k_.algorithmicOps = static_cast<uint64_t>(4 * s.states * s.seq * s.dk * s.dv);
+    if (s.seq <= kFewTokens) {
+      // Columns of a workgroup: as many as leave two workgroups for every CU.
+      int64_t te = 128;
+      while (te > 16 && (te / 2 >= s.dv || s.states * ceilDiv(s.dv, te) < 2 * cus_)) te /= 2;
+      const int64_t tiles = ceilDiv(s.dv, te);
+      std::vector<std::string> scalars = {"akg_batch", "akg_seq"};
+      if (l_.hasSlots) scalars.push_back("akg_pool");
+      std::ostringstream b;
+      b << "  const akg::linear::Walk akg_w = {" << inName(0) << ", " << inName(1) << ", " << inName(2) << ", " << outName(0) << ", " << inName(3) << ", " << state << ", "
+        << outName(1) << ", " << lengths << ", " << slots << ", nullptr, akg_seq, " << (l_.hasSlots ? "akg_pool" : "akg_batch") << ", 0, 1, " << number(l_.scale) << "};\n"
+        << "  akg::linear::tokens<" << trait() << ", " << s.dk << ", " << s.dv << ", " << te << ", " << s.heads << ", " << s.kvHeads << ", " << flag(l_.headsFirst) << ", " << kFewTokens
+        << ">(akg_w, blockIdx.x / " << tiles << ", static_cast<int>(blockIdx.x % " << tiles << "));\n";
+      o << kernel(k_.kernelName, 256, signature(scalars, false), b.str());
+      k_.scalarArgs = {s.batch, s.seq};
+      if (l_.hasSlots) k_.scalarArgs.push_back(in(4).shape[0]);
+      k_.grid[0] = checkGrid(s.states * tiles, 256);
+      k_.block[0] = 256;
+      k_.family = KernelFamily::LinearAttention;
+      k_.scheduleNote = "token after token, columns of a workgroup " + std::to_string(te);
+      k_.source = o.str();
+      return;
+    }
+    std::vector<std::string> scalars = {"akg_batch", "akg_seq", "akg_segment", "akg_segments"};
+    if (l_.hasSlots) scalars.push_back("akg_pool");
+    WalkOf w{inName(0), inName(1), inName(2), outName(0), state, outName(1), s.dk, s.dv, s.heads, s.kvHeads, s.kvHeads, false, false, wanted(0) ? "Storage" : "None"};
+    std::vector<WalkOf> all{w};
+    std::vector<KernelPhase> phases;
+    // (whether there is a workspace is known only behind the schedule: the text is made twice where there is none)
+    std::ostringstream text;
+    k_.workspaceBytes = static_cast<uint64_t>(walks(text, phases, all, s, signature(scalars, true), inName(3), lengths, slots, 0, false));
+    if (k_.workspaceBytes == 0) {
+      text.str("");
+      phases.clear();
+      walks(text, phases, all, s, signature(scalars, false), inName(3), lengths, slots, 0, false);
+    }
+    o << text.str();
+    lastPhase(phases);
+    k_.source = o.str();
+  }
+
+  void linearAttentionGrad() {
+    const LinearSizes s = linearSizes(in(1), in(3));
+    size_t next = 5;
+    const std::string state = l_.hasState ? inName(next++) : "nullptr", dstate = l_.hasStateGradient ? inName(next++) : "nullptr";
+    const std::string lengths = l_.hasLengths ? inName(next++) : "nullptr";
+    const std::string dout = inName(0), q = inName(1), k = inName(2), v = inName(3);
+    std::ostringstream o;
+    o << head("#include \"akg_attention.hpp\"\n#include \"akg_linear_attention.hpp\"\n");
+    const int64_t h = s.heads, kv = s.kvHeads, rows = s.states * s.seq;
+    const bool shared = h != kv;
+    // gradients of shared heads: every head's own in float32 first
+    const int64_t dkBytes = shared && wanted(1) ? 4 * rows * s.dk : 0, dvBytes = shared && wanted(2) ? 4 * rows * s.dv : 0;
+    const std::string dvAt = wanted(1) ? "akg_batch * akg_seq * " + std::to_string(h * s.dk) + "L" : "0L";
+    std::vector<WalkOf> all;
+    const char *part = shared ? "Float" : "Storage";
+    if (wanted(0)) all.push_back({dout, v, k, outName(0), state, "nullptr", s.dv, s.dk, h, kv, kv, false, true, "Storage"});
+    if (wanted(1)) all.push_back({v, dout, q, shared ? "akg_ws" : outName(1), dstate, "nullptr", s.dv, s.dk, kv, h, h, true, true, part});
+    if (wanted(2) || wanted(3)) {
+      all.push_back({k, q, dout, !wanted(2) ? "nullptr" : shared ? "akg_ws + " + dvAt : outName(2), dstate, outName(3), s.dk, s.dv, kv, h, h, true, false, wanted(2) ? part : "None"});
+    }
+    if (all.empty()) throw LoweringError("op " + op_.name + ": none of its results is an output");
+    const bool more = dkBytes + dvBytes > 0;
+    const std::vector<std::string> scalars = {"akg_batch", "akg_seq", "akg_segment", "akg_segments"};
+    std::vector<KernelPhase> phases;
+    std::ostringstream text;
+    k_.workspaceBytes = static_cast<uint64_t>(walks(text, phases, all, s, signature(scalars, true), inName(4), lengths, "nullptr", dkBytes + dvBytes, more));
+    if (k_.workspaceBytes == 0) {
+      text.str("");
+      phases.clear();
+      walks(text, phases, all, s, signature(scalars, false), inName(4), lengths, "nullptr", 0, more);
+    }
+    o << text.str();
+    if (more) {
+      KernelPhase p;
+      p.kernelName = k_.kernelName;
+      p.grid[0] = checkGrid(ceilDiv(s.batch * kv * s.seq * ((dkBytes ? s.dk : 0) + (dvBytes ? s.dv : 0)) / 4, 256), 256);
+      p.block[0] = 256;
+      phases.push_back(p);
+      std::ostringstream b;
+      b << "  long akg_at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;\n";
+      auto one = [&](int64_t d, const std::string &from, const std::string &to) {
+        b << "  if (akg_at < akg_batch * akg_seq * " << kv * d / 4 << "L) {\n    akg::linear::share<" << trait() << ", " << d << ", " << h << ", " << kv << ", " << flag(l_.headsFirst) << ">("
+          << from << ", " << to << ", akg_batch, akg_seq, akg_at);\n    return;\n  }\n  akg_at -= akg_batch * akg_seq * " << kv * d / 4 << "L;\n";
+      };
+      if (dkBytes) one(s.dk, "akg_ws", outName(1));
+      if (dvBytes) one(s.dv, "akg_ws + " + dvAt, outName(2));
+      o << kernel(p.kernelName, 256, signature(scalars, true), b.str());
+    }
+    lastPhase(phases);
+    k_.source = o.str();
+    // (both states, and a product for every result)
+    k_.algorithmicOps = static_cast<uint64_t>((wanted(0) ? 4 : 0) + (wanted(1) || wanted(2) || wanted(3) ? 2 : 0) + (wanted(1) ? 2 : 0) + (wanted(2) ? 2 : 0)) *
+                        static_cast<uint64_t>(s.states * s.seq * s.dk * s.dv);
   }
 };
 

@@ -105,6 +105,8 @@ const OpTableEntry kOpTable[] = {
   {"Attention", OpKind::Attention},
   {"AttentionGrad", OpKind::AttentionGrad},
   {"CacheAttention", OpKind::CacheAttention},
+  {"LinearAttention", OpKind::LinearAttention},
+  {"LinearAttentionGrad", OpKind::LinearAttentionGrad},
 };
 
 OpKind lookupOpKind(const std::string &name) {
@@ -641,6 +643,20 @@ class GraphBuilder {
       } else if (scaling != "none") {
         throw TranslateError(at + "scaling must be none, linear or wavelength");
       }
+      if (const json::Value *a = findAttr(attrs, "sections")) {
+        if (!a->isArray() || a->asDoubleVector().empty()) throw TranslateError(at + "sections must be a list of whole numbers");
+        for (double n : a->asDoubleVector()) {
+          if (!(n >= 0.0 && n < 2147483648.0) || n != std::floor(n)) throw TranslateError(at + "sections must be whole numbers of pairs");
+          l.sections.push_back(static_cast<int64_t>(n));
+        }
+        if (l.sections.size() > 16) throw TranslateError(at + "positions have at most 16 axes");
+      }
+      const std::string order = textAttr(attrs, "axis_order", "blocks"), axisRates = textAttr(attrs, "axis_rates", "shared");
+      if (order != "blocks" && order != "cycle") throw TranslateError(at + "axis_order must be blocks or cycle");
+      if (axisRates != "shared" && axisRates != "own") throw TranslateError(at + "axis_rates must be shared or own");
+      l.axisCycle = order == "cycle";
+      l.axisOwnRates = axisRates == "own";
+      if (l.sections.empty() && (l.axisCycle || l.axisOwnRates)) throw TranslateError(at + "axis_order and axis_rates need sections");
       if (!(l.base > 1.0) || !(l.factor >= 1.0)) throw TranslateError(at + "base must be above 1 and factor at least 1");
       if (node->inputs.size() != 2 && node->inputs.size() != 3) throw TranslateError(at + "takes one or two tensors and their positions");
       return node->inputs.size();
@@ -652,6 +668,15 @@ class GraphBuilder {
     if (node->kind == OpKind::CacheAttention) {
       if (l.headsFirst) throw TranslateError(at + "layout must be BSND");
       return 7;
+    }
+    if (node->kind == OpKind::LinearAttention || node->kind == OpKind::LinearAttentionGrad) {
+      const bool grad = node->kind == OpKind::LinearAttentionGrad;
+      l.hasState = boolAttr(attrs, "has_state");
+      l.hasLengths = boolAttr(attrs, "has_lengths");
+      if (grad) l.hasStateGradient = boolAttr(attrs, "has_state_gradient");
+      if (!grad) l.hasSlots = boolAttr(attrs, "has_slots");
+      if (l.hasSlots && !l.hasState) throw TranslateError(at + "slots need the states that they are slots of");
+      return (grad ? 5u : 4u) + (l.hasState ? 1 : 0) + (l.hasSlots ? 1 : 0) + (l.hasStateGradient ? 1 : 0) + (l.hasLengths ? 1 : 0);
     }
     l.causal = boolAttr(attrs, "causal");
     l.hasMask = boolAttr(attrs, "has_mask");
@@ -695,6 +720,16 @@ class GraphBuilder {
       }
       const TensorValue &p = operand(tensors);
       need(p.dtype == DType::I32 || p.dtype == DType::I64, "positions must be int32 or int64");
+      if (!l.sections.empty()) {
+        int64_t pairs = 0;
+        for (int64_t n : l.sections) pairs += n;
+        need(2 * pairs == l.rotaryDims, "sections must add up to half of rotary_dims");
+        const int64_t axes = static_cast<int64_t>(l.sections.size());
+        const size_t rank = p.shape.size();
+        need((rank == 2 || (rank == 3 && (p.shape[1] == batch || p.shape[1] == 1))) && p.shape[0] == axes && p.shape[rank - 1] == seq,
+             "positions must be [axes, sequence] or [axes, batch, sequence]");
+        return out;
+      }
       need((p.shape.size() == 1 && p.shape[0] == seq) || (p.shape.size() == 2 && (p.shape[0] == batch || p.shape[0] == 1) && p.shape[1] == seq),
            "positions must be [sequence] or [batch, sequence]");
       return out;
@@ -716,6 +751,45 @@ class GraphBuilder {
       need(results == 1, "has one result");
       if (l.scale == 0.0) l.scale = 1.0 / std::sqrt(static_cast<double>(dim));
       return {like(x)};
+    }
+    if (node.kind == OpKind::LinearAttention || node.kind == OpKind::LinearAttentionGrad) {
+      const size_t at0 = node.kind == OpKind::LinearAttentionGrad ? 1 : 0;   // (behind dout)
+      const TensorValue &q = operand(at0), &k = operand(at0 + 1), &v = operand(at0 + 2), &decay = operand(at0 + 3);
+      need(q.shape.size() == 4 && k.shape.size() == 4 && v.shape.size() == 4, "tensors of heads must have four dimensions");
+      need(q.dtype == x.dtype && k.dtype == x.dtype && v.dtype == x.dtype, "queries, keys and values must have one type");
+      need(q.shape[0] == batch && q.shape[seqDim] == seq && q.shape[headDim] == heads, "the gradient must have the shape of the result");
+      need(k.shape[0] == batch && v.shape[0] == batch && k.shape[seqDim] == seq && v.shape[seqDim] == seq, "queries, keys and values differ in batch or sequence");
+      need(k.shape[headDim] == v.shape[headDim] && heads % k.shape[headDim] == 0, "keys and values must have the same heads, and queries a multiple of them");
+      need(k.shape[3] == q.shape[3], "queries and keys differ in the channels of a head");
+      need(decay.dtype == DType::F32 && decay.shape == std::vector<int64_t>{heads}, "log_decay must be float32 [heads]");
+      if (l.scale == 0.0) l.scale = 1.0 / std::sqrt(static_cast<double>(q.shape[3]));
+      TensorValue out = like(q), state;
+      out.shape[3] = v.shape[3];
+      state.dtype = DType::F32;
+      state.shape = {batch, heads, q.shape[3], v.shape[3]};
+      size_t next = at0 + 4;
+      if (l.hasState) {
+        const TensorValue &s = operand(next++);
+        need(s.dtype == DType::F32 && s.shape.size() == 4, "states must be float32 with four dimensions");
+        if (l.hasSlots) state.shape[0] = s.shape[0];
+        need(s.shape == state.shape, "states must be [batch (or slots), heads, channels of the keys, channels of the values]");
+      }
+      if (l.hasSlots) lengths(next++, "slots");
+      if (l.hasStateGradient) {
+        need(operand(next).dtype == DType::F32 && operand(next).shape == state.shape, "the state's gradient must be float32 [batch, heads, channels of the keys, channels of the values]");
+        ++next;
+      }
+      if (l.hasLengths) lengths(next++, "lengths");
+      if (at0 == 0) {
+        need(results == 1 || results == 2, "has one or two results: the values read and the last state");
+        if (results == 1) return {out};
+        return {out, state};
+      }
+      need(x.shape == out.shape, "the gradient must have the shape of the result");
+      need(results == (l.hasState ? 4u : 3u), "has a result for each of queries, keys, values and the state given");
+      std::vector<TensorValue> grads{like(q), like(k), like(v)};
+      if (l.hasState) grads.push_back(state);
+      return grads;
     }
     // Attention: q, k, v ...; AttentionGrad: dout, q, k, v, out, lse ...
     const bool grad = node.kind == OpKind::AttentionGrad;
@@ -974,6 +1048,8 @@ OperatorTemplate templateOfOp(const OpGraph &g, const OpNode &op) {
     case OpKind::Attention:
     case OpKind::AttentionGrad:
     case OpKind::CacheAttention:
+    case OpKind::LinearAttention:
+    case OpKind::LinearAttentionGrad:
       return OperatorTemplate::Matmul;
     case OpKind::Reshape:
       return OperatorTemplate::Reshape;
@@ -1127,6 +1203,8 @@ const char *opKindName(OpKind k) {
     case OpKind::Attention: return "attention";
     case OpKind::AttentionGrad: return "attention_grad";
     case OpKind::CacheAttention: return "cache_attention";
+    case OpKind::LinearAttention: return "linear_attention";
+    case OpKind::LinearAttentionGrad: return "linear_attention_grad";
     case OpKind::Assign: return "inplace_assign";
     case OpKind::Unsupported: return "unsupported";
     case OpKind::Unknown: return "unknown";
@@ -1135,7 +1213,8 @@ const char *opKindName(OpKind k) {
 }
 
 bool isLayerKind(OpKind k) {
-  return k == OpKind::RotaryEmbedding || k == OpKind::Attention || k == OpKind::AttentionGrad || k == OpKind::CacheAttention;
+  return k == OpKind::RotaryEmbedding || k == OpKind::Attention || k == OpKind::AttentionGrad || k == OpKind::CacheAttention ||
+         k == OpKind::LinearAttention || k == OpKind::LinearAttentionGrad;
 }
 
 const char *operatorTemplateName(OperatorTemplate t) {
@@ -1431,8 +1510,14 @@ std::string printOpGraph(const OpGraph &g) {
         static const char *const kScaling[] = {"none", "linear", "wavelength"};
         os << ", base = " << l.base << ", rotary_dims = " << l.rotaryDims << ", interleaved = " << (l.interleaved ? "true" : "false")
            << ", inverse = " << (l.inverse ? "true" : "false") << ", scaling = \"" << kScaling[static_cast<int>(l.scaling)] << "\"";
+        if (!l.sections.empty()) {
+          os << ", sections = [";
+          for (size_t i = 0; i < l.sections.size(); ++i) os << (i ? ", " : "") << l.sections[i];
+          os << "], axis_order = \"" << (l.axisCycle ? "cycle" : "blocks") << "\", axis_rates = \"" << (l.axisOwnRates ? "own" : "shared") << "\"";
+        }
       } else {
-        os << ", scale = " << l.scale << ", causal = " << (l.causal ? "true" : "false");
+        os << ", scale = " << l.scale;
+        if (op.kind != OpKind::LinearAttention && op.kind != OpKind::LinearAttentionGrad) os << ", causal = " << (l.causal ? "true" : "false");
       }
       os << "}";
     }

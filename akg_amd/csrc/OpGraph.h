@@ -56,7 +56,7 @@ enum class OpKind {
   // contraction
   MatMul,
   // the operators of an attention layer, each a kernel of its own (LayerAttributes)
-  RotaryEmbedding, Attention, AttentionGrad, CacheAttention,
+  RotaryEmbedding, Attention, AttentionGrad, CacheAttention, LinearAttention, LinearAttentionGrad,
   // n-ary
   AddN,
   // Assign / InplaceAssign: the result is the second operand; as a side effect it is also written over the first
@@ -69,7 +69,7 @@ enum class OpKind {
 };
 
 const char *opKindName(OpKind k);
-// RotaryEmbedding, Attention, AttentionGrad, CacheAttention.
+// RotaryEmbedding, Attention, AttentionGrad, CacheAttention, LinearAttention, LinearAttentionGrad.
 bool isLayerKind(OpKind k);
 
 // OperatorTemplate lattice of akg-mlir/include/akg/Utils/AnalysisCommon.hpp:127; the fusion class of a kernel
@@ -93,13 +93,15 @@ struct TensorValue {
   int64_t numel() const;
 };
 
-// Attributes of RotaryEmbedding, Attention, AttentionGrad and CacheAttention.
+// Attributes of the operators of an attention layer.
 struct LayerAttributes {
   bool headsFirst = false;        // "layout": "BSND" (default) or "BNSD"
   // Attention and its gradient: optional operands behind the fixed ones, in this order
   bool hasMask = false, hasQueryLengths = false, hasKeyLengths = false;
   bool causal = false;
   double scale = 0.0;             // of the scores; the translator puts 1 / sqrt(channels) where none is given
+  // LinearAttention and its gradient: optional operands behind the fixed ones, in this order
+  bool hasState = false, hasSlots = false, hasStateGradient = false, hasLengths = false;
   // RotaryEmbedding
   double base = 10000.0, magnitude = 1.0;
   int64_t rotaryDims = 0;         // leading channels of a head that are turned
@@ -107,6 +109,9 @@ struct LayerAttributes {
   bool inverse = false;           // turned back: the gradient
   enum class Scaling { None, Linear, Wavelength } scaling = Scaling::None;
   double factor = 1.0, low = 1.0, high = 4.0, originalLength = 0.0;
+  std::vector<int64_t> sections;  // pairs of every axis of the positions (empty: positions have one axis)
+  bool axisCycle = false;         // pairs dealt to the axes in turn (else a block of pairs for every axis)
+  bool axisOwnRates = false;      // the pairs of an axis have the rates of a head of their own
 };
 
 struct OpNode {

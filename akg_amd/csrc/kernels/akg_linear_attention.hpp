@@ -1,0 +1,620 @@
+/**
+ * Linear attention with a decay for each head, for gfx950. The state of a head is a matrix, keys by values, in float32:
+ *
+ *   S[t] = exp(g) S[t-1] + k[t] v[t]^T,   out[t] = scale q[t] S[t]
+ *
+ * A walk over tokens takes a chunk of them at a time, S being the state in front of the chunk (r, c: tokens inside it):
+ *
+ *   out[r] = scale ( exp(g (r + 1)) q[r] S + sum_{c <= r} exp(g (r - c)) (q[r] . k[c]) v[c] )
+ *   S     <- exp(g n) S + sum_c exp(g (n - 1 - c)) k[c] v[c]^T        (n: tokens of the chunk)
+ *
+ * No exponent is positive where g is not, so nothing overflows however long the walk is. The gradient is three walks of
+ * the same form, with dS[t] = scale q[t] dout[t]^T + exp(g) dS[t+1]:
+ *
+ *   dq[t] = scale dout[t] S[t]^T   (dout, v, k), dk[t] = v[t] dS[t]^T   (v, dout, q) backward, dv[t] = k[t] dS[t]   (k, q, dout) backward
+ *
+ * so the kernel is written for (a, b, c) -> out with a state of b by c, forward or backward in time (a backward walk
+ * numbers the tokens from the last one on). A state that a backward walk is given is that of its first token already: there
+ * the exponents of what comes from outside the chunk are one less, and those of what goes on one more.
+ *
+ * Products run on v_mfma_f32_32x32x16_bf16 with float32 accumulators. A wavefront owns 32 columns of the state (channels
+ * of c) as accumulators: what one matrix instruction leaves in a lane is, rounded, the operand of the next one, so the
+ * state never leaves the registers. Two quads of channels change places in the transposing LDS reads for that: lane m of a
+ * transposed operand holds channel m with bits 2 and 3 swapped, so the rows that a lane holds of a result are eight
+ * adjacent channels (the contracted ones of the next product, read from LDS as 16 bytes, and 16 bytes of a row of `out`).
+ * The wavefronts share the masked products of a chunk (a . b) through LDS, in the form of the operand that they become.
+ *
+ * Rounding: bfloat16 operands are exact; products a . b and the state are rounded to bfloat16 (2^-9 of each term) where they
+ * are contracted again. What is added to the state, exp(g ..) c, goes as two bfloat16 parts (2^-17), since the state is a
+ * result in float32 and lives long. float16 operands, and everything contracted with them, go as two bfloat16 parts
+ * throughout: three products for one, no range but that of float32, and 2^-16 of each term.
+ */
+#pragma once
+
+namespace akg {
+namespace linear {
+
+using attn::BF16;
+using attn::chunk_at;
+using attn::f32x16;
+using attn::f32x4;
+using attn::kLog2e;
+using attn::padded;
+using attn::pitch;
+using attn::records;
+using attn::u32x2;
+using attn::u32x4;
+
+// Channel of a 32-channel unit that lane `m` (mod 32) of a transposed operand holds.
+constexpr int swapped(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1); }
+
+// exp(g n) from g log2 e: 1 for n = 0 (also where g is -inf).
+AKG_DEV float power(float g2, int n) { return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(g2 * static_cast<float>(n)); }
+// exp(g n) - 1, with the digits that are left of it near 0: a state that is faded by s + s (exp(g n) - 1) is off by half a
+// step of float32 a chunk, in either direction; with the rounded factor it would be off by the same share every time.
+AKG_DEV float power_less_one(float g, int n) {
+  const float x = g * static_cast<float>(n);
+  if (n == 0) return 0.0f;
+  if (!(__builtin_fabsf(x) < 0.125f)) return __builtin_amdgcn_exp2f(x * kLog2e) - 1.0f;
+  float p = __builtin_fmaf(x, 1.0f / 720.0f, 1.0f / 120.0f);   // x^7 / 7! is below 2^-33 x there
+  p = __builtin_fmaf(x, p, 1.0f / 24.0f);
+  p = __builtin_fmaf(x, p, 1.0f / 6.0f);
+  p = __builtin_fmaf(x, p, 0.5f);
+  return __builtin_fmaf(x * x, p, x);
+}
+
+// Eight float32 values as PARTS operands of bfloat16 whose sum they are, to 2^-9 or 2^-17.
+template <int PARTS>
+AKG_DEV void split(const float (&x)[8], u32x4 (&parts)[PARTS]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const u32 w = BF16::pack(x[2 * e], x[2 * e + 1]);
+    parts[0][e] = w;
+    if constexpr (PARTS == 2) parts[1][e] = BF16::pack(x[2 * e] - BF16::low(w), x[2 * e + 1] - BF16::high(w));
+  }
+}
+
+// c += a b, both in parts (the product of the two rests is below every digit kept).
+template <int PA, int PB>
+AKG_DEV f32x16 product(const u32x4 (&a)[PA], const u32x4 (&b)[PB], f32x16 c) {
+  if constexpr (PB == 2) c = BF16::mma(a[0], b[1], c);
+  if constexpr (PA == 2) c = BF16::mma(a[1], b[0], c);
+  return BF16::mma(a[0], b[0], c);
+}
+
+// A lane's places in a tile of W channels (as attn::Reader, with the quads of transposed reads swapped).
+template <int W>
+struct Places {
+  int along[2], across[2];
+  AKG_DEV explicit Places(int lane) {
+    const int row = lane & 31, h = lane >> 5;
+    along[0] = chunk_at<W>(row, h);
+    along[1] = chunk_at<W>(row, 2 + h);
+    const int i = lane & 15, r = 4 * h + (i >> 2), quad = ((i & 1) << 1) | ((i & 2) >> 1), chunk = 2 * ((lane >> 4) & 1) + (quad >> 1);
+    across[0] = chunk_at<W>(r, chunk) + (quad & 1) * 8;
+    across[1] = chunk_at<W>(r + 8, chunk) + (quad & 1) * 8;
+  }
+  // Channels 16 c + 8 (lane / 32) .. + 7 of row `row0 + lane % 32`.
+  AKG_DEV u32x4 row(const u8 *tile, int row0, int c) const {
+    return *reinterpret_cast<const u32x4 *>(tile + along[c & 1] + (row0 * pitch(W) + 64 * (c >> 1)));
+  }
+  // Channel 32 unit + swapped(lane % 32) of the rows row0 + 4 h .. 4 h + 3 and row0 + 8 + 4 h .. (h = lane / 32).
+  AKG_DEV u32x4 transposed(const u8 *tile, int row0, int unit) const {
+    const int more = row0 * pitch(W) + 64 * unit;
+    const attn::s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn::s16x4 *)(tile + across[0] + more));
+    const attn::s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn::s16x4 *)(tile + across[1] + more));
+    const u32x2 l = __builtin_bit_cast(u32x2, lo), u = __builtin_bit_cast(u32x2, hi);
+    return u32x4{l[0], l[1], u[0], u[1]};
+  }
+};
+
+// ROWS tokens of W channels on their way from memory to LDS. Tokens and channels that do not exist read zeros.
+template <int ROWS, int W, int THREADS, int PARTS>
+struct Stage {
+  static constexpr int kPerRow = W / 8, kChunks = ROWS * kPerRow, kEach = (kChunks + THREADS - 1) / THREADS;
+  static constexpr bool kWhole = kChunks % THREADS == 0;
+  static constexpr int kTileBytes = ROWS * pitch(W);
+  u32x4 held[kEach];
+  // Row i is `count - 1 - i` rows (BACK) or i rows behind `first`; `channels` of a row are read.
+  template <bool BACK>
+  AKG_DEV void load(const char *first, long step, int count, int channels, int tid) {
+    const Buffer buf = make_buffer(first, count > 0 ? records((count - 1) * step + 2L * channels) : 0);
+    const int from = BACK ? (count - 1) * static_cast<int>(step) : 0, each = BACK ? -static_cast<int>(step) : static_cast<int>(step);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int c = tid + i * THREADS, row = c / kPerRow, at = c % kPerRow * 8;
+      // (a row in front of `first` has an offset of almost 2^32: beyond the descriptor too)
+      const u32 off = static_cast<u32>(from + row * each + 2 * at);
+      held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, (kWhole || c < kChunks) && row < count && at < channels ? off : kBeyondEveryBuffer, 0, 0));
+    }
+  }
+  AKG_DEV void store(u8 *tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int c = tid + i * THREADS, row = c / kPerRow, chunk = c % kPerRow;
+      if (!kWhole && c >= kChunks) continue;
+      u8 *to = tile + chunk_at<W>(row, chunk);
+      if constexpr (PARTS == 1) {
+        *reinterpret_cast<u32x4 *>(to) = held[i];
+      } else {   // float16
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[2 * e] = attn::F16::low(held[i][e]);
+          x[2 * e + 1] = attn::F16::high(held[i][e]);
+        }
+        u32x4 parts[2];
+        split<2>(x, parts);
+        *reinterpret_cast<u32x4 *>(to) = parts[0];
+        *reinterpret_cast<u32x4 *>(to + kTileBytes) = parts[1];
+      }
+    }
+  }
+};
+
+// What the emitted kernel states about a walk: the operands' type in parts, channels of a and b (D) and of c and the result
+// (E), 32-token tiles of a chunk (CT), wavefronts (NW, 32 channels of c each), heads of the states (H) and of each operand,
+// whether it runs backward, whether states given and left are the transposed ones ([E][D] in memory).
+enum class Result { None, Storage, Float };
+template <typename T_, int D_, int E_, int CT_, int NW_, int H_, int HA_, int HB_, int HC_, bool HEADS_FIRST_, bool BACK_, bool TURNED_, Result RESULT_>
+struct Config {
+  typedef T_ T;   // attn::BF16 or attn::F16
+  static constexpr int PARTS = T::kNarrowRange ? 2 : 1, D = D_, E = E_, CT = CT_, NW = NW_, H = H_, HA = HA_, HB = HB_, HC = HC_;
+  static constexpr bool HEADS_FIRST = HEADS_FIRST_, BACK = BACK_, TURNED = TURNED_;
+  static constexpr Result RESULT = RESULT_;
+  static constexpr int kChunk = 32 * CT, kColumns = 32 * NW, kThreads = 64 * NW, kTiles = (E + kColumns - 1) / kColumns;
+};
+
+template <typename C>
+struct Lds {
+  static constexpr int kPairs = C::CT * (C::CT + 1) / 2;   // 32 x 32 tiles of the masked products
+  u8 a[C::PARTS][C::kChunk * pitch(C::D)], b[C::PARTS][C::kChunk * pitch(C::D)], c[C::PARTS][C::kChunk * pitch(C::kColumns)];
+  u32x4 pairs[C::PARTS][kPairs][2][64];
+};
+template <typename C>
+struct StateLds {
+  u8 b[C::PARTS][C::kChunk * pitch(C::D)], c[C::PARTS][C::kChunk * pitch(C::kColumns)];
+};
+
+// Where the tokens of one head of a tensor with X heads of W channels of 2 bytes lie.
+template <int X, int W, bool HEADS_FIRST, int H>
+struct Tokens {
+  const char *base;
+  long step;
+  AKG_DEV Tokens(const void *p, long b, int h, long seq, int size = 2) {
+    const long head = h / (H / X);
+    step = static_cast<long>(size) * W * (HEADS_FIRST ? 1 : X);
+    base = static_cast<const char *>(p) + static_cast<long>(size) * W * (HEADS_FIRST ? (b * X + head) * seq : b * seq * X + head);
+  }
+};
+
+// A walk's arguments. `starts`: states in front of every segment, [head][segment][D][E], written by the launches before (none
+// where there is one segment); a walk over states alone leaves there what its segment adds.
+struct Walk {
+  const void *a, *b, *c;
+  void *out;
+  const float *log_decay, *first;   // [H]; given state (or null)
+  float *last;                      // state behind the last token (or null)
+  const int *lengths, *slots;       // [batch] or null; slots: which entry of `first` and `last` a sequence has
+  float *starts;
+  long seq, pool;                   // entries of `first` and `last`
+  int segment, segments;            // tokens of a segment (a multiple of the chunk), their number
+  float scale;
+};
+
+AKG_DEV long length_of(const int *lengths, long b, long seq) {
+  if (lengths == nullptr) return seq;
+  const long n = lengths[b];
+  return n < 0 ? 0 : n < seq ? n : seq;
+}
+// Entry of sequence b in the pool of states, -1: none.
+AKG_DEV long entry_of(const int *slots, long b, long pool) {
+  if (slots == nullptr) return b;
+  const long n = slots[b];
+  return n >= 0 && n < pool ? n : -1;
+}
+
+// One segment of one head, 32 NW channels of c. STATES: only what the segment adds to a state.
+template <typename C, bool STATES>
+AKG_DEV void walk(const Walk &w, typename attn::conditional<STATES, StateLds<C>, Lds<C>>::type &lds, long head, int tile, int seg) {
+  constexpr int D = C::D, E = C::E, PARTS = C::PARTS, CT = C::CT, NW = C::NW, kChunk = C::kChunk, kThreads = C::kThreads;
+  constexpr int kUnits = padded(D) / 32, kSteps = 2 * CT;
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const long b = head / C::H;
+  const int h = static_cast<int>(head % C::H), e0 = tile * C::kColumns;
+  const long len = length_of(w.lengths, b, w.seq);
+  const long from = static_cast<long>(seg) * w.segment, upto = from + w.segment < w.seq ? from + w.segment : w.seq, end = upto < len ? upto : len;
+  const float g = w.log_decay[h], g2 = g * kLog2e;
+  const int column = e0 + 32 * wave + swapped(lane & 31);   // of the state, in this lane
+
+  const Tokens<C::HA, D, C::HEADS_FIRST, C::H> ta(w.a, b, h, w.seq);
+  const Tokens<C::HB, D, C::HEADS_FIRST, C::H> tb(w.b, b, h, w.seq);
+  const Tokens<C::HC, E, C::HEADS_FIRST, C::H> tc(w.c, b, h, w.seq);
+  Stage<kChunk, D, kThreads, PARTS> sa, sb;
+  Stage<kChunk, C::kColumns, kThreads, PARTS> sc;
+  auto count_at = [&](long r0) { return static_cast<int>(end - r0 < kChunk ? (end > r0 ? end - r0 : 0) : kChunk); };
+  auto fetch = [&](long r0) {
+    const int n = count_at(r0);
+    const long first = C::BACK ? len - r0 - n : r0;   // the lowest of the tokens
+    if constexpr (!STATES) sa.template load<C::BACK>(ta.base + first * ta.step, ta.step, n, D, tid);
+    sb.template load<C::BACK>(tb.base + first * tb.step, tb.step, n, D, tid);
+    sc.template load<C::BACK>(tc.base + first * tc.step + 2 * e0, tc.step, n, E - e0 < C::kColumns ? E - e0 : C::kColumns, tid);
+  };
+  fetch(from);
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    if constexpr (!STATES) attn::clear_padding<kChunk, D, kThreads>(lds.a[p], tid);
+    attn::clear_padding<kChunk, D, kThreads>(lds.b[p], tid);
+  }
+
+  // Row of unit u in register r: channel 32 u + 16 (r / 8) + 8 half + r % 8.
+  f32x16 state[kUnits];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) state[u] = {};
+  const long entry = entry_of(w.slots, b, w.pool);
+  float *starts = w.starts + (w.starts != nullptr ? (head * w.segments + seg) * (static_cast<long>(D) * E) : 0);
+  if constexpr (!STATES) {
+    const bool turned = C::TURNED && w.segments == 1;   // (starts in the workspace never are)
+    const float *given = w.segments > 1 ? starts : w.first != nullptr && entry >= 0 ? w.first + (entry * C::H + h) * (static_cast<long>(D) * E) : nullptr;
+    if (given != nullptr && column < E) {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = 32 * u + 16 * (r >> 3) + 8 * half + (r & 7);
+          if (D % 32 == 0 || d < D) state[u][r] = given[turned ? static_cast<long>(column) * D + d : static_cast<long>(d) * E + column];
+        }
+      }
+    }
+  }
+
+  // Weights: of the masked products (register r: key token 8 (r / 4) + 4 half + r % 4 of its 32, query token lane % 32), of
+  // the rows of a . S, and of what a token adds to the state.
+  constexpr int kAfter = C::BACK ? 1 : 0;
+  const float grow = C::BACK ? w.scale : 1.0f, show = C::BACK ? 1.0f : w.scale;
+  // pairs of tiles (query tile, key tile): 0 = (0, 0), 1 = (1, 0), 2 = (1, 1)
+  constexpr bool kAlone = NW == 1 && CT == 2;   // (one wavefront has them all)
+  float mask[kAlone ? 2 : 1][16], shown[CT];
+  float added[kSteps][8];
+  if constexpr (!STATES) {
+#pragma unroll
+    for (int k = 0; k < (kAlone ? 2 : 1); ++k) {
+      const int apart = kAlone ? 32 * k : CT == 2 && wave == 1 ? 32 : 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int n = apart + (lane & 31) - (8 * (r >> 2) + 4 * half + (r & 3));
+        mask[k][r] = n < 0 ? 0.0f : power(g2, n) * w.scale;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < CT; ++i) shown[i] = power(g2, 32 * i + (lane & 31) + 1 - kAfter) * show;
+  }
+  float fade;
+  auto weigh = [&](int n) {
+    fade = power_less_one(g, n);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int left = n - 1 - (16 * s + 8 * (e >> 2) + 4 * half + (e & 3));
+        added[s][e] = left < 0 ? 0.0f : power(g2, left + kAfter) * grow;
+      }
+    }
+  };
+  weigh(kChunk);
+
+  const Places<D> pd(lane);
+  const Places<C::kColumns> pc(lane);
+  for (long r0 = from; r0 < end; r0 += kChunk) {
+    const int n = count_at(r0);
+    if constexpr (!STATES) sa.store(lds.a[0], tid);
+    sb.store(lds.b[0], tid);
+    sc.store(lds.c[0], tid);
+    __syncthreads();
+    if (r0 + kChunk < end) fetch(r0 + kChunk);
+    if (n != kChunk) weigh(n);
+
+    f32x16 out[CT];
+    if constexpr (!STATES) {
+      // this wavefront's share of the masked products, in the form of an operand whose columns are the query tokens
+      auto pair = [&](int which, const float (&weights)[16]) {
+        const int qt = which > 0 ? 1 : 0, kt = which > 1 ? 1 : 0;
+        f32x16 s = {};
+#pragma unroll
+        for (int x = 0; x < 2 * kUnits; ++x) {
+          u32x4 keys[PARTS], queries[PARTS];
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) {
+            keys[p] = pd.row(lds.b[p], 32 * kt, x);
+            queries[p] = pd.row(lds.a[p], 32 * qt, x);
+          }
+          s = product(keys, queries, s);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float v[8];
+          const bool outside = which != 1;   // (on the diagonal: where the weight is 0 the product does not count, whatever it is)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = outside && weights[8 * x + e] == 0.0f ? 0.0f : s[8 * x + e] * weights[8 * x + e];
+          u32x4 parts[PARTS];
+          split<PARTS>(v, parts);
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) lds.pairs[p][which][x][lane] = parts[p];
+        }
+      };
+      if constexpr (CT == 1) {
+        if (wave == 0) pair(0, mask[0]);
+      } else if constexpr (kAlone) {
+        pair(0, mask[0]);
+        pair(1, mask[1]);
+        pair(2, mask[0]);
+      } else {
+        if (wave == 0) pair(0, mask[0]);
+        if (wave == 1) pair(1, mask[0]);
+        if (wave == (NW > 2 ? 2 : 0)) pair(2, mask[0]);
+      }
+      // a . S
+#pragma unroll
+      for (int i = 0; i < CT; ++i) out[i] = {};
+#pragma unroll
+      for (int x = 0; x < 2 * kUnits; ++x) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = state[x >> 1][8 * (x & 1) + e];
+        u32x4 s[PARTS];
+        split<PARTS>(v, s);
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+          u32x4 queries[PARTS];
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) queries[p] = pd.row(lds.a[p], 32 * i, x);
+          out[i] = product(s, queries, out[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) out[i][r] *= shown[i];
+      }
+      __syncthreads();
+    }
+    // the masked products with c, and what c adds to the state
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) state[u][r] = __builtin_fmaf(state[u][r], fade, state[u][r]);
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      u32x4 values[PARTS];
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) values[p] = pc.transposed(lds.c[p], 16 * s, wave);
+      if constexpr (!STATES) {
+#pragma unroll
+        for (int i = s / 2; i < CT; ++i) {
+          const int which = i == 0 ? 0 : 1 + s / 2;
+          u32x4 pairs[PARTS];
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) pairs[p] = lds.pairs[p][which][s & 1][lane];
+          out[i] = product(values, pairs, out[i]);
+        }
+      }
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[2 * e] = BF16::low(values[0][e]);
+        v[2 * e + 1] = BF16::high(values[0][e]);
+        if constexpr (PARTS == 2) {
+          v[2 * e] += BF16::low(values[1][e]);
+          v[2 * e + 1] += BF16::high(values[1][e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= added[s][e];
+      u32x4 more[2];
+      split<2>(v, more);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        u32x4 keys[PARTS];
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) keys[p] = pd.transposed(lds.b[p], 16 * s, u);
+        state[u] = product(keys, more, state[u]);
+      }
+    }
+    if constexpr (!STATES && C::RESULT != Result::None) {
+      constexpr bool kFloat = C::RESULT == Result::Float;
+      constexpr int kSize = kFloat ? 4 : 2;
+      // (a result in float32 is one of the walk's own heads, heads first)
+      const Tokens<C::H, E, kFloat || C::HEADS_FIRST, C::H> to(w.out, b, h, w.seq, kSize);
+      const long lowest = C::BACK ? len - r0 - n : r0;
+      const Buffer buf = make_buffer(to.base + lowest * to.step, records((n - 1) * to.step + static_cast<long>(kSize) * E));
+#pragma unroll
+      for (int i = 0; i < CT; ++i) {
+        const int row = 32 * i + (lane & 31);
+        const int at = (C::BACK ? n - 1 - row : row) * static_cast<int>(to.step);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int d = e0 + 32 * wave + 16 * x + 8 * half;
+          const u32 off = row < n && d < E ? static_cast<u32>(at + kSize * d) : kBeyondEveryBuffer;
+          if constexpr (kFloat) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              f32x4 v;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = out[i][8 * x + 4 * y + e];
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), buf, off + (off == kBeyondEveryBuffer ? 0u : 16u * y), 0, 0);
+            }
+          } else {
+            u32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = C::T::pack(out[i][8 * x + 2 * e], out[i][8 * x + 2 * e + 1]);
+            __builtin_amdgcn_raw_buffer_store_b128(v, buf, off, 0, 0);
+          }
+        }
+      }
+    }
+    __syncthreads();   // (the tiles have been read)
+  }
+
+  if constexpr (STATES) {
+    if (column < E) {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = 32 * u + 16 * (r >> 3) + 8 * half + (r & 7);
+          if (D % 32 == 0 || d < D) starts[static_cast<long>(d) * E + column] = state[u][r];
+        }
+      }
+    }
+  } else {
+    if constexpr (C::RESULT != Result::None) {   // rows behind the length: zeros
+      constexpr bool kFloat = C::RESULT == Result::Float;
+      constexpr int kSize = kFloat ? 4 : 2, kPieces = C::kColumns * kSize / 16;
+      const Tokens<C::H, E, kFloat || C::HEADS_FIRST, C::H> to(w.out, b, h, w.seq, kSize);
+      const long none = from > len ? from : len;
+      for (long x = tid; x < (upto - none) * kPieces; x += kThreads) {
+        const int d = e0 + static_cast<int>(x % kPieces) * (16 / kSize);
+        if (d < E) *reinterpret_cast<u32x4 *>(const_cast<char *>(to.base) + (none + x / kPieces) * to.step + kSize * d) = u32x4{0, 0, 0, 0};
+      }
+    }
+    // the segment that holds the last token has the last state
+    const bool ends = seg == (len > 0 ? static_cast<int>((len - 1) / w.segment) : 0);
+    if (w.last != nullptr && ends && entry >= 0 && column < E) {
+      float *to = w.last + (entry * C::H + h) * (static_cast<long>(D) * E);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = 32 * u + 16 * (r >> 3) + 8 * half + (r & 7);
+          if (D % 32 == 0 || d < D) to[C::TURNED ? static_cast<long>(column) * D + d : static_cast<long>(d) * E + column] = state[u][r];
+        }
+      }
+    }
+  }
+}
+
+// The states in front of every segment from what the segments add: start[s + 1] = exp(g tokens of s) start[s] + added[s].
+// A thread has four adjacent values of one head.
+template <typename C>
+AKG_DEV void scan(const Walk &w, long heads, long at) {
+  constexpr int D = C::D, E = C::E, kEach = D * E / 4;
+  const long head = at / kEach;
+  if (head >= heads) return;
+  const int x = static_cast<int>(at % kEach) * 4, h = static_cast<int>(head % C::H);
+  const long b = head / C::H, len = length_of(w.lengths, b, w.seq), entry = entry_of(w.slots, b, w.pool);
+  const float g2 = w.log_decay[h] * kLog2e;
+  f32x4 start = {};
+  if (w.first != nullptr && entry >= 0) {
+    const float *given = w.first + (entry * C::H + h) * (static_cast<long>(D) * E);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) start[e] = given[C::TURNED ? (x % E + e) * D + x / E : x + e];   // (E is a multiple of 4)
+  }
+  float *to = w.starts + head * w.segments * (static_cast<long>(D) * E) + x;
+  for (int s = 0; s < w.segments; ++s, to += D * E) {
+    const long left = len - static_cast<long>(s) * w.segment;
+    const int n = left <= 0 ? 0 : left < w.segment ? static_cast<int>(left) : w.segment;
+    f32x4 add = {};
+    if (s + 1 < w.segments) __builtin_memcpy(&add, to, 16);
+    __builtin_memcpy(to, &start, 16);
+    const float fade = power(g2, n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) start[e] = __builtin_fmaf(start[e], fade, add[e]);
+  }
+}
+
+// Gradients of heads that share keys and values: the sum over those heads, in their order. `part`: [batch][H][seq][W] in
+// float32; a thread has four channels of one token of one key head.
+template <typename T, int W, int H, int HKV, bool HEADS_FIRST>
+AKG_DEV void share(const float *part, void *out, long batch, long seq, long at) {
+  constexpr int G = H / HKV;
+  const long d = at % (W / 4) * 4, token = at / (W / 4) % seq, head = at / (W / 4) / seq;
+  if (head >= batch * HKV) return;
+  const float *from = part + (head * G * seq + token) * W + d;
+  f32x4 sum = {};
+#pragma unroll
+  for (int k = 0; k < G; ++k) sum += *reinterpret_cast<const f32x4 *>(from + k * seq * W);
+  const long b = head / HKV, hkv = head % HKV;
+  const u32x2 v = {T::pack(sum[0], sum[1]), T::pack(sum[2], sum[3])};
+  *reinterpret_cast<u32x2 *>(static_cast<u16 *>(out) + (HEADS_FIRST ? (head * seq + token) * W : ((b * seq + token) * HKV + hkv) * W) + d) = v;
+}
+
+// ---- few tokens: the recurrence itself ----------------------------------------------------------------------------------
+// A workgroup has TE channels of v of one head (TE / 4 lanes side by side) and all D channels of k, a thread D / (1024 / TE)
+// adjacent ones of those; the state stays in registers over the tokens. Bound by the state, read and written once.
+template <typename T, int D, int E, int TE, int H, int HKV, bool HEADS_FIRST, int MOST>
+AKG_DEV void tokens(const Walk &w, long head, int tile) {
+  constexpr int kLanes = TE / 4, kGroups = 256 / kLanes, kRows = (D + kGroups - 1) / kGroups, kPerWave = 64 / kLanes;
+  typedef typename T::dtype::storage S;
+  __shared__ float qs[MOST][kGroups * kRows], ks[MOST][kGroups * kRows];
+  __shared__ f32x4 parts[MOST][4][kLanes];
+  const int tid = static_cast<int>(threadIdx.x), e = tile * TE + tid % kLanes * 4, row0 = tid / kLanes * kRows;
+  const long b = head / H;
+  const int h = static_cast<int>(head % H);
+  const int seq = static_cast<int>(w.seq), len = static_cast<int>(length_of(w.lengths, b, w.seq));
+  const long entry = entry_of(w.slots, b, w.pool);
+  const bool live = e < E;
+  f32x4 state[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) state[r] = {};
+  const long at = (entry * H + h) * (static_cast<long>(D) * E) + e;
+  if (w.first != nullptr && entry >= 0 && live) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (D % kGroups == 0 || row0 + r < D) __builtin_memcpy(&state[r], w.first + at + static_cast<long>(row0 + r) * E, 16);
+    }
+  }
+  const Tokens<H, D, HEADS_FIRST, H> tq(w.a, b, h, w.seq);
+  const Tokens<HKV, D, HEADS_FIRST, H> tk(w.b, b, h, w.seq);
+  const Tokens<HKV, E, HEADS_FIRST, H> tv(w.c, b, h, w.seq);
+  for (int x = tid; x < len * kGroups * kRows; x += 256) {
+    const int t = x / (kGroups * kRows), d = x % (kGroups * kRows);
+    qs[t][d] = d < D ? T::dtype::load(reinterpret_cast<const S *>(tq.base + t * tq.step)[d]) * w.scale : 0.0f;
+    ks[t][d] = d < D ? T::dtype::load(reinterpret_cast<const S *>(tk.base + t * tk.step)[d]) : 0.0f;
+  }
+  const float fade = power(w.log_decay[h] * kLog2e, 1);
+  __syncthreads();
+  for (int t = 0; t < len; ++t) {
+    f32x4 v = {}, out = {};
+    if (live) {
+      S raw[4];
+      __builtin_memcpy(raw, tv.base + t * tv.step + 2 * e, 8);
+#pragma unroll
+      for (int z = 0; z < 4; ++z) v[z] = T::dtype::load(raw[z]);
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float k = ks[t][row0 + r], q = qs[t][row0 + r];
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        state[r][z] = __builtin_fmaf(state[r][z], fade, k * v[z]);
+        out[z] = __builtin_fmaf(state[r][z], q, out[z]);
+      }
+    }
+#pragma unroll
+    for (int step = kLanes; step < 64; step *= 2) {
+#pragma unroll
+      for (int z = 0; z < 4; ++z) out[z] += __shfl_xor(out[z], step);
+    }
+    if ((tid & 63) < kLanes) parts[t][tid >> 6][tid & 63] = out;
+  }
+  if (w.last != nullptr && entry >= 0 && live) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (D % kGroups == 0 || row0 + r < D) __builtin_memcpy(w.last + at + static_cast<long>(row0 + r) * E, &state[r], 16);
+    }
+  }
+  if (w.out == nullptr) return;
+  __syncthreads();
+  const Tokens<H, E, HEADS_FIRST, H> to(w.out, b, h, w.seq);
+  for (int x = tid; x < seq * kLanes; x += 256) {
+    const int t = x / kLanes, lane = x % kLanes, d = tile * TE + lane * 4;
+    f32x4 sum = {};
+    if (t < len) sum = (parts[t][0][lane] + parts[t][1][lane]) + (parts[t][2][lane] + parts[t][3][lane]);
+    const u32x2 v = {T::pack(sum[0], sum[1]), T::pack(sum[2], sum[3])};
+    if (d < E) __builtin_memcpy(const_cast<char *>(to.base) + t * to.step + 2 * d, &v, 8);
+  }
+}
+
+}  // namespace linear
+}  // namespace akg

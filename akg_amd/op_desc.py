@@ -573,7 +573,7 @@ def attention_probabilities(batch, m, k, n, dtype="bfloat16", name=None):
 
 def _layer(b, name, inputs, outs, attrs):
     """One op entry with several results: `outs` is a list of (shape, dtype), `attrs` of (name, value)."""
-    kinds = {bool: "bool", float: "float", int: "int", str: "str"}
+    kinds = {bool: "bool", float: "float", int: "int", str: "str", list: "listInt"}
     results = []
     for shape, dtype in outs:
         results.append(Tensor("output_0_%d" % b._n_out, shape, dtype))
@@ -586,19 +586,27 @@ def _layer(b, name, inputs, outs, attrs):
 
 
 def rotary_embedding(b, xs, positions, layout="BSND", base=10000.0, rotary_dims=0, interleaved=False, inverse=False, scaling=None,
-                     magnitude=1.0):
+                     magnitude=1.0, sections=None, axis_order="blocks", axis_rates="shared"):
     """Rotary positions of one or two tensors of heads ([batch, sequence, heads, channels], or "BNSD"; they may differ in
     their heads only), `positions` int32 / int64 [sequence] or [batch, sequence]. The first `rotary_dims` channels (0: all)
     are turned in pairs - channel i with i + rotary_dims / 2, or adjacent ones where `interleaved` - by position *
     base^(-2 i / rotary_dims); `inverse` turns back (the gradient). `scaling`: None, {"kind": "linear", "factor"} or {"kind":
     "wavelength", "factor", "original_length", "low", "high"} (rates that turn fewer than `low` times over the original
     length are divided by the factor, those that turn more than `high` times are not, the ones between in part). `magnitude`
-    multiplies the result of the turned channels. Returns one result per tensor."""
+    multiplies the result of the turned channels.
+
+    Tokens with several positions (time, height and width of a video's): `sections` holds the number of pairs of every axis, in
+    all rotary_dims / 2, and `positions` is [axes, sequence] or [axes, batch, sequence]. `axis_order`: "blocks" (the first
+    sections[0] pairs turn by the first axis, and so on) or "cycle" (pairs are dealt to the axes in turn, an axis that has all
+    of its own left out). `axis_rates`: "shared" (the rate of pair i whatever its axis) or "own" (the j-th of n pairs of an
+    axis has the rate of pair j of a head with 2 n channels). Returns one result per tensor."""
     attrs = [("layout", layout), ("base", float(base)), ("rotary_dims", int(rotary_dims)), ("interleaved", bool(interleaved)),
              ("inverse", bool(inverse)), ("magnitude", float(magnitude)), ("scaling", scaling["kind"] if scaling else "none")]
     for key in ("factor", "original_length", "low", "high"):
         if scaling and key in scaling:
             attrs.append((key, float(scaling[key])))
+    if sections is not None:
+        attrs += [("sections", [int(n) for n in sections]), ("axis_order", axis_order), ("axis_rates", axis_rates)]
     return _layer(b, "RotaryEmbedding", list(xs) + [positions], [(x.shape, x.dtype) for x in xs], attrs)
 
 
@@ -636,6 +644,39 @@ def cache_attention(b, q, key_cache, value_cache, key_scale, value_scale, block_
     the first length - queries + 1 + i). Entries of the table outside the pool hold no tokens. Returns the result."""
     attrs = [] if scale is None else [("scale", float(scale))]
     return _layer(b, "CacheAttention", [q, key_cache, value_cache, key_scale, value_scale, block_table, lengths], [(q.shape, q.dtype)], attrs)[0]
+
+
+def _linear_attrs(layout, scale, optional):
+    attrs = [("layout", layout)] + [("has_" + n, t is not None) for n, t in optional]
+    if scale is not None:
+        attrs.append(("scale", float(scale)))
+    return attrs, [t for _, t in optional if t is not None]
+
+
+def linear_attention(b, q, k, v, log_decay, state=None, slots=None, lengths=None, layout="BSND", scale=None, last_state=False):
+    """Attention without a softmax, whose past is a state: state[t] = exp(log_decay) state[t-1] + k[t] v[t]^T, out[t] = scale
+    q[t] state[t] (scale: 1 / sqrt(channels) where none is given). Heads of q may share those of k and v; every head of q has
+    a decay of its own, `log_decay` float32 [heads] (at most 0; -inf forgets everything), and so a state of its own, float32
+    [batch, heads, channels of k, channels of v]. `state`: the one in front of the first token (none: zeros). `slots` int32
+    [batch]: `state` and the last state are pools [slots, heads, ..], of which a sequence has the entry named (all different;
+    one outside the pool: starts from zeros, and leaves none). The last state may be written over the state given. `lengths`
+    int32 [batch]: tokens of a sequence; the rows behind them are zeros. Returns [out] or [out, last state]. A few tokens (a
+    decoding step, drafted tokens) run as the recurrence, more in chunks."""
+    attrs, more = _linear_attrs(layout, scale, [("state", state), ("slots", slots), ("lengths", lengths)])
+    heads = q.shape[1] if layout == "BNSD" else q.shape[2]
+    outs = [(q.shape[:3] + v.shape[3:], q.dtype)]
+    if last_state:
+        outs.append((state.shape if state is not None else [q.shape[0], heads, q.shape[3], v.shape[3]], "float32"))
+    return _layer(b, "LinearAttention", [q, k, v, log_decay] + more, outs, attrs)
+
+
+def linear_attention_grad(b, dout, q, k, v, log_decay, state=None, dstate=None, lengths=None, layout="BSND", scale=None):
+    """Gradients [dq, dk, dv] of `linear_attention` from that of its first result and, where the last state was used too, of the
+    last state (`dstate`); with `state`, the one that the forward pass was given, its gradient is a fourth result. The
+    states in between are computed again. The decays get none."""
+    attrs, more = _linear_attrs(layout, scale, [("state", state), ("state_gradient", dstate), ("lengths", lengths)])
+    outs = [(t.shape, t.dtype) for t in (q, k, v)] + ([(state.shape, "float32")] if state is not None else [])
+    return _layer(b, "LinearAttentionGrad", [dout, q, k, v, log_decay] + more, outs, attrs)
 
 
 def sgd_clip_by_global_norm(rows, cols, dtype="float32", lr=0.01, clip=1.0, name=None):
