@@ -575,9 +575,9 @@ class LayerEmitter {
     if (s.seq >= (1LL << 31) - 8192) throw LoweringError("op " + op_.name + ": more than 2^31 tokens");
     return s;
   }
-  std::string walkConfig(const WalkOf &w, const LinearSizes &s, int ct, int64_t nw) const {
+  std::string walkConfig(const WalkOf &w, const LinearSizes &s, int ct, int64_t nw, int sets) const {
     std::ostringstream o;
-    o << "akg::linear::Config<" << trait() << ", " << w.d << ", " << w.e << ", " << ct << ", " << nw << ", " << s.heads << ", " << w.ha << ", " << w.hb << ", " << w.hc
+    o << "akg::linear::Config<" << trait() << ", " << w.d << ", " << w.e << ", " << ct << ", " << nw << ", " << sets << ", " << s.heads << ", " << w.ha << ", " << w.hb << ", " << w.hc
       << ", " << flag(l_.headsFirst) << ", " << flag(w.back) << ", " << flag(w.turned) << ", akg::linear::Result::" << w.result << ">";
     return o.str();
   }
@@ -586,29 +586,38 @@ class LayerEmitter {
   // workspace in front of theirs. The workspace's bytes are returned.
   int64_t walks(std::ostringstream &o, std::vector<KernelPhase> &phases, std::vector<WalkOf> &all, const LinearSizes &s, const std::string &args, const std::string &decay,
                 const std::string &lengths, const std::string &slots, int64_t space, bool more) {
-    int64_t widest = 0, deepest = 0;
+    int64_t widest = 0, deepestD = 0;
     for (const WalkOf &w : all) {
       widest = std::max(widest, w.e);
-      deepest = std::max(deepest, std::max(w.d, w.e));
+      deepestD = std::max(deepestD, w.d);
     }
     const bool pairsOfParts = in(0).dtype == DType::F16;
-    const int ct = pairsOfParts ? 1 : 2;
-    const int64_t units = ceilDiv(widest, 32), nw = std::max<int64_t>(2, ceilDiv(units, ceilDiv(units, 4)));
+    int ct = pairsOfParts ? 1 : 2;
+    const int64_t units = ceilDiv(widest, 32);
+    int64_t nw = std::max<int64_t>(2, ceilDiv(units, ceilDiv(units, 4)));
+    // Two sets of tiles where LDS holds them (attn::pitch), chunks of 32 tokens before one set.
+    const int64_t parts = pairsOfParts ? 2 : 1;
+    auto pitchOf = [](int64_t d) { return ceilDiv(d, 32) % 2 == 1 ? ceilDiv(d, 32) * 64 : ceilDiv(d, 32) * 64 + 64; };
+    auto setBytes = [&](int tiles) { return parts * 32 * tiles * (2 * pitchOf(deepestD) + pitchOf(32 * nw)); };
+    int sets = 2;
+    const int64_t room = 160 * 1024 - parts * 6144;
+    if (2 * setBytes(ct) > room) ct = 1;
+    if (2 * setBytes(ct) > room) sets = 1;
     int64_t groups = 0, values = 0;
     for (WalkOf &w : all) {
       w.tiles = ceilDiv(w.e, 32 * nw);
       groups += s.states * w.tiles;
       values += w.d * w.e;
     }
-    int64_t segments = std::max<int64_t>(1, std::min<int64_t>(2 * cus_ / groups, s.seq / 256));
+    int64_t segments = std::max<int64_t>(1, std::min<int64_t>(cus_ / groups, s.seq / 256));
     while (limit_ > 0 && segments > 1 && space + 4 * s.states * segments * values > limit_) --segments;
     const int64_t chunk = 32 * ct, segment = ceilDiv(ceilDiv(s.seq, segments), chunk) * chunk;
     segments = ceilDiv(s.seq, segment);
     k_.scalarArgs = {s.batch, s.seq, segment, segments};
     if (l_.hasSlots) k_.scalarArgs.push_back(in(4).shape[0]);
     std::vector<std::string> names;
-    o << "typedef " << walkConfig(all[0], s, ct, nw) << " akg_C0;\n";
-    for (size_t i = 1; i < all.size(); ++i) o << "typedef " << walkConfig(all[i], s, ct, nw) << " akg_C" << i << ";\n";
+    o << "typedef " << walkConfig(all[0], s, ct, nw, sets) << " akg_C0;\n";
+    for (size_t i = 1; i < all.size(); ++i) o << "typedef " << walkConfig(all[i], s, ct, nw, sets) << " akg_C" << i << ";\n";
     o << "\n";
     int64_t before = space;
     std::vector<std::string> structs;
@@ -621,16 +630,16 @@ class LayerEmitter {
       structs.push_back(b.str());
       before += 4 * s.heads * w.d * w.e;
     }
-    const int threads = static_cast<int>(64 * nw);
-    const int hint = deepest <= 128 ? 2 : 0;
+    const int threads = static_cast<int>(128 * nw);
+    int hint = 2;
     // every walk has the workgroups from `from` on; a head's are on one XCD (attn::head_and_tile)
     auto body = [&](bool states) {
       std::ostringstream b;
-      const char *kind = states ? "StateLds" : "Lds";
       b << "  __shared__ __attribute__((aligned(16))) akg::u8 akg_lds[";
-      std::string size = std::string("sizeof(akg::linear::") + kind + "<akg_C0>)";
+      auto lds = [&](size_t i) { return "akg::linear::Lds<akg_C" + std::to_string(i) + ", " + flag(states) + ">"; };
+      std::string size = "sizeof(" + lds(0) + ")";
       for (size_t i = 1; i < all.size(); ++i) {
-        const std::string other = std::string("sizeof(akg::linear::") + kind + "<akg_C" + std::to_string(i) + ">)";
+        const std::string other = "sizeof(" + lds(i) + ")";
         size = "(" + size + " > " + other + " ? " + size + " : " + other + ")";
       }
       b << size << "];\n  long akg_id = blockIdx.x, akg_head, akg_rest;\n  const long akg_heads = akg_batch * " << s.heads << ", akg_parts = " << (states ? "akg_segments - 1" : "akg_segments") << ";\n";
@@ -638,8 +647,7 @@ class LayerEmitter {
         const std::string n = std::to_string(i);
         b << "  if (akg_id < akg_heads * akg_parts * akg_C" << n << "::kTiles) {\n    const akg::linear::Walk akg_w = " << structs[i] << ";\n"
           << "    akg::attn::head_and_tile(akg_id, akg_heads, akg_head, akg_rest);\n"
-          << "    akg::linear::walk<akg_C" << n << ", " << flag(states) << ">(akg_w, *reinterpret_cast<akg::linear::" << kind << "<akg_C" << n
-          << "> *>(akg_lds), akg_head, static_cast<int>(akg_rest % akg_C" << n << "::kTiles), static_cast<int>(akg_rest / akg_C" << n << "::kTiles));\n    return;\n  }\n"
+          << "    akg::linear::walk<akg_C" << n << ", " << flag(states) << ">(akg_w, *reinterpret_cast<" << lds(i) << " *>(akg_lds), akg_head, static_cast<int>(akg_rest % akg_C" << n << "::kTiles), static_cast<int>(akg_rest / akg_C" << n << "::kTiles));\n    return;\n  }\n"
           << "  akg_id -= akg_heads * akg_parts * akg_C" << n << "::kTiles;\n";
       }
       return b.str();

@@ -63,15 +63,20 @@ AKG_DEV float power_less_one(float g, int n) {
   return __builtin_fmaf(x * x, p, x);
 }
 
-// Eight float32 values as PARTS operands of bfloat16 whose sum they are, to 2^-9 or 2^-17.
+// Float32 values as PARTS values of bfloat16 whose sum they are, to 2^-8 or 2^-16 of them: word `e` of an operand.
+template <int PARTS>
+AKG_DEV void split_pair(float lo, float hi, u32x4 (&parts)[PARTS], int e) {
+  u32 w = BF16::pack(lo, hi);
+  if constexpr (PARTS == 2) {
+    asm("" : "+v"(w));   // (one rounding, not another one for the rest)
+    parts[1][e] = BF16::pack(lo - BF16::low(w), hi - BF16::high(w));
+  }
+  parts[0][e] = w;
+}
 template <int PARTS>
 AKG_DEV void split(const float (&x)[8], u32x4 (&parts)[PARTS]) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const u32 w = BF16::pack(x[2 * e], x[2 * e + 1]);
-    parts[0][e] = w;
-    if constexpr (PARTS == 2) parts[1][e] = BF16::pack(x[2 * e] - BF16::low(w), x[2 * e + 1] - BF16::high(w));
-  }
+  for (int e = 0; e < 4; ++e) split_pair<PARTS>(x[2 * e], x[2 * e + 1], parts, e);
 }
 
 // c += a b, both in parts (the product of the two rests is below every digit kept).
@@ -113,27 +118,28 @@ template <int ROWS, int W, int THREADS, int PARTS>
 struct Stage {
   static constexpr int kPerRow = W / 8, kChunks = ROWS * kPerRow, kEach = (kChunks + THREADS - 1) / THREADS;
   static constexpr bool kWhole = kChunks % THREADS == 0;
+  // (the rows of a thread then lie a constant number of rows apart, at the same place of their swizzle)
+  static constexpr bool kEven = kWhole && THREADS % kPerRow == 0 && THREADS / kPerRow % 16 == 0;
   static constexpr int kTileBytes = ROWS * pitch(W);
   u32x4 held[kEach];
-  // Row i is `count - 1 - i` rows (BACK) or i rows behind `first`; `channels` of a row are read.
+  // The last `count` rows, of which row ROWS - 1 - i is i (BACK) or count - 1 - i rows behind `first`; `channels` of a row are read.
   template <bool BACK>
   AKG_DEV void load(const char *first, long step, int count, int channels, int tid) {
     const Buffer buf = make_buffer(first, count > 0 ? records((count - 1) * step + 2L * channels) : 0);
-    const int from = BACK ? (count - 1) * static_cast<int>(step) : 0, each = BACK ? -static_cast<int>(step) : static_cast<int>(step);
+    const int each = BACK ? -static_cast<int>(step) : static_cast<int>(step), from = BACK ? (ROWS - 1) * static_cast<int>(step) : (count - ROWS) * static_cast<int>(step);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int c = tid + i * THREADS, row = c / kPerRow, at = c % kPerRow * 8;
-      // (a row in front of `first` has an offset of almost 2^32: beyond the descriptor too)
-      const u32 off = static_cast<u32>(from + row * each + 2 * at);
-      held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, (kWhole || c < kChunks) && row < count && at < channels ? off : kBeyondEveryBuffer, 0, 0));
+      const bool there = row >= ROWS - count && at < channels && (kWhole || c < kChunks);
+      held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, there ? static_cast<u32>(from + row * each + 2 * at) : kBeyondEveryBuffer, 0, 0));
     }
   }
   AKG_DEV void store(u8 *tile, int tid) const {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int c = tid + i * THREADS, row = c / kPerRow, chunk = c % kPerRow;
+      const int c = tid + i * THREADS;
       if (!kWhole && c >= kChunks) continue;
-      u8 *to = tile + chunk_at<W>(row, chunk);
+      u8 *to = tile + (kEven ? chunk_at<W>(tid / kPerRow, tid % kPerRow) + i * (THREADS / kPerRow) * pitch(W) : chunk_at<W>(c / kPerRow, c % kPerRow));
       if constexpr (PARTS == 1) {
         *reinterpret_cast<u32x4 *>(to) = held[i];
       } else {   // float16
@@ -153,27 +159,30 @@ struct Stage {
 };
 
 // What the emitted kernel states about a walk: the operands' type in parts, channels of a and b (D) and of c and the result
-// (E), 32-token tiles of a chunk (CT), wavefronts (NW, 32 channels of c each), heads of the states (H) and of each operand,
-// whether it runs backward, whether states given and left are the transposed ones ([E][D] in memory).
+// (E), 32-token tiles of a chunk (CT), pairs of wavefronts (NW, 32 channels of c each), sets of tiles in LDS (SETS), heads of the
+// states (H) and of each operand, whether it runs backward, whether states given and left are the transposed ones ([E][D] in
+// memory).
 enum class Result { None, Storage, Float };
-template <typename T_, int D_, int E_, int CT_, int NW_, int H_, int HA_, int HB_, int HC_, bool HEADS_FIRST_, bool BACK_, bool TURNED_, Result RESULT_>
+template <typename T_, int D_, int E_, int CT_, int NW_, int SETS_, int H_, int HA_, int HB_, int HC_, bool HEADS_FIRST_, bool BACK_, bool TURNED_, Result RESULT_>
 struct Config {
+  static_assert(NW_ >= 2, "two wavefronts at least share the masked products of a chunk");
   typedef T_ T;   // attn::BF16 or attn::F16
-  static constexpr int PARTS = T::kNarrowRange ? 2 : 1, D = D_, E = E_, CT = CT_, NW = NW_, H = H_, HA = HA_, HB = HB_, HC = HC_;
+  static constexpr int PARTS = T::kNarrowRange ? 2 : 1, D = D_, E = E_, CT = CT_, NW = NW_, SETS = SETS_, H = H_, HA = HA_, HB = HB_, HC = HC_;
   static constexpr bool HEADS_FIRST = HEADS_FIRST_, BACK = BACK_, TURNED = TURNED_;
   static constexpr Result RESULT = RESULT_;
-  static constexpr int kChunk = 32 * CT, kColumns = 32 * NW, kThreads = 64 * NW, kTiles = (E + kColumns - 1) / kColumns;
+  static constexpr int kChunk = 32 * CT, kColumns = 32 * NW, kTiles = (E + kColumns - 1) / kColumns;
 };
 
-template <typename C>
+// Tiles of a chunk, and its masked products as operands. STATES: what a walk over states alone needs.
+template <typename C, bool STATES>
+struct Set {
+  u8 b[C::PARTS][C::kChunk * pitch(C::D)], c[C::PARTS][C::kChunk * pitch(C::kColumns)], a[STATES ? 0 : C::PARTS][C::kChunk * pitch(C::D)];
+};
+template <typename C, bool STATES>
 struct Lds {
   static constexpr int kPairs = C::CT * (C::CT + 1) / 2;   // 32 x 32 tiles of the masked products
-  u8 a[C::PARTS][C::kChunk * pitch(C::D)], b[C::PARTS][C::kChunk * pitch(C::D)], c[C::PARTS][C::kChunk * pitch(C::kColumns)];
-  u32x4 pairs[C::PARTS][kPairs][2][64];
-};
-template <typename C>
-struct StateLds {
-  u8 b[C::PARTS][C::kChunk * pitch(C::D)], c[C::PARTS][C::kChunk * pitch(C::kColumns)];
+  Set<C, STATES> sets[C::SETS];
+  u32x4 pairs[STATES ? 0 : C::PARTS][kPairs][2][64];
 };
 
 // Where the tokens of one head of a tensor with X heads of W channels of 2 bytes lie.
@@ -215,39 +224,152 @@ AKG_DEV long entry_of(const int *slots, long b, long pool) {
 }
 
 // One segment of one head, 32 NW channels of c. STATES: only what the segment adds to a state.
+//
+// NW wavefronts hold the state and do what needs it. As many others fetch: two chunks ahead into registers, from there to LDS
+// (float16 in parts), and compute the masked products, the first of two steps of a chunk, beside a . S; in the second, beside the
+// products with c, they put the next chunk's tiles in place. (With both in the same wavefronts, one behind the other, a chunk
+// of 64 tokens of 128 channels took 3.3 us whatever was fetched ahead, since registers left no room to read operands ahead.)
 template <typename C, bool STATES>
-AKG_DEV void walk(const Walk &w, typename attn::conditional<STATES, StateLds<C>, Lds<C>>::type &lds, long head, int tile, int seg) {
-  constexpr int D = C::D, E = C::E, PARTS = C::PARTS, CT = C::CT, NW = C::NW, kChunk = C::kChunk, kThreads = C::kThreads;
-  constexpr int kUnits = padded(D) / 32, kSteps = 2 * CT;
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int seg) {
+  constexpr int D = C::D, E = C::E, PARTS = C::PARTS, CT = C::CT, NW = C::NW, SETS = C::SETS, kChunk = C::kChunk, kThreads = 64 * NW;
+  constexpr int kUnits = padded(D) / 32, kSteps = 2 * CT, kAfter = C::BACK ? 1 : 0;
+  const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const long b = head / C::H;
   const int h = static_cast<int>(head % C::H), e0 = tile * C::kColumns;
   const long len = length_of(w.lengths, b, w.seq);
   const long from = static_cast<long>(seg) * w.segment, upto = from + w.segment < w.seq ? from + w.segment : w.seq, end = upto < len ? upto : len;
   const float g = w.log_decay[h], g2 = g * kLog2e;
-  const int column = e0 + 32 * wave + swapped(lane & 31);   // of the state, in this lane
-
-  const Tokens<C::HA, D, C::HEADS_FIRST, C::H> ta(w.a, b, h, w.seq);
-  const Tokens<C::HB, D, C::HEADS_FIRST, C::H> tb(w.b, b, h, w.seq);
-  const Tokens<C::HC, E, C::HEADS_FIRST, C::H> tc(w.c, b, h, w.seq);
-  Stage<kChunk, D, kThreads, PARTS> sa, sb;
-  Stage<kChunk, C::kColumns, kThreads, PARTS> sc;
   auto count_at = [&](long r0) { return static_cast<int>(end - r0 < kChunk ? (end > r0 ? end - r0 : 0) : kChunk); };
-  auto fetch = [&](long r0) {
-    const int n = count_at(r0);
-    const long first = C::BACK ? len - r0 - n : r0;   // the lowest of the tokens
-    if constexpr (!STATES) sa.template load<C::BACK>(ta.base + first * ta.step, ta.step, n, D, tid);
-    sb.template load<C::BACK>(tb.base + first * tb.step, tb.step, n, D, tid);
-    sc.template load<C::BACK>(tc.base + first * tc.step + 2 * e0, tc.step, n, E - e0 < C::kColumns ? E - e0 : C::kColumns, tid);
-  };
-  fetch(from);
+  // the lowest of the tokens of a chunk, whose last rows they are
+  auto lowest_at = [&](long r0, int n) { return C::BACK ? len - r0 - n : r0; };
+  const Places<D> pd(lane);
+
+  if (wave >= NW) {
+    const int tid = static_cast<int>(threadIdx.x) - kThreads, helper = wave - NW;
+    const Tokens<C::HA, D, C::HEADS_FIRST, C::H> ta(w.a, b, h, w.seq);
+    const Tokens<C::HB, D, C::HEADS_FIRST, C::H> tb(w.b, b, h, w.seq);
+    const Tokens<C::HC, E, C::HEADS_FIRST, C::H> tc(w.c, b, h, w.seq);
+    Stage<kChunk, D, kThreads, PARTS> sa[2], sb[2];
+    Stage<kChunk, C::kColumns, kThreads, PARTS> sc[2];
+    auto fetch = [&](int to, long r0) {   // (behind the end: nothing is asked of memory)
+      const int n = count_at(r0);
+      const long first = lowest_at(r0, n);
+      if constexpr (!STATES) sa[to].template load<C::BACK>(ta.base + first * ta.step, ta.step, n, D, tid);
+      sb[to].template load<C::BACK>(tb.base + first * tb.step, tb.step, n, D, tid);
+      sc[to].template load<C::BACK>(tc.base + first * tc.step + 2 * e0, tc.step, n, E - e0 < C::kColumns ? E - e0 : C::kColumns, tid);
+    };
+    auto place = [&](int x) {
+      Set<C, STATES> &set = lds.sets[x % SETS];
+      if constexpr (!STATES) sa[x].store(set.a[0], tid);
+      sb[x].store(set.b[0], tid);
+      sc[x].store(set.c[0], tid);
+    };
+    // Weights of the masked products (register r: key token 8 (r / 4) + 4 half + r % 4 of its 32, query token lane % 32). Pairs
+    // of tiles (query tile, key tile): 0 = (0, 0), 1 = (1, 0), 2 = (1, 1).
+    float mask[16];
+    if constexpr (!STATES) {
+      const int apart = CT == 2 && helper == 1 ? 32 : 0;
 #pragma unroll
-  for (int p = 0; p < PARTS; ++p) {
-    if constexpr (!STATES) attn::clear_padding<kChunk, D, kThreads>(lds.a[p], tid);
-    attn::clear_padding<kChunk, D, kThreads>(lds.b[p], tid);
+      for (int r = 0; r < 16; ++r) {
+        const int n = apart + (lane & 31) - (8 * (r >> 2) + 4 * half + (r & 3));
+        mask[r] = n < 0 ? 0.0f : power(g2, n) * w.scale;
+      }
+    }
+    auto pair = [&](const Set<C, STATES> &set, int which) {
+      const int qt = which > 0 ? 1 : 0, kt = which > 1 ? 1 : 0;
+      f32x16 s = {};
+      constexpr int kAhead = 3;
+      u32x4 keys[2 * kUnits][PARTS], queries[2 * kUnits][PARTS];
+      auto read = [&](int x) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          keys[x][p] = pd.row(set.b[p], 32 * kt, x);
+          queries[x][p] = pd.row(set.a[p], 32 * qt, x);
+        }
+      };
+#pragma unroll
+      for (int x = 0; x < kAhead && x < 2 * kUnits; ++x) read(x);
+#pragma unroll
+      for (int x = 0; x < 2 * kUnits; ++x) {
+        __builtin_amdgcn_sched_barrier(0);
+        s = product(keys[x], queries[x], s);
+        if (x + kAhead < 2 * kUnits) read(x + kAhead);
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float v[8];
+        // (on the diagonal: where the weight is 0 the product does not count, whatever it is)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = which != 1 && mask[8 * x + e] == 0.0f ? 0.0f : s[8 * x + e] * mask[8 * x + e];
+        u32x4 parts[PARTS];
+        split<PARTS>(v, parts);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) lds.pairs[p][which][x][lane] = parts[p];
+      }
+    };
+    auto multiply = [&](const Set<C, STATES> &set) {
+      if (helper == 0) pair(set, 0);
+      if constexpr (CT == 2) {
+        if (helper == 1) pair(set, 1);
+        if (helper == (NW > 2 ? 2 : 0)) pair(set, 2);
+      }
+    };
+    if (from < end) {
+      fetch(0, from);
+      fetch(1, from + kChunk);
+#pragma unroll
+      for (int x = 0; x < SETS; ++x) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          if constexpr (!STATES) attn::clear_padding<kChunk, D, kThreads>(lds.sets[x].a[p], tid);
+          attn::clear_padding<kChunk, D, kThreads>(lds.sets[x].b[p], tid);
+        }
+      }
+      place(0);
+      fetch(0, from + 2 * kChunk);
+      __syncthreads();
+      if constexpr (!STATES) {
+        multiply(lds.sets[0]);
+        __syncthreads();
+      }
+    }
+    // Beside chunk r0: the next one, which is held in `k`.
+    auto chunk = [&](auto k, long r0) {
+      constexpr int K = decltype(k)::value;
+      const bool more = r0 + kChunk < end;
+      if constexpr (SETS == 1) {
+        if constexpr (!STATES) __syncthreads();
+        if (!more) return;
+        __syncthreads();   // (the tiles have been read)
+      }
+      if (more) {
+        place(K);
+        fetch(K, r0 + 3L * kChunk);
+      }
+      if (!STATES || more) __syncthreads();
+      if (STATES || !more) return;
+      multiply(lds.sets[K % SETS]);
+      __syncthreads();
+    };
+    for (long r0 = from; r0 < end; r0 += 2 * kChunk) {
+      chunk(attn::IntTag<1>(), r0);
+      if (r0 + kChunk < end) chunk(attn::IntTag<0>(), r0 + kChunk);
+    }
+    if constexpr (!STATES && C::RESULT != Result::None) {   // rows behind the length: zeros
+      constexpr bool kFloat = C::RESULT == Result::Float;
+      constexpr int kSize = kFloat ? 4 : 2, kPieces = C::kColumns * kSize / 16;
+      const Tokens<C::H, E, kFloat || C::HEADS_FIRST, C::H> to(w.out, b, h, w.seq, kSize);
+      const long none = from > len ? from : len;
+      for (long x = tid; x < (upto - none) * kPieces; x += kThreads) {
+        const int d = e0 + static_cast<int>(x % kPieces) * (16 / kSize);
+        if (d < E) *reinterpret_cast<u32x4 *>(const_cast<char *>(to.base) + (none + x / kPieces) * to.step + kSize * d) = u32x4{0, 0, 0, 0};
+      }
+    }
+    return;
   }
 
   // Row of unit u in register r: channel 32 u + 16 (r / 8) + 8 half + r % 8.
+  const int column = e0 + 32 * wave + swapped(lane & 31);   // of the state, in this lane
   f32x16 state[kUnits];
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) state[u] = {};
@@ -267,108 +389,99 @@ AKG_DEV void walk(const Walk &w, typename attn::conditional<STATES, StateLds<C>,
       }
     }
   }
-
-  // Weights: of the masked products (register r: key token 8 (r / 4) + 4 half + r % 4 of its 32, query token lane % 32), of
-  // the rows of a . S, and of what a token adds to the state.
-  constexpr int kAfter = C::BACK ? 1 : 0;
+  // What a token adds to the state fades with the tokens of its chunk behind it: 16 (kSteps - 1 - s) + 15 - j for token j of step
+  // s (the tokens are the last rows of their tile, however few).
   const float grow = C::BACK ? w.scale : 1.0f, show = C::BACK ? 1.0f : w.scale;
-  // pairs of tiles (query tile, key tile): 0 = (0, 0), 1 = (1, 0), 2 = (1, 1)
-  constexpr bool kAlone = NW == 1 && CT == 2;   // (one wavefront has them all)
-  float mask[kAlone ? 2 : 1][16], shown[CT];
-  float added[kSteps][8];
-  if constexpr (!STATES) {
+  float added[8], steps[kSteps], shown[CT], fade = 0.0f;
 #pragma unroll
-    for (int k = 0; k < (kAlone ? 2 : 1); ++k) {
-      const int apart = kAlone ? 32 * k : CT == 2 && wave == 1 ? 32 : 0;
+  for (int e = 0; e < 8; ++e) added[e] = power(g2, 15 - (8 * (e >> 2) + 4 * half + (e & 3)) + kAfter) * grow;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int n = apart + (lane & 31) - (8 * (r >> 2) + 4 * half + (r & 3));
-        mask[k][r] = n < 0 ? 0.0f : power(g2, n) * w.scale;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < CT; ++i) shown[i] = power(g2, 32 * i + (lane & 31) + 1 - kAfter) * show;
-  }
-  float fade;
+  for (int s = 0; s < kSteps; ++s) steps[s] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, power(g2, 16 * (kSteps - 1 - s)))));
   auto weigh = [&](int n) {
     fade = power_less_one(g, n);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int left = n - 1 - (16 * s + 8 * (e >> 2) + 4 * half + (e & 3));
-        added[s][e] = left < 0 ? 0.0f : power(g2, left + kAfter) * grow;
-      }
+    for (int i = 0; i < CT; ++i) {
+      const int row = 32 * i + (lane & 31) - (kChunk - n);
+      shown[i] = row < 0 ? 0.0f : power(g2, row + 1 - kAfter) * show;
     }
   };
   weigh(kChunk);
 
-  const Places<D> pd(lane);
   const Places<C::kColumns> pc(lane);
+  if (from < end) {   // (the first tiles are in place, and their masked products)
+    __syncthreads();
+    if constexpr (!STATES) __syncthreads();
+  }
+  int at = 0;   // the set
   for (long r0 = from; r0 < end; r0 += kChunk) {
     const int n = count_at(r0);
-    if constexpr (!STATES) sa.store(lds.a[0], tid);
-    sb.store(lds.b[0], tid);
-    sc.store(lds.c[0], tid);
-    __syncthreads();
-    if (r0 + kChunk < end) fetch(r0 + kChunk);
+    const Set<C, STATES> &set = lds.sets[at];
+    at = at + 1 < SETS ? at + 1 : 0;
     if (n != kChunk) weigh(n);
-
+    // Matrix instructions one by one, each with its share of what stands beside it: operands of later ones read from LDS,
+    // values of later ones rounded or weighted. (The barriers keep that order: left to itself the compiler reads an operand in
+    // front of its use and waits.)
     f32x16 out[CT];
-    if constexpr (!STATES) {
-      // this wavefront's share of the masked products, in the form of an operand whose columns are the query tokens
-      auto pair = [&](int which, const float (&weights)[16]) {
-        const int qt = which > 0 ? 1 : 0, kt = which > 1 ? 1 : 0;
-        f32x16 s = {};
+    constexpr int kGroup = kUnits == 8 ? 4 : kUnits == 6 ? 3 : kUnits;   // units of the state at a time
+    u32x4 values[kSteps][PARTS], more[kSteps][2], keys[kSteps * kUnits][PARTS];
+    auto value = [&](int s) {
 #pragma unroll
-        for (int x = 0; x < 2 * kUnits; ++x) {
-          u32x4 keys[PARTS], queries[PARTS];
+      for (int p = 0; p < PARTS; ++p) values[s][p] = pc.transposed(set.c[p], 16 * s, wave);
+    };
+    auto key = [&](int x) {
 #pragma unroll
-          for (int p = 0; p < PARTS; ++p) {
-            keys[p] = pd.row(lds.b[p], 32 * kt, x);
-            queries[p] = pd.row(lds.a[p], 32 * qt, x);
-          }
-          s = product(keys, queries, s);
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float v[8];
-          const bool outside = which != 1;   // (on the diagonal: where the weight is 0 the product does not count, whatever it is)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = outside && weights[8 * x + e] == 0.0f ? 0.0f : s[8 * x + e] * weights[8 * x + e];
-          u32x4 parts[PARTS];
-          split<PARTS>(v, parts);
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p) lds.pairs[p][which][x][lane] = parts[p];
-        }
-      };
-      if constexpr (CT == 1) {
-        if (wave == 0) pair(0, mask[0]);
-      } else if constexpr (kAlone) {
-        pair(0, mask[0]);
-        pair(1, mask[1]);
-        pair(2, mask[0]);
-      } else {
-        if (wave == 0) pair(0, mask[0]);
-        if (wave == 1) pair(1, mask[0]);
-        if (wave == (NW > 2 ? 2 : 0)) pair(2, mask[0]);
+      for (int p = 0; p < PARTS; ++p) keys[x][p] = pd.transposed(set.b[p], 16 * (x / kUnits), x % kUnits);
+    };
+    // (pair e of the eight values of step s)
+    auto weighted = [&](int s, int e) {
+      float lo = BF16::low(values[s][0][e]), hi = BF16::high(values[s][0][e]);
+      if constexpr (PARTS == 2) {
+        lo += BF16::low(values[s][1][e]);
+        hi += BF16::high(values[s][1][e]);
       }
-      // a . S
+      split_pair<2>(lo * (added[2 * e] * steps[s]), hi * (added[2 * e + 1] * steps[s]), more[s], e);
+    };
+    if constexpr (!STATES) {
+      // a . S; the state fades behind its use
 #pragma unroll
       for (int i = 0; i < CT; ++i) out[i] = {};
+      constexpr int kAll = 2 * kUnits * CT, kAhead = 6;
+      u32x4 queries[kAll][PARTS], parts[2 * kUnits][PARTS], pairs[kSteps][CT][PARTS];
+      auto query = [&](int y) {
 #pragma unroll
-      for (int x = 0; x < 2 * kUnits; ++x) {
-        float v[8];
+        for (int p = 0; p < PARTS; ++p) queries[y][p] = pd.row(set.a[p], 32 * (y % CT), y / CT);
+      };
+      // (pair e of the eight rows x)
+      auto rounded = [&](int x, int e) {
+        const int r = 8 * (x & 1) + 2 * e;
+        const float lo = state[x >> 1][r], hi = state[x >> 1][r + 1];
+        split_pair<PARTS>(lo, hi, parts[x], e);
+        state[x >> 1][r] = __builtin_fmaf(lo, fade, lo);
+        state[x >> 1][r + 1] = __builtin_fmaf(hi, fade, hi);
+      };
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = state[x >> 1][8 * (x & 1) + e];
-        u32x4 s[PARTS];
-        split<PARTS>(v, s);
+      for (int y = 0; y < kAhead && y < kAll; ++y) query(y);
 #pragma unroll
-        for (int i = 0; i < CT; ++i) {
-          u32x4 queries[PARTS];
+      for (int e = 0; e < 4; ++e) rounded(0, e);
 #pragma unroll
-          for (int p = 0; p < PARTS; ++p) queries[p] = pd.row(lds.a[p], 32 * i, x);
-          out[i] = product(s, queries, out[i]);
+      for (int y = 0; y < kAll; ++y) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int x = y / CT, i = y % CT;
+        out[i] = product(parts[x], queries[y], out[i]);
+        if (y + kAhead < kAll) query(y + kAhead);
+        if (x + 1 < 2 * kUnits) {
+#pragma unroll
+          for (int e = i * 4 / CT; e < (i + 1) * 4 / CT; ++e) rounded(x + 1, e);
+        }
+      }
+      // ... and the masked products with c
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        value(s);
+#pragma unroll
+        for (int i = s / 2; i < CT; ++i) {
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) pairs[s][i][p] = lds.pairs[p][i == 0 ? 0 : 1 + s / 2][s & 1][lane];
         }
       }
 #pragma unroll
@@ -376,119 +489,105 @@ AKG_DEV void walk(const Walk &w, typename attn::conditional<STATES, StateLds<C>,
 #pragma unroll
         for (int r = 0; r < 16; ++r) out[i][r] *= shown[i];
       }
-      __syncthreads();
-    }
-    // the masked products with c, and what c adds to the state
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) state[u][r] = __builtin_fmaf(state[u][r], fade, state[u][r]);
-    }
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      u32x4 values[PARTS];
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p) values[p] = pc.transposed(lds.c[p], 16 * s, wave);
-      if constexpr (!STATES) {
+      for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
         for (int i = s / 2; i < CT; ++i) {
-          const int which = i == 0 ? 0 : 1 + s / 2;
-          u32x4 pairs[PARTS];
+          __builtin_amdgcn_sched_barrier(0);
+          out[i] = product(values[s], pairs[s][i], out[i]);
+          if (s == 0 && i == 0) {
 #pragma unroll
-          for (int p = 0; p < PARTS; ++p) pairs[p] = lds.pairs[p][which][s & 1][lane];
-          out[i] = product(values, pairs, out[i]);
-        }
-      }
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[2 * e] = BF16::low(values[0][e]);
-        v[2 * e + 1] = BF16::high(values[0][e]);
-        if constexpr (PARTS == 2) {
-          v[2 * e] += BF16::low(values[1][e]);
-          v[2 * e + 1] += BF16::high(values[1][e]);
+            for (int e = 0; e < 4; ++e) weighted(0, e);
+          }
         }
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= added[s][e];
-      u32x4 more[2];
-      split<2>(v, more);
+      for (int u = 0; u < kGroup; ++u) key(u);
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) value(s);
+#pragma unroll
+      for (int u = 0; u < kGroup; ++u) key(u);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
-        u32x4 keys[PARTS];
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) keys[p] = pd.transposed(lds.b[p], 16 * s, u);
-        state[u] = product(keys, more, state[u]);
+        for (int r = 0; r < 16; ++r) state[u][r] = __builtin_fmaf(state[u][r], fade, state[u][r]);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) weighted(0, e);
     }
-    if constexpr (!STATES && C::RESULT != Result::None) {
-      constexpr bool kFloat = C::RESULT == Result::Float;
-      constexpr int kSize = kFloat ? 4 : 2;
-      // (a result in float32 is one of the walk's own heads, heads first)
-      const Tokens<C::H, E, kFloat || C::HEADS_FIRST, C::H> to(w.out, b, h, w.seq, kSize);
-      const long lowest = C::BACK ? len - r0 - n : r0;
-      const Buffer buf = make_buffer(to.base + lowest * to.step, records((n - 1) * to.step + static_cast<long>(kSize) * E));
+    // a result in float32 is one of the walk's own heads, heads first
+    constexpr bool kFloat = C::RESULT == Result::Float, kShow = !STATES && C::RESULT != Result::None;
+    constexpr int kSize = kFloat ? 4 : 2;
+    const Tokens<C::H, E, kFloat || C::HEADS_FIRST, C::H> to(w.out, b, h, w.seq, kSize);
+    const Buffer buf = make_buffer(to.base + lowest_at(r0, n) * to.step, kShow ? records((n - 1) * to.step + static_cast<long>(kSize) * E) : 0);
+    // (half x of query tile i: 16 channels of a row in a pair of lanes)
+    auto write = [&](int i, int x) {
+      const int row = 32 * i + (lane & 31), behind = C::BACK ? kChunk - 1 - row : row - (kChunk - n), d = e0 + 32 * wave + 16 * x + 8 * half;
+      const u32 off = row >= kChunk - n && d < E ? static_cast<u32>(behind * static_cast<int>(to.step) + kSize * d) : kBeyondEveryBuffer;
+      if constexpr (kFloat) {
 #pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        const int row = 32 * i + (lane & 31);
-        const int at = (C::BACK ? n - 1 - row : row) * static_cast<int>(to.step);
+        for (int y = 0; y < 2; ++y) {
+          f32x4 v;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int d = e0 + 32 * wave + 16 * x + 8 * half;
-          const u32 off = row < n && d < E ? static_cast<u32>(at + kSize * d) : kBeyondEveryBuffer;
-          if constexpr (kFloat) {
+          for (int e = 0; e < 4; ++e) v[e] = out[i][8 * x + 4 * y + e];
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), buf, off + (off == kBeyondEveryBuffer ? 0u : 16u * y), 0, 0);
+        }
+      } else {
+        u32x4 v;
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              f32x4 v;
+        for (int e = 0; e < 4; ++e) v[e] = C::T::pack(out[i][8 * x + 2 * e], out[i][8 * x + 2 * e + 1]);
+        __builtin_amdgcn_raw_buffer_store_b128(v, buf, off, 0, 0);
+      }
+    };
+    // What c adds to the state: a few units at a time, first the products with the rests; the keys of the units behind them are
+    // read meanwhile, the next tokens weighted, the rows of the result written.
+    constexpr int kPasses = PARTS + 1, kGroups = kSteps * kUnits / kGroup;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] = out[i][8 * x + 4 * y + e];
-              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), buf, off + (off == kBeyondEveryBuffer ? 0u : 16u * y), 0, 0);
+    for (int q = 0; q < kGroups; ++q) {
+      const int s = q * kGroup / kUnits, u0 = q * kGroup % kUnits;
+#pragma unroll
+      for (int pass = 0; pass < kPasses; ++pass) {
+#pragma unroll
+        for (int v = 0; v < kGroup; ++v) {
+          __builtin_amdgcn_sched_barrier(0);
+          const int u = u0 + v;
+          state[u] = BF16::mma(keys[q * kGroup + v][PARTS == 2 && pass == 1 ? 1 : 0], more[s][pass == 0 ? 1 : 0], state[u]);
+          if (pass == 0 && q + 1 < kGroups) key((q + 1) * kGroup + v);
+          if (u0 == 0 && pass + 1 == kPasses && s + 1 < kSteps) {
+#pragma unroll
+            for (int e = v * 4 / kGroup; e < (v + 1) * 4 / kGroup; ++e) weighted(s + 1, e);
+          }
+          if constexpr (kShow) {
+            if (pass == kPasses - 2 && v == 0) {
+#pragma unroll
+              for (int y = q * 2 * CT / kGroups; y < (q + 1) * 2 * CT / kGroups; ++y) write(y / 2, y % 2);
             }
-          } else {
-            u32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = C::T::pack(out[i][8 * x + 2 * e], out[i][8 * x + 2 * e + 1]);
-            __builtin_amdgcn_raw_buffer_store_b128(v, buf, off, 0, 0);
           }
         }
       }
     }
-    __syncthreads();   // (the tiles have been read)
+    __builtin_amdgcn_sched_barrier(0);
+    if (r0 + kChunk < end) {
+      if constexpr (SETS == 1) {
+        __syncthreads();
+        if constexpr (!STATES) __syncthreads();
+      }
+      __syncthreads();   // (the next chunk's tiles are in place, and their masked products)
+    }
   }
 
-  if constexpr (STATES) {
-    if (column < E) {
+  // a walk over states leaves them in the workspace; else the segment that holds the last token has the last state
+  const bool ends = seg == (len > 0 ? static_cast<int>((len - 1) / w.segment) : 0);
+  float *to = STATES ? starts : w.last != nullptr && ends && entry >= 0 ? w.last + (entry * C::H + h) * (static_cast<long>(D) * E) : nullptr;
+  if (to != nullptr && column < E) {
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
+    for (int u = 0; u < kUnits; ++u) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int d = 32 * u + 16 * (r >> 3) + 8 * half + (r & 7);
-          if (D % 32 == 0 || d < D) starts[static_cast<long>(d) * E + column] = state[u][r];
-        }
-      }
-    }
-  } else {
-    if constexpr (C::RESULT != Result::None) {   // rows behind the length: zeros
-      constexpr bool kFloat = C::RESULT == Result::Float;
-      constexpr int kSize = kFloat ? 4 : 2, kPieces = C::kColumns * kSize / 16;
-      const Tokens<C::H, E, kFloat || C::HEADS_FIRST, C::H> to(w.out, b, h, w.seq, kSize);
-      const long none = from > len ? from : len;
-      for (long x = tid; x < (upto - none) * kPieces; x += kThreads) {
-        const int d = e0 + static_cast<int>(x % kPieces) * (16 / kSize);
-        if (d < E) *reinterpret_cast<u32x4 *>(const_cast<char *>(to.base) + (none + x / kPieces) * to.step + kSize * d) = u32x4{0, 0, 0, 0};
-      }
-    }
-    // the segment that holds the last token has the last state
-    const bool ends = seg == (len > 0 ? static_cast<int>((len - 1) / w.segment) : 0);
-    if (w.last != nullptr && ends && entry >= 0 && column < E) {
-      float *to = w.last + (entry * C::H + h) * (static_cast<long>(D) * E);
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int d = 32 * u + 16 * (r >> 3) + 8 * half + (r & 7);
-          if (D % 32 == 0 || d < D) to[C::TURNED ? static_cast<long>(column) * D + d : static_cast<long>(d) * E + column] = state[u][r];
-        }
+      for (int r = 0; r < 16; ++r) {
+        const int d = 32 * u + 16 * (r >> 3) + 8 * half + (r & 7);
+        if (D % 32 == 0 || d < D) to[C::TURNED && !STATES ? static_cast<long>(column) * D + d : static_cast<long>(d) * E + column] = state[u][r];
       }
     }
   }
