@@ -552,6 +552,7 @@ class LayerEmitter {
     int64_t d, e, ha, hb, hc;
     bool back, turned;
     const char *result;   // of linear::Result
+    bool rest;            // the last state is a result
     int64_t tiles = 1;
   };
   struct LinearSizes {
@@ -575,9 +576,9 @@ class LayerEmitter {
     if (s.seq >= (1LL << 31) - 8192) throw LoweringError("op " + op_.name + ": more than 2^31 tokens");
     return s;
   }
-  std::string walkConfig(const WalkOf &w, const LinearSizes &s, int ct, int64_t nw, int sets) const {
+  std::string walkConfig(const WalkOf &w, const LinearSizes &s, int ct, int64_t nw, bool tight) const {
     std::ostringstream o;
-    o << "akg::linear::Config<" << trait() << ", " << w.d << ", " << w.e << ", " << ct << ", " << nw << ", " << sets << ", " << s.heads << ", " << w.ha << ", " << w.hb << ", " << w.hc
+    o << "akg::linear::Config<" << trait() << ", " << w.d << ", " << w.e << ", " << ct << ", " << nw << ", " << flag(tight) << ", " << flag(w.rest) << ", " << s.heads << ", " << w.ha << ", " << w.hb << ", " << w.hc
       << ", " << flag(l_.headsFirst) << ", " << flag(w.back) << ", " << flag(w.turned) << ", akg::linear::Result::" << w.result << ">";
     return o.str();
   }
@@ -586,38 +587,77 @@ class LayerEmitter {
   // workspace in front of theirs. The workspace's bytes are returned.
   int64_t walks(std::ostringstream &o, std::vector<KernelPhase> &phases, std::vector<WalkOf> &all, const LinearSizes &s, const std::string &args, const std::string &decay,
                 const std::string &lengths, const std::string &slots, int64_t space, bool more) {
-    int64_t widest = 0, deepestD = 0;
+    int64_t widest = 0, deepest = 0, values = 0;
     for (const WalkOf &w : all) {
       widest = std::max(widest, w.e);
-      deepestD = std::max(deepestD, w.d);
-    }
-    const bool pairsOfParts = in(0).dtype == DType::F16;
-    int ct = pairsOfParts ? 1 : 2;
-    const int64_t units = ceilDiv(widest, 32);
-    int64_t nw = std::max<int64_t>(2, ceilDiv(units, ceilDiv(units, 4)));
-    // Two sets of tiles where LDS holds them (attn::pitch), chunks of 32 tokens before one set.
-    const int64_t parts = pairsOfParts ? 2 : 1;
-    auto pitchOf = [](int64_t d) { return ceilDiv(d, 32) % 2 == 1 ? ceilDiv(d, 32) * 64 : ceilDiv(d, 32) * 64 + 64; };
-    auto setBytes = [&](int tiles) { return parts * 32 * tiles * (2 * pitchOf(deepestD) + pitchOf(32 * nw)); };
-    int sets = 2;
-    const int64_t room = 160 * 1024 - parts * 6144;
-    if (2 * setBytes(ct) > room) ct = 1;
-    if (2 * setBytes(ct) > room) sets = 1;
-    int64_t groups = 0, values = 0;
-    for (WalkOf &w : all) {
-      w.tiles = ceilDiv(w.e, 32 * nw);
-      groups += s.states * w.tiles;
+      deepest = std::max(deepest, w.d);
       values += w.d * w.e;
     }
-    int64_t segments = std::max<int64_t>(1, std::min<int64_t>(cus_ / groups, s.seq / 256));
+    const int parts = in(0).dtype == DType::F16 ? 2 : 1;
+    const int64_t units = ceilDiv(widest, 32);
+    // How many wavefronts hold the state of a workgroup (32 columns each: fewer make more workgroups, which all fetch a and b and
+    // multiply them), and how many segments share the tokens (each but the last adds a pass over b and c in front): what is
+    // expected to take least. A chunk of 64 tokens of 128 channels takes 1.4, 1.5 and 2.0 us with one, two and four such wavefronts
+    // (one workgroup a CU), of 32 tokens of 256 channels 1.2, 1.2 and 1.5, of 32 tokens of 128 in float16 1.8 and 2.4 with two and
+    // four, a walk over states alone about half; memory gives 4.8 TB/s; two launches more and a state to be
+    // joined take some 10 us. us at 4 x 4096 tokens of 32 heads of 128: two 121, four 145, four and two segments 157; 2 x 2048:
+    // one 48, two 56, four 69, four and four segments 53; 16384 of 16 heads: four and 1, 8, 16, 32 segments 522, 132, 102, 117;
+    // 4 x 4096 of 16 heads of 64: one 76, two and 1, 4, 8 segments 91, 50, 56; gradient of 2 x 1021 of 16/4 heads of 128: one, two,
+    // four 59, 40, 49; of 4 x 4096 of 32 heads: two, four 351, 297.
+    struct Schedule {
+      double time;
+      int64_t nw, segments;
+      int ct;
+      bool tight;
+    } best = {};
+    auto tilesOf = [&](int64_t nw) {
+      int64_t n = 0;
+      for (const WalkOf &w : all) n += ceilDiv(w.e, 32 * nw);
+      return n;
+    };
+    for (int64_t nw = std::min<int64_t>(units, 4); nw >= 1; --nw) {
+      if (nw > 2 && nw != ceilDiv(units, ceilDiv(units, 4))) continue;
+      // Tiles of a few chunks (linear::Lds, linear::pitch) where LDS holds them, of chunks of 32 tokens before those of one chunk only.
+      auto pitchOf = [](int64_t d) { return ceilDiv(d, 32) * 64 + 32; };
+      auto ldsBytes = [&](int64_t tiles) { return parts * (32 * tiles * (5 * pitchOf(deepest) + 3 * pitchOf(32 * nw)) + 2 * 2048 * (tiles * (tiles + 1) / 2)); };
+      int ct = parts == 2 || ldsBytes(2) > 160 * 1024 ? 1 : 2;
+      const bool tight = ldsBytes(ct) > 160 * 1024;
+      const int64_t groups = s.states * tilesOf(nw), chunks = ceilDiv(s.seq, 32 * ct);
+      const double each = (0.9 + ct * (0.15 + (parts == 2 ? 0.08 : 0.026) * static_cast<double>(nw * ceilDiv(deepest, 32)))) * (tight ? 1.5 : 1.0);
+      const double bytes = static_cast<double>(2 * s.states * s.seq) / 4.8e6;   // us for a channel of every token
+      for (int64_t segments = 1; segments <= std::max<int64_t>(1, std::min<int64_t>(cus_ / groups, chunks / 2)); ++segments) {
+        const double steps = static_cast<double>(ceilDiv(chunks, segments));
+        double moved = 0.0, movedStates = 0.0;
+        for (const WalkOf &w : all) {
+          // (a and b once more for every further workgroup of a head, most of it from the L2)
+          const double again = 1.0 + 0.2 * static_cast<double>(ceilDiv(w.e, 32 * nw) - 1);
+          moved += bytes * (static_cast<double>(2 * w.d) * again + static_cast<double>(2 * w.e));
+          movedStates += bytes * (static_cast<double>(w.d) * again + static_cast<double>(w.e));
+        }
+        // (what chunks take and what memory takes overlap, not wholly)
+        auto both = [](double x, double y) { return std::max(x, y) + 0.25 * std::min(x, y); };
+        double time = both(static_cast<double>(ceilDiv(groups * segments, cus_)) * steps * each, moved);
+        if (segments > 1) {
+          time += both(static_cast<double>(ceilDiv(groups * (segments - 1), cus_)) * steps * each * 0.55, movedStates) + 10.0 +
+                  static_cast<double>(8 * s.states * segments * values) / 4.8e6;
+        }
+        if (best.nw == 0 || time < best.time) best = {time, nw, segments, ct, tight};
+      }
+    }
+    const int64_t nw = best.nw;
+    const int ct = best.ct;
+    const bool tight = best.tight;
+    for (WalkOf &w : all) w.tiles = ceilDiv(w.e, 32 * nw);
+    const int64_t groups = s.states * tilesOf(nw);
+    int64_t segments = best.segments;
     while (limit_ > 0 && segments > 1 && space + 4 * s.states * segments * values > limit_) --segments;
     const int64_t chunk = 32 * ct, segment = ceilDiv(ceilDiv(s.seq, segments), chunk) * chunk;
     segments = ceilDiv(s.seq, segment);
     k_.scalarArgs = {s.batch, s.seq, segment, segments};
     if (l_.hasSlots) k_.scalarArgs.push_back(in(4).shape[0]);
     std::vector<std::string> names;
-    o << "typedef " << walkConfig(all[0], s, ct, nw, sets) << " akg_C0;\n";
-    for (size_t i = 1; i < all.size(); ++i) o << "typedef " << walkConfig(all[i], s, ct, nw, sets) << " akg_C" << i << ";\n";
+    o << "typedef " << walkConfig(all[0], s, ct, nw, tight) << " akg_C0;\n";
+    for (size_t i = 1; i < all.size(); ++i) o << "typedef " << walkConfig(all[i], s, ct, nw, tight) << " akg_C" << i << ";\n";
     o << "\n";
     int64_t before = space;
     std::vector<std::string> structs;
@@ -630,25 +670,27 @@ class LayerEmitter {
       structs.push_back(b.str());
       before += 4 * s.heads * w.d * w.e;
     }
-    const int threads = static_cast<int>(128 * nw);
+    const int threads = static_cast<int>(64 * (nw + 4));   // (linear::kHelpers)
     int hint = 2;
-    // every walk has the workgroups from `from` on; a head's are on one XCD (attn::head_and_tile)
+    // A head's workgroups are neighbours on one XCD, whose L2 they share: the walks of a gradient read the same tensors, those
+    // backward in time at the same time.
+    int64_t tiles = 0;
+    for (const WalkOf &w : all) tiles += w.tiles;
     auto body = [&](bool states) {
       std::ostringstream b;
-      b << "  __shared__ __attribute__((aligned(16))) akg::u8 akg_lds[";
+      b << "  const int akg_parts = static_cast<int>(akg_segments" << (states ? " - 1" : "") << ");\n  __shared__ __attribute__((aligned(16))) akg::u8 akg_lds[";
       auto lds = [&](size_t i) { return "akg::linear::Lds<akg_C" + std::to_string(i) + ", " + flag(states) + ">"; };
       std::string size = "sizeof(" + lds(0) + ")";
       for (size_t i = 1; i < all.size(); ++i) {
         const std::string other = "sizeof(" + lds(i) + ")";
         size = "(" + size + " > " + other + " ? " + size + " : " + other + ")";
       }
-      b << size << "];\n  long akg_id = blockIdx.x, akg_head, akg_rest;\n  const long akg_heads = akg_batch * " << s.heads << ", akg_parts = " << (states ? "akg_segments - 1" : "akg_segments") << ";\n";
+      b << size << "];\n  const int akg_id = akg::xcd_contiguous_id(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));\n  const long akg_head = akg_id / (akg_parts * " << tiles
+        << ");\n  int akg_part = static_cast<int>(akg_id % (akg_parts * " << tiles << ")), akg_tile = akg_part % " << tiles << ";\n  akg_part /= " << tiles << ";\n";
       for (size_t i = 0; i < all.size(); ++i) {
         const std::string n = std::to_string(i);
-        b << "  if (akg_id < akg_heads * akg_parts * akg_C" << n << "::kTiles) {\n    const akg::linear::Walk akg_w = " << structs[i] << ";\n"
-          << "    akg::attn::head_and_tile(akg_id, akg_heads, akg_head, akg_rest);\n"
-          << "    akg::linear::walk<akg_C" << n << ", " << flag(states) << ">(akg_w, *reinterpret_cast<" << lds(i) << " *>(akg_lds), akg_head, static_cast<int>(akg_rest % akg_C" << n << "::kTiles), static_cast<int>(akg_rest / akg_C" << n << "::kTiles));\n    return;\n  }\n"
-          << "  akg_id -= akg_heads * akg_parts * akg_C" << n << "::kTiles;\n";
+        b << "  if (akg_tile < akg_C" << n << "::kTiles) {\n    const akg::linear::Walk akg_w = " << structs[i] << ";\n    akg::linear::walk<akg_C" << n << ", " << flag(states)
+          << ">(akg_w, *reinterpret_cast<" << lds(i) << " *>(akg_lds), akg_head, akg_tile, akg_part);\n    return;\n  }\n  akg_tile -= akg_C" << n << "::kTiles;\n";
       }
       return b.str();
     };
@@ -714,7 +756,7 @@ class LayerEmitter {
     }
     std::vector<std::string> scalars = {"akg_batch", "akg_seq", "akg_segment", "akg_segments"};
     if (l_.hasSlots) scalars.push_back("akg_pool");
-    WalkOf w{inName(0), inName(1), inName(2), outName(0), state, outName(1), s.dk, s.dv, s.heads, s.kvHeads, s.kvHeads, false, false, wanted(0) ? "Storage" : "None"};
+    WalkOf w{inName(0), inName(1), inName(2), outName(0), state, outName(1), s.dk, s.dv, s.heads, s.kvHeads, s.kvHeads, false, false, wanted(0) ? "Storage" : "None", op_.outputs.size() > 1};
     std::vector<WalkOf> all{w};
     std::vector<KernelPhase> phases;
     // (whether there is a workspace is known only behind the schedule: the text is made twice where there is none)
@@ -745,10 +787,10 @@ class LayerEmitter {
     const std::string dvAt = wanted(1) ? "akg_batch * akg_seq * " + std::to_string(h * s.dk) + "L" : "0L";
     std::vector<WalkOf> all;
     const char *part = shared ? "Float" : "Storage";
-    if (wanted(0)) all.push_back({dout, v, k, outName(0), state, "nullptr", s.dv, s.dk, h, kv, kv, false, true, "Storage"});
-    if (wanted(1)) all.push_back({v, dout, q, shared ? "akg_ws" : outName(1), dstate, "nullptr", s.dv, s.dk, kv, h, h, true, true, part});
+    if (wanted(0)) all.push_back({dout, v, k, outName(0), state, "nullptr", s.dv, s.dk, h, kv, kv, false, true, "Storage", false});
+    if (wanted(1)) all.push_back({v, dout, q, shared ? "akg_ws" : outName(1), dstate, "nullptr", s.dv, s.dk, kv, h, h, true, true, part, false});
     if (wanted(2) || wanted(3)) {
-      all.push_back({k, q, dout, !wanted(2) ? "nullptr" : shared ? "akg_ws + " + dvAt : outName(2), dstate, outName(3), s.dk, s.dv, kv, h, h, true, false, wanted(2) ? part : "None"});
+      all.push_back({k, q, dout, !wanted(2) ? "nullptr" : shared ? "akg_ws + " + dvAt : outName(2), dstate, outName(3), s.dk, s.dv, kv, h, h, true, false, wanted(2) ? part : "None", l_.hasState});
     }
     if (all.empty()) throw LoweringError("op " + op_.name + ": none of its results is an output");
     const bool more = dkBytes + dvBytes > 0;

@@ -24,9 +24,9 @@
  * adjacent channels (the contracted ones of the next product, read from LDS as 16 bytes, and 16 bytes of a row of `out`).
  * The wavefronts share the masked products of a chunk (a . b) through LDS, in the form of the operand that they become.
  *
- * Rounding: bfloat16 operands are exact; products a . b and the state are rounded to bfloat16 (2^-9 of each term) where they
- * are contracted again. What is added to the state, exp(g ..) c, goes as two bfloat16 parts (2^-17), since the state is a
- * result in float32 and lives long. float16 operands, and everything contracted with them, go as two bfloat16 parts
+ * Rounding: bfloat16 operands are exact; products a . b and the state are rounded to bfloat16 (2^-8 of each term at most) where they
+ * are contracted again. What is added to the state, exp(g ..) c, is rounded likewise where the state is only read on the way,
+ * and goes as two bfloat16 parts (2^-16) where the last state is a result, in float32. float16 operands, and everything contracted with them, go as two bfloat16 parts
  * throughout: three products for one, no range but that of float32, and 2^-16 of each term.
  */
 #pragma once
@@ -35,15 +35,31 @@ namespace akg {
 namespace linear {
 
 using attn::BF16;
-using attn::chunk_at;
 using attn::f32x16;
 using attn::f32x4;
 using attn::kLog2e;
 using attn::padded;
-using attn::pitch;
 using attn::records;
 using attn::u32x2;
 using attn::u32x4;
+
+// A tile of W channels in LDS: rows an odd multiple of 32 bytes apart, so that four neighbouring rows of 32 bytes (transposed
+// reads, sixteen lanes at a time) and eight of 16 bytes lie in banks of their own; chunks of 16 bytes change places in pairs in every
+// second eight rows, so that sixteen of 16 bytes do (rows read by 128 bits, sixteen lanes at a time). (The tiles of
+// akg_attention.hpp have 64 bytes more a row instead of 32: three chunks' tiles would not fit.)
+constexpr int pitch(int w) { return padded(w) * 2 + 32; }
+template <int W>
+AKG_DEV int chunk_at(int row, int chunk) {
+  return row * pitch(W) + ((chunk ^ ((row >> 3) & 1)) << 4);
+}
+// The channels behind W of a tile's rows (to the next multiple of 32) hold zeros: written once, never again.
+template <int ROWS, int W, int THREADS>
+AKG_DEV void clear_padding(u8 *tile, int tid) {
+  if constexpr (W % 32 != 0) {
+    constexpr int kPad = (padded(W) - W) / 8;
+    for (int c = tid; c < ROWS * kPad; c += THREADS) *reinterpret_cast<u32x4 *>(tile + chunk_at<W>(c / kPad, W / 8 + c % kPad)) = u32x4{0, 0, 0, 0};
+  }
+}
 
 // Channel of a 32-channel unit that lane `m` (mod 32) of a transposed operand holds.
 constexpr int swapped(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1); }
@@ -90,20 +106,16 @@ AKG_DEV f32x16 product(const u32x4 (&a)[PA], const u32x4 (&b)[PB], f32x16 c) {
 // A lane's places in a tile of W channels (as attn::Reader, with the quads of transposed reads swapped).
 template <int W>
 struct Places {
-  int along[2], across[2];
+  int along, across[2];
   AKG_DEV explicit Places(int lane) {
-    const int row = lane & 31, h = lane >> 5;
-    along[0] = chunk_at<W>(row, h);
-    along[1] = chunk_at<W>(row, 2 + h);
-    const int i = lane & 15, r = 4 * h + (i >> 2), quad = ((i & 1) << 1) | ((i & 2) >> 1), chunk = 2 * ((lane >> 4) & 1) + (quad >> 1);
+    const int h = lane >> 5, i = lane & 15, r = 4 * h + (i >> 2), quad = ((i & 1) << 1) | ((i & 2) >> 1), chunk = 2 * ((lane >> 4) & 1) + (quad >> 1);
+    along = chunk_at<W>(lane & 31, h);
     across[0] = chunk_at<W>(r, chunk) + (quad & 1) * 8;
     across[1] = chunk_at<W>(r + 8, chunk) + (quad & 1) * 8;
   }
-  // Channels 16 c + 8 (lane / 32) .. + 7 of row `row0 + lane % 32`.
-  AKG_DEV u32x4 row(const u8 *tile, int row0, int c) const {
-    return *reinterpret_cast<const u32x4 *>(tile + along[c & 1] + (row0 * pitch(W) + 64 * (c >> 1)));
-  }
-  // Channel 32 unit + swapped(lane % 32) of the rows row0 + 4 h .. 4 h + 3 and row0 + 8 + 4 h .. (h = lane / 32).
+  // Channels 16 c + 8 (lane / 32) .. + 7 of row `row0 + lane % 32` (row0 a multiple of 32).
+  AKG_DEV u32x4 row(const u8 *tile, int row0, int c) const { return *reinterpret_cast<const u32x4 *>(tile + along + (row0 * pitch(W) + 32 * c)); }
+  // Channel 32 unit + swapped(lane % 32) of the rows row0 + 4 h .. 4 h + 3 and row0 + 8 + 4 h .. (h = lane / 32; row0 a multiple of 16).
   AKG_DEV u32x4 transposed(const u8 *tile, int row0, int unit) const {
     const int more = row0 * pitch(W) + 64 * unit;
     const attn::s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn::s16x4 *)(tile + across[0] + more));
@@ -113,7 +125,18 @@ struct Places {
   }
 };
 
-// ROWS tokens of W channels on their way from memory to LDS. Tokens and channels that do not exist read zeros.
+// The last `count` of the rows of a tile in memory: row ROWS - 1 - i is i (BACK) or count - 1 - i rows behind `first`; `channels`
+// of a row are read.
+template <int ROWS, bool BACK>
+struct Rows {
+  Buffer buf;
+  int from, each, missing, channels;
+  AKG_DEV Rows(const char *first, long step, int count, int channels_)
+      : buf(make_buffer(first, count > 0 ? records((count - 1) * step + 2L * channels_) : 0)), from((BACK ? ROWS - 1 : count - ROWS) * static_cast<int>(step)),
+        each(BACK ? -static_cast<int>(step) : static_cast<int>(step)), missing(ROWS - count), channels(channels_) {}
+};
+// ROWS tokens of W channels on their way from memory to LDS, in kEach pieces of a thread. Tokens and channels that do not exist
+// read zeros.
 template <int ROWS, int W, int THREADS, int PARTS>
 struct Stage {
   static constexpr int kPerRow = W / 8, kChunks = ROWS * kPerRow, kEach = (kChunks + THREADS - 1) / THREADS;
@@ -122,17 +145,11 @@ struct Stage {
   static constexpr bool kEven = kWhole && THREADS % kPerRow == 0 && THREADS / kPerRow % 16 == 0;
   static constexpr int kTileBytes = ROWS * pitch(W);
   u32x4 held[kEach];
-  // The last `count` rows, of which row ROWS - 1 - i is i (BACK) or count - 1 - i rows behind `first`; `channels` of a row are read.
   template <bool BACK>
-  AKG_DEV void load(const char *first, long step, int count, int channels, int tid) {
-    const Buffer buf = make_buffer(first, count > 0 ? records((count - 1) * step + 2L * channels) : 0);
-    const int each = BACK ? -static_cast<int>(step) : static_cast<int>(step), from = BACK ? (ROWS - 1) * static_cast<int>(step) : (count - ROWS) * static_cast<int>(step);
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int c = tid + i * THREADS, row = c / kPerRow, at = c % kPerRow * 8;
-      const bool there = row >= ROWS - count && at < channels && (kWhole || c < kChunks);
-      held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, there ? static_cast<u32>(from + row * each + 2 * at) : kBeyondEveryBuffer, 0, 0));
-    }
+  AKG_DEV void load(const Rows<ROWS, BACK> &rows, int i, int tid) {
+    const int c = tid + i * THREADS, row = c / kPerRow, at = c % kPerRow * 8;
+    const bool there = row >= rows.missing && at < rows.channels && (kWhole || c < kChunks);
+    held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows.buf, there ? static_cast<u32>(rows.from + row * rows.each + 2 * at) : kBeyondEveryBuffer, 0, 0));
   }
   AKG_DEV void store(u8 *tile, int tid) const {
 #pragma unroll
@@ -159,30 +176,27 @@ struct Stage {
 };
 
 // What the emitted kernel states about a walk: the operands' type in parts, channels of a and b (D) and of c and the result
-// (E), 32-token tiles of a chunk (CT), pairs of wavefronts (NW, 32 channels of c each), sets of tiles in LDS (SETS), heads of the
-// states (H) and of each operand, whether it runs backward, whether states given and left are the transposed ones ([E][D] in
-// memory).
+// (E), 32-token tiles of a chunk (CT), wavefronts that hold the state (NW, 32 channels of c each), whether LDS holds one chunk's
+// tiles only (TIGHT), whether what is added to the state goes in two parts (REST), heads of the states (H) and of each operand, whether it runs backward, whether states given and left are
+// the transposed ones ([E][D] in memory).
 enum class Result { None, Storage, Float };
-template <typename T_, int D_, int E_, int CT_, int NW_, int SETS_, int H_, int HA_, int HB_, int HC_, bool HEADS_FIRST_, bool BACK_, bool TURNED_, Result RESULT_>
+constexpr int kHelpers = 4;   // wavefronts that fetch and multiply
+template <typename T_, int D_, int E_, int CT_, int NW_, bool TIGHT_, bool REST_, int H_, int HA_, int HB_, int HC_, bool HEADS_FIRST_, bool BACK_, bool TURNED_, Result RESULT_>
 struct Config {
-  static_assert(NW_ >= 2, "two wavefronts at least share the masked products of a chunk");
   typedef T_ T;   // attn::BF16 or attn::F16
-  static constexpr int PARTS = T::kNarrowRange ? 2 : 1, D = D_, E = E_, CT = CT_, NW = NW_, SETS = SETS_, H = H_, HA = HA_, HB = HB_, HC = HC_;
-  static constexpr bool HEADS_FIRST = HEADS_FIRST_, BACK = BACK_, TURNED = TURNED_;
+  static constexpr int PARTS = T::kNarrowRange ? 2 : 1, D = D_, E = E_, CT = CT_, NW = NW_, H = H_, HA = HA_, HB = HB_, HC = HC_;
+  static constexpr bool TIGHT = TIGHT_, REST = REST_ || T::kNarrowRange, HEADS_FIRST = HEADS_FIRST_, BACK = BACK_, TURNED = TURNED_;
   static constexpr Result RESULT = RESULT_;
   static constexpr int kChunk = 32 * CT, kColumns = 32 * NW, kTiles = (E + kColumns - 1) / kColumns;
 };
 
-// Tiles of a chunk, and its masked products as operands. STATES: what a walk over states alone needs.
-template <typename C, bool STATES>
-struct Set {
-  u8 b[C::PARTS][C::kChunk * pitch(C::D)], c[C::PARTS][C::kChunk * pitch(C::kColumns)], a[STATES ? 0 : C::PARTS][C::kChunk * pitch(C::D)];
-};
+// Tiles of a few chunks, and masked products as operands. STATES: what a walk over states alone needs.
 template <typename C, bool STATES>
 struct Lds {
   static constexpr int kPairs = C::CT * (C::CT + 1) / 2;   // 32 x 32 tiles of the masked products
-  Set<C, STATES> sets[C::SETS];
-  u32x4 pairs[STATES ? 0 : C::PARTS][kPairs][2][64];
+  static constexpr int kA = C::TIGHT ? 1 : 2, kB = C::TIGHT ? 1 : 3;
+  u8 b[kB][C::PARTS][C::kChunk * pitch(C::D)], c[kB][C::PARTS][C::kChunk * pitch(C::kColumns)], a[STATES ? 0 : kA][C::PARTS][C::kChunk * pitch(C::D)];
+  u32x4 pairs[STATES ? 0 : kA][C::PARTS][kPairs][2][64];
 };
 
 // Where the tokens of one head of a tensor with X heads of W channels of 2 bytes lie.
@@ -225,66 +239,101 @@ AKG_DEV long entry_of(const int *slots, long b, long pool) {
 
 // One segment of one head, 32 NW channels of c. STATES: only what the segment adds to a state.
 //
-// NW wavefronts hold the state and do what needs it. As many others fetch: two chunks ahead into registers, from there to LDS
-// (float16 in parts), and compute the masked products, the first of two steps of a chunk, beside a . S; in the second, beside the
-// products with c, they put the next chunk's tiles in place. (With both in the same wavefronts, one behind the other, a chunk
-// of 64 tokens of 128 channels took 3.3 us whatever was fetched ahead, since registers left no room to read operands ahead.)
+// NW wavefronts hold the state and do what needs it. Four others fetch into registers, two chunks ahead of what they put into
+// LDS (float16 in parts), and compute the masked products. Between two barriers the first have what chunk t adds to the state, its
+// masked products with c, and a . S of chunk t + 1; the others the masked products of t + 1, and a, b and c of t + 2 to put in
+// place of tiles that nothing reads any more. TIGHT: one after the other.
 template <typename C, bool STATES>
 AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int seg) {
-  constexpr int D = C::D, E = C::E, PARTS = C::PARTS, CT = C::CT, NW = C::NW, SETS = C::SETS, kChunk = C::kChunk, kThreads = 64 * NW;
+  constexpr int D = C::D, E = C::E, PARTS = C::PARTS, CT = C::CT, NW = C::NW, kChunk = C::kChunk, kThreads = 64 * kHelpers;
   constexpr int kUnits = padded(D) / 32, kSteps = 2 * CT, kAfter = C::BACK ? 1 : 0;
+  constexpr int kTerms = C::REST ? 2 : 1;   // parts of what is added to the state
+  constexpr bool TIGHT = C::TIGHT;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const long b = head / C::H;
   const int h = static_cast<int>(head % C::H), e0 = tile * C::kColumns;
   const long len = length_of(w.lengths, b, w.seq);
   const long from = static_cast<long>(seg) * w.segment, upto = from + w.segment < w.seq ? from + w.segment : w.seq, end = upto < len ? upto : len;
+  const int chunks = end > from ? static_cast<int>((end - from + kChunk - 1) / kChunk) : 0;
   const float g = w.log_decay[h], g2 = g * kLog2e;
-  auto count_at = [&](long r0) { return static_cast<int>(end - r0 < kChunk ? (end > r0 ? end - r0 : 0) : kChunk); };
+  auto count_of = [&](int t) {
+    const long left = end - from - static_cast<long>(t) * kChunk;
+    return static_cast<int>(left < kChunk ? (left > 0 ? left : 0) : kChunk);
+  };
   // the lowest of the tokens of a chunk, whose last rows they are
-  auto lowest_at = [&](long r0, int n) { return C::BACK ? len - r0 - n : r0; };
+  auto lowest_of = [&](int t, int n) {
+    const long r0 = from + static_cast<long>(t) * kChunk;
+    return C::BACK ? len - r0 - n : r0;
+  };
   const Places<D> pd(lane);
 
   if (wave >= NW) {
-    const int tid = static_cast<int>(threadIdx.x) - kThreads, helper = wave - NW;
+    const int tid = static_cast<int>(threadIdx.x) - 64 * NW, helper = wave - NW;
     const Tokens<C::HA, D, C::HEADS_FIRST, C::H> ta(w.a, b, h, w.seq);
     const Tokens<C::HB, D, C::HEADS_FIRST, C::H> tb(w.b, b, h, w.seq);
     const Tokens<C::HC, E, C::HEADS_FIRST, C::H> tc(w.c, b, h, w.seq);
-    Stage<kChunk, D, kThreads, PARTS> sa[2], sb[2];
-    Stage<kChunk, C::kColumns, kThreads, PARTS> sc[2];
-    auto fetch = [&](int to, long r0) {   // (behind the end: nothing is asked of memory)
-      const int n = count_at(r0);
-      const long first = lowest_at(r0, n);
-      if constexpr (!STATES) sa[to].template load<C::BACK>(ta.base + first * ta.step, ta.step, n, D, tid);
-      sb[to].template load<C::BACK>(tb.base + first * tb.step, tb.step, n, D, tid);
-      sc[to].template load<C::BACK>(tc.base + first * tc.step + 2 * e0, tc.step, n, E - e0 < C::kColumns ? E - e0 : C::kColumns, tid);
+    const int channels = E - e0 < C::kColumns ? E - e0 : C::kColumns;
+    typedef Stage<kChunk, D, kThreads, PARTS> StageD;
+    typedef Stage<kChunk, C::kColumns, kThreads, PARTS> StageE;
+    StageD sa[2], sb[2];
+    StageE sc[2];
+    // Piece i of all pieces of chunk t's tiles (behind the last chunk nothing is asked of memory).
+    constexpr int kPiecesA = STATES ? 0 : StageD::kEach, kPieces = kPiecesA + StageD::kEach + StageE::kEach;
+    struct Sources {
+      Rows<kChunk, C::BACK> a, b, c;
     };
-    auto place = [&](int x) {
-      Set<C, STATES> &set = lds.sets[x % SETS];
-      if constexpr (!STATES) sa[x].store(set.a[0], tid);
-      sb[x].store(set.b[0], tid);
-      sc[x].store(set.c[0], tid);
+    auto sources = [&](int t) {
+      const int n = count_of(t);
+      const long first = lowest_of(t, n);
+      return Sources{Rows<kChunk, C::BACK>(ta.base + first * ta.step, ta.step, n, D), Rows<kChunk, C::BACK>(tb.base + first * tb.step, tb.step, n, D),
+                     Rows<kChunk, C::BACK>(tc.base + first * tc.step + 2 * e0, tc.step, n, channels)};
+    };
+    auto fetch_piece = [&](int to, const Sources &from_, int i) {
+      if (i < kPiecesA) {
+        sa[to].load(from_.a, i, tid);
+      } else if (i < kPiecesA + StageD::kEach) {
+        sb[to].load(from_.b, i - kPiecesA, tid);
+      } else {
+        sc[to].load(from_.c, i - kPiecesA - StageD::kEach, tid);
+      }
+    };
+    auto fetch = [&](int to, int t) {
+      const Sources from_ = sources(t);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) fetch_piece(to, from_, i);
+    };
+    auto place = [&](int held, int ia, int ib) {
+      if constexpr (!STATES) sa[held].store(lds.a[ia][0], tid);
+      sb[held].store(lds.b[ib][0], tid);
+      sc[held].store(lds.c[ib][0], tid);
     };
     // Weights of the masked products (register r: key token 8 (r / 4) + 4 half + r % 4 of its 32, query token lane % 32). Pairs
-    // of tiles (query tile, key tile): 0 = (0, 0), 1 = (1, 0), 2 = (1, 1).
+    // of tiles (query tile, key tile): 0 = (0, 0), 1 = (1, 0), 2 = (1, 1), one to a wavefront.
+    constexpr int kPairs = CT * (CT + 1) / 2;
+    const int qt = helper > 0 ? 1 : 0, kt = helper > 1 ? 1 : 0;
     float mask[16];
     if constexpr (!STATES) {
-      const int apart = CT == 2 && helper == 1 ? 32 : 0;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int n = apart + (lane & 31) - (8 * (r >> 2) + 4 * half + (r & 3));
+        const int n = 32 * (qt - kt) + (lane & 31) - (8 * (r >> 2) + 4 * half + (r & 3));
         mask[r] = n < 0 ? 0.0f : power(g2, n) * w.scale;
       }
     }
-    auto pair = [&](const Set<C, STATES> &set, int which) {
-      const int qt = which > 0 ? 1 : 0, kt = which > 1 ? 1 : 0;
+    // ..., and the pieces of chunk t meanwhile
+    auto multiply = [&](int ia, int ib, int to, int t) {
+      if (STATES || helper >= kPairs) {
+        fetch(to, t);
+        return;
+      }
+      const Sources from_ = sources(t);
       f32x16 s = {};
-      constexpr int kAhead = 3;
+      constexpr int kAhead = 4;
       u32x4 keys[2 * kUnits][PARTS], queries[2 * kUnits][PARTS];
       auto read = [&](int x) {
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-          keys[x][p] = pd.row(set.b[p], 32 * kt, x);
-          queries[x][p] = pd.row(set.a[p], 32 * qt, x);
+          keys[x][p] = pd.row(lds.b[ib][p] + 32 * pitch(D) * kt, 0, x);
+          queries[x][p] = pd.row(lds.a[ia][p] + 32 * pitch(D) * qt, 0, x);
         }
       };
 #pragma unroll
@@ -294,66 +343,69 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
         __builtin_amdgcn_sched_barrier(0);
         s = product(keys[x], queries[x], s);
         if (x + kAhead < 2 * kUnits) read(x + kAhead);
+#pragma unroll
+        for (int i = x * kPieces / (2 * kUnits); i < (x + 1) * kPieces / (2 * kUnits); ++i) fetch_piece(to, from_, i);
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         float v[8];
         // (on the diagonal: where the weight is 0 the product does not count, whatever it is)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = which != 1 && mask[8 * x + e] == 0.0f ? 0.0f : s[8 * x + e] * mask[8 * x + e];
+        for (int e = 0; e < 8; ++e) v[e] = qt == kt && mask[8 * x + e] == 0.0f ? 0.0f : s[8 * x + e] * mask[8 * x + e];
         u32x4 parts[PARTS];
         split<PARTS>(v, parts);
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) lds.pairs[p][which][x][lane] = parts[p];
+        for (int p = 0; p < PARTS; ++p) lds.pairs[ia][p][helper][x][lane] = parts[p];
       }
     };
-    auto multiply = [&](const Set<C, STATES> &set) {
-      if (helper == 0) pair(set, 0);
-      if constexpr (CT == 2) {
-        if (helper == 1) pair(set, 1);
-        if (helper == (NW > 2 ? 2 : 0)) pair(set, 2);
-      }
-    };
-    if (from < end) {
-      fetch(0, from);
-      fetch(1, from + kChunk);
+    if (chunks > 0) {
+      fetch(0, 0);
+      fetch(1, 1);
+      typedef Lds<C, STATES> L;
 #pragma unroll
-      for (int x = 0; x < SETS; ++x) {
+      for (int p = 0; p < PARTS; ++p) {
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-          if constexpr (!STATES) attn::clear_padding<kChunk, D, kThreads>(lds.sets[x].a[p], tid);
-          attn::clear_padding<kChunk, D, kThreads>(lds.sets[x].b[p], tid);
+        for (int x = 0; x < L::kB; ++x) clear_padding<kChunk, D, kThreads>(lds.b[x][p], tid);
+#pragma unroll
+        for (int x = 0; x < L::kA; ++x) {
+          if constexpr (!STATES) clear_padding<kChunk, D, kThreads>(lds.a[x][p], tid);
         }
       }
-      place(0);
-      fetch(0, from + 2 * kChunk);
-      __syncthreads();
-      if constexpr (!STATES) {
-        multiply(lds.sets[0]);
+      place(0, 0, 0);
+      if constexpr (TIGHT) {
+        __syncthreads();
+        multiply(0, 0, 0, 2);
+      } else {
+        fetch(0, 2);
+        place(1, 1, 1);
+        __syncthreads();
+        multiply(0, 0, 1, 3);
+      }
+      if constexpr (!STATES) __syncthreads();
+    }
+    // Beside chunk t; `k`: t mod 2.
+    int third = 1;   // t + 1 mod 3
+    auto beside = [&](auto k, int t) {
+      constexpr int K = decltype(k)::value;
+      if (t + 1 >= chunks) return;
+      if constexpr (TIGHT) {
+        __syncthreads();   // (the tiles have been read)
+        place(1 - K, 0, 0);
+        __syncthreads();
+        multiply(0, 0, 1 - K, t + 3);
+        if constexpr (!STATES) __syncthreads();
+      } else {
+        const int then = third + 1 < 3 ? third + 1 : 0;
+        place(K, K, then);
+        multiply(1 - K, third, K, t + 4);
+        third = then;
         __syncthreads();
       }
-    }
-    // Beside chunk r0: the next one, which is held in `k`.
-    auto chunk = [&](auto k, long r0) {
-      constexpr int K = decltype(k)::value;
-      const bool more = r0 + kChunk < end;
-      if constexpr (SETS == 1) {
-        if constexpr (!STATES) __syncthreads();
-        if (!more) return;
-        __syncthreads();   // (the tiles have been read)
-      }
-      if (more) {
-        place(K);
-        fetch(K, r0 + 3L * kChunk);
-      }
-      if (!STATES || more) __syncthreads();
-      if (STATES || !more) return;
-      multiply(lds.sets[K % SETS]);
-      __syncthreads();
     };
-    for (long r0 = from; r0 < end; r0 += 2 * kChunk) {
-      chunk(attn::IntTag<1>(), r0);
-      if (r0 + kChunk < end) chunk(attn::IntTag<0>(), r0 + kChunk);
+    for (int t = 0; t < chunks; t += 2) {
+      beside(attn::IntTag<0>(), t);
+      beside(attn::IntTag<1>(), t + 1);
     }
     if constexpr (!STATES && C::RESULT != Result::None) {   // rows behind the length: zeros
       constexpr bool kFloat = C::RESULT == Result::Float;
@@ -405,123 +457,113 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
       shown[i] = row < 0 ? 0.0f : power(g2, row + 1 - kAfter) * show;
     }
   };
-  weigh(kChunk);
-
+  weigh(count_of(0));
   const Places<C::kColumns> pc(lane);
-  if (from < end) {   // (the first tiles are in place, and their masked products)
-    __syncthreads();
+
+  // Matrix instructions one by one, each with its share of what stands beside it: operands of later ones read from LDS,
+  // values of later ones rounded or weighted. (The barriers keep that order: left to itself the compiler reads an operand in
+  // front of its use and waits.)
+  f32x16 out[CT];
+  constexpr bool kWide = kUnits > 4;   // (the state leaves few registers to read ahead)
+  constexpr int kAll = 2 * kUnits * CT, kAhead = kWide ? 3 : 6;
+  u32x4 queries[kAll][PARTS];
+  auto query = [&](int ia, int y) {
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) queries[y][p] = pd.row(lds.a[ia][p], 32 * (y % CT), y / CT);
+  };
+  constexpr int kGroup = !kWide ? kUnits : kUnits % 2 == 0 ? 2 : 1, kPasses = PARTS + kTerms - 1;   // units of the state at a time
+  constexpr int kAllKeys = kSteps * kUnits, kKeysAhead = kWide ? 3 : kPasses == 1 && 2 * kGroup <= kAllKeys ? 2 * kGroup : kGroup;
+  u32x4 values[kSteps][PARTS], more[kSteps][kTerms], keys[kAllKeys][PARTS];
+  auto key = [&](int ib, int x) {
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) keys[x][p] = pd.transposed(lds.b[ib][p], 16 * (x / kUnits), x % kUnits);
+  };
+  // (pair e of the eight values of step s)
+  auto weighted = [&](int s, int e) {
+    float lo = BF16::low(values[s][0][e]), hi = BF16::high(values[s][0][e]);
+    if constexpr (PARTS == 2) {
+      lo += BF16::low(values[s][1][e]);
+      hi += BF16::high(values[s][1][e]);
+    }
+    split_pair<kTerms>(lo * (added[2 * e] * steps[s]), hi * (added[2 * e + 1] * steps[s]), more[s], e);
+  };
+  // What chunk ib's part of the state begins with.
+  auto ready = [&](int ib) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) values[s][p] = pc.transposed(lds.c[ib][p], 16 * s, wave);
+    }
+#pragma unroll
+    for (int x = 0; x < kKeysAhead; ++x) key(ib, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) weighted(0, e);
+  };
+  // a . S with the first kAhead operands read already; the state fades behind its use
+  auto through = [&](int ia) {
+#pragma unroll
+    for (int i = 0; i < CT; ++i) out[i] = {};
+    u32x4 parts[2 * kUnits][PARTS];
+    // (pair e of the eight rows x)
+    auto rounded = [&](int x, int e) {
+      const int r = 8 * (x & 1) + 2 * e;
+      const float lo = state[x >> 1][r], hi = state[x >> 1][r + 1];
+      split_pair<PARTS>(lo, hi, parts[x], e);
+      state[x >> 1][r] = __builtin_fmaf(lo, fade, lo);
+      state[x >> 1][r + 1] = __builtin_fmaf(hi, fade, hi);
+    };
+#pragma unroll
+    for (int e = 0; e < 4; ++e) rounded(0, e);
+#pragma unroll
+    for (int y = 0; y < kAll; ++y) {
+      __builtin_amdgcn_sched_barrier(0);
+      const int x = y / CT, i = y % CT;
+      out[i] = product(parts[x], queries[y], out[i]);
+      if (y + kAhead < kAll) query(ia, y + kAhead);
+      if (x + 1 < 2 * kUnits) {
+#pragma unroll
+        for (int e = i * 4 / CT; e < (i + 1) * 4 / CT; ++e) rounded(x + 1, e);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (chunks > 0) {
+    __syncthreads();   // (the first tiles are in place)
+    if constexpr (!STATES) {
+#pragma unroll
+      for (int y = 0; y < kAhead && y < kAll; ++y) query(0, y);
+      through(0);
+    }
+    ready(0);
     if constexpr (!STATES) __syncthreads();
   }
-  int at = 0;   // the set
-  for (long r0 = from; r0 < end; r0 += kChunk) {
-    const int n = count_at(r0);
-    const Set<C, STATES> &set = lds.sets[at];
-    at = at + 1 < SETS ? at + 1 : 0;
-    if (n != kChunk) weigh(n);
-    // Matrix instructions one by one, each with its share of what stands beside it: operands of later ones read from LDS,
-    // values of later ones rounded or weighted. (The barriers keep that order: left to itself the compiler reads an operand in
-    // front of its use and waits.)
-    f32x16 out[CT];
-    constexpr int kGroup = kUnits == 8 ? 4 : kUnits == 6 ? 3 : kUnits;   // units of the state at a time
-    u32x4 values[kSteps][PARTS], more[kSteps][2], keys[kSteps * kUnits][PARTS];
-    auto value = [&](int s) {
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p) values[s][p] = pc.transposed(set.c[p], 16 * s, wave);
-    };
-    auto key = [&](int x) {
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p) keys[x][p] = pd.transposed(set.b[p], 16 * (x / kUnits), x % kUnits);
-    };
-    // (pair e of the eight values of step s)
-    auto weighted = [&](int s, int e) {
-      float lo = BF16::low(values[s][0][e]), hi = BF16::high(values[s][0][e]);
-      if constexpr (PARTS == 2) {
-        lo += BF16::low(values[s][1][e]);
-        hi += BF16::high(values[s][1][e]);
-      }
-      split_pair<2>(lo * (added[2 * e] * steps[s]), hi * (added[2 * e + 1] * steps[s]), more[s], e);
-    };
+  int third = 0;   // t mod 3
+  for (int t = 0; t < chunks; ++t) {
+    const int n = count_of(t), ia = TIGHT ? 0 : t & 1, ib = TIGHT ? 0 : third;
+    third = third + 1 < 3 ? third + 1 : 0;
+    u32x4 pairs[kSteps][CT][PARTS];
     if constexpr (!STATES) {
-      // a . S; the state fades behind its use
-#pragma unroll
-      for (int i = 0; i < CT; ++i) out[i] = {};
-      constexpr int kAll = 2 * kUnits * CT, kAhead = 6;
-      u32x4 queries[kAll][PARTS], parts[2 * kUnits][PARTS], pairs[kSteps][CT][PARTS];
-      auto query = [&](int y) {
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) queries[y][p] = pd.row(set.a[p], 32 * (y % CT), y / CT);
-      };
-      // (pair e of the eight rows x)
-      auto rounded = [&](int x, int e) {
-        const int r = 8 * (x & 1) + 2 * e;
-        const float lo = state[x >> 1][r], hi = state[x >> 1][r + 1];
-        split_pair<PARTS>(lo, hi, parts[x], e);
-        state[x >> 1][r] = __builtin_fmaf(lo, fade, lo);
-        state[x >> 1][r + 1] = __builtin_fmaf(hi, fade, hi);
-      };
-#pragma unroll
-      for (int y = 0; y < kAhead && y < kAll; ++y) query(y);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) rounded(0, e);
-#pragma unroll
-      for (int y = 0; y < kAll; ++y) {
-        __builtin_amdgcn_sched_barrier(0);
-        const int x = y / CT, i = y % CT;
-        out[i] = product(parts[x], queries[y], out[i]);
-        if (y + kAhead < kAll) query(y + kAhead);
-        if (x + 1 < 2 * kUnits) {
-#pragma unroll
-          for (int e = i * 4 / CT; e < (i + 1) * 4 / CT; ++e) rounded(x + 1, e);
-        }
-      }
-      // ... and the masked products with c
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        value(s);
-#pragma unroll
-        for (int i = s / 2; i < CT; ++i) {
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p) pairs[s][i][p] = lds.pairs[p][i == 0 ? 0 : 1 + s / 2][s & 1][lane];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < CT; ++i) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) out[i][r] *= shown[i];
-      }
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
         for (int i = s / 2; i < CT; ++i) {
-          __builtin_amdgcn_sched_barrier(0);
-          out[i] = product(values[s], pairs[s][i], out[i]);
-          if (s == 0 && i == 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) weighted(0, e);
-          }
+          for (int p = 0; p < PARTS; ++p) pairs[s][i][p] = lds.pairs[ia][p][i == 0 ? 0 : 1 + s / 2][s & 1][lane];
         }
       }
-#pragma unroll
-      for (int u = 0; u < kGroup; ++u) key(u);
-      __syncthreads();
     } else {
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) value(s);
-#pragma unroll
-      for (int u = 0; u < kGroup; ++u) key(u);
+      if (n != kChunk) weigh(n);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) state[u][r] = __builtin_fmaf(state[u][r], fade, state[u][r]);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) weighted(0, e);
     }
     // a result in float32 is one of the walk's own heads, heads first
     constexpr bool kFloat = C::RESULT == Result::Float, kShow = !STATES && C::RESULT != Result::None;
     constexpr int kSize = kFloat ? 4 : 2;
     const Tokens<C::H, E, kFloat || C::HEADS_FIRST, C::H> to(w.out, b, h, w.seq, kSize);
-    const Buffer buf = make_buffer(to.base + lowest_at(r0, n) * to.step, kShow ? records((n - 1) * to.step + static_cast<long>(kSize) * E) : 0);
+    const Buffer buf = make_buffer(to.base + lowest_of(t, n) * to.step, kShow ? records((n - 1) * to.step + static_cast<long>(kSize) * E) : 0);
     // (half x of query tile i: 16 channels of a row in a pair of lanes)
     auto write = [&](int i, int x) {
       const int row = 32 * i + (lane & 31), behind = C::BACK ? kChunk - 1 - row : row - (kChunk - n), d = e0 + 32 * wave + 16 * x + 8 * half;
@@ -541,9 +583,9 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
         __builtin_amdgcn_raw_buffer_store_b128(v, buf, off, 0, 0);
       }
     };
-    // What c adds to the state: a few units at a time, first the products with the rests; the keys of the units behind them are
-    // read meanwhile, the next tokens weighted, the rows of the result written.
-    constexpr int kPasses = PARTS + 1, kGroups = kSteps * kUnits / kGroup;
+    // What c adds to the state: a few units at a time, first the products with the rests; keys are read ahead, the next tokens
+    // weighted. Behind the first units: the masked products with c, then row by row of the result.
+    constexpr int kGroups = kAllKeys / kGroup;
 #pragma unroll
     for (int q = 0; q < kGroups; ++q) {
       const int s = q * kGroup / kUnits, u0 = q * kGroup % kUnits;
@@ -552,30 +594,63 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
 #pragma unroll
         for (int v = 0; v < kGroup; ++v) {
           __builtin_amdgcn_sched_barrier(0);
-          const int u = u0 + v;
-          state[u] = BF16::mma(keys[q * kGroup + v][PARTS == 2 && pass == 1 ? 1 : 0], more[s][pass == 0 ? 1 : 0], state[u]);
-          if (pass == 0 && q + 1 < kGroups) key((q + 1) * kGroup + v);
+          const int u = u0 + v, x = q * kGroup + v;
+          state[u] = BF16::mma(keys[x][PARTS == 2 && pass == 1 ? 1 : 0], more[s][kTerms == 2 && pass == 0 ? 1 : 0], state[u]);
+          if (pass == 0 && x + kKeysAhead < kAllKeys) key(ib, x + kKeysAhead);
           if (u0 == 0 && pass + 1 == kPasses && s + 1 < kSteps) {
 #pragma unroll
             for (int e = v * 4 / kGroup; e < (v + 1) * 4 / kGroup; ++e) weighted(s + 1, e);
           }
-          if constexpr (kShow) {
-            if (pass == kPasses - 2 && v == 0) {
+          if constexpr (!STATES) {
+            if (q == 0 && pass == 0) {
 #pragma unroll
-              for (int y = q * 2 * CT / kGroups; y < (q + 1) * 2 * CT / kGroups; ++y) write(y / 2, y % 2);
+              for (int r = v * 16 * CT / kGroup; r < (v + 1) * 16 * CT / kGroup; ++r) out[r / 16][r % 16] *= shown[r / 16];
+            }
+          }
+          if constexpr (kShow) {
+            if (q > 0 && pass == 0 && v == 0) {
+#pragma unroll
+              for (int y = (q - 1) * 2 * CT / (kGroups - 1); y < q * 2 * CT / (kGroups - 1); ++y) write(y / 2, y % 2);
+            }
+          }
+          if constexpr (!STATES && !TIGHT) {   // (of the next chunk's a; behind the last one nothing uses them)
+            if (q + 1 == kGroups && pass + 1 == kPasses && v == 0) {
+#pragma unroll
+              for (int y = 0; y < kAhead && y < kAll; ++y) query(1 - ia, y);
+            }
+          }
+        }
+      }
+      if constexpr (!STATES) {
+        if (q == 0) {
+#pragma unroll
+          for (int z = 0; z < kSteps; ++z) {
+#pragma unroll
+            for (int i = z / 2; i < CT; ++i) {
+              __builtin_amdgcn_sched_barrier(0);
+              out[i] = product(values[z], pairs[z][i], out[i]);
             }
           }
         }
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (r0 + kChunk < end) {
-      if constexpr (SETS == 1) {
-        __syncthreads();
-        if constexpr (!STATES) __syncthreads();
-      }
-      __syncthreads();   // (the next chunk's tiles are in place, and their masked products)
+    if (t + 1 >= chunks) break;
+    if constexpr (TIGHT) {
+      __syncthreads();
+      __syncthreads();   // (the next chunk's tiles are in place)
     }
+    if constexpr (!STATES) {
+      const int then = count_of(t + 1);
+      if (then != kChunk) weigh(then);
+      if constexpr (TIGHT) {
+#pragma unroll
+        for (int y = 0; y < kAhead && y < kAll; ++y) query(0, y);
+      }
+      through(TIGHT ? 0 : 1 - ia);
+    }
+    ready(TIGHT ? 0 : third);
+    if constexpr (!STATES || !TIGHT) __syncthreads();
   }
 
   // a walk over states leaves them in the workspace; else the segment that holds the last token has the last state
@@ -610,15 +685,24 @@ AKG_DEV void scan(const Walk &w, long heads, long at) {
     for (int e = 0; e < 4; ++e) start[e] = given[C::TURNED ? (x % E + e) * D + x / E : x + e];   // (E is a multiple of 4)
   }
   float *to = w.starts + head * w.segments * (static_cast<long>(D) * E) + x;
-  for (int s = 0; s < w.segments; ++s, to += D * E) {
-    const long left = len - static_cast<long>(s) * w.segment;
-    const int n = left <= 0 ? 0 : left < w.segment ? static_cast<int>(left) : w.segment;
-    f32x4 add = {};
-    if (s + 1 < w.segments) __builtin_memcpy(&add, to, 16);
-    __builtin_memcpy(to, &start, 16);
-    const float fade = power(g2, n);
+  constexpr int kAtOnce = 8;   // (asked for together: one behind the other 16 segments of 16 states of 128 x 128 took 16 us)
+  for (int s0 = 0; s0 < w.segments; s0 += kAtOnce) {
+    f32x4 add[kAtOnce];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) start[e] = __builtin_fmaf(start[e], fade, add[e]);
+    for (int k = 0; k < kAtOnce; ++k) {
+      add[k] = f32x4{};
+      if (s0 + k + 1 < w.segments) __builtin_memcpy(&add[k], to + static_cast<long>(s0 + k) * (D * E), 16);
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (s0 + k >= w.segments) break;
+      const long left = len - static_cast<long>(s0 + k) * w.segment;
+      const int n = left <= 0 ? 0 : left < w.segment ? static_cast<int>(left) : w.segment;
+      __builtin_memcpy(to + static_cast<long>(s0 + k) * (D * E), &start, 16);
+      const float fade = power(g2, n);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) start[e] = __builtin_fmaf(start[e], fade, add[k][e]);
+    }
   }
 }
 

@@ -329,7 +329,7 @@ def test_without_allocations_and_at_odd_addresses(tmp_path):
 
 @pytest.mark.gpu
 def test_fewer_segments_without_allocations(tmp_path):
-    t = make(("bfloat16", "BSND", 1, 8192, 16, 16, 128, 128, "slow", True, None))
+    t = make(("bfloat16", "BSND", 1, 4096, 8, 8, 256, 256, "slow", True, None))
     text, inputs = describe(t, "BSND")
     kernel = driver.HipKernel(text, out_dir=str(tmp_path))
     assert kernel.workspace_bytes > 16 << 20 and "_within" in kernel.source
