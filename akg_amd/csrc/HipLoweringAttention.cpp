@@ -22,7 +22,9 @@ namespace {
 using lowering::dtypeTag;
 
 int64_t ceilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-constexpr int64_t kFewTokens = 8;   // up to which linear attention goes token after token
+// Tokens up to which linear attention goes token after token: us that way, in chunks: 16 x 2, 4, 8, 12 of 16/4 heads of 64, float16,
+// 4.6, 4.8, 6.2, 7.9 and 6.1; 16 x 2, 4, 8, 16 of 32 heads of 128 12.8, 14.7, 18.1, 24.9 and 21.4, 21.5, 21.7, 22.2.
+constexpr int64_t kFewTokens = 8;
 
 class LayerEmitter {
  public:
@@ -576,9 +578,9 @@ class LayerEmitter {
     if (s.seq >= (1LL << 31) - 8192) throw LoweringError("op " + op_.name + ": more than 2^31 tokens");
     return s;
   }
-  std::string walkConfig(const WalkOf &w, const LinearSizes &s, int ct, int64_t nw, bool tight) const {
+  std::string walkConfig(const WalkOf &w, const LinearSizes &s, int ct, int64_t nw, int helpers, bool tight) const {
     std::ostringstream o;
-    o << "akg::linear::Config<" << trait() << ", " << w.d << ", " << w.e << ", " << ct << ", " << nw << ", " << flag(tight) << ", " << flag(w.rest) << ", " << s.heads << ", " << w.ha << ", " << w.hb << ", " << w.hc
+    o << "akg::linear::Config<" << trait() << ", " << w.d << ", " << w.e << ", " << ct << ", " << nw << ", " << helpers << ", " << flag(tight) << ", " << flag(w.rest) << ", " << s.heads << ", " << w.ha << ", " << w.hb << ", " << w.hc
       << ", " << flag(l_.headsFirst) << ", " << flag(w.back) << ", " << flag(w.turned) << ", akg::linear::Result::" << w.result << ">";
     return o.str();
   }
@@ -618,7 +620,7 @@ class LayerEmitter {
     for (int64_t nw = std::min<int64_t>(units, 4); nw >= 1; --nw) {
       if (nw > 2 && nw != ceilDiv(units, ceilDiv(units, 4))) continue;
       // Tiles of a few chunks (linear::Lds, linear::pitch) where LDS holds them, of chunks of 32 tokens before those of one chunk only.
-      auto pitchOf = [](int64_t d) { return ceilDiv(d, 32) * 64 + 32; };
+      auto pitchOf = [](int64_t d) { return d <= 32 ? 64 : d <= 64 ? 128 : d <= 128 ? 256 : 512; };
       auto ldsBytes = [&](int64_t tiles) { return parts * (32 * tiles * (5 * pitchOf(deepest) + 3 * pitchOf(32 * nw)) + 2 * 2048 * (tiles * (tiles + 1) / 2)); };
       int ct = parts == 2 || ldsBytes(2) > 160 * 1024 ? 1 : 2;
       const bool tight = ldsBytes(ct) > 160 * 1024;
@@ -653,11 +655,13 @@ class LayerEmitter {
     while (limit_ > 0 && segments > 1 && space + 4 * s.states * segments * values > limit_) --segments;
     const int64_t chunk = 32 * ct, segment = ceilDiv(ceilDiv(s.seq, segments), chunk) * chunk;
     segments = ceilDiv(s.seq, segment);
+    // Two wavefronts that fetch instead of four where two workgroups to a CU are then resident (gradient of 8 x 200 tokens of 12 heads
+    // of 64, float16: 16.7 us instead of 22.6; 8 x 77 with a workgroup a CU 7.5 instead of 7.2).
+    int helpers = nw <= 2 && deepest <= 64 && groups * segments > cus_ ? 2 : 4;
     k_.scalarArgs = {s.batch, s.seq, segment, segments};
     if (l_.hasSlots) k_.scalarArgs.push_back(in(4).shape[0]);
-    std::vector<std::string> names;
-    o << "typedef " << walkConfig(all[0], s, ct, nw, tight) << " akg_C0;\n";
-    for (size_t i = 1; i < all.size(); ++i) o << "typedef " << walkConfig(all[i], s, ct, nw, tight) << " akg_C" << i << ";\n";
+    o << "typedef " << walkConfig(all[0], s, ct, nw, helpers, tight) << " akg_C0;\n";
+    for (size_t i = 1; i < all.size(); ++i) o << "typedef " << walkConfig(all[i], s, ct, nw, helpers, tight) << " akg_C" << i << ";\n";
     o << "\n";
     int64_t before = space;
     std::vector<std::string> structs;
@@ -670,7 +674,7 @@ class LayerEmitter {
       structs.push_back(b.str());
       before += 4 * s.heads * w.d * w.e;
     }
-    const int threads = static_cast<int>(64 * (nw + 4));   // (linear::kHelpers)
+    const int threads = static_cast<int>(64 * (nw + helpers));
     int hint = 2;
     // A head's workgroups are neighbours on one XCD, whose L2 they share: the walks of a gradient read the same tensors, those
     // backward in time at the same time.
@@ -678,7 +682,7 @@ class LayerEmitter {
     for (const WalkOf &w : all) tiles += w.tiles;
     auto body = [&](bool states) {
       std::ostringstream b;
-      b << "  const int akg_parts = static_cast<int>(akg_segments" << (states ? " - 1" : "") << ");\n  __shared__ __attribute__((aligned(16))) akg::u8 akg_lds[";
+      b << "  const int akg_parts = static_cast<int>(akg_segments" << (states ? " - 1" : "") << ");\n  __shared__ __attribute__((aligned(256))) akg::u8 akg_lds[";
       auto lds = [&](size_t i) { return "akg::linear::Lds<akg_C" + std::to_string(i) + ", " + flag(states) + ">"; };
       std::string size = "sizeof(" + lds(0) + ")";
       for (size_t i = 1; i < all.size(); ++i) {

@@ -43,14 +43,15 @@ using attn::records;
 using attn::u32x2;
 using attn::u32x4;
 
-// A tile of W channels in LDS: rows an odd multiple of 32 bytes apart, so that four neighbouring rows of 32 bytes (transposed
-// reads, sixteen lanes at a time) and eight of 16 bytes lie in banks of their own; chunks of 16 bytes change places in pairs in every
-// second eight rows, so that sixteen of 16 bytes do (rows read by 128 bits, sixteen lanes at a time). (The tiles of
-// akg_attention.hpp have 64 bytes more a row instead of 32: three chunks' tiles would not fit.)
-constexpr int pitch(int w) { return padded(w) * 2 + 32; }
+// A tile of W channels in LDS: rows of 64, 128, 256 or 512 bytes without any between them, whose chunks of 16 bytes change places
+// by exclusive or with bits of the row. Four neighbouring rows of 64 bytes (transposed reads, half a wavefront at a time) and
+// sixteen of 16 bytes (rows read by 128 bits) then lie in banks of their own. The places of a lane differ by an exclusive or with
+// a constant. (With 32 and 64 bytes more a row instead, transposed reads met in the banks, or three chunks' tiles did not fit.)
+constexpr int pitch(int w) { return w <= 32 ? 64 : w <= 64 ? 128 : w <= 128 ? 256 : 512; }
+constexpr int turn(int w, int row) { return (w <= 32 ? 0 : w <= 64 ? (row & 2) << 1 : (row & 3) << 2) | ((row >> 2) & 3); }
 template <int W>
 AKG_DEV int chunk_at(int row, int chunk) {
-  return row * pitch(W) + ((chunk ^ ((row >> 3) & 1)) << 4);
+  return row * pitch(W) + ((chunk ^ turn(W, row)) << 4);
 }
 // The channels behind W of a tile's rows (to the next multiple of 32) hold zeros: written once, never again.
 template <int ROWS, int W, int THREADS>
@@ -103,7 +104,8 @@ AKG_DEV f32x16 product(const u32x4 (&a)[PA], const u32x4 (&b)[PB], f32x16 c) {
   return BF16::mma(a[0], b[0], c);
 }
 
-// A lane's places in a tile of W channels (as attn::Reader, with the quads of transposed reads swapped).
+// A lane's places in a tile of W channels (as attn::Reader, with the quads of transposed reads swapped). A tile lies `tile` bytes
+// behind `lds`, both multiples of 256.
 template <int W>
 struct Places {
   int along, across[2];
@@ -114,12 +116,13 @@ struct Places {
     across[1] = chunk_at<W>(r + 8, chunk) + (quad & 1) * 8;
   }
   // Channels 16 c + 8 (lane / 32) .. + 7 of row `row0 + lane % 32` (row0 a multiple of 32).
-  AKG_DEV u32x4 row(const u8 *tile, int row0, int c) const { return *reinterpret_cast<const u32x4 *>(tile + along + (row0 * pitch(W) + 32 * c)); }
+  AKG_DEV u32x4 row(const u8 *lds, int tile, int row0, int c) const {
+    return *reinterpret_cast<const u32x4 *>(lds + ((tile + along) ^ (32 * c)) + row0 * pitch(W));
+  }
   // Channel 32 unit + swapped(lane % 32) of the rows row0 + 4 h .. 4 h + 3 and row0 + 8 + 4 h .. (h = lane / 32; row0 a multiple of 16).
-  AKG_DEV u32x4 transposed(const u8 *tile, int row0, int unit) const {
-    const int more = row0 * pitch(W) + 64 * unit;
-    const attn::s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn::s16x4 *)(tile + across[0] + more));
-    const attn::s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn::s16x4 *)(tile + across[1] + more));
+  AKG_DEV u32x4 transposed(const u8 *lds, int tile, int row0, int unit) const {
+    const attn::s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn::s16x4 *)(lds + ((tile + across[0]) ^ (64 * unit)) + row0 * pitch(W)));
+    const attn::s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn::s16x4 *)(lds + ((tile + across[1]) ^ (64 * unit)) + row0 * pitch(W)));
     const u32x2 l = __builtin_bit_cast(u32x2, lo), u = __builtin_bit_cast(u32x2, hi);
     return u32x4{l[0], l[1], u[0], u[1]};
   }
@@ -176,15 +179,14 @@ struct Stage {
 };
 
 // What the emitted kernel states about a walk: the operands' type in parts, channels of a and b (D) and of c and the result
-// (E), 32-token tiles of a chunk (CT), wavefronts that hold the state (NW, 32 channels of c each), whether LDS holds one chunk's
+// (E), 32-token tiles of a chunk (CT), wavefronts that hold the state (NW, 32 channels of c each), wavefronts that fetch and multiply (HELPERS, two or four), whether LDS holds one chunk's
 // tiles only (TIGHT), whether what is added to the state goes in two parts (REST), heads of the states (H) and of each operand, whether it runs backward, whether states given and left are
 // the transposed ones ([E][D] in memory).
 enum class Result { None, Storage, Float };
-constexpr int kHelpers = 4;   // wavefronts that fetch and multiply
-template <typename T_, int D_, int E_, int CT_, int NW_, bool TIGHT_, bool REST_, int H_, int HA_, int HB_, int HC_, bool HEADS_FIRST_, bool BACK_, bool TURNED_, Result RESULT_>
+template <typename T_, int D_, int E_, int CT_, int NW_, int HELPERS_, bool TIGHT_, bool REST_, int H_, int HA_, int HB_, int HC_, bool HEADS_FIRST_, bool BACK_, bool TURNED_, Result RESULT_>
 struct Config {
   typedef T_ T;   // attn::BF16 or attn::F16
-  static constexpr int PARTS = T::kNarrowRange ? 2 : 1, D = D_, E = E_, CT = CT_, NW = NW_, H = H_, HA = HA_, HB = HB_, HC = HC_;
+  static constexpr int PARTS = T::kNarrowRange ? 2 : 1, D = D_, E = E_, CT = CT_, NW = NW_, HELPERS = HELPERS_, H = H_, HA = HA_, HB = HB_, HC = HC_;
   static constexpr bool TIGHT = TIGHT_, REST = REST_ || T::kNarrowRange, HEADS_FIRST = HEADS_FIRST_, BACK = BACK_, TURNED = TURNED_;
   static constexpr Result RESULT = RESULT_;
   static constexpr int kChunk = 32 * CT, kColumns = 32 * NW, kTiles = (E + kColumns - 1) / kColumns;
@@ -239,13 +241,13 @@ AKG_DEV long entry_of(const int *slots, long b, long pool) {
 
 // One segment of one head, 32 NW channels of c. STATES: only what the segment adds to a state.
 //
-// NW wavefronts hold the state and do what needs it. Four others fetch into registers, two chunks ahead of what they put into
+// NW wavefronts hold the state and do what needs it. The others fetch into registers, two chunks ahead of what they put into
 // LDS (float16 in parts), and compute the masked products. Between two barriers the first have what chunk t adds to the state, its
 // masked products with c, and a . S of chunk t + 1; the others the masked products of t + 1, and a, b and c of t + 2 to put in
 // place of tiles that nothing reads any more. TIGHT: one after the other.
 template <typename C, bool STATES>
 AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int seg) {
-  constexpr int D = C::D, E = C::E, PARTS = C::PARTS, CT = C::CT, NW = C::NW, kChunk = C::kChunk, kThreads = 64 * kHelpers;
+  constexpr int D = C::D, E = C::E, PARTS = C::PARTS, CT = C::CT, NW = C::NW, kChunk = C::kChunk, kThreads = 64 * C::HELPERS;
   constexpr int kUnits = padded(D) / 32, kSteps = 2 * CT, kAfter = C::BACK ? 1 : 0;
   constexpr int kTerms = C::REST ? 2 : 1;   // parts of what is added to the state
   constexpr bool TIGHT = C::TIGHT;
@@ -266,6 +268,8 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
     return C::BACK ? len - r0 - n : r0;
   };
   const Places<D> pd(lane);
+  const u8 *mem = reinterpret_cast<const u8 *>(&lds);
+  auto place_of = [&](const u8 *tile_) { return static_cast<int>(tile_ - mem); };
 
   if (wave >= NW) {
     const int tid = static_cast<int>(threadIdx.x) - 64 * NW, helper = wave - NW;
@@ -308,32 +312,26 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
       sc[held].store(lds.c[ib][0], tid);
     };
     // Weights of the masked products (register r: key token 8 (r / 4) + 4 half + r % 4 of its 32, query token lane % 32). Pairs
-    // of tiles (query tile, key tile): 0 = (0, 0), 1 = (1, 0), 2 = (1, 1), one to a wavefront.
-    constexpr int kPairs = CT * (CT + 1) / 2;
-    const int qt = helper > 0 ? 1 : 0, kt = helper > 1 ? 1 : 0;
+    // of tiles (query tile, key tile): 0 = (0, 0), 1 = (1, 0), 2 = (1, 1), one to a wavefront, or 0 and 2 to the first of two.
     float mask[16];
     if constexpr (!STATES) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int n = 32 * (qt - kt) + (lane & 31) - (8 * (r >> 2) + 4 * half + (r & 3));
+        const int n = (CT == 2 && helper == 1 ? 32 : 0) + (lane & 31) - (8 * (r >> 2) + 4 * half + (r & 3));
         mask[r] = n < 0 ? 0.0f : power(g2, n) * w.scale;
       }
     }
-    // ..., and the pieces of chunk t meanwhile
-    auto multiply = [&](int ia, int ib, int to, int t) {
-      if (STATES || helper >= kPairs) {
-        fetch(to, t);
-        return;
-      }
-      const Sources from_ = sources(t);
+    // `load`: what is asked of memory behind every matrix instruction.
+    auto pair = [&](int which, int ia, int ib, auto load) {
+      const int qt = which > 0 ? 1 : 0, kt = which > 1 ? 1 : 0;
       f32x16 s = {};
       constexpr int kAhead = 4;
       u32x4 keys[2 * kUnits][PARTS], queries[2 * kUnits][PARTS];
       auto read = [&](int x) {
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-          keys[x][p] = pd.row(lds.b[ib][p] + 32 * pitch(D) * kt, 0, x);
-          queries[x][p] = pd.row(lds.a[ia][p] + 32 * pitch(D) * qt, 0, x);
+          keys[x][p] = pd.row(mem, place_of(lds.b[ib][p]) + 32 * pitch(D) * kt, 0, x);
+          queries[x][p] = pd.row(mem, place_of(lds.a[ia][p]) + 32 * pitch(D) * qt, 0, x);
         }
       };
 #pragma unroll
@@ -343,8 +341,7 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
         __builtin_amdgcn_sched_barrier(0);
         s = product(keys[x], queries[x], s);
         if (x + kAhead < 2 * kUnits) read(x + kAhead);
-#pragma unroll
-        for (int i = x * kPieces / (2 * kUnits); i < (x + 1) * kPieces / (2 * kUnits); ++i) fetch_piece(to, from_, i);
+        load(x);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -356,7 +353,23 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
         u32x4 parts[PARTS];
         split<PARTS>(v, parts);
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) lds.pairs[ia][p][helper][x][lane] = parts[p];
+        for (int p = 0; p < PARTS; ++p) lds.pairs[ia][p][which][x][lane] = parts[p];
+      }
+    };
+    // The masked products of a chunk, and the pieces of chunk t on their way meanwhile.
+    auto multiply = [&](int ia, int ib, int to, int t) {
+      constexpr int kPairs = CT * (CT + 1) / 2;
+      if (STATES || helper >= kPairs) {
+        fetch(to, t);
+        return;
+      }
+      const Sources from_ = sources(t);
+      pair(helper, ia, ib, [&](int x) {
+#pragma unroll
+        for (int i = x * kPieces / (2 * kUnits); i < (x + 1) * kPieces / (2 * kUnits); ++i) fetch_piece(to, from_, i);
+      });
+      if constexpr (kPairs > C::HELPERS) {
+        if (helper == 0) pair(2, ia, ib, [](int) {});
       }
     };
     if (chunks > 0) {
@@ -469,14 +482,14 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
   u32x4 queries[kAll][PARTS];
   auto query = [&](int ia, int y) {
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) queries[y][p] = pd.row(lds.a[ia][p], 32 * (y % CT), y / CT);
+    for (int p = 0; p < PARTS; ++p) queries[y][p] = pd.row(mem, place_of(lds.a[ia][p]), 32 * (y % CT), y / CT);
   };
   constexpr int kGroup = !kWide ? kUnits : kUnits % 2 == 0 ? 2 : 1, kPasses = PARTS + kTerms - 1;   // units of the state at a time
   constexpr int kAllKeys = kSteps * kUnits, kKeysAhead = kWide ? 3 : kPasses == 1 && 2 * kGroup <= kAllKeys ? 2 * kGroup : kGroup;
   u32x4 values[kSteps][PARTS], more[kSteps][kTerms], keys[kAllKeys][PARTS];
   auto key = [&](int ib, int x) {
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) keys[x][p] = pd.transposed(lds.b[ib][p], 16 * (x / kUnits), x % kUnits);
+    for (int p = 0; p < PARTS; ++p) keys[x][p] = pd.transposed(mem, place_of(lds.b[ib][p]), 16 * (x / kUnits), x % kUnits);
   };
   // (pair e of the eight values of step s)
   auto weighted = [&](int s, int e) {
@@ -492,7 +505,7 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p) values[s][p] = pc.transposed(lds.c[ib][p], 16 * s, wave);
+      for (int p = 0; p < PARTS; ++p) values[s][p] = pc.transposed(mem, place_of(lds.c[ib][p]), 16 * s, wave);
     }
 #pragma unroll
     for (int x = 0; x < kKeysAhead; ++x) key(ib, x);
