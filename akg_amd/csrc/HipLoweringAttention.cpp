@@ -578,9 +578,9 @@ class LayerEmitter {
     if (s.seq >= (1LL << 31) - 8192) throw LoweringError("op " + op_.name + ": more than 2^31 tokens");
     return s;
   }
-  std::string walkConfig(const WalkOf &w, const LinearSizes &s, int ct, int64_t nw, int helpers, bool tight) const {
+  std::string walkConfig(const WalkOf &w, const LinearSizes &s, int ct, int64_t nw, int halves, int helpers, bool tight) const {
     std::ostringstream o;
-    o << "akg::linear::Config<" << trait() << ", " << w.d << ", " << w.e << ", " << ct << ", " << nw << ", " << helpers << ", " << flag(tight) << ", " << flag(w.rest) << ", " << s.heads << ", " << w.ha << ", " << w.hb << ", " << w.hc
+    o << "akg::linear::Config<" << trait() << ", " << w.d << ", " << w.e << ", " << ct << ", " << nw << ", " << (w.d > 128 ? halves : 1) << ", " << helpers << ", " << flag(tight) << ", " << flag(w.rest) << ", " << s.heads << ", " << w.ha << ", " << w.hb << ", " << w.hc
       << ", " << flag(l_.headsFirst) << ", " << flag(w.back) << ", " << flag(w.turned) << ", akg::linear::Result::" << w.result << ">";
     return o.str();
   }
@@ -597,6 +597,12 @@ class LayerEmitter {
     }
     const int parts = in(0).dtype == DType::F16 ? 2 : 1;
     const int64_t units = ceilDiv(widest, 32);
+    // Two wavefronts share the rows of 32 columns of a state where one has too few registers for them: above 128 channels with
+    // operands or terms of the state in several parts (4 x 2048 tokens of 16/4 heads of 256, the last state kept: 117 us instead of 328;
+    // float16 288, 1339; without that 4 x 4096 of 8 heads in bfloat16 135 with one, 153 with two, its gradient 246, 334).
+    bool rest = false;
+    for (const WalkOf &w : all) rest = rest || w.rest;
+    const int halves = deepest > 128 && (parts == 2 || rest) ? 2 : 1;
     // How many wavefronts hold the state of a workgroup (32 columns each: fewer make more workgroups, which all fetch a and b and
     // multiply them), and how many segments share the tokens (each but the last adds a pass over b and c in front): what is
     // expected to take least. A chunk of 64 tokens of 128 channels takes 1.4, 1.5 and 2.0 us with one, two and four such wavefronts
@@ -617,11 +623,11 @@ class LayerEmitter {
       for (const WalkOf &w : all) n += ceilDiv(w.e, 32 * nw);
       return n;
     };
-    for (int64_t nw = std::min<int64_t>(units, 4); nw >= 1; --nw) {
+    for (int64_t nw = std::min<int64_t>(units, 4 / halves); nw >= 1; --nw) {
       if (nw > 2 && nw != ceilDiv(units, ceilDiv(units, 4))) continue;
       // Tiles of a few chunks (linear::Lds, linear::pitch) where LDS holds them, of chunks of 32 tokens before those of one chunk only.
       auto pitchOf = [](int64_t d) { return d <= 32 ? 64 : d <= 64 ? 128 : d <= 128 ? 256 : 512; };
-      auto ldsBytes = [&](int64_t tiles) { return parts * (32 * tiles * (5 * pitchOf(deepest) + 3 * pitchOf(32 * nw)) + 2 * 2048 * (tiles * (tiles + 1) / 2)); };
+      auto ldsBytes = [&](int64_t tiles) { return parts * (32 * tiles * (5 * pitchOf(deepest) + 3 * pitchOf(32 * nw)) + 2 * 2048 * (tiles * (tiles + 1) / 2)) + (halves == 2 ? 2 * 4096 * nw * tiles : 0); };
       int ct = parts == 2 || ldsBytes(2) > 160 * 1024 ? 1 : 2;
       const bool tight = ldsBytes(ct) > 160 * 1024;
       const int64_t groups = s.states * tilesOf(nw), chunks = ceilDiv(s.seq, 32 * ct);
@@ -660,8 +666,8 @@ class LayerEmitter {
     int helpers = nw <= 2 && deepest <= 64 && groups * segments > cus_ ? 2 : 4;
     k_.scalarArgs = {s.batch, s.seq, segment, segments};
     if (l_.hasSlots) k_.scalarArgs.push_back(in(4).shape[0]);
-    o << "typedef " << walkConfig(all[0], s, ct, nw, helpers, tight) << " akg_C0;\n";
-    for (size_t i = 1; i < all.size(); ++i) o << "typedef " << walkConfig(all[i], s, ct, nw, helpers, tight) << " akg_C" << i << ";\n";
+    o << "typedef " << walkConfig(all[0], s, ct, nw, halves, helpers, tight) << " akg_C0;\n";
+    for (size_t i = 1; i < all.size(); ++i) o << "typedef " << walkConfig(all[i], s, ct, nw, halves, helpers, tight) << " akg_C" << i << ";\n";
     o << "\n";
     int64_t before = space;
     std::vector<std::string> structs;
@@ -674,7 +680,7 @@ class LayerEmitter {
       structs.push_back(b.str());
       before += 4 * s.heads * w.d * w.e;
     }
-    const int threads = static_cast<int>(64 * (nw + helpers));
+    const int threads = static_cast<int>(64 * (nw * halves + helpers));
     int hint = 2;
     // A head's workgroups are neighbours on one XCD, whose L2 they share: the walks of a gradient read the same tensors, those
     // backward in time at the same time.

@@ -46,18 +46,21 @@ using attn::u32x4;
 // A tile of W channels in LDS: rows of 64, 128, 256 or 512 bytes without any between them, whose chunks of 16 bytes change places
 // by exclusive or with bits of the row. Four neighbouring rows of 64 bytes (transposed reads, half a wavefront at a time) and
 // sixteen of 16 bytes (rows read by 128 bits) then lie in banks of their own. The places of a lane differ by an exclusive or with
-// a constant. (With 32 and 64 bytes more a row instead, transposed reads met in the banks, or three chunks' tiles did not fit.)
+// a constant. (With 32 and 64 bytes more a row instead, transposed reads met in the banks, or three chunks' tiles did not fit; a
+// gradient of 4 x 4096 tokens of 8 heads of 256 took 334 us instead of 247.)
 constexpr int pitch(int w) { return w <= 32 ? 64 : w <= 64 ? 128 : w <= 128 ? 256 : 512; }
 constexpr int turn(int w, int row) { return (w <= 32 ? 0 : w <= 64 ? (row & 2) << 1 : (row & 3) << 2) | ((row >> 2) & 3); }
+// (above 128 channels two wavefronts may share the rows of a state: a multiple of 64)
+constexpr int whole(int w) { return w <= 128 ? padded(w) : (w + 63) / 64 * 64; }
 template <int W>
 AKG_DEV int chunk_at(int row, int chunk) {
   return row * pitch(W) + ((chunk ^ turn(W, row)) << 4);
 }
-// The channels behind W of a tile's rows (to the next multiple of 32) hold zeros: written once, never again.
+// The channels behind W of a tile's rows, up to whole(W), hold zeros: written once, never again.
 template <int ROWS, int W, int THREADS>
 AKG_DEV void clear_padding(u8 *tile, int tid) {
-  if constexpr (W % 32 != 0) {
-    constexpr int kPad = (padded(W) - W) / 8;
+  if constexpr (whole(W) != W) {
+    constexpr int kPad = (whole(W) - W) / 8;
     for (int c = tid; c < ROWS * kPad; c += THREADS) *reinterpret_cast<u32x4 *>(tile + chunk_at<W>(c / kPad, W / 8 + c % kPad)) = u32x4{0, 0, 0, 0};
   }
 }
@@ -80,15 +83,19 @@ AKG_DEV float power_less_one(float g, int n) {
   return __builtin_fmaf(x * x, p, x);
 }
 
-// Float32 values as PARTS values of bfloat16 whose sum they are, to 2^-8 or 2^-16 of them: word `e` of an operand.
+// Float32 values as PARTS values of bfloat16 whose sum they are, to 2^-8, 2^-16 or 2^-24 of them: word `e` of an operand.
 template <int PARTS>
 AKG_DEV void split_pair(float lo, float hi, u32x4 (&parts)[PARTS], int e) {
-  u32 w = BF16::pack(lo, hi);
-  if constexpr (PARTS == 2) {
-    asm("" : "+v"(w));   // (one rounding, not another one for the rest)
-    parts[1][e] = BF16::pack(lo - BF16::low(w), hi - BF16::high(w));
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    u32 w = BF16::pack(lo, hi);
+    if (p + 1 < PARTS) {
+      asm("" : "+v"(w));   // (one rounding, not another one for the rest)
+      lo -= BF16::low(w);
+      hi -= BF16::high(w);
+    }
+    parts[p][e] = w;
   }
-  parts[0][e] = w;
 }
 template <int PARTS>
 AKG_DEV void split(const float (&x)[8], u32x4 (&parts)[PARTS]) {
@@ -179,15 +186,15 @@ struct Stage {
 };
 
 // What the emitted kernel states about a walk: the operands' type in parts, channels of a and b (D) and of c and the result
-// (E), 32-token tiles of a chunk (CT), wavefronts that hold the state (NW, 32 channels of c each), wavefronts that fetch and multiply (HELPERS, two or four), whether LDS holds one chunk's
+// (E), 32-token tiles of a chunk (CT), wavefronts that hold the state (NW, 32 channels of c each, times HALVES of its rows), wavefronts that fetch and multiply (HELPERS, two or four), whether LDS holds one chunk's
 // tiles only (TIGHT), whether what is added to the state goes in two parts (REST), heads of the states (H) and of each operand, whether it runs backward, whether states given and left are
 // the transposed ones ([E][D] in memory).
 enum class Result { None, Storage, Float };
-template <typename T_, int D_, int E_, int CT_, int NW_, int HELPERS_, bool TIGHT_, bool REST_, int H_, int HA_, int HB_, int HC_, bool HEADS_FIRST_, bool BACK_, bool TURNED_, Result RESULT_>
+template <typename T_, int D_, int E_, int CT_, int NW_, int HALVES_, int HELPERS_, bool TIGHT_, bool REST_, int H_, int HA_, int HB_, int HC_, bool HEADS_FIRST_, bool BACK_, bool TURNED_, Result RESULT_>
 struct Config {
   typedef T_ T;   // attn::BF16 or attn::F16
-  static constexpr int PARTS = T::kNarrowRange ? 2 : 1, D = D_, E = E_, CT = CT_, NW = NW_, HELPERS = HELPERS_, H = H_, HA = HA_, HB = HB_, HC = HC_;
-  static constexpr bool TIGHT = TIGHT_, REST = REST_ || T::kNarrowRange, HEADS_FIRST = HEADS_FIRST_, BACK = BACK_, TURNED = TURNED_;
+  static constexpr int PARTS = T::kNarrowRange ? 2 : 1, D = D_, E = E_, CT = CT_, NW = NW_, HALVES = HALVES_, HELPERS = HELPERS_, H = H_, HA = HA_, HB = HB_, HC = HC_;
+  static constexpr bool TIGHT = TIGHT_, REST = REST_, HEADS_FIRST = HEADS_FIRST_, BACK = BACK_, TURNED = TURNED_;
   static constexpr Result RESULT = RESULT_;
   static constexpr int kChunk = 32 * CT, kColumns = 32 * NW, kTiles = (E + kColumns - 1) / kColumns;
 };
@@ -199,6 +206,7 @@ struct Lds {
   static constexpr int kA = C::TIGHT ? 1 : 2, kB = C::TIGHT ? 1 : 3;
   u8 b[kB][C::PARTS][C::kChunk * pitch(C::D)], c[kB][C::PARTS][C::kChunk * pitch(C::kColumns)], a[STATES ? 0 : kA][C::PARTS][C::kChunk * pitch(C::D)];
   u32x4 pairs[STATES ? 0 : kA][C::PARTS][kPairs][2][64];
+  f32x4 other[STATES || C::HALVES == 1 ? 0 : kA][C::NW][C::CT][4][64];   // a . S of the second half of the rows
 };
 
 // Where the tokens of one head of a tensor with X heads of W channels of 2 bytes lie.
@@ -241,15 +249,16 @@ AKG_DEV long entry_of(const int *slots, long b, long pool) {
 
 // One segment of one head, 32 NW channels of c. STATES: only what the segment adds to a state.
 //
-// NW wavefronts hold the state and do what needs it. The others fetch into registers, two chunks ahead of what they put into
+// NW wavefronts hold the state and do what needs it (with HALVES 2 NW, half of the rows each, since a state of 256 leaves a wavefront
+// few registers: the second half's a . S reaches the first through LDS). The others fetch into registers, two chunks ahead of what they put into
 // LDS (float16 in parts), and compute the masked products. Between two barriers the first have what chunk t adds to the state, its
 // masked products with c, and a . S of chunk t + 1; the others the masked products of t + 1, and a, b and c of t + 2 to put in
 // place of tiles that nothing reads any more. TIGHT: one after the other.
 template <typename C, bool STATES>
 AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int seg) {
   constexpr int D = C::D, E = C::E, PARTS = C::PARTS, CT = C::CT, NW = C::NW, kChunk = C::kChunk, kThreads = 64 * C::HELPERS;
-  constexpr int kUnits = padded(D) / 32, kSteps = 2 * CT, kAfter = C::BACK ? 1 : 0;
-  constexpr int kTerms = C::REST ? 2 : 1;   // parts of what is added to the state
+  constexpr int kHalves = C::HALVES, kWaves = NW * kHalves, kUnits = whole(D) / 32 / kHalves, kSteps = 2 * CT, kAfter = C::BACK ? 1 : 0;
+  constexpr int kTerms = C::REST ? 3 : 2;   // parts of what is added to the state
   constexpr bool TIGHT = C::TIGHT;
   const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), half = lane >> 5;
   const long b = head / C::H;
@@ -271,8 +280,10 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
   const u8 *mem = reinterpret_cast<const u8 *>(&lds);
   auto place_of = [&](const u8 *tile_) { return static_cast<int>(tile_ - mem); };
 
-  if (wave >= NW) {
-    const int tid = static_cast<int>(threadIdx.x) - 64 * NW, helper = wave - NW;
+  if (wave >= kWaves + C::HELPERS) return;   // (walks of other channels in the same launch have more; who has ended is not waited for)
+  if (wave >= kWaves) {
+    const int tid = static_cast<int>(threadIdx.x) - 64 * kWaves, helper = wave - kWaves;
+    constexpr int kDeep = 2 * kUnits * kHalves;   // of 16 channels
     const Tokens<C::HA, D, C::HEADS_FIRST, C::H> ta(w.a, b, h, w.seq);
     const Tokens<C::HB, D, C::HEADS_FIRST, C::H> tb(w.b, b, h, w.seq);
     const Tokens<C::HC, E, C::HEADS_FIRST, C::H> tc(w.c, b, h, w.seq);
@@ -325,8 +336,8 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
     auto pair = [&](int which, int ia, int ib, auto load) {
       const int qt = which > 0 ? 1 : 0, kt = which > 1 ? 1 : 0;
       f32x16 s = {};
-      constexpr int kAhead = 4;
-      u32x4 keys[2 * kUnits][PARTS], queries[2 * kUnits][PARTS];
+      constexpr int kAhead = kDeep * PARTS > 16 ? 2 : 4;   // (as registers allow)
+      u32x4 keys[kDeep][PARTS], queries[kDeep][PARTS];
       auto read = [&](int x) {
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
@@ -335,12 +346,12 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
         }
       };
 #pragma unroll
-      for (int x = 0; x < kAhead && x < 2 * kUnits; ++x) read(x);
+      for (int x = 0; x < kAhead && x < kDeep; ++x) read(x);
 #pragma unroll
-      for (int x = 0; x < 2 * kUnits; ++x) {
+      for (int x = 0; x < kDeep; ++x) {
         __builtin_amdgcn_sched_barrier(0);
         s = product(keys[x], queries[x], s);
-        if (x + kAhead < 2 * kUnits) read(x + kAhead);
+        if (x + kAhead < kDeep) read(x + kAhead);
         load(x);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -366,7 +377,7 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
       const Sources from_ = sources(t);
       pair(helper, ia, ib, [&](int x) {
 #pragma unroll
-        for (int i = x * kPieces / (2 * kUnits); i < (x + 1) * kPieces / (2 * kUnits); ++i) fetch_piece(to, from_, i);
+        for (int i = x * kPieces / kDeep; i < (x + 1) * kPieces / kDeep; ++i) fetch_piece(to, from_, i);
       });
       if constexpr (kPairs > C::HELPERS) {
         if (helper == 0) pair(2, ia, ib, [](int) {});
@@ -434,7 +445,9 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
   }
 
   // Row of unit u in register r: channel 32 u + 16 (r / 8) + 8 half + r % 8.
-  const int column = e0 + 32 * wave + swapped(lane & 31);   // of the state, in this lane
+  // (of unit 0 .. kUnits - 1 of this wavefront's half of the rows)
+  const int block = wave % NW, part = wave / NW, unit0 = part * kUnits;
+  const int column = e0 + 32 * block + swapped(lane & 31);   // of the state, in this lane
   f32x16 state[kUnits];
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) state[u] = {};
@@ -448,8 +461,8 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
       for (int u = 0; u < kUnits; ++u) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int d = 32 * u + 16 * (r >> 3) + 8 * half + (r & 7);
-          if (D % 32 == 0 || d < D) state[u][r] = given[turned ? static_cast<long>(column) * D + d : static_cast<long>(d) * E + column];
+          const int d = 32 * (unit0 + u) + 16 * (r >> 3) + 8 * half + (r & 7);
+          if (D == whole(D) || d < D) state[u][r] = given[turned ? static_cast<long>(column) * D + d : static_cast<long>(d) * E + column];
         }
       }
     }
@@ -477,19 +490,19 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
   // values of later ones rounded or weighted. (The barriers keep that order: left to itself the compiler reads an operand in
   // front of its use and waits.)
   f32x16 out[CT];
-  constexpr bool kWide = kUnits > 4;   // (the state leaves few registers to read ahead)
-  constexpr int kAll = 2 * kUnits * CT, kAhead = kWide ? 3 : 6;
+  constexpr bool kWide = kUnits > 4;   // (few registers to read ahead)
+  constexpr int kAll = 2 * kUnits * CT, kAhead = kWide || C::REST ? 3 : 6;
   u32x4 queries[kAll][PARTS];
   auto query = [&](int ia, int y) {
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) queries[y][p] = pd.row(mem, place_of(lds.a[ia][p]), 32 * (y % CT), y / CT);
+    for (int p = 0; p < PARTS; ++p) queries[y][p] = pd.row(mem, place_of(lds.a[ia][p]), 32 * (y % CT), 2 * unit0 + y / CT);
   };
-  constexpr int kGroup = !kWide ? kUnits : kUnits % 2 == 0 ? 2 : 1, kPasses = PARTS + kTerms - 1;   // units of the state at a time
-  constexpr int kAllKeys = kSteps * kUnits, kKeysAhead = kWide ? 3 : kPasses == 1 && 2 * kGroup <= kAllKeys ? 2 * kGroup : kGroup;
+  constexpr int kGroup = !kWide ? kUnits : kUnits % 2 == 0 ? 2 : 1, kPasses = PARTS == 1 ? kTerms : 2 * kTerms - 1;   // units of the state at a time
+  constexpr int kAllKeys = kSteps * kUnits, kKeysAhead = kWide ? 3 : kGroup;
   u32x4 values[kSteps][PARTS], more[kSteps][kTerms], keys[kAllKeys][PARTS];
   auto key = [&](int ib, int x) {
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) keys[x][p] = pd.transposed(mem, place_of(lds.b[ib][p]), 16 * (x / kUnits), x % kUnits);
+    for (int p = 0; p < PARTS; ++p) keys[x][p] = pd.transposed(mem, place_of(lds.b[ib][p]), 16 * (x / kUnits), unit0 + x % kUnits);
   };
   // (pair e of the eight values of step s)
   auto weighted = [&](int s, int e) {
@@ -505,7 +518,7 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p) values[s][p] = pc.transposed(mem, place_of(lds.c[ib][p]), 16 * s, wave);
+      for (int p = 0; p < PARTS; ++p) values[s][p] = pc.transposed(mem, place_of(lds.c[ib][p]), 16 * s, block);
     }
 #pragma unroll
     for (int x = 0; x < kKeysAhead; ++x) key(ib, x);
@@ -539,6 +552,15 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
       }
     }
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kHalves == 2) {
+      if (part == 1) {
+#pragma unroll
+        for (int i = 0; i < CT; ++i) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) lds.other[ia][block][i][x][lane] = f32x4{out[i][4 * x], out[i][4 * x + 1], out[i][4 * x + 2], out[i][4 * x + 3]};
+        }
+      }
+    }
   };
   if (chunks > 0) {
     __syncthreads();   // (the first tiles are in place)
@@ -556,6 +578,19 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
     third = third + 1 < 3 ? third + 1 : 0;
     u32x4 pairs[kSteps][CT][PARTS];
     if constexpr (!STATES) {
+      if constexpr (kHalves == 2) {
+        if (part == 0) {
+#pragma unroll
+          for (int i = 0; i < CT; ++i) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const f32x4 v = lds.other[ia][block][i][x][lane];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) out[i][4 * x + e] += v[e];
+            }
+          }
+        }
+      }
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
@@ -576,10 +611,10 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
     constexpr bool kFloat = C::RESULT == Result::Float, kShow = !STATES && C::RESULT != Result::None;
     constexpr int kSize = kFloat ? 4 : 2;
     const Tokens<C::H, E, kFloat || C::HEADS_FIRST, C::H> to(w.out, b, h, w.seq, kSize);
-    const Buffer buf = make_buffer(to.base + lowest_of(t, n) * to.step, kShow ? records((n - 1) * to.step + static_cast<long>(kSize) * E) : 0);
+    const Buffer buf = make_buffer(to.base + lowest_of(t, n) * to.step, kShow && part == 0 ? records((n - 1) * to.step + static_cast<long>(kSize) * E) : 0);
     // (half x of query tile i: 16 channels of a row in a pair of lanes)
     auto write = [&](int i, int x) {
-      const int row = 32 * i + (lane & 31), behind = C::BACK ? kChunk - 1 - row : row - (kChunk - n), d = e0 + 32 * wave + 16 * x + 8 * half;
+      const int row = 32 * i + (lane & 31), behind = C::BACK ? kChunk - 1 - row : row - (kChunk - n), d = e0 + 32 * block + 16 * x + 8 * half;
       const u32 off = row >= kChunk - n && d < E ? static_cast<u32>(behind * static_cast<int>(to.step) + kSize * d) : kBeyondEveryBuffer;
       if constexpr (kFloat) {
 #pragma unroll
@@ -608,7 +643,9 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
         for (int v = 0; v < kGroup; ++v) {
           __builtin_amdgcn_sched_barrier(0);
           const int u = u0 + v, x = q * kGroup + v;
-          state[u] = BF16::mma(keys[x][PARTS == 2 && pass == 1 ? 1 : 0], more[s][kTerms == 2 && pass == 0 ? 1 : 0], state[u]);
+          // (parts of the key and of the value, the smallest products first: those below 2^-16, or 2^-24, are left out)
+          const int kp = PARTS == 1 ? 0 : pass % 2, mt = PARTS == 1 ? kTerms - 1 - pass : kTerms - 1 - (pass + 1) / 2;
+          state[u] = BF16::mma(keys[x][kp], more[s][mt], state[u]);
           if (pass == 0 && x + kKeysAhead < kAllKeys) key(ib, x + kKeysAhead);
           if (u0 == 0 && pass + 1 == kPasses && s + 1 < kSteps) {
 #pragma unroll
@@ -674,8 +711,8 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
     for (int u = 0; u < kUnits; ++u) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int d = 32 * u + 16 * (r >> 3) + 8 * half + (r & 7);
-        if (D % 32 == 0 || d < D) to[C::TURNED && !STATES ? static_cast<long>(column) * D + d : static_cast<long>(d) * E + column] = state[u][r];
+        const int d = 32 * (unit0 + u) + 16 * (r >> 3) + 8 * half + (r & 7);
+        if (D == whole(D) || d < D) to[C::TURNED && !STATES ? static_cast<long>(column) * D + d : static_cast<long>(d) * E + column] = state[u][r];
       }
     }
   }
