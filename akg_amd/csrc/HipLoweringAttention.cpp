@@ -631,7 +631,7 @@ class LayerEmitter {
       int ct = parts == 2 || ldsBytes(2) > 160 * 1024 ? 1 : 2;
       const bool tight = ldsBytes(ct) > 160 * 1024;
       const int64_t groups = s.states * tilesOf(nw), chunks = ceilDiv(s.seq, 32 * ct);
-      const double each = (0.9 + ct * (0.15 + (parts == 2 ? 0.08 : 0.026) * static_cast<double>(nw * ceilDiv(deepest, 32)))) * (tight ? 1.5 : 1.0);
+      const double each = (0.9 + ct * ((rest ? 0.33 : 0.15) + (parts == 2 ? 0.08 : 0.026) * static_cast<double>(nw * ceilDiv(deepest, 32)))) * (tight ? 1.5 : 1.0);
       const double bytes = static_cast<double>(2 * s.states * s.seq) / 4.8e6;   // us for a channel of every token
       for (int64_t segments = 1; segments <= std::max<int64_t>(1, std::min<int64_t>(cus_ / groups, chunks / 2)); ++segments) {
         const double steps = static_cast<double>(ceilDiv(chunks, segments));
@@ -646,7 +646,7 @@ class LayerEmitter {
         auto both = [](double x, double y) { return std::max(x, y) + 0.25 * std::min(x, y); };
         double time = both(static_cast<double>(ceilDiv(groups * segments, cus_)) * steps * each, moved);
         if (segments > 1) {
-          time += both(static_cast<double>(ceilDiv(groups * (segments - 1), cus_)) * steps * each * 0.55, movedStates) + 10.0 +
+          time += both(static_cast<double>(ceilDiv(groups * (segments - 1), cus_)) * steps * each * 0.55, movedStates) + 8.0 +
                   static_cast<double>(8 * s.states * segments * values) / 4.8e6;
         }
         if (best.nw == 0 || time < best.time) best = {time, nw, segments, ct, tight};

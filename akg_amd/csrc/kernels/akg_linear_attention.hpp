@@ -611,7 +611,9 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
     constexpr bool kFloat = C::RESULT == Result::Float, kShow = !STATES && C::RESULT != Result::None;
     constexpr int kSize = kFloat ? 4 : 2;
     const Tokens<C::H, E, kFloat || C::HEADS_FIRST, C::H> to(w.out, b, h, w.seq, kSize);
-    const Buffer buf = make_buffer(to.base + lowest_of(t, n) * to.step, kShow && part == 0 ? records((n - 1) * to.step + static_cast<long>(kSize) * E) : 0);
+    // (in a scalar register: the compiler would test every store's descriptor for each lane otherwise)
+    const int bytes = __builtin_amdgcn_readfirstlane(static_cast<int>(kShow && part == 0 ? records((n - 1) * to.step + static_cast<long>(kSize) * E) : 0));
+    const Buffer buf = make_buffer(to.base + lowest_of(t, n) * to.step, bytes);
     // (half x of query tile i: 16 channels of a row in a pair of lanes)
     auto write = [&](int i, int x) {
       const int row = 32 * i + (lane & 31), behind = C::BACK ? kChunk - 1 - row : row - (kChunk - n), d = e0 + 32 * block + 16 * x + 8 * half;
