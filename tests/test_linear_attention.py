@@ -458,6 +458,95 @@ def test_large_and_small_values_in_float16(seq, tmp_path):
             assert ((x.to(F) - exact).abs() <= bound)[fits].all(), n
 
 
+@pytest.mark.gpu
+def test_long_texts_in_a_pool_in_place(tmp_path):
+    """Segments, entries of a pool read and written in place: one of them whole, one sequence without an entry, one without
+    tokens, whose entry stays as it was, bit for bit, as do those that no sequence has."""
+    heads, dim, seq = 2, 64, 3000
+    g, pool = decays("slow", heads), normal((5, heads, dim, dim), "float32", 1, 2.0)
+    t = {n: normal((3, seq, heads, dim), "bfloat16", 2 + i) for i, n in enumerate(("q", "k", "v"))}
+    t = dict(t, log_decay=g, state=pool, slots=torch.tensor([3, -1, 0], dtype=torch.int32), lengths=torch.tensor([seq, 50, 0], dtype=torch.int32))
+    text, inputs = describe(t, "BSND", scale=0.25)
+    kernel = driver.HipKernel(text, out_dir=str(tmp_path))
+    assert kernel.workspace_bytes > 0
+    ins = [x.cuda() for x in inputs]
+    out = empties(kernel)[0]
+    kernel.launch(ins + [out, ins[4]])
+    r = check_forward(t, "BSND", [out.cpu()], scale=0.25)
+    after = ins[4].cpu()
+    close(after[3], r["last"][0], ref.state_bound(r["last_rough"][0], dim, seq), "entry")
+    others = [0, 1, 2, 4]
+    assert torch.equal(after[others], pool[others])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seq", [2, 150, 2000])
+def test_one_entry_read_by_several_sequences(seq, tmp_path):
+    """A prefix that sequences share: the same entry for all of them, and none left behind."""
+    heads, dim = 2, 64
+    g, pool = decays("mixed", heads), normal((3, heads, dim, dim), "float32", 1, 2.0)
+    t = dict({n: normal((3, seq, heads, dim), "bfloat16", 2 + i) for i, n in enumerate(("q", "k", "v"))}, log_decay=g)
+    text, inputs = describe(dict(t, state=pool, slots=torch.tensor([1, 1, 1], dtype=torch.int32)), "BSND", last=False, name="Fused_SharedEntry")
+    shared = launch(text, inputs, tmp_path)[0]
+    text, inputs = describe(dict(t, state=pool[1:2].expand(3, -1, -1, -1).contiguous()), "BSND", last=False, name="Fused_OwnState")
+    assert torch.equal(shared, launch(text, inputs, tmp_path)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seq", [70, 1600])
+@pytest.mark.parametrize("given_", ["state", "dstate"])
+def test_gradient_with_one_of_the_states(seq, given_, tmp_path):
+    t = make(("bfloat16", "BSND", 2, seq, 4, 2, 64, 40, "slow", True, "padded"))
+    del t["state" if given_ == "dstate" else "dstate"]
+    text, inputs = describe_grad(t, "BSND", scale=0.5)
+    got = launch(text, inputs, tmp_path)
+    assert len(got) == (4 if given_ == "state" else 3)
+    check_gradient(t, "BSND", got, scale=0.5)
+
+
+@pytest.mark.gpu
+def test_one_handle_on_two_streams(tmp_path):
+    """Launches of one handle with a workspace that overlap on two streams: each has the results it has alone."""
+    t = make(("bfloat16", "BSND", 2, 1500, 2, 1, 128, 128, "slow", True, None))
+    for f in (describe, describe_grad):
+        text, inputs = f(t, "BSND")
+        kernel = driver.HipKernel(text, out_dir=str(tmp_path))
+        assert kernel.workspace_bytes > 0
+        kernel.prepare()
+        sets = [[x.cuda() for x in inputs], [x.cuda() * (0.5 if x.is_floating_point() and x.dim() == 4 else 1) for x in inputs]]
+        alone, both = [empties(kernel) for _ in sets], [empties(kernel) for _ in sets]
+        for ins, outs in zip(sets, alone):
+            kernel.launch(ins + outs)
+            torch.cuda.synchronize()
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for _ in range(5):
+            for stream, ins, outs in zip(streams, sets, both):
+                with torch.cuda.stream(stream):
+                    kernel.launch(ins + outs)
+        torch.cuda.synchronize()
+        for a, o in zip(alone, both):
+            assert all(torch.equal(x, y) for x, y in zip(a, o))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seq,at,kept", [(6, 3, 3), (300, 200, 128), (2500, 1700, 1664)])
+def test_values_that_are_not_finite_stay_in_their_head(seq, at, kept, tmp_path):
+    """Infinity and NaN in one head of one sequence: every other head and sequence has its results, bit for bit, and so have the
+    head's own tokens in front of the chunk (of few tokens: in front of the token)."""
+    t = make(("bfloat16", "BSND", 2, seq, 4, 4, 64, 64, "slow", True, None))
+    text, inputs = describe(t, "BSND")
+    clean = launch(text, inputs, tmp_path)
+    for n, x in (("v", math.inf), ("k", math.nan)):
+        t[n][1, at, 2, 5] = x
+    text, inputs = describe(t, "BSND")
+    got = launch(text, inputs, tmp_path)
+    for a, o in zip(clean, got):
+        assert torch.equal(a[0], o[0])
+    for h in (0, 1, 3):
+        assert torch.equal(clean[0][1, :, h], got[0][1, :, h]) and torch.equal(clean[1][1, h], got[1][1, h])
+    assert torch.equal(clean[0][1, :kept, 2], got[0][1, :kept, 2]) and torch.isnan(got[0][1, at:, 2]).all()
+
+
 # ---- what is refused ------------------------------------------------------------------------------------------------
 def text_of(dtype="bfloat16", q=(2, 9, 4, 64), k=(2, 9, 2, 64), v=(2, 9, 2, 32), decay=([4], "float32"), state=None, slots=None, lengths=None, grad=False, dout=None,
             dstate=None, **options):
