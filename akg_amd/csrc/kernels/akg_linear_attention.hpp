@@ -497,7 +497,7 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) queries[y][p] = pd.row(mem, place_of(lds.a[ia][p]), 32 * (y % CT), 2 * unit0 + y / CT);
   };
-  constexpr int kGroup = !kWide ? kUnits : kUnits % 2 == 0 ? 2 : 1, kPasses = PARTS == 1 ? kTerms : 2 * kTerms - 1;   // units of the state at a time
+  constexpr int kGroup = !kWide && !C::REST ? kUnits : kUnits % 2 == 0 ? 2 : 1, kPasses = PARTS == 1 ? kTerms : 2 * kTerms - 1;   // units of the state at a time
   constexpr int kAllKeys = kSteps * kUnits, kKeysAhead = kWide ? 3 : kGroup;
   u32x4 values[kSteps][PARTS], more[kSteps][kTerms], keys[kAllKeys][PARTS];
   auto key = [&](int ib, int x) {
@@ -533,8 +533,13 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
     // (pair e of the eight rows x)
     auto rounded = [&](int x, int e) {
       const int r = 8 * (x & 1) + 2 * e;
-      const float lo = state[x >> 1][r], hi = state[x >> 1][r + 1];
+      float lo = state[x >> 1][r], hi = state[x >> 1][r + 1];
       split_pair<PARTS>(lo, hi, parts[x], e);
+      if constexpr (PARTS == 1 || !C::REST) {
+        u32 w = parts[x][PARTS - 1][e];
+        asm("" : "+v"(w), "+v"(lo), "+v"(hi));   // (rounded before it fades, which then needs no register more)
+        parts[x][PARTS - 1][e] = w;
+      }
       state[x >> 1][r] = __builtin_fmaf(lo, fade, lo);
       state[x >> 1][r + 1] = __builtin_fmaf(hi, fade, hi);
     };
@@ -564,16 +569,31 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
   };
   if (chunks > 0) {
     __syncthreads();   // (the first tiles are in place)
-    if constexpr (!STATES) {
+    if constexpr (!STATES && !TIGHT) {
 #pragma unroll
       for (int y = 0; y < kAhead && y < kAll; ++y) query(0, y);
-      through(0);
     }
-    ready(0);
-    if constexpr (!STATES) __syncthreads();
   }
   int third = 0;   // t mod 3
-  for (int t = 0; t < chunks; ++t) {
+  // What needs the state in front of chunk t, and the tiles that the rest of it begins with.
+  auto front = [&](int t) __attribute__((always_inline)) {
+    const int n = count_of(t), ia = TIGHT ? 0 : t & 1, ib = TIGHT ? 0 : third;
+    if (t > 0 && n != kChunk) weigh(n);
+    if (TIGHT && t > 0) {
+      __syncthreads();
+      __syncthreads();   // (the chunk's tiles are in place)
+    }
+    if constexpr (!STATES) {
+      if constexpr (TIGHT) {
+#pragma unroll
+        for (int y = 0; y < kAhead && y < kAll; ++y) query(0, y);
+      }
+      through(ia);
+    }
+    ready(ib);
+    if (!STATES || (!TIGHT && t > 0)) __syncthreads();
+  };
+  auto back = [&](int t) __attribute__((always_inline)) {
     const int n = count_of(t), ia = TIGHT ? 0 : t & 1, ib = TIGHT ? 0 : third;
     third = third + 1 < 3 ? third + 1 : 0;
     u32x4 pairs[kSteps][CT][PARTS];
@@ -600,7 +620,6 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
         }
       }
     } else {
-      if (n != kChunk) weigh(n);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
 #pragma unroll
@@ -687,22 +706,21 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (t + 1 >= chunks) break;
-    if constexpr (TIGHT) {
-      __syncthreads();
-      __syncthreads();   // (the next chunk's tiles are in place)
+  };
+  // One body for both where registers hold it (4 x 4096 tokens of 8 heads of 256 231 us with it, 125 without, of 32 of 128 in
+  // float16 269, 223; with the last state kept 4 x 2048 of 16/4 heads of 256 111, 115, 16384 of 16 of 128 105, 107).
+  if constexpr (PARTS == 1 && !kWide) {
+    for (int t = 0; t < chunks; ++t) {
+      front(t);
+      back(t);
     }
-    if constexpr (!STATES) {
-      const int then = count_of(t + 1);
-      if (then != kChunk) weigh(then);
-      if constexpr (TIGHT) {
-#pragma unroll
-        for (int y = 0; y < kAhead && y < kAll; ++y) query(0, y);
-      }
-      through(TIGHT ? 0 : 1 - ia);
+  } else if (chunks > 0) {
+    front(0);
+    for (int t = 0;; ++t) {
+      back(t);
+      if (t + 1 >= chunks) break;
+      front(t + 1);
     }
-    ready(TIGHT ? 0 : third);
-    if constexpr (!STATES || !TIGHT) __syncthreads();
   }
 
   // a walk over states leaves them in the workspace; else the segment that holds the last token has the last state
