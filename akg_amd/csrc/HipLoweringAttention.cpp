@@ -23,7 +23,7 @@ using lowering::dtypeTag;
 
 int64_t ceilDiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Tokens up to which linear attention goes token after token: us that way, in chunks: 16 x 2, 4, 8, 12 of 16/4 heads of 64, float16,
-// 4.6, 4.8, 6.2, 7.9 and 6.1; 16 x 2, 4, 8, 16 of 32 heads of 128 12.8, 14.7, 18.1, 24.9 and 21.4, 21.5, 21.7, 22.2.
+// 4.5, 4.6, 6.2, 7.9 and 6.4; 16 x 2, 4, 8, 16 of 32 heads of 128 12.8, 14.7, 18.2, 24.9 and 21.4, 21.5, 21.7, 22.1.
 constexpr int64_t kFewTokens = 8;
 
 class LayerEmitter {
@@ -580,7 +580,8 @@ class LayerEmitter {
   }
   std::string walkConfig(const WalkOf &w, const LinearSizes &s, int ct, int64_t nw, int halves, int helpers, bool tight) const {
     std::ostringstream o;
-    o << "akg::linear::Config<" << trait() << ", " << w.d << ", " << w.e << ", " << ct << ", " << nw << ", " << (w.d > 128 ? halves : 1) << ", " << helpers << ", " << flag(tight) << ", " << flag(w.rest) << ", " << s.heads << ", " << w.ha << ", " << w.hb << ", " << w.hc
+    o << "akg::linear::Config<" << trait() << ", " << w.d << ", " << w.e << ", " << ct << ", " << nw << ", " << (w.d > 128 ? halves : 1) << ", " << helpers
+      << ", " << flag(tight) << ", " << flag(w.rest) << ", " << s.heads << ", " << w.ha << ", " << w.hb << ", " << w.hc
       << ", " << flag(l_.headsFirst) << ", " << flag(w.back) << ", " << flag(w.turned) << ", akg::linear::Result::" << w.result << ">";
     return o.str();
   }
@@ -598,20 +599,20 @@ class LayerEmitter {
     const int parts = in(0).dtype == DType::F16 ? 2 : 1;
     const int64_t units = ceilDiv(widest, 32);
     // Two wavefronts share the rows of 32 columns of a state where one has too few registers for them: above 128 channels with
-    // operands or terms of the state in several parts (4 x 2048 tokens of 16/4 heads of 256, the last state kept: 117 us instead of 328;
-    // float16 288, 1339; without that 4 x 4096 of 8 heads in bfloat16 135 with one, 153 with two, its gradient 246, 334).
+    // operands in two parts or terms of the state in three (4 x 2048 tokens of 16/4 heads of 256, the last state kept: 113 us instead
+    // of 319; float16 248, 941; without that 4 x 4096 of 8 heads in bfloat16 127 with one, 159 with two, its gradient 237, 337).
     bool rest = false;
     for (const WalkOf &w : all) rest = rest || w.rest;
     const int halves = deepest > 128 && (parts == 2 || rest) ? 2 : 1;
     // How many wavefronts hold the state of a workgroup (32 columns each: fewer make more workgroups, which all fetch a and b and
     // multiply them), and how many segments share the tokens (each but the last adds a pass over b and c in front): what is
-    // expected to take least. A chunk of 64 tokens of 128 channels takes 1.4, 1.5 and 2.0 us with one, two and four such wavefronts
-    // (one workgroup a CU), of 32 tokens of 256 channels 1.2, 1.2 and 1.5, of 32 tokens of 128 in float16 1.8 and 2.4 with two and
-    // four, a walk over states alone about half; memory gives 4.8 TB/s; two launches more and a state to be
-    // joined take some 10 us. us at 4 x 4096 tokens of 32 heads of 128: two 121, four 145, four and two segments 157; 2 x 2048:
-    // one 48, two 56, four 69, four and four segments 53; 16384 of 16 heads: four and 1, 8, 16, 32 segments 522, 132, 102, 117;
-    // 4 x 4096 of 16 heads of 64: one 76, two and 1, 4, 8 segments 91, 50, 56; gradient of 2 x 1021 of 16/4 heads of 128: one, two,
-    // four 59, 40, 49; of 4 x 4096 of 32 heads: two, four 351, 297.
+    // expected to take least. A chunk of 64 tokens of 128 channels takes 1.5, 1.7 and 2.3 us with one, two and four such wavefronts
+    // (one workgroup a CU), with terms of the state in three parts some 20 % more, a walk over states alone about half; memory gives
+    // 4.8 TB/s; two launches more and a state to be joined take some 8 us. us at 4 x 4096 tokens of 32 heads of 128: one 192, two 128,
+    // four 160, four and two segments 157; 2 x 2048: one 52, two 60, four 76, four and four segments 57; 16384 of 16 heads, the last
+    // state kept: four and 1, 8, 16, 32 segments 597, 148, 107, 123, two and eight 126; 4 x 4096 of 16 heads of 64: one 77, two and 1,
+    // 4, 8 segments 93, 51, 55; 4 x 1003 of 16/4 of 96/80: one 31, three and 1, 4 segments 32, 27; gradient of 2 x 1021 of 16/4 heads
+    // of 128: one, two, four 68, 44, 51; of 4 x 4096 of 32 heads: two, four 358, 332.
     struct Schedule {
       double time;
       int64_t nw, segments;

@@ -25,9 +25,17 @@
  * The wavefronts share the masked products of a chunk (a . b) through LDS, in the form of the operand that they become.
  *
  * Rounding: bfloat16 operands are exact; products a . b and the state are rounded to bfloat16 (2^-8 of each term at most) where they
- * are contracted again. What is added to the state, exp(g ..) c, is rounded likewise where the state is only read on the way,
- * and goes as two bfloat16 parts (2^-16) where the last state is a result, in float32. float16 operands, and everything contracted with them, go as two bfloat16 parts
- * throughout: three products for one, no range but that of float32, and 2^-16 of each term.
+ * are contracted again. What is added to the state, exp(g ..) c, goes as two bfloat16 parts (2^-16 of it), since a state gathers what
+ * thousands of tokens add, and as three (2^-24) where the last state is a result, in float32. float16 operands, and everything
+ * contracted with them, go as two bfloat16 parts throughout: three products for one, no range but that of float32, and 2^-16 of each
+ * term.
+ *
+ * What bounds it: a wavefront that holds a state issues a vector instruction every 5.2 cycles, a matrix instruction of its own every
+ * 33, and has 340 of the first (the state rounded and faded, c weighed and split) and 54 of the second for 64 tokens of 128
+ * channels; all CUs at work, the clock falls to 1.5 GHz. 4 x 4096 tokens of 32 heads of 128 take 128 us, 4.2 TB/s, 16 x 4096 447 us,
+ * 4.8 TB/s; the gradient of the first 312 us for seven tensors, of which it moves ten. (c weighed by the wavefronts that fetch, and
+ * read from LDS in parts: a gradient of 2 x 1021 tokens of 16/4 heads 41 us instead of 45, of 4 x 4096 of 32 heads 356 instead of 312,
+ * since four wavefronts' tiles then have 32 tokens.)
  */
 #pragma once
 
@@ -47,7 +55,7 @@ using attn::u32x4;
 // by exclusive or with bits of the row. Four neighbouring rows of 64 bytes (transposed reads, half a wavefront at a time) and
 // sixteen of 16 bytes (rows read by 128 bits) then lie in banks of their own. The places of a lane differ by an exclusive or with
 // a constant. (With 32 and 64 bytes more a row instead, transposed reads met in the banks, or three chunks' tiles did not fit; a
-// gradient of 4 x 4096 tokens of 8 heads of 256 took 334 us instead of 247.)
+// gradient of 4 x 4096 tokens of 8 heads of 256 took 334 us instead of 242.)
 constexpr int pitch(int w) { return w <= 32 ? 64 : w <= 64 ? 128 : w <= 128 ? 256 : 512; }
 constexpr int turn(int w, int row) { return (w <= 32 ? 0 : w <= 64 ? (row & 2) << 1 : (row & 3) << 2) | ((row >> 2) & 3); }
 // (above 128 channels two wavefronts may share the rows of a state: a multiple of 64)
@@ -185,12 +193,14 @@ struct Stage {
   }
 };
 
-// What the emitted kernel states about a walk: the operands' type in parts, channels of a and b (D) and of c and the result
-// (E), 32-token tiles of a chunk (CT), wavefronts that hold the state (NW, 32 channels of c each, times HALVES of its rows), wavefronts that fetch and multiply (HELPERS, two or four), whether LDS holds one chunk's
-// tiles only (TIGHT), whether what is added to the state goes in two parts (REST), heads of the states (H) and of each operand, whether it runs backward, whether states given and left are
-// the transposed ones ([E][D] in memory).
+// What the emitted kernel states about a walk: the operands' type, channels of a and b (D) and of c and the result (E), 32-token
+// tiles of a chunk (CT), wavefronts that hold the state (NW, 32 channels of c each, times HALVES of its rows), wavefronts that fetch
+// and multiply (HELPERS, two or four), whether LDS holds one chunk's tiles only (TIGHT), whether what is added to the state goes in
+// three parts instead of two (REST), heads of the states (H) and of each operand, whether it runs backward, whether states given and
+// left are the transposed ones ([E][D] in memory).
 enum class Result { None, Storage, Float };
-template <typename T_, int D_, int E_, int CT_, int NW_, int HALVES_, int HELPERS_, bool TIGHT_, bool REST_, int H_, int HA_, int HB_, int HC_, bool HEADS_FIRST_, bool BACK_, bool TURNED_, Result RESULT_>
+template <typename T_, int D_, int E_, int CT_, int NW_, int HALVES_, int HELPERS_, bool TIGHT_, bool REST_, int H_, int HA_, int HB_, int HC_,
+          bool HEADS_FIRST_, bool BACK_, bool TURNED_, Result RESULT_>
 struct Config {
   typedef T_ T;   // attn::BF16 or attn::F16
   static constexpr int PARTS = T::kNarrowRange ? 2 : 1, D = D_, E = E_, CT = CT_, NW = NW_, HALVES = HALVES_, HELPERS = HELPERS_, H = H_, HA = HA_, HB = HB_, HC = HC_;
@@ -250,10 +260,10 @@ AKG_DEV long entry_of(const int *slots, long b, long pool) {
 // One segment of one head, 32 NW channels of c. STATES: only what the segment adds to a state.
 //
 // NW wavefronts hold the state and do what needs it (with HALVES 2 NW, half of the rows each, since a state of 256 leaves a wavefront
-// few registers: the second half's a . S reaches the first through LDS). The others fetch into registers, two chunks ahead of what they put into
-// LDS (float16 in parts), and compute the masked products. Between two barriers the first have what chunk t adds to the state, its
-// masked products with c, and a . S of chunk t + 1; the others the masked products of t + 1, and a, b and c of t + 2 to put in
-// place of tiles that nothing reads any more. TIGHT: one after the other.
+// few registers: the second half's a . S reaches the first through LDS). The others fetch into registers, two chunks ahead of what
+// they put into LDS (float16 in parts), and compute the masked products. Between two barriers the first have what chunk t adds to
+// the state, its masked products with c, and a . S of chunk t + 1; the others the masked products of t + 1, and a, b and c of t + 2
+// to put in place of tiles that nothing reads any more. TIGHT: one after the other.
 template <typename C, bool STATES>
 AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int seg) {
   constexpr int D = C::D, E = C::E, PARTS = C::PARTS, CT = C::CT, NW = C::NW, kChunk = C::kChunk, kThreads = 64 * C::HELPERS;
@@ -535,7 +545,7 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
       const int r = 8 * (x & 1) + 2 * e;
       float lo = state[x >> 1][r], hi = state[x >> 1][r + 1];
       split_pair<PARTS>(lo, hi, parts[x], e);
-      if constexpr (PARTS == 1 || !C::REST) {
+      if constexpr (PARTS == 1 || !C::REST) {   // (in parts, three of them added, it copied the whole state instead)
         u32 w = parts[x][PARTS - 1][e];
         asm("" : "+v"(w), "+v"(lo), "+v"(hi));   // (rounded before it fades, which then needs no register more)
         parts[x][PARTS - 1][e] = w;
@@ -708,7 +718,7 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
     __builtin_amdgcn_sched_barrier(0);
   };
   // One body for both where registers hold it (4 x 4096 tokens of 8 heads of 256 231 us with it, 125 without, of 32 of 128 in
-  // float16 269, 223; with the last state kept 4 x 2048 of 16/4 heads of 256 111, 115, 16384 of 16 of 128 105, 107).
+  // float16 269, 223; with the last state kept 4 x 2048 of 16/4 heads of 256 111, 115, gradient of 2 x 1021 of 16/4 of 128 45, 47).
   if constexpr (PARTS == 1 && !kWide) {
     for (int t = 0; t < chunks; ++t) {
       front(t);

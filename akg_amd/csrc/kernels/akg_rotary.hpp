@@ -9,6 +9,8 @@
  * dropped terms are below 2^-28 there. Bound by memory: a thread turns the pairs of 16-byte accesses of one head (4 x 4096
  * tokens of 32 + 8 heads of 128 channels in bfloat16 take 59 us, 5.7 TB/s; with the angles computed once for two, four
  * and eight heads a thread 2, 6 and 8 % more: the arithmetic hides behind the accesses, the longer chains do not).
+ * Tokens with several positions: a table holds the axis of every pair, and pairs of a thread that have one read its position
+ * once (three axes, the same tokens, 60.5 us, 5.5 TB/s).
  */
 #pragma once
 
