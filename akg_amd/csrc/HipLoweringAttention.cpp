@@ -608,11 +608,16 @@ class LayerEmitter {
     // multiply them), and how many segments share the tokens (each but the last adds a pass over b and c in front): what is
     // expected to take least. A chunk of 64 tokens of 128 channels takes 1.5, 1.7 and 2.3 us with one, two and four such wavefronts
     // (one workgroup a CU), with terms of the state in three parts some 20 % more, a walk over states alone about half; memory gives
-    // 4.8 TB/s; two launches more and a state to be joined take some 8 us. us at 4 x 4096 tokens of 32 heads of 128: one 192, two 128,
+    // 4.8 TB/s; a launch more takes some 5 us, two and a state to be joined 8. us at 4 x 4096 tokens of 32 heads of 128: one 192, two 128,
     // four 160, four and two segments 157; 2 x 2048: one 52, two 60, four 76, four and four segments 57; 16384 of 16 heads, the last
     // state kept: four and 1, 8, 16, 32 segments 597, 148, 107, 123, two and eight 126; 4 x 4096 of 16 heads of 64: one 77, two and 1,
-    // 4, 8 segments 93, 51, 55; 4 x 1003 of 16/4 of 96/80: one 31, three and 1, 4 segments 32, 27; gradient of 2 x 1021 of 16/4 heads
+    // 4, 8 segments 93, 49, 55; 4 x 1003 of 16/4 of 96/80: one 31, three and 1, 4 segments 32, 24; gradient of 2 x 1021 of 16/4 heads
     // of 128: one, two, four 68, 44, 51; of 4 x 4096 of 32 heads: two, four 358, 332.
+    // A few segments' states are added up by the walks themselves, without a launch for it (1 x 512 tokens of 12 heads of 64 in float16,
+    // eight segments, 11.6 us instead of 14.2, 4 x 1003 of 16/4 of 96/80, four, 23.6 instead of 26.9, 2048 of 16 heads of 128, eight, 28
+    // instead of 31; 8192 of 8 heads of 128, sixteen, 49 instead of 45), where a wavefront has at most 128 of their rows (4 x 4096 of 8
+    // heads of 256, four, 182 instead of 131).
+    auto joins = [&](int64_t segments) { return segments > 1 && segments <= 8 && deepest <= 128 * halves; };
     struct Schedule {
       double time;
       int64_t nw, segments;
@@ -647,7 +652,7 @@ class LayerEmitter {
         auto both = [](double x, double y) { return std::max(x, y) + 0.25 * std::min(x, y); };
         double time = both(static_cast<double>(ceilDiv(groups * segments, cus_)) * steps * each, moved);
         if (segments > 1) {
-          time += both(static_cast<double>(ceilDiv(groups * (segments - 1), cus_)) * steps * each * 0.55, movedStates) + 8.0 +
+          time += both(static_cast<double>(ceilDiv(groups * (segments - 1), cus_)) * steps * each * 0.55, movedStates) + (joins(segments) ? 4.6 + 0.4 * static_cast<double>(segments) : 8.0) +
                   static_cast<double>(8 * s.states * segments * values) / 4.8e6;
         }
         if (best.nw == 0 || time < best.time) best = {time, nw, segments, ct, tight};
@@ -670,6 +675,7 @@ class LayerEmitter {
     o << "typedef " << walkConfig(all[0], s, ct, nw, halves, helpers, tight) << " akg_C0;\n";
     for (size_t i = 1; i < all.size(); ++i) o << "typedef " << walkConfig(all[i], s, ct, nw, halves, helpers, tight) << " akg_C" << i << ";\n";
     o << "\n";
+    const bool join = joins(segments);
     int64_t before = space;
     std::vector<std::string> structs;
     for (const WalkOf &w : all) {
@@ -677,7 +683,7 @@ class LayerEmitter {
       b << "{" << w.a << ", " << w.b << ", " << w.c << ", " << w.out << ", " << decay << ", " << w.first << ", " << w.last << ", " << lengths << ", " << slots << ", ";
       if (segments > 1) b << "akg_ws + (" << space / 4 << "L + " << (before - space) / 4 << "L * akg_batch * akg_segments)";
       else b << "nullptr";
-      b << ", akg_seq, " << (l_.hasSlots ? "akg_pool" : "akg_batch") << ", static_cast<int>(akg_segment), static_cast<int>(akg_segments), " << number(l_.scale) << "}";
+      b << ", akg_seq, " << (l_.hasSlots ? "akg_pool" : "akg_batch") << ", static_cast<int>(akg_segment), static_cast<int>(akg_segments), " << number(l_.scale) << ", " << flag(join) << "}";
       structs.push_back(b.str());
       before += 4 * s.heads * w.d * w.e;
     }
@@ -715,6 +721,8 @@ class LayerEmitter {
     };
     if (segments > 1) {
       launch(name_ + "_states", groups * (segments - 1), threads, body(true), hint);
+    }
+    if (segments > 1 && !join) {
       std::ostringstream b;
       b << "  long akg_at = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;\n  const long akg_heads = akg_batch * " << s.heads << ";\n";
       for (size_t i = 0; i < all.size(); ++i) {

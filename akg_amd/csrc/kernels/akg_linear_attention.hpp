@@ -231,8 +231,8 @@ struct Tokens {
   }
 };
 
-// A walk's arguments. `starts`: states in front of every segment, [head][segment][D][E], written by the launches before (none
-// where there is one segment); a walk over states alone leaves there what its segment adds.
+// A walk's arguments. `starts`: [head][segment][D][E], what every segment adds to a state, left by a walk over states alone, then
+// the states in front of them (none where there is one segment).
 struct Walk {
   const void *a, *b, *c;
   void *out;
@@ -243,6 +243,7 @@ struct Walk {
   long seq, pool;                   // entries of `first` and `last`
   int segment, segments;            // tokens of a segment (a multiple of the chunk), their number
   float scale;
+  bool join;                        // no launch makes the one of the other: a walk adds up what stands in front of its segment
 };
 
 AKG_DEV long length_of(const int *lengths, long b, long seq) {
@@ -255,6 +256,12 @@ AKG_DEV long entry_of(const int *slots, long b, long pool) {
   if (slots == nullptr) return b;
   const long n = slots[b];
   return n >= 0 && n < pool ? n : -1;
+}
+
+// Tokens of segment s of a sequence of `len`.
+AKG_DEV int tokens_of(const Walk &w, long len, int s) {
+  const long left = len - static_cast<long>(s) * w.segment;
+  return left <= 0 ? 0 : left < w.segment ? static_cast<int>(left) : w.segment;
 }
 
 // One segment of one head, 32 NW channels of c. STATES: only what the segment adds to a state.
@@ -464,8 +471,8 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
   const long entry = entry_of(w.slots, b, w.pool);
   float *starts = w.starts + (w.starts != nullptr ? (head * w.segments + seg) * (static_cast<long>(D) * E) : 0);
   if constexpr (!STATES) {
-    const bool turned = C::TURNED && w.segments == 1;   // (starts in the workspace never are)
-    const float *given = w.segments > 1 ? starts : w.first != nullptr && entry >= 0 ? w.first + (entry * C::H + h) * (static_cast<long>(D) * E) : nullptr;
+    const bool turned = C::TURNED && (w.segments == 1 || w.join);   // (starts in the workspace never are)
+    const float *given = w.segments > 1 && !w.join ? starts : w.first != nullptr && entry >= 0 ? w.first + (entry * C::H + h) * (static_cast<long>(D) * E) : nullptr;
     if (given != nullptr && column < E) {
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
@@ -473,6 +480,20 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
         for (int r = 0; r < 16; ++r) {
           const int d = 32 * (unit0 + u) + 16 * (r >> 3) + 8 * half + (r & 7);
           if (D == whole(D) || d < D) state[u][r] = given[turned ? static_cast<long>(column) * D + d : static_cast<long>(d) * E + column];
+        }
+      }
+    }
+    if (w.join && column < E) {
+      for (int s = 0; s < seg; ++s) {
+        const float *add = starts - static_cast<long>(seg - s) * (D * E);
+        const float over = power(g2, tokens_of(w, len, s));
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int d = 32 * (unit0 + u) + 16 * (r >> 3) + 8 * half + (r & 7);
+            if (D == whole(D) || d < D) state[u][r] = __builtin_fmaf(state[u][r], over, add[static_cast<long>(d) * E + column]);
+          }
         }
       }
     }
@@ -776,10 +797,8 @@ AKG_DEV void scan(const Walk &w, long heads, long at) {
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
       if (s0 + k >= w.segments) break;
-      const long left = len - static_cast<long>(s0 + k) * w.segment;
-      const int n = left <= 0 ? 0 : left < w.segment ? static_cast<int>(left) : w.segment;
       __builtin_memcpy(to + static_cast<long>(s0 + k) * (D * E), &start, 16);
-      const float fade = power(g2, n);
+      const float fade = power(g2, tokens_of(w, len, s0 + k));
 #pragma unroll
       for (int e = 0; e < 4; ++e) start[e] = __builtin_fmaf(start[e], fade, add[k][e]);
     }

@@ -328,12 +328,14 @@ def test_without_allocations_and_at_odd_addresses(tmp_path):
 
 
 @pytest.mark.gpu
-def test_fewer_segments_without_allocations(tmp_path):
-    """A gradient whose heads' own gradients and states in front of segments take more than 16 MiB together."""
-    t = make(("bfloat16", "BSND", 1, 2048, 4, 2, 128, 128, "slow", False, "padded"))
+@pytest.mark.parametrize("seq", [2048, 3500])
+def test_fewer_segments_without_allocations(seq, tmp_path):
+    """A gradient whose heads' own gradients (4 KiB a token) and states in front of segments take almost, or more than, 16 MiB."""
+    t = make(("bfloat16", "BSND", 1, seq, 4, 2, 128, 128, "slow", False, "padded"))
     text, inputs = describe_grad(t, "BSND")
     kernel = driver.HipKernel(text, out_dir=str(tmp_path))
-    assert kernel.workspace_bytes > 16 << 20 and "_within" in kernel.source
+    assert kernel.workspace_bytes > seq * 4096 and ("_within" in kernel.source) == (kernel.workspace_bytes > 16 << 20)
+    assert seq == 2048 or "_within" in kernel.source
     kernel.prepare()
     ins, outs = [x.cuda() for x in inputs], empties(kernel)
     kernel.launch_static_scratch_ptrs([x.data_ptr() for x in ins + outs], torch.cuda.current_stream().cuda_stream)
