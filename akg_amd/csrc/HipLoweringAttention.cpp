@@ -611,11 +611,11 @@ class LayerEmitter {
     // 4.8 TB/s; a launch more takes some 5 us, two and a state to be joined 8. us at 4 x 4096 tokens of 32 heads of 128: one 192, two 128,
     // four 160, four and two segments 157; 2 x 2048: one 52, two 60, four 76, four and four segments 57; 16384 of 16 heads, the last
     // state kept: four and 1, 8, 16, 32 segments 597, 148, 107, 123, two and eight 126; 4 x 4096 of 16 heads of 64: one 77, two and 1,
-    // 4, 8 segments 93, 49, 55; 4 x 1003 of 16/4 of 96/80: one 31, three and 1, 4 segments 32, 24; gradient of 2 x 1021 of 16/4 heads
+    // 4, 8 segments 93, 49, 55; 4 x 1003 of 16/4 of 96/80: one 31, three and 1, 4 segments 32, 25; gradient of 2 x 1021 of 16/4 heads
     // of 128: one, two, four 68, 44, 51; of 4 x 4096 of 32 heads: two, four 358, 332.
     // A few segments' states are added up by the walks themselves, without a launch for it (1 x 512 tokens of 12 heads of 64 in float16,
-    // eight segments, 11.6 us instead of 14.2, 4 x 1003 of 16/4 of 96/80, four, 23.6 instead of 26.9, 2048 of 16 heads of 128, eight, 28
-    // instead of 31; 8192 of 8 heads of 128, sixteen, 49 instead of 45), where a wavefront has at most 128 of their rows (4 x 4096 of 8
+    // eight segments, 11.6 us instead of 14.2, 4 x 1003 of 16/4 of 96/80, four, 24.7 instead of 26.9, 2048 of 16 heads of 128, eight, 29.5
+    // instead of 30.8; 8192 of 8 heads of 128, sixteen, 49 instead of 45), where a wavefront has at most 128 of their rows (4 x 4096 of 8
     // heads of 256, four, 182 instead of 131).
     auto joins = [&](int64_t segments) { return segments > 1 && segments <= 8 && deepest <= 128 * halves; };
     struct Schedule {

@@ -469,10 +469,14 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) state[u] = {};
   const long entry = entry_of(w.slots, b, w.pool);
-  float *starts = w.starts + (w.starts != nullptr ? (head * w.segments + seg) * (static_cast<long>(D) * E) : 0);
-  if constexpr (!STATES) {
-    const bool turned = C::TURNED && (w.segments == 1 || w.join);   // (starts in the workspace never are)
-    const float *given = w.segments > 1 && !w.join ? starts : w.first != nullptr && entry >= 0 ? w.first + (entry * C::H + h) * (static_cast<long>(D) * E) : nullptr;
+  float *own = w.starts + (w.starts != nullptr ? head * w.segments * (static_cast<long>(D) * E) : 0), *starts = own + seg * (static_cast<long>(D) * E);
+  const float *first = w.first != nullptr && entry >= 0 ? w.first + (entry * C::H + h) * (static_cast<long>(D) * E) : nullptr;
+  // Walks that join the segments' states take the one given from the last segment's place, which needs none, since the last state may
+  // be written over it before another segment's workgroup begins.
+  float *copy = own + (w.segments - 1) * (static_cast<long>(D) * E);
+  if (!STATES || (w.join && seg == 0)) {
+    const bool turned = C::TURNED && (STATES || w.segments == 1);   // (what lies in the workspace never is)
+    const float *given = STATES || w.segments == 1 ? first : !w.join ? starts : first != nullptr ? copy : nullptr;
     if (given != nullptr && column < E) {
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
@@ -482,8 +486,17 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
           if (D == whole(D) || d < D) state[u][r] = given[turned ? static_cast<long>(column) * D + d : static_cast<long>(d) * E + column];
         }
       }
+#pragma unroll
+      for (int u = 0; STATES && u < kUnits; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = 32 * (unit0 + u) + 16 * (r >> 3) + 8 * half + (r & 7);
+          if (D == whole(D) || d < D) copy[static_cast<long>(d) * E + column] = state[u][r];
+          state[u][r] = 0.0f;
+        }
+      }
     }
-    if (w.join && column < E) {
+    if (!STATES && w.join && column < E) {
       for (int s = 0; s < seg; ++s) {
         const float *add = starts - static_cast<long>(seg - s) * (D * E);
         const float over = power(g2, tokens_of(w, len, s));

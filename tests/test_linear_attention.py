@@ -482,6 +482,32 @@ def test_long_texts_in_a_pool_in_place(tmp_path):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seq,joined", [(700, True), (6000, False)])
+def test_the_last_state_over_the_one_given_beside_other_work(seq, joined, tmp_path):
+    """Several segments, whose workgroups other work on the card keeps from starting together: in place as apart, bit for bit."""
+    heads, dim = 4, 64
+    t = dict({n: normal((2, seq, heads, dim), "bfloat16", 2 + i) for i, n in enumerate(("q", "k", "v"))}, log_decay=decays("slow", heads),
+             state=normal((2, heads, dim, dim), "float32", 1, 2.0))
+    text, inputs = describe(t, "BSND")
+    kernel = driver.HipKernel(text, out_dir=str(tmp_path))
+    assert kernel.workspace_bytes > 0 and ("_starts" not in kernel.source) == joined
+    kernel.prepare()
+    ins, apart = [x.cuda() for x in inputs], empties(kernel)
+    kernel.launch(ins + apart)
+    torch.cuda.synchronize()
+    check_forward(t, "BSND", [x.cpu() for x in apart])
+    side, a = torch.cuda.Stream(), torch.randn(2048, 2048, device="cuda")
+    for _ in range(6):
+        with torch.cuda.stream(side):
+            for _ in range(4):
+                a @ a
+        out, where = torch.empty_like(apart[0]), ins[4].clone()
+        kernel.launch(ins[:4] + [where] + [out, where])
+        torch.cuda.synchronize()
+        assert torch.equal(out, apart[0]) and torch.equal(where, apart[1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("seq", [2, 150, 2000])
 def test_one_entry_read_by_several_sequences(seq, tmp_path):
     """A prefix that sequences share: the same entry for all of them, and none left behind."""
