@@ -751,6 +751,10 @@ class LayerEmitter {
     std::ostringstream o;
     o << head("#include \"akg_attention.hpp\"\n#include \"akg_linear_attention.hpp\"\n");
     k_.algorithmicOps = static_cast<uint64_t>(4 * s.states * s.seq * s.dk * s.dv);
+    if (l_.hasSlots) {   // (of the pool, at most an entry for every sequence)
+      const int64_t idle = std::max<int64_t>(0, in(4).shape[0] - s.batch) * s.heads * s.dk * s.dv;
+      k_.algorithmicBytes = lowering::countAlgorithmicBytes(g_) - static_cast<uint64_t>(4 * idle * (wanted(1) ? 2 : 1));
+    }
     if (s.seq <= kFewTokens) {
       // Columns of a workgroup: as many as leave two workgroups for every CU.
       int64_t te = 128;

@@ -623,6 +623,15 @@ def test_refusals():
     refused(json.dumps(doc), -3, "does not follow")
 
 
+def test_bytes_count_the_entries_of_a_pool_that_sequences_have(tmp_path):
+    def moved(entries, **options):
+        text = text_of(state=([entries, 4, 64, 32], "float32"), slots=([2], "int32"), **options)
+        return driver.HipKernel(text, out_dir=str(tmp_path)).algorithmic_bytes
+    for last in (False, True):
+        assert moved(2, last_state=last) == moved(70, last_state=last)
+    assert moved(2, last_state=True) - moved(2) == 4 * 2 * 4 * 64 * 32
+
+
 def test_long_texts_of_few_heads_are_cut_into_segments(tmp_path):
     def kernel(seq, batch=1, **options):
         return driver.HipKernel(text_of(q=(batch, seq, 4, 64), k=(batch, seq, 4, 64), v=(batch, seq, 4, 64), **options), out_dir=str(tmp_path))
