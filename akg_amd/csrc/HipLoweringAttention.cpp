@@ -676,6 +676,8 @@ class LayerEmitter {
     for (size_t i = 1; i < all.size(); ++i) o << "typedef " << walkConfig(all[i], s, ct, nw, halves, helpers, tight) << " akg_C" << i << ";\n";
     o << "\n";
     const bool join = joins(segments);
+    // (one segment is stated as such: its walks have no workspace, and what would read a null one has to be known as dead)
+    const std::string parted = segments > 1 ? "static_cast<int>(akg_segments)" : "1";
     int64_t before = space;
     std::vector<std::string> structs;
     for (const WalkOf &w : all) {
@@ -683,7 +685,7 @@ class LayerEmitter {
       b << "{" << w.a << ", " << w.b << ", " << w.c << ", " << w.out << ", " << decay << ", " << w.first << ", " << w.last << ", " << lengths << ", " << slots << ", ";
       if (segments > 1) b << "akg_ws + (" << space / 4 << "L + " << (before - space) / 4 << "L * akg_batch * akg_segments)";
       else b << "nullptr";
-      b << ", akg_seq, " << (l_.hasSlots ? "akg_pool" : "akg_batch") << ", static_cast<int>(akg_segment), static_cast<int>(akg_segments), " << number(l_.scale) << ", " << flag(join) << "}";
+      b << ", akg_seq, " << (l_.hasSlots ? "akg_pool" : "akg_batch") << ", static_cast<int>(akg_segment), " << parted << ", " << number(l_.scale) << ", " << flag(join) << "}";
       structs.push_back(b.str());
       before += 4 * s.heads * w.d * w.e;
     }
@@ -695,7 +697,7 @@ class LayerEmitter {
     for (const WalkOf &w : all) tiles += w.tiles;
     auto body = [&](bool states) {
       std::ostringstream b;
-      b << "  const int akg_parts = static_cast<int>(akg_segments" << (states ? " - 1" : "") << ");\n  __shared__ __attribute__((aligned(256))) akg::u8 akg_lds[";
+      b << "  const int akg_parts = " << parted << (states ? " - 1" : "") << ";\n  __shared__ __attribute__((aligned(256))) akg::u8 akg_lds[";
       auto lds = [&](size_t i) { return "akg::linear::Lds<akg_C" + std::to_string(i) + ", " + flag(states) + ">"; };
       std::string size = "sizeof(" + lds(0) + ")";
       for (size_t i = 1; i < all.size(); ++i) {
