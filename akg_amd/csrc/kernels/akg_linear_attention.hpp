@@ -78,18 +78,36 @@ constexpr int swapped(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1
 
 // exp(g n) from g log2 e: 1 for n = 0 (also where g is -inf).
 AKG_DEV float power(float g2, int n) { return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(g2 * static_cast<float>(n)); }
-// exp(g n) - 1, with the digits that are left of it near 0: a state that is faded by s + s (exp(g n) - 1) is off by half a
-// step of float32 a chunk, in either direction; with the rounded factor it would be off by the same share every time.
-AKG_DEV float power_less_one(float g, int n) {
-  const float x = g * static_cast<float>(n);
-  if (n == 0) return 0.0f;
-  if (!(__builtin_fabsf(x) < 0.125f)) return __builtin_amdgcn_exp2f(x * kLog2e) - 1.0f;
-  float p = __builtin_fmaf(x, 1.0f / 720.0f, 1.0f / 120.0f);   // x^7 / 7! is below 2^-33 x there
-  p = __builtin_fmaf(x, p, 1.0f / 24.0f);
-  p = __builtin_fmaf(x, p, 1.0f / 6.0f);
-  p = __builtin_fmaf(x, p, 0.5f);
-  return __builtin_fmaf(x * x, p, x);
-}
+// What a state fades by with every chunk: exp(g n) as `whole`, a float32 number, and `rest`, what that leaves of it near 1. A factor
+// that is rounded once is off by the same share every time, over 256 chunks by 2^-17; so each chunk's is rounded with what is
+// `owed` since the first, and their product stays within a step of float32. (A state faded by s + s (exp(g n) - 1) does not
+// drift either, but is off by half a step of what it was, not of what is left of it: with exp(g n) of 2^-24 by all of that.)
+struct Fade {
+  float whole, rest, owed = 0.0f;
+  AKG_DEV void set(float g, int n) {
+    const float x = g * static_cast<float>(n);
+    rest = 0.0f;
+    if (n == 0) {
+      whole = 1.0f;
+    } else if (!(__builtin_fabsf(x) < 0.125f)) {
+      whole = __builtin_amdgcn_exp2f(x * kLog2e);
+    } else {
+      float p = __builtin_fmaf(x, 1.0f / 720.0f, 1.0f / 120.0f);   // exp(x) - 1: x^7 / 7! is below 2^-30 x there
+      p = __builtin_fmaf(x, p, 1.0f / 24.0f);
+      p = __builtin_fmaf(x, p, 1.0f / 6.0f);
+      p = __builtin_fmaf(x, p, 0.5f);
+      p = __builtin_fmaf(x * x, p, x);
+      whole = 1.0f + p;
+      rest = p - (whole - 1.0f);
+    }
+  }
+  AKG_DEV float next() {
+    owed += rest;
+    const float f = whole + owed;
+    owed -= f - whole;
+    return f;
+  }
+};
 
 // Float32 values as PARTS values of bfloat16 whose sum they are, to 2^-8, 2^-16 or 2^-24 of them: word `e` of an operand.
 template <int PARTS>
@@ -515,12 +533,13 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
   // s (the tokens are the last rows of their tile, however few).
   const float grow = C::BACK ? w.scale : 1.0f, show = C::BACK ? 1.0f : w.scale;
   float added[8], steps[kSteps], shown[CT], fade = 0.0f;
+  Fade fades;
 #pragma unroll
   for (int e = 0; e < 8; ++e) added[e] = power(g2, 15 - (8 * (e >> 2) + 4 * half + (e & 3)) + kAfter) * grow;
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) steps[s] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, power(g2, 16 * (kSteps - 1 - s)))));
   auto weigh = [&](int n) {
-    fade = power_less_one(g, n);
+    fades.set(g, n);
 #pragma unroll
     for (int i = 0; i < CT; ++i) {
       const int row = 32 * i + (lane & 31) - (kChunk - n);
@@ -584,8 +603,8 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
         asm("" : "+v"(w), "+v"(lo), "+v"(hi));   // (rounded before it fades, which then needs no register more)
         parts[x][PARTS - 1][e] = w;
       }
-      state[x >> 1][r] = __builtin_fmaf(lo, fade, lo);
-      state[x >> 1][r + 1] = __builtin_fmaf(hi, fade, hi);
+      state[x >> 1][r] = lo * fade;
+      state[x >> 1][r + 1] = hi * fade;
     };
 #pragma unroll
     for (int e = 0; e < 4; ++e) rounded(0, e);
@@ -623,6 +642,7 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
   auto front = [&](int t) __attribute__((always_inline)) {
     const int n = count_of(t), ia = TIGHT ? 0 : t & 1, ib = TIGHT ? 0 : third;
     if (t > 0 && n != kChunk) weigh(n);
+    fade = fades.next();
     if (TIGHT && t > 0) {
       __syncthreads();
       __syncthreads();   // (the chunk's tiles are in place)
@@ -667,7 +687,7 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) state[u][r] = __builtin_fmaf(state[u][r], fade, state[u][r]);
+        for (int r = 0; r < 16; ++r) state[u][r] *= fade;
       }
     }
     // a result in float32 is one of the walk's own heads, heads first
