@@ -6,7 +6,7 @@ import linear_reference as ref
 from akg_amd import driver
 from test_attention_ops import launch, normal
 from test_attention_use import empties
-from test_linear_attention import describe, describe_grad
+from test_linear_attention import decays, describe, describe_grad, make
 
 F = torch.float64
 STEP = 2.0 ** -24   # half a step of float32, relative to the value
@@ -84,3 +84,49 @@ def test_fading_does_not_drift_over_a_long_text(tmp_path):
     once = torch.exp(g.to(F) * 64).float().to(F) ** (tokens // 64) / torch.exp(g.to(F) * tokens) - 1
     assert (once.abs() > 2 * bound).any()   # (that it would show)
     assert (share.abs() <= bound).all(), share
+
+
+# What is added to a state that is a result goes as three bfloat16 parts: 2^-27 of it is left, two would leave 2^-18. Float32 adds,
+# over 1024 tokens with the decays taken here, at most 54 roundings that count of 2^-25.5 on average, and weights off by
+# some 4 half steps each: 3e-7 of a state in the mean square.
+DIGITS = 2.0 ** -20
+
+
+def kept(dtype):
+    t = make((dtype, "BSND", 2, 1024, 4, 2, 64, 64, "slow", True, None))
+    t["state"], t["dstate"] = t["state"] * 0, t["dstate"] * 0
+    return t
+
+
+def mean_square(got, exact):
+    return float(((got.to(F) - exact).square().mean((0, 2, 3)) / exact.square().mean((0, 2, 3))).sqrt().max())
+
+
+def test_two_parts_would_show():
+    t = kept("bfloat16")
+    g = decays("slow", 4).to(F)
+    k, v = (t[n].to(F).transpose(1, 2).repeat_interleave(2, 1) for n in ("k", "v"))
+    at = torch.arange(1024)
+    inside, behind = (torch.exp(g[:, None] * n)[None, :, :, None] for n in (63 - at % 64, 1023 - at - (63 - at % 64)))
+    exact = (k * inside * behind).transpose(2, 3) @ v
+    rest, left = (v * inside).float(), {}
+    whole = torch.zeros_like(v)
+    for n in (1, 2, 3):
+        part = rest.to(torch.bfloat16).float()
+        rest, whole = rest - part, whole + part.to(F)
+        left[n] = mean_square((k * behind).transpose(2, 3) @ whole, exact)
+    assert left[3] < DIGITS / 16 and left[2] > 2 * DIGITS
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1024, 960])
+def test_what_is_added_to_a_state_keeps_its_digits(tokens, tmp_path):
+    """Of a state that is a result, forward and backward."""
+    t = kept("bfloat16")
+    t = {n: x[:, :tokens].contiguous() if n in ("q", "k", "v", "dout") else x for n, x in t.items()}
+    text, inputs = describe(t, "BSND")
+    off = mean_square(launch(text, inputs, tmp_path)[1], ref.forward(t["q"], t["k"], t["v"], t["log_decay"])["last"])
+    assert off <= DIGITS, off
+    text, inputs = describe_grad(t, "BSND")
+    off = mean_square(launch(text, inputs, tmp_path)[3], ref.gradient(t["dout"], t["q"], t["k"], t["v"], t["log_decay"])["dstate"][0])
+    assert off <= DIGITS, off
