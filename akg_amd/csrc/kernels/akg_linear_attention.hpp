@@ -8,7 +8,9 @@
  *   out[r] = scale ( exp(g (r + 1)) q[r] S + sum_{c <= r} exp(g (r - c)) (q[r] . k[c]) v[c] )
  *   S     <- exp(g n) S + sum_c exp(g (n - 1 - c)) k[c] v[c]^T        (n: tokens of the chunk)
  *
- * No exponent is positive where g is not, so nothing overflows however long the walk is. The gradient is three walks of
+ * No exponent is positive where g is not, so nothing overflows however long the walk is. Where g is positive, a weight that no two tokens of
+ * a walk are far enough apart for counts as 0 (rows of a tile that hold no token would meet infinity otherwise), and so does what a
+ * state of 0 grows to. The gradient is three walks of
  * the same form, with dS[t] = scale q[t] dout[t]^T + exp(g) dS[t+1]:
  *
  *   dq[t] = scale dout[t] S[t]^T   (dout, v, k), dk[t] = v[t] dS[t]^T   (v, dout, q) backward, dv[t] = k[t] dS[t]   (k, q, dout) backward
@@ -78,6 +80,8 @@ constexpr int swapped(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1
 
 // exp(g n) from g log2 e: 1 for n = 0 (also where g is -inf).
 AKG_DEV float power(float g2, int n) { return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(g2 * static_cast<float>(n)); }
+// What a segment makes of the state in front of it (nothing of nothing, whatever the factor).
+AKG_DEV float grown(float state, float factor, float added) { return state == 0.0f ? added : __builtin_fmaf(state, factor, added); }
 // What a state fades by with every chunk: exp(g n) as `whole`, a float32 number, and `rest`, what that leaves of it near 1. A factor
 // that is rounded once is off by the same share every time, over 256 chunks by 2^-17; so each chunk's is rounded with what is
 // `owed` since the first, and their product stays within a step of float32. (A state faded by s + s (exp(g n) - 1) does not
@@ -361,10 +365,11 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
     // of tiles (query tile, key tile): 0 = (0, 0), 1 = (1, 0), 2 = (1, 1), one to a wavefront, or 0 and 2 to the first of two.
     float mask[16];
     if constexpr (!STATES) {
+      const int most = count_of(0);   // (a walk of fewer tokens than a chunk is its first chunk)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int n = (CT == 2 && helper == 1 ? 32 : 0) + (lane & 31) - (8 * (r >> 2) + 4 * half + (r & 3));
-        mask[r] = n < 0 ? 0.0f : power(g2, n) * w.scale;
+        mask[r] = n < 0 || n >= most ? 0.0f : power(g2, n) * w.scale;
       }
     }
     // `load`: what is asked of memory behind every matrix instruction.
@@ -523,7 +528,7 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int d = 32 * (unit0 + u) + 16 * (r >> 3) + 8 * half + (r & 7);
-            if (D == whole(D) || d < D) state[u][r] = __builtin_fmaf(state[u][r], over, add[static_cast<long>(d) * E + column]);
+            if (D == whole(D) || d < D) state[u][r] = grown(state[u][r], over, add[static_cast<long>(d) * E + column]);
           }
         }
       }
@@ -537,7 +542,10 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
 #pragma unroll
   for (int e = 0; e < 8; ++e) added[e] = power(g2, 15 - (8 * (e >> 2) + 4 * half + (e & 3)) + kAfter) * grow;
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) steps[s] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, power(g2, 16 * (kSteps - 1 - s)))));
+  for (int s = 0; s < kSteps; ++s) {
+    const int n = 16 * (kSteps - 1 - s);
+    steps[s] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, n >= count_of(0) ? 0.0f : power(g2, n))));
+  }
   auto weigh = [&](int n) {
     fades.set(g, n);
 #pragma unroll
@@ -833,7 +841,7 @@ AKG_DEV void scan(const Walk &w, long heads, long at) {
       __builtin_memcpy(to + static_cast<long>(s0 + k) * (D * E), &start, 16);
       const float fade = power(g2, tokens_of(w, len, s0 + k));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) start[e] = __builtin_fmaf(start[e], fade, add[k][e]);
+      for (int e = 0; e < 4; ++e) start[e] = grown(start[e], fade, add[k][e]);
     }
   }
 }
