@@ -280,6 +280,11 @@ AKG_DEV long entry_of(const int *slots, long b, long pool) {
   return n >= 0 && n < pool ? n : -1;
 }
 
+// Whether nothing is left of the state given behind the first token, whatever it holds (0 times that may be no number). Backward the
+// first token has it already.
+template <bool BACK>
+AKG_DEV bool forgets(float g, long len) { return !BACK && len > 0 && g == -__builtin_inff(); }
+
 // Tokens of segment s of a sequence of `len`.
 AKG_DEV int tokens_of(const Walk &w, long len, int s) {
   const long left = len - static_cast<long>(s) * w.segment;
@@ -493,7 +498,7 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
   for (int u = 0; u < kUnits; ++u) state[u] = {};
   const long entry = entry_of(w.slots, b, w.pool);
   float *own = w.starts + (w.starts != nullptr ? head * w.segments * (static_cast<long>(D) * E) : 0), *starts = own + seg * (static_cast<long>(D) * E);
-  const float *first = w.first != nullptr && entry >= 0 ? w.first + (entry * C::H + h) * (static_cast<long>(D) * E) : nullptr;
+  const float *first = w.first != nullptr && entry >= 0 && !forgets<C::BACK>(g, len) ? w.first + (entry * C::H + h) * (static_cast<long>(D) * E) : nullptr;
   // Walks that join the segments' states take the one given from the last segment's place, which needs none, since the last state may
   // be written over it before another segment's workgroup begins.
   float *copy = own + (w.segments - 1) * (static_cast<long>(D) * E);
@@ -819,9 +824,9 @@ AKG_DEV void scan(const Walk &w, long heads, long at) {
   if (head >= heads) return;
   const int x = static_cast<int>(at % kEach) * 4, h = static_cast<int>(head % C::H);
   const long b = head / C::H, len = length_of(w.lengths, b, w.seq), entry = entry_of(w.slots, b, w.pool);
-  const float g2 = w.log_decay[h] * kLog2e;
+  const float g = w.log_decay[h], g2 = g * kLog2e;
   f32x4 start = {};
-  if (w.first != nullptr && entry >= 0) {
+  if (w.first != nullptr && entry >= 0 && !forgets<C::BACK>(g, len)) {
     const float *given = w.first + (entry * C::H + h) * (static_cast<long>(D) * E);
 #pragma unroll
     for (int e = 0; e < 4; ++e) start[e] = given[C::TURNED ? (x % E + e) * D + x / E : x + e];   // (E is a multiple of 4)
@@ -895,7 +900,8 @@ AKG_DEV void tokens(const Walk &w, long head, int tile) {
     qs[t][d] = d < D ? T::dtype::load(reinterpret_cast<const S *>(tq.base + t * tq.step)[d]) * w.scale : 0.0f;
     ks[t][d] = d < D ? T::dtype::load(reinterpret_cast<const S *>(tk.base + t * tk.step)[d]) : 0.0f;
   }
-  const float fade = power(w.log_decay[h] * kLog2e, 1);
+  const float g = w.log_decay[h], fade = power(g * kLog2e, 1);
+  const bool forget = forgets<false>(g, len);
   __syncthreads();
   for (int t = 0; t < len; ++t) {
     f32x4 v = {}, out = {};
@@ -904,6 +910,10 @@ AKG_DEV void tokens(const Walk &w, long head, int tile) {
       __builtin_memcpy(raw, tv.base + t * tv.step + 2 * e, 8);
 #pragma unroll
       for (int z = 0; z < 4; ++z) v[z] = T::dtype::load(raw[z]);
+    }
+    if (forget) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) state[r] = {};
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {

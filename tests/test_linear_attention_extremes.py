@@ -1,4 +1,7 @@
-"""Linear attention where numbers are extreme: decays above 0."""
+"""Linear attention where numbers are extreme: decays above 0, decays of -infinity before states that are not finite, values that are
+not finite behind the tokens whose results are looked at."""
+import math
+
 import pytest
 import torch
 
@@ -49,3 +52,32 @@ def test_growing_behind_tokens_that_add_nothing(tokens, tmp_path):
     # rounded by itself, so that the sizes of the terms count, not those of their sums
     close(got[0][:, quiet:], r["out"], ref.bound(r["out"], [r["rough"][1]] * 2, "bfloat16", 64, tokens), "out")
     close(got[1], r["last"], ref.state_bound(r["last_rough"], 64, tokens), "last state")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,tokens,dim", [("bfloat16", 1, 64), ("float16", 6, 96), ("bfloat16", 70, 64), ("float16", 70, 256), ("bfloat16", 1200, 64), ("bfloat16", 6000, 64)])
+@pytest.mark.parametrize("pool", [False, True])
+def test_nothing_is_left_of_a_state_where_the_decay_is_infinite(dtype, tokens, dim, pool, tmp_path):
+    """An entry of a pool may hold anything where a head forgets everything; a sequence without tokens leaves it as it is."""
+    t = make((dtype, "BSND", 3, tokens, 4, 2, dim, dim, "all", True, None))
+    t["lengths"] = torch.tensor([tokens, 0, max(1, tokens - 5)], dtype=torch.int32)
+    if pool:
+        t["slots"] = torch.tensor([2, 0, 1], dtype=torch.int32)
+    text, inputs = describe(t, "BSND")
+    clean = launch(text, inputs, tmp_path)
+    forgets = torch.isinf(t["log_decay"])
+    t["state"][:, forgets] = torch.tensor([math.nan, math.inf, -math.inf]).repeat(dim * dim)[:dim * dim].view(dim, dim)
+    text, inputs = describe(t, "BSND")
+    out, last = launch(text, inputs, tmp_path)
+    assert torch.equal(out, clean[0])
+    idle = 0 if pool else 1
+    others = [i for i in range(3) if i != idle]
+    assert torch.equal(last[others], clean[1][others])
+    assert torch.equal(last[idle].view(torch.int32), t["state"][idle].view(torch.int32))
+    if not pool and tokens > 8:
+        t["state"] = t["state"] * 1
+        text, inputs = describe_grad(t, "BSND", wanted=[0], name="Fused_QueriesOnly")
+        dirty = launch(text, inputs, tmp_path)[0]
+        t["state"][:, forgets] = 0
+        text, inputs = describe_grad(t, "BSND", wanted=[0], name="Fused_QueriesOnly")
+        assert torch.equal(dirty, launch(text, inputs, tmp_path)[0])
