@@ -633,7 +633,7 @@ class LayerEmitter {
       if (nw > 2 && nw != ceilDiv(units, ceilDiv(units, 4))) continue;
       // Tiles of a few chunks (linear::Lds, linear::pitch) where LDS holds them, of chunks of 32 tokens before those of one chunk only.
       auto pitchOf = [](int64_t d) { return d <= 32 ? 64 : d <= 64 ? 128 : d <= 128 ? 256 : 512; };
-      auto ldsBytes = [&](int64_t tiles) { return parts * (32 * tiles * (5 * pitchOf(deepest) + 3 * pitchOf(32 * nw)) + 2 * 2048 * (tiles * (tiles + 1) / 2)) + (halves == 2 ? 2 * 4096 * nw * tiles : 0); };
+      auto ldsBytes = [&](int64_t tiles) { return parts * (32 * tiles * (5 * pitchOf(deepest) + 3 * pitchOf(32 * nw)) + 2 * 2048 * (tiles * (tiles + 1) / 2)) + (halves == 2 ? 2 * 4096 * nw * tiles : 0) + 512 * nw + 16; };
       int ct = parts == 2 || ldsBytes(2) > 160 * 1024 ? 1 : 2;
       const bool tight = ldsBytes(ct) > 160 * 1024;
       const int64_t groups = s.states * tilesOf(nw), chunks = ceilDiv(s.seq, 32 * ct);

@@ -182,12 +182,40 @@ struct Stage {
   // (the rows of a thread then lie a constant number of rows apart, at the same place of their swizzle)
   static constexpr bool kEven = kWhole && THREADS % kPerRow == 0 && THREADS / kPerRow % 16 == 0;
   static constexpr int kTileBytes = ROWS * pitch(W);
+  static constexpr u32 kInfinity = PARTS == 1 ? 0x7f80 : 0x7c00;   // of bfloat16, float16
   u32x4 held[kEach];
   template <bool BACK>
   AKG_DEV void load(const Rows<ROWS, BACK> &rows, int i, int tid) {
     const int c = tid + i * THREADS, row = c / kPerRow, at = c % kPerRow * 8;
     const bool there = row >= rows.missing && at < rows.channels && (kWhole || c < kChunks);
     held[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows.buf, there ? static_cast<u32>(rows.from + row * rows.each + 2 * at) : kBeyondEveryBuffer, 0, 0));
+  }
+  // Whether a piece of this thread holds a value that is not finite.
+  AKG_DEV bool odd() const {
+    typedef u16 u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, held[i][e] & 0x7fff7fffu));
+    }
+    return most[0] >= kInfinity || most[1] >= kInfinity;
+  }
+  // Zeros in place of such values; the first row of each channel that has one (`row0`: of the tile's first), if it comes before what
+  // `spoilt` has.
+  AKG_DEV void clean(int *spoilt, int row0, int tid) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int c = tid + i * THREADS, row = row0 + c / kPerRow, at = c % kPerRow * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const u32 bits = 0x7fffu << 16 * (e & 1);
+        if (((held[i][e / 2] & bits) >> 16 * (e & 1)) >= kInfinity) {
+          __hip_atomic_fetch_min(spoilt + at + e, row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          held[i][e / 2] &= ~bits;
+        }
+      }
+    }
   }
   AKG_DEV void store(u8 *tile, int tid) const {
 #pragma unroll
@@ -237,7 +265,11 @@ struct Lds {
   u8 b[kB][C::PARTS][C::kChunk * pitch(C::D)], c[kB][C::PARTS][C::kChunk * pitch(C::kColumns)], a[STATES ? 0 : kA][C::PARTS][C::kChunk * pitch(C::D)];
   u32x4 pairs[STATES ? 0 : kA][C::PARTS][kPairs][2][64];
   f32x4 other[STATES || C::HALVES == 1 ? 0 : kA][C::NW][C::CT][4][64];   // a . S of the second half of the rows
+  // By every wavefront that fetches: the first token of the segment whose c is not finite, for each channel, and whether there is one.
+  int spoilt[STATES ? 0 : C::HELPERS][C::kColumns];
+  __attribute__((aligned(16))) int odd[STATES ? 0 : C::HELPERS];
 };
+constexpr int kNever = 0x7fffffff;
 
 // Where the tokens of one head of a tensor with X heads of W channels of 2 bytes lie.
 template <int X, int W, bool HEADS_FIRST, int H>
@@ -359,9 +391,17 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) fetch_piece(to, from_, i);
     };
-    auto place = [&](int held, int ia, int ib) {
+    // Chunk t's tiles. A value of c that is not finite would spoil rows that do not see it (their weights are 0, and 0 times it is no
+    // number): the tile has 0 there, and the rows that do see it, and the state's column, become no numbers behind the walk.
+    auto place = [&](int t, int held, int ia, int ib) {
       if constexpr (!STATES) sa[held].store(lds.a[ia][0], tid);
       sb[held].store(lds.b[ib][0], tid);
+      if constexpr (!STATES) {   // (behind the others' stores, which then need not wait for c)
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(sc[held].odd()) != 0, 0)) {
+          sc[held].clean(lds.spoilt[helper], t * kChunk - (kChunk - count_of(t)), tid);
+          if (lane == 0) lds.odd[helper] = 1;
+        }
+      }
       sc[held].store(lds.c[ib][0], tid);
     };
     // Weights of the masked products (register r: key token 8 (r / 4) + 4 half + r % 4 of its 32, query token lane % 32). Pairs
@@ -429,6 +469,10 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
     if (chunks > 0) {
       fetch(0, 0);
       fetch(1, 1);
+      if constexpr (!STATES) {
+        for (int x = lane; x < C::kColumns; x += 64) lds.spoilt[helper][x] = kNever;
+        if (lane == 0) lds.odd[helper] = 0;
+      }
       typedef Lds<C, STATES> L;
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) {
@@ -439,13 +483,13 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
           if constexpr (!STATES) clear_padding<kChunk, D, kThreads>(lds.a[x][p], tid);
         }
       }
-      place(0, 0, 0);
+      place(0, 0, 0, 0);
       if constexpr (TIGHT) {
         __syncthreads();
         multiply(0, 0, 0, 2);
       } else {
         fetch(0, 2);
-        place(1, 1, 1);
+        place(1, 1, 1, 1);
         __syncthreads();
         multiply(0, 0, 1, 3);
       }
@@ -458,13 +502,13 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
       if (t + 1 >= chunks) return;
       if constexpr (TIGHT) {
         __syncthreads();   // (the tiles have been read)
-        place(1 - K, 0, 0);
+        place(t + 1, 1 - K, 0, 0);
         __syncthreads();
         multiply(0, 0, 1 - K, t + 3);
         if constexpr (!STATES) __syncthreads();
       } else {
         const int then = third + 1 < 3 ? third + 1 : 0;
-        place(K, K, then);
+        place(t + 2, K, K, then);
         multiply(1 - K, third, K, t + 4);
         third = then;
         __syncthreads();
@@ -816,6 +860,43 @@ AKG_DEV void walk(const Walk &w, Lds<C, STATES> &lds, long head, int tile, int s
       back(t);
       if (t + 1 >= chunks) break;
       front(t + 1);
+    }
+  }
+
+  // Rows from a value of c on that is not finite, and the state's column behind it: no numbers (the tiles had 0 in its place).
+  if constexpr (!STATES) {
+    int odd = 0;
+#pragma unroll
+    for (int i = 0; i < C::HELPERS; ++i) odd |= chunks > 0 ? lds.odd[i] : 0;
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(odd) != 0, 0)) {
+      auto first_of = [&](int channel) {
+        int n = kNever;
+#pragma unroll
+        for (int i = 0; i < C::HELPERS; ++i) n = n < lds.spoilt[i][channel] ? n : lds.spoilt[i][channel];
+        return n;
+      };
+      if (first_of(column - e0) != kNever) {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) state[u][r] = __builtin_nanf("");
+        }
+      }
+      if constexpr (C::RESULT != Result::None) {
+        constexpr bool kFloat = C::RESULT == Result::Float;
+        const Tokens<C::H, E, kFloat || C::HEADS_FIRST, C::H> to(w.out, b, h, w.seq, kFloat ? 4 : 2);
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "agent");   // (behind this wavefront's own stores)
+        for (int x = 0; part == 0 && x < 32 && e0 + 32 * block + x < E; ++x) {
+          for (long i = static_cast<long>(first_of(32 * block + x)) + lane; i < end - from; i += 64) {
+            char *at = const_cast<char *>(to.base) + (C::BACK ? len - 1 - from - i : from + i) * to.step;
+            if constexpr (kFloat) {
+              reinterpret_cast<float *>(at)[e0 + 32 * block + x] = __builtin_nanf("");
+            } else {
+              reinterpret_cast<u16 *>(at)[e0 + 32 * block + x] = PARTS == 1 ? 0x7fc0 : 0x7e00;
+            }
+          }
+        }
+      }
     }
   }
 
