@@ -39,6 +39,9 @@ class LayerEmitter {
       }
     }
     k_.kernelName = name_ + "_kernel";
+    k_.family = op_.kind == OpKind::RotaryEmbedding ? KernelFamily::Rotary
+                : op_.kind == OpKind::LinearAttention || op_.kind == OpKind::LinearAttentionGrad ? KernelFamily::LinearAttention
+                                                                                                 : KernelFamily::Attention;
     switch (op_.kind) {
       case OpKind::RotaryEmbedding: rotary(); break;
       case OpKind::Attention: attention(); break;
@@ -98,7 +101,7 @@ class LayerEmitter {
     return o.str();
   }
   std::string head(const char *header) const {
-    return "// Generated by the akg HIP lowering for gfx950. Op description: " + g_.name + "\n// family: attention, op: " + op_.name +
+    return "// Generated by the akg HIP lowering for gfx950. Op description: " + g_.name + "\n// family: " + kernelFamilyName(k_.family) + ", op: " + op_.name +
            "\n#include \"akg_rt.hpp\"\n" + header + "\n";
   }
   // `wavesPerSimd`: how many the registers have to leave room for (0: the compiler's choice).
@@ -210,7 +213,6 @@ class LayerEmitter {
     }
     o << kernel(k_.kernelName, 256, signature({"akg_batch", "akg_seq"}, false), b.str());
     k_.source = o.str();
-    k_.family = KernelFamily::Rotary;
     k_.scalarArgs = {batch, seq};
     k_.grid[0] = checkGrid(ceilDiv(batch * seq * chunks * all, 256), 256);
     k_.block[0] = 256;
@@ -365,7 +367,6 @@ class LayerEmitter {
       k_.block[0] = static_cast<unsigned>(64 * nw);
     }
     k_.source = o.str();
-    k_.family = KernelFamily::Attention;
     k_.scalarArgs = {s.batch, s.sq, s.sk, splits};
     k_.algorithmicOps = static_cast<uint64_t>(2 * (s.dk + s.dv) * s.batch * s.heads * pairs(s, l_.causal));
     k_.scheduleNote = "32 rows per wavefront, wavefronts " + std::to_string(nw) + ", key ranges " + std::to_string(splits);
@@ -478,7 +479,6 @@ class LayerEmitter {
     phases.pop_back();
     k_.earlierPhases = phases;
     k_.source = o.str();
-    k_.family = KernelFamily::Attention;
     k_.scalarArgs = {s.batch, s.sq, s.sk};
     if (splits > 1) k_.scalarArgs.push_back(splits);
     // scores, dout v (but for dv alone), and a product for each result
@@ -537,7 +537,6 @@ class LayerEmitter {
       k_.block[0] = 256;
     }
     k_.source = o.str();
-    k_.family = KernelFamily::Attention;
     k_.scalarArgs = {batch, sq, blocks, perSequence, splits};
     // (of the pool, at most the blocks that the table names)
     const uint64_t live = static_cast<uint64_t>(std::min(blocks, batch * perSequence));
@@ -734,7 +733,6 @@ class LayerEmitter {
       launch(name_ + "_starts", ceilDiv(s.states * values / 4, 256), 256, b.str(), 0);
     }
     launch(more ? name_ + "_walks" : k_.kernelName, groups * segments, threads, body(false), hint);
-    k_.family = KernelFamily::LinearAttention;
     k_.scheduleNote = "tokens of a chunk " + std::to_string(chunk) + ", wavefronts " + std::to_string(nw) + ", segments " + std::to_string(segments);
     return segments > 1 ? space + 4 * s.states * segments * values : space;
   }
@@ -774,7 +772,6 @@ class LayerEmitter {
       if (l_.hasSlots) k_.scalarArgs.push_back(in(4).shape[0]);
       k_.grid[0] = checkGrid(s.states * tiles, 256);
       k_.block[0] = 256;
-      k_.family = KernelFamily::LinearAttention;
       k_.scheduleNote = "token after token, columns of a workgroup " + std::to_string(te);
       k_.source = o.str();
       return;

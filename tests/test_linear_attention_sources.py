@@ -5,6 +5,8 @@ import subprocess
 
 import pytest
 
+from akg_amd import driver, op_desc
+from test_attention_ops import builder
 from test_linear_attention import text_of
 
 TOOL = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "akg_amd", "akg-hip")
@@ -34,3 +36,12 @@ def test_the_installed_compiler_takes_them(name, tmp_path):
     text.write_text(described(**SOURCES[name]))
     done = subprocess.run([TOOL, "info", str(text)], capture_output=True, text=True, env=dict(os.environ, AKG_HIP_NO_CACHE="1"), timeout=300)
     assert done.returncode == 0 and "linear_attention" in done.stdout, (done.returncode, done.stderr[-500:])
+
+
+def test_a_source_names_its_family(tmp_path):
+    for name, family in (("few", "linear_attention"), ("joined", "linear_attention"), ("gradient", "linear_attention")):
+        kernel = driver.HipKernel(described(**SOURCES[name]), out_dir=str(tmp_path))
+        assert kernel.family == family and "// family: %s, op: " % family in kernel.source
+    b = builder()
+    kernel = driver.HipKernel(b.dumps(op_desc.rotary_embedding(b, [b.input([1, 3, 2, 8], "float32")], b.input([3], "int32"))), out_dir=str(tmp_path))
+    assert kernel.family == "rotary" and "// family: rotary, op: " in kernel.source
