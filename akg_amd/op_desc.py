@@ -7,6 +7,7 @@ and `output_desc`. Scalar constants are op inputs of shape [1] that carry a nume
 Only op names of the reference's op table (:417-486) are emitted, and this backend's own operators of an attention layer.
 """
 import json
+import operator
 import re
 
 _IDENT = re.compile(r"^[A-Za-z_][A-Za-z0-9_]*$")
@@ -606,7 +607,9 @@ def rotary_embedding(b, xs, positions, layout="BSND", base=10000.0, rotary_dims=
         if scaling and key in scaling:
             attrs.append((key, float(scaling[key])))
     if sections is not None:
-        attrs += [("sections", [int(n) for n in sections]), ("axis_order", axis_order), ("axis_rates", axis_rates)]
+        attrs.append(("sections", [operator.index(n) for n in sections]))   # (no fraction is cut off)
+    if sections is not None or axis_order != "blocks" or axis_rates != "shared":
+        attrs += [("axis_order", axis_order), ("axis_rates", axis_rates)]
     return _layer(b, "RotaryEmbedding", list(xs) + [positions], [(x.shape, x.dtype) for x in xs], attrs)
 
 
