@@ -1030,6 +1030,16 @@ class GraphBuilder {
       graph_.outputs.push_back(it->second);
     }
     if (graph_.outputs.empty()) throw TranslateError("op description has no outputs");
+    // A pool of last states holds the entries that sequences name, the others are what its memory held before: between two ops
+    // that would be anything.
+    for (const OpNode &op : graph_.ops) {
+      if (op.kind != OpKind::LinearAttention || !op.layer.hasSlots || op.outputs.size() < 2 || graph_.tensor(op.outputs[1]).outputIndex >= 0) continue;
+      for (const OpNode &other : graph_.ops) {
+        if (std::find(other.inputs.begin(), other.inputs.end(), op.outputs[1]) != other.inputs.end()) {
+          throw TranslateError("op " + op.name + ": a pool of last states that another op reads has to be a result of the description");
+        }
+      }
+    }
   }
 };
 

@@ -660,10 +660,10 @@ def linear_attention(b, q, k, v, log_decay, state=None, slots=None, lengths=None
     """Attention without a softmax, whose past is a state: state[t] = exp(log_decay) state[t-1] + k[t] v[t]^T, out[t] = scale
     q[t] state[t] (scale: 1 / sqrt(channels) where none is given). Heads of q may share those of k and v; every head of q has
     a decay of its own, `log_decay` float32 [heads] (at most 0; -inf forgets everything; above 0, times 64 tokens, it has to stay
-    below 88), and so a state of its own, float32
-    [batch, heads, channels of k, channels of v]. `state`: the one in front of the first token (none: zeros). `slots` int32
+    below 88), and so a state of its own, float32 [batch, heads, channels of k, channels of v]. `state`: the one in front of the first token (none: zeros). `slots` int32
     [batch]: `state` and the last state are pools [slots, heads, ..], of which a sequence has the entry named (all different;
-    one outside the pool: starts from zeros, and leaves none). The last state may be written over the state given. `lengths`
+    one outside the pool: starts from zeros, and leaves none; entries that nobody names stay as they are in the result's buffer).
+    The last state may be written over the state given where no other op reads that. `lengths`
     int32 [batch]: tokens of a sequence; the rows behind them are zeros. Returns [out] or [out, last state]. A few tokens (a
     decoding step, drafted tokens) run as the recurrence, more in chunks."""
     attrs, more = _linear_attrs(layout, scale, [("state", state), ("slots", slots), ("lengths", lengths)])
