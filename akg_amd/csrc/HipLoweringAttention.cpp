@@ -553,7 +553,8 @@ class LayerEmitter {
     int64_t d, e, ha, hb, hc;
     bool back, turned;
     const char *result;   // of linear::Result
-    bool rest;            // the last state is a result
+    // The op has the last state as a result, asked for or not: what a description returns does not change the bits of it.
+    bool rest;
     int64_t tiles = 1;
   };
   struct LinearSizes {
