@@ -8,10 +8,9 @@
  *   out[r] = scale ( exp(g (r + 1)) q[r] S + sum_{c <= r} exp(g (r - c)) (q[r] . k[c]) v[c] )
  *   S     <- exp(g n) S + sum_c exp(g (n - 1 - c)) k[c] v[c]^T        (n: tokens of the chunk)
  *
- * No exponent is positive where g is not, so nothing overflows however long the walk is. Where g is positive, a weight that no two tokens of
- * a walk are far enough apart for counts as 0 (rows of a tile that hold no token would meet infinity otherwise), and so does what a
- * state of 0 grows to. The gradient is three walks of
- * the same form, with dS[t] = scale q[t] dout[t]^T + exp(g) dS[t+1]:
+ * No exponent is positive where g is not, so nothing overflows however long the walk is. Where g is positive, weights of distances that
+ * no two tokens of a walk have are 0 (rows of a tile without a token would meet infinity otherwise), and a state of 0 stays 0. The
+ * gradient is three walks of the same form, with dS[t] = scale q[t] dout[t]^T + exp(g) dS[t+1]:
  *
  *   dq[t] = scale dout[t] S[t]^T   (dout, v, k), dk[t] = v[t] dS[t]^T   (v, dout, q) backward, dv[t] = k[t] dS[t]   (k, q, dout) backward
  *
