@@ -33,8 +33,8 @@
  *
  * What bounds it: a wavefront that holds a state issues a vector instruction every 5.2 cycles, a matrix instruction of its own every
  * 33, and has 340 of the first (the state rounded and faded, c weighed and split) and 54 of the second for 64 tokens of 128
- * channels; all CUs at work, the clock falls to 1.5 GHz. 4 x 4096 tokens of 32 heads of 128 take 128 us, 4.2 TB/s, 16 x 4096 447 us,
- * 4.8 TB/s; the gradient of the first 312 us for seven tensors, of which it moves ten. (c weighed by the wavefronts that fetch, and
+ * channels; all CUs at work, the clock falls to 1.5 GHz. 4 x 4096 tokens of 32 heads of 128 take 128 us, 4.2 TB/s, 16 x 4096 441 us,
+ * 4.9 TB/s; the gradient of the first 303 us for seven tensors, of which it moves ten. (c weighed by the wavefronts that fetch, and
  * read from LDS in parts: a gradient of 2 x 1021 tokens of 16/4 heads 41 us instead of 45, of 4 x 4096 of 32 heads 356 instead of 312,
  * since four wavefronts' tiles then have 32 tokens.)
  */
